@@ -31,4 +31,44 @@ int decode_embed(const int64_t* tok, const int64_t* pos, const uint16_t* E, int6
 int few_rows_logits(const uint16_t* X, int64_t ldx, const uint16_t* W, const uint16_t* norm_w, float eps, float* out, int64_t M,
                     int64_t N, int64_t K, void* stream);
 
+// ---- drafted decoding ----
+
+// Attention of a tree of drafted tokens over a cache (tree.hip).  Strides in elements; b / t / h (cache),
+// b / n / h (q, new keys and values), b / n (tree).
+struct TreeArgs {
+    const uint16_t *q, *k, *v, *knew, *vnew;
+    const int32_t* ctx;
+    const int64_t* tree;
+    uint16_t* o;
+    float *lse, *work;
+    int64_t qb, qn, qh, kb, kt, kh, vb, vt, vh, knb, knn, knh, vnb, vnn, vnh, treeb, treen;
+    int32_t B, N, first, H, Hkv, Tmax, D;
+    float scale;
+};
+int64_t tree_attention_workspace(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t Tmax, int32_t D);
+int tree_attention(const TreeArgs& a, void* stream);
+
+// probs (rows, V) fp32 = softmax(logits / temperature) over the top_k largest logits of a row and their
+// equals (top_k <= 0 or >= V: over all); logits (rows, V) contiguous, fp32 or (bf16) bfloat16.  A row
+// without a finite maximum: zeros where every logit is -inf, else NaN.
+int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, int64_t V, double temperature, int64_t top_k, void* stream);
+
+// The walk of drafted trees (draft.hip).  probs, draft (B, N, V) fp32 contiguous (draft may be null),
+// tokens (B, N) int64, parents (B, N) int32, uniform (B, N) fp32; out (B, N) int64, path (B, N) int32,
+// counts (B) int32.
+int verify_draft(const float* probs, const float* draft, const int64_t* tokens, const int32_t* parents, const float* uniform,
+                 int64_t* out, int32_t* path, int32_t* counts, int32_t B, int32_t N, int64_t V, void* stream);
+
+// Rows of caches moved: row ctx[b] + path[b, d] -> ctx[b] + d for d < counts[b], in the order of d; ctx_out = ctx +
+// counts.  Caches (B, T, H, D) of one shape with strides b / t / h.
+constexpr int kCompactTensors = 64;
+struct CompactArgs {
+    uint16_t* at[kCompactTensors];
+    int64_t sb[kCompactTensors], st[kCompactTensors], sh[kCompactTensors];
+    const int32_t *ctx, *path, *counts;
+    int32_t* ctx_out;   // null: another launch writes it
+    int32_t count, B, T, H, D, N;
+};
+int compact_cache(const CompactArgs& a, void* stream);
+
 }  // namespace fx

@@ -10,8 +10,10 @@
 // raise the error or make the aligned copy.
 #include <torch/extension.h>
 #include <torch/csrc/utils/pybind.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <tuple>
 #include <vector>
@@ -457,6 +459,137 @@ OptT few_rows_logits(const Tensor& x, const Tensor& w, const Tensor& norm_w, dou
     return out;
 }
 
+// ---- drafted decoding --------------------------------------------------------------------
+
+bool rows16(const Tensor& t, int64_t dims) {
+    if (!is_bf(t) || !t.is_cuda() || t.dim() != dims || t.stride(dims - 1) != 1 || !aligned(t)) return false;
+    for (int64_t i = 0; i < dims - 1; ++i)
+        if (t.stride(i) % 8) return false;
+    return true;
+}
+
+// (o, lse or None) of checked tensors, or None when a check fails
+std::optional<std::tuple<Tensor, OptT>> tree_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ctx,
+                                                       const Tensor& tree, int64_t first, double scale, bool want_lse,
+                                                       const OptT& knew, const OptT& vnew) {
+    if (!rows16(q, 4) || !rows16(k, 4) || !rows16(v, 4) || v.sizes() != k.sizes() || knew.has_value() != vnew.has_value())
+        return std::nullopt;
+    const int64_t B = q.size(0), N = q.size(1), H = q.size(2), D = q.size(3), T = k.size(1), Hkv = k.size(2);
+    if ((D != 64 && D != 128) || B < 1 || N < 1 || H < 1 || Hkv < 1 || H % Hkv || k.size(0) != B || k.size(3) != D || T < 1 ||
+        first < 0 || first > 63 || first + N > 64 || B > 0x7fffffff || H > 0x7fffffff || T > 0x7fffffff - 128)
+        return std::nullopt;
+    if (ctx.dim() != 1 || ctx.size(0) != B || ctx.scalar_type() != at::kInt || !ctx.is_cuda() || !ctx.is_contiguous() ||
+        tree.dim() != 2 || tree.size(0) != B || tree.size(1) != N || tree.scalar_type() != at::kLong || !tree.is_cuda())
+        return std::nullopt;
+    if (knew.has_value())
+        for (const Tensor* t : {&*knew, &*vnew})
+            if (!rows16(*t, 4) || t->size(0) != B || t->size(1) != N || t->size(2) != Hkv || t->size(3) != D) return std::nullopt;
+    same_gpu(q, k, v, ctx, tree, knew, vnew);
+    const c10::DeviceGuard guard(q.device());   // launches and the allocations below go to q's GPU
+    fx::TreeArgs a{};
+    a.q = bf(q), a.k = bf(k), a.v = bf(v), a.knew = bf(knew), a.vnew = bf(vnew);
+    a.ctx = static_cast<int32_t*>(ctx.data_ptr());
+    a.tree = static_cast<int64_t*>(tree.data_ptr());
+    a.qb = q.stride(0), a.qn = q.stride(1), a.qh = q.stride(2);
+    a.kb = k.stride(0), a.kt = k.stride(1), a.kh = k.stride(2);
+    a.vb = v.stride(0), a.vt = v.stride(1), a.vh = v.stride(2);
+    if (knew.has_value()) {
+        a.knb = knew->stride(0), a.knn = knew->stride(1), a.knh = knew->stride(2);
+        a.vnb = vnew->stride(0), a.vnn = vnew->stride(1), a.vnh = vnew->stride(2);
+    }
+    a.treeb = tree.stride(0), a.treen = tree.stride(1);
+    a.B = (int32_t)B, a.N = (int32_t)N, a.first = (int32_t)first, a.H = (int32_t)H, a.Hkv = (int32_t)Hkv;
+    a.Tmax = (int32_t)T, a.D = (int32_t)D;
+    a.scale = (float)scale;
+    Tensor o = at::empty({B, N, H, D}, q.options()), work;
+    OptT lse;
+    if (want_lse) lse = at::empty({B, N, H}, as_f32(q));
+    a.o = bf(o);
+    a.lse = want_lse ? f32(*lse) : nullptr;
+    const int64_t nbytes = fx::tree_attention_workspace(a.B, a.N, a.H, a.Hkv, a.Tmax, a.D);
+    if (nbytes) work = at::empty({nbytes / 4}, as_f32(q));
+    a.work = nbytes ? f32(work) : nullptr;
+    check(fx::tree_attention(a, stream_of(q)), "tree_attention");
+    return std::make_tuple(o, lse);
+}
+
+// fp32 probabilities shaped like the logits, or None when a check fails
+OptT sampling_probs(const Tensor& logits, double temperature, int64_t top_k) {
+    const bool b = is_bf(logits);
+    if ((!b && logits.scalar_type() != at::kFloat) || !logits.is_cuda() || logits.dim() < 1 || logits.size(-1) < 1 ||
+        !logits.is_contiguous() || !aligned(logits))
+        return std::nullopt;
+    const c10::DeviceGuard guard(logits.device());
+    Tensor p = at::empty(logits.sizes(), as_f32(logits));
+    const int64_t V = logits.size(-1);
+    check(fx::sampling_probs(logits.data_ptr(), b, f32(p), logits.numel() / V, V, temperature, top_k, stream_of(logits)),
+          "sampling_probs");
+    return p;
+}
+
+// (tokens, path, counts), or None when a check fails
+std::optional<std::tuple<Tensor, Tensor, Tensor>> verify_draft(const Tensor& probs, const Tensor& tokens, const Tensor& parents,
+                                                               const Tensor& uniform, const OptT& draft) {
+    if (probs.dim() != 3 || probs.size(1) < 1 || probs.size(1) > 64 || probs.size(2) < 1 || tokens.dim() != 2 ||
+        tokens.scalar_type() != at::kLong || parents.scalar_type() != at::kInt)
+        return std::nullopt;
+    const int64_t B = probs.size(0), N = probs.size(1), V = probs.size(2);
+    if (B > 0x7fffffff || (draft.has_value() && draft->sizes() != probs.sizes())) return std::nullopt;
+    for (const Tensor* t : {&tokens, &parents, &uniform})
+        if (t->dim() != 2 || t->size(0) != B || t->size(1) != N || !t->is_cuda() || !t->is_contiguous()) return std::nullopt;
+    for (const Tensor* t : {&probs, &uniform, draft.has_value() ? &*draft : &probs})
+        if (t->scalar_type() != at::kFloat || !t->is_cuda() || !t->is_contiguous()) return std::nullopt;
+    same_gpu(probs, tokens, parents, uniform, draft);
+    const c10::DeviceGuard guard(probs.device());
+    Tensor out = at::empty({B, N}, tokens.options()), path = at::empty({B, N}, parents.options()),
+           counts = at::empty({B}, parents.options());
+    check(fx::verify_draft(f32(probs), draft.has_value() ? f32(*draft) : nullptr, static_cast<int64_t*>(tokens.data_ptr()),
+                           static_cast<int32_t*>(parents.data_ptr()), f32(uniform), static_cast<int64_t*>(out.data_ptr()),
+                           static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(counts.data_ptr()), (int32_t)B, (int32_t)N, V,
+                           stream_of(probs)),
+          "verify_draft");
+    return std::make_tuple(out, path, counts);
+}
+
+// ctx + counts, or None when a check fails; the caches' rows moved in place
+OptT compact_cache(const std::vector<Tensor>& caches, const Tensor& ctx, const Tensor& path, const Tensor& counts) {
+    if (caches.empty() || path.dim() != 2 || path.size(1) < 1) return std::nullopt;
+    const Tensor& c = caches[0];
+    if (c.dim() != 4) return std::nullopt;
+    const int64_t B = c.size(0), T = c.size(1), H = c.size(2), D = c.size(3);
+    if (B < 1 || B > 65535 || T < 1 || T > 0x7fffffff || H < 1 || D < 8 || D % 8 || H * D > 0x7fffffff || path.size(0) != B ||
+        path.size(1) > 0x7fffffff)
+        return std::nullopt;
+    for (const Tensor* t : {&ctx, &counts})
+        if (t->dim() != 1 || t->size(0) != B) return std::nullopt;
+    for (const Tensor* t : {&ctx, &path, &counts})
+        if (t->scalar_type() != at::kInt || !t->is_cuda() || !t->is_contiguous()) return std::nullopt;
+    for (const Tensor& t : caches) {
+        if (!rows16(t, 4) || t.sizes() != c.sizes()) return std::nullopt;
+        same_gpu(c, t);
+    }
+    same_gpu(c, ctx, path, counts);
+    const c10::DeviceGuard guard(c.device());
+    Tensor out = at::empty({B}, ctx.options());
+    fx::CompactArgs a{};
+    a.ctx = static_cast<int32_t*>(ctx.data_ptr());
+    a.path = static_cast<int32_t*>(path.data_ptr());
+    a.counts = static_cast<int32_t*>(counts.data_ptr());
+    a.B = (int32_t)B, a.T = (int32_t)T, a.H = (int32_t)H, a.D = (int32_t)D, a.N = (int32_t)path.size(1);
+    const size_t most = std::min<size_t>(fx::kCompactTensors, 65535 / (size_t)B);
+    for (size_t i = 0; i < caches.size(); i += most) {
+        a.count = (int32_t)std::min(most, caches.size() - i);
+        a.ctx_out = i == 0 ? static_cast<int32_t*>(out.data_ptr()) : nullptr;
+        for (int32_t j = 0; j < a.count; ++j) {
+            const Tensor& t = caches[i + j];
+            a.at[j] = bf(t);
+            a.sb[j] = t.stride(0), a.st[j] = t.stride(1), a.sh[j] = t.stride(2);
+        }
+        check(fx::compact_cache(a, stream_of(c)), "compact_cache");
+    }
+    return out;
+}
+
 // ---- optimiser -------------------------------------------------------------------------
 
 // The flat layout of FlatAdamW: per parameter its offset, size and weight-decay flag.
@@ -547,6 +680,10 @@ PYBIND11_MODULE(_host, m) {
     FX_DEF(decode_inputs);
     FX_DEF(decode_embed);
     FX_DEF(few_rows_logits);
+    FX_DEF(tree_attention);
+    FX_DEF(sampling_probs);
+    FX_DEF(verify_draft);
+    FX_DEF(compact_cache);
     FX_DEF(ce_inv_nvalid);
     FX_DEF(ce_rows);
     FX_DEF(ce_finalize);

@@ -1,0 +1,489 @@
+// Attention of a tree of drafted tokens over a KV cache, for gfx950.
+//
+// Sequence b has ctx[b] keys in its cache; its tree's node j (a drafted token; node 0 the last
+// token that is not drafted) has cache row ctx[b] + j.  A query of node i sees every row below
+// ctx[b] and the rows of the nodes in its bit set tree[b, i]:
+//
+//   o[b, i, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[b, i, h] . k_j),
+//
+// over those rows j, in one pass with a running maximum and sum.  A node whose own bit is clear
+// is padding: its output is zero and its row is nobody's key.  Query heads share key heads
+// (H a multiple of Hkv): the N H / Hkv queries of one key head are the rows of one product.
+//
+// HBM-bound: every cached key and value is read once (4 D bytes a row and key head).  So the
+// rows of a key head stay in one workgroup, 32 to a wave's MFMA tile, and the keys are split:
+// over the workgroup's waves, and over workgroups ("units") for as many as fill the CUs at once.
+// A unit's length comes from the sequences' own lengths on the device, so a long sequence among
+// short ones gets more units and the cache's size costs nothing; a second kernel joins the units
+// of a row by their maxima and sums.  See the launch shape below for when keys are not split.
+#include <math.h>
+
+#include "fx_internal.h"
+#include "fx_mfma.h"
+
+namespace fx {
+
+constexpr int kTreeWaves = 8;
+constexpr int kTreeThreads = 64 * kTreeWaves;
+constexpr int kTreeTile = 32;    // keys of a wave's step, rows of its queries
+constexpr float kTreeNegInf = -__builtin_huge_valf();
+constexpr float kTreeLazy = 8.f;   // the running maximum moves only past this (log2 units): p stays <= 2^8
+
+// what a kernel needs besides the arguments: units a launch aims at (0: keys are not split), the
+// fewest tiles of a unit, query row groups of a key head
+struct TreePlan {
+    int32_t units, least, groups, wq;
+};
+
+__device__ __forceinline__ int tree_len(const TreeArgs& a, int b) {
+    const int c = a.ctx[b];
+    const int64_t e = (int64_t)(c < 0 ? 0 : c) + a.first + a.N;
+    return (int)(e < a.Tmax ? e : a.Tmax);
+}
+
+// Tiles of a unit: as many as let all sequences' tiles fit the units, in whole steps of the
+// workgroup.  Every wave computes it by itself, 64 sequences at a time.
+template <int WK>
+__device__ __forceinline__ uint32_t tree_unit_tiles(const TreeArgs& a, const TreePlan& p, int lane) {
+    uint32_t sum = 0;
+    for (int b = lane; b < a.B; b += 64) sum += (uint32_t)((tree_len(a, b) + kTreeTile - 1) / kTreeTile);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    sum *= (uint32_t)(p.groups * a.Hkv);
+    const uint32_t t = max((sum + p.units - 1) / (uint32_t)p.units, (uint32_t)p.least);
+    return (t + WK - 1) / WK * WK;
+}
+
+__device__ __forceinline__ uint32_t tree_seq_units(const TreeArgs& a, int b, uint32_t tiles) {
+    const uint32_t n = (uint32_t)((tree_len(a, b) + kTreeTile - 1) / kTreeTile);
+    return max(1u, (n + tiles - 1) / tiles);
+}
+
+// The sequence that holds unit u of those counted a sequence at a time (u in units of one key head
+// and row group), its first unit and its number of units; false past the last sequence.
+__device__ __forceinline__ bool tree_find(const TreeArgs& a, uint32_t u, uint32_t tiles, int lane, int& b, uint32_t& first,
+                                          uint32_t& count) {
+    uint32_t before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const uint32_t n = b0 + lane < a.B ? tree_seq_units(a, b0 + lane, tiles) : 0u;
+        uint32_t up = n;   // inclusive scan
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t o = __shfl_up(up, off, 64);
+            if (lane >= off) up += o;
+        }
+        const uint64_t past = __ballot(before + up > u);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            b = __builtin_amdgcn_readfirstlane(b0 + l);
+            count = __builtin_amdgcn_readfirstlane(__shfl(n, l, 64));
+            first = __builtin_amdgcn_readfirstlane(before + __shfl(up, l, 64)) - count;
+            return true;
+        }
+        before += __shfl(up, 63, 64);
+    }
+    return false;
+}
+
+// bits of the tree's nodes that are keys: drafted before this call (below `first`), or queries of it
+// that are no padding, and inside the cache
+__device__ __forceinline__ uint64_t tree_live(const TreeArgs& a, int b, int ctx, int lane) {
+    bool real = false;
+    if (lane < a.N) real = (a.tree[b * a.treeb + lane * a.treen] >> (a.first + lane)) & 1;
+    uint64_t live = (uint64_t)__ballot(real);
+    live = a.first ? (live << a.first) | ((1ull << a.first) - 1) : live;
+    const int room = a.Tmax - ctx;
+    return room >= 64 ? live : live & ((1ull << (room > 0 ? room : 0)) - 1);
+}
+
+__device__ __forceinline__ bool bf16_not_finite(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
+__device__ __forceinline__ bool any_not_finite(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= bf16_not_finite(w[i]) || bf16_not_finite(w[i] >> 16);
+    return bad;
+}
+
+// A wave's LDS operations are done in the order of its instructions; this keeps the compiler from moving
+// them past each other where lanes read what other lanes wrote.
+__device__ __forceinline__ void tree_wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Workgroup: WQ groups of 32 query rows x WK = 8 / WQ streams of keys; wave (wq, wk) takes the unit's
+// tiles wk, wk + WK, ...  Per tile S^T = K Q^T (a lane holds 16 of the 32 keys of one query), the
+// softmax, and O^T += V^T P^T with V read transposed from the wave's own LDS (fx_mfma.h has the
+// layouts); the next tile's keys and values are in flight in registers meanwhile, no barrier in the
+// loop.  The WK streams of a row join through LDS.
+template <int D, int WQ>
+__global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, TreePlan plan) {
+    constexpr int WK = kTreeWaves / WQ;
+    constexpr int LPR = D / 8;        // lanes of a row in 16-byte loads
+    constexpr int RPI = 64 / LPR;     // rows of a wave-wide load
+    constexpr int NV = kTreeTile / RPI;
+    constexpr int KS = D / 16;        // steps of the score product
+    constexpr int DT = D / 32;
+    constexpr int VLD = D + 32;       // LDS row of V: 4 rows of a transposed read fall in distinct banks
+    constexpr int OLD = D + 4;        // LDS row of a wave's fp32 output
+    constexpr int kVBytes = kTreeWaves * kTreeTile * VLD * 2;
+    constexpr int kOBytes = kTreeWaves * kTreeTile * OLD * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kVBytes > kOBytes ? kVBytes : kOBytes];
+    __shared__ float2 ml[kTreeWaves][kTreeTile];
+
+    const int lane = threadIdx.x & 63, ln = lane & 31, g = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wq = w % WQ, wk = w / WQ;
+    const int G = a.H / a.Hkv, heads = plan.groups * a.Hkv;
+
+    // the unit: sequence, key head, row group, tiles [t0, t1)
+    int b, hr;
+    uint32_t count = 1, t0 = 0, t1 = 0xffffffffu;
+    if (plan.units == 0) {
+        b = blockIdx.x / heads;
+        hr = blockIdx.x - b * heads;
+    } else {
+        const uint32_t tiles = tree_unit_tiles<WK>(a, plan, lane);
+        const uint32_t u = blockIdx.x / heads;
+        hr = blockIdx.x - u * heads;
+        uint32_t first;
+        if (!tree_find(a, u, tiles, lane, b, first, count)) return;
+        t0 = (u - first) * tiles;
+        t1 = t0 + tiles;
+    }
+    const int h = hr % a.Hkv, rg = hr / a.Hkv;
+    int ctx = __builtin_amdgcn_readfirstlane(a.ctx[b]);
+    ctx = ctx < 0 ? 0 : (ctx > a.Tmax ? a.Tmax : ctx);
+    const int end = tree_len(a, b);
+    t1 = min(t1, (uint32_t)((end + kTreeTile - 1) / kTreeTile));
+    const uint64_t live = tree_live(a, b, ctx, lane);
+    const int newrow = a.knew ? ctx + a.first : a.Tmax;   // rows from here on come from knew / vnew
+
+    // this lane's query row: node and head
+    const int rows = a.N * G;
+    const int r = (rg * WQ + wq) * kTreeTile + ln;
+    const int node = r < rows ? r / G : 0;
+    uint64_t bits = r < rows ? (uint64_t)a.tree[b * a.treeb + node * a.treen] : 0ull;
+    if (!((bits >> (a.first + node)) & 1)) bits = 0;
+    bits &= live;
+    bf16x8 qf[KS];
+    {
+        const uint16_t* qp = a.q + b * a.qb + node * a.qn + (int64_t)(h * G + (r < rows ? r - node * G : 0)) * a.qh + 8 * g;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * s));
+    }
+
+    uint16_t* vt = reinterpret_cast<uint16_t*>(lds) + w * kTreeTile * VLD;
+    const int vr = lane / LPR, vc = (lane % LPR) * 8;   // V: this lane's row of a load and its column
+    const uint16_t* kb = a.k + b * a.kb + h * a.kh + 8 * g;
+    const uint16_t* vb = a.v + b * a.vb + h * a.vh + vc;
+    const uint16_t* kn = a.knew + b * a.knb + h * a.knh + 8 * g;
+    const uint16_t* vn = a.vnew + b * a.vnb + h * a.vnh + vc;
+
+    bf16x8 kf[KS];
+    uint4 vf[NV];
+    auto load_k = [&](int j0) {
+        const int j = min(j0 + ln, end - 1);
+        const uint16_t* p = j >= newrow ? kn + (j - newrow) * a.knn : kb + (int64_t)j * a.kt;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kf[s] = __builtin_bit_cast(bf16x8, ld16(p + 16 * s));
+    };
+    auto load_v = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = j0 + i * RPI + vr;
+            // a row that is nobody's key may hold anything: zeros
+            const bool ok = j < ctx || (j < end && ((live >> (j - ctx)) & 1));
+            const uint16_t* p = j >= newrow ? vn + (j - newrow) * a.vnn : vb + (int64_t)j * a.vt;
+            vf[i] = ok ? ld16(p) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+
+    const float sc = a.scale * kLog2e;
+    float m = kTreeNegInf, l = 0.f;
+    f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+
+    uint32_t t = t0 + wk;
+    if (t < t1) {
+        load_k((int)t * kTreeTile);
+        load_v((int)t * kTreeTile);
+    }
+    for (; t < t1; t += WK) {
+        const int j0 = (int)t * kTreeTile;
+        const bool more = t + WK < t1;
+        f32x16 s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KS; ++c) s = mfma32(kf[c], qf[c], s);
+        if (more) load_k(j0 + WK * kTreeTile);
+        bool odd_v = false;
+        if (j0 + kTreeTile > ctx)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) odd_v |= any_not_finite(vf[i]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) st16(vt + (i * RPI + vr) * VLD + vc, vf[i]);
+        tree_wave_order();
+        if (more) load_v(j0 + WK * kTreeTile);
+
+        if (j0 + kTreeTile > ctx) {   // the tree's rows: one bit a key
+            const uint32_t see = j0 < ctx ? (uint32_t)(bits << (ctx - j0)) | ((1u << (ctx - j0)) - 1u)
+                                          : (j0 - ctx < 64 ? (uint32_t)(bits >> (j0 - ctx)) : 0u);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!((see >> (8 * (i >> 2) + (i & 3) + 4 * g)) & 1u)) s[i] = kTreeNegInf;
+        }
+        float mc = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mc = fmaxf(mc, s[i]);
+        mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
+        if (__ballot(mc * sc > m * sc + kTreeLazy)) {
+            const float mn = fmaxf(m, mc);
+            const float mu = mn == kTreeNegInf ? 0.f : mn;
+            const float f = exp2_fast((m - mu) * sc);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+            m = mn;
+        }
+        const float ms = m == kTreeNegInf ? 0.f : m * sc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = exp2_fast(fmaf(s[i], sc, -ms));
+            l += s[i];
+        }
+        if (__ballot(odd_v)) {
+            // An infinity or a NaN among the tree's values belongs to the queries that see its row
+            // alone, and a product with the others' zeros would give them a NaN: such values are
+            // added here, row by row, and leave the tile.
+            for (int j = 0; j < kTreeTile; ++j) {
+                float p = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (8 * (i >> 2) + (i & 3) == (j & ~4)) p = s[i];
+                p = __shfl(p, ln + 32 * ((j >> 2) & 1), 64);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const uint32_t x = vt[j * VLD + 32 * d + 8 * (e >> 2) + 4 * g + (e & 3)];
+                        if (bf16_not_finite(x) && p > 0.f) acc[d][e] += p * bf16_to_f32((uint16_t)x);
+                    }
+            }
+            tree_wave_order();
+            for (int i = 0; i < NV * 8; ++i) {
+                uint16_t* x = vt + ((i >> 3) * RPI + vr) * VLD + vc + (i & 7);
+                if (bf16_not_finite(*x)) *x = 0;
+            }
+            tree_wave_order();
+        }
+        bf16x8 pf[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const f32x8 x = c == 0 ? __builtin_shufflevector(s, s, 0, 1, 2, 3, 4, 5, 6, 7)
+                                   : __builtin_shufflevector(s, s, 8, 9, 10, 11, 12, 13, 14, 15);
+            pf[c] = __builtin_convertvector(x, bf16x8);   // p <= 2^8 in bf16, 2^-9 off at most; the sums take it unrounded
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] = mfma32(lds_op_t(vt, VLD, 16 * c, 32 * d, lane), pf[c], acc[d]);
+        tree_wave_order();   // before the next tile's values are written over this one's
+    }
+
+    // join the WK streams of a row
+    l += __shfl_xor(l, 32, 64);
+    const float ms = m * sc;   // -inf where the stream had no key
+    __syncthreads();           // V tiles are done with
+    {
+        float* op = reinterpret_cast<float*>(lds) + (w * kTreeTile + ln) * OLD;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4*>(op + 32 * d + 8 * q + 4 * g) =
+                    make_float4(acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]);
+        if (g == 0) ml[w][ln] = make_float2(ms, l);
+    }
+    __syncthreads();
+    const int64_t per = (int64_t)32 * WQ * (D + 2);   // floats of a unit's partial
+    float* part = a.work + (int64_t)blockIdx.x * per;
+    for (int i = threadIdx.x; i < 32 * WQ * LPR; i += kTreeThreads) {
+        const int rr = i / LPR, c = (i % LPR) * 8;      // row of the unit, columns c..c+7
+        const int row = rg * WQ * kTreeTile + rr;
+        if (row >= rows) continue;
+        const int wr = rr >> 5, lr = rr & 31;
+        float M = kTreeNegInf;
+#pragma unroll
+        for (int x = 0; x < WK; ++x) M = fmaxf(M, ml[x * WQ + wr][lr].x);
+        const float mu = M == kTreeNegInf ? 0.f : M;
+        float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < WK; ++x) {
+            const float2 z = ml[x * WQ + wr][lr];
+            const float f = exp2_fast(z.x - mu);
+            L += z.y * f;
+            const float* op = reinterpret_cast<const float*>(lds) + ((x * WQ + wr) * kTreeTile + lr) * OLD + c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] += op[e] * f;
+        }
+        if (count == 1) {
+            const int n = row / G;
+            const bool pad = !((a.tree[b * a.treeb + n * a.treen] >> (a.first + n)) & 1);
+            const float inv = pad || L == 0.f ? 0.f : 1.f / L;
+            const int64_t at = ((int64_t)b * a.N + n) * a.H + h * G + row - n * G;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = pad || L == 0.f ? 0.f : o[e] * inv;
+            st16(a.o + at * D + c, pack8(o));
+            if (a.lse && c == 0) a.lse[at] = pad || L == 0.f ? kTreeNegInf : (M + log2_fast(L)) * kLn2;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e += 4)
+                *reinterpret_cast<float4*>(part + rr * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            if (c == 0) *reinterpret_cast<float2*>(part + 32 * WQ * D + 2 * rr) = make_float2(M, L);
+        }
+    }
+    // the new rows into the cache, by the sequence's last unit
+    if (a.knew && rg == 0 && t1 * kTreeTile >= (uint32_t)end) {
+        for (int i = threadIdx.x; i < a.N * LPR; i += kTreeThreads) {
+            const int n = i / LPR, c = (i % LPR) * 8;
+            if (!((live >> (a.first + n)) & 1)) continue;
+            const int64_t j = newrow + n;
+            st16(const_cast<uint16_t*>(a.k) + b * a.kb + h * a.kh + j * a.kt + c, ld16(kn - 8 * g + n * a.knn + c));
+            st16(const_cast<uint16_t*>(a.v) + b * a.vb + h * a.vh + j * a.vt + c, ld16(vn - vc + n * a.vnn + c));
+        }
+    }
+}
+
+// Join the units of one query row: a workgroup a row, D / 4 lanes for a unit's row of D floats.
+template <int D>
+__global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, TreePlan plan) {
+    constexpr int LPR = D / 4, NS = 256 / LPR;   // units read side by side
+    __shared__ float sm[NS], sl[NS];
+    __shared__ __attribute__((aligned(16))) float so[NS][D];
+    const int lane = threadIdx.x & 63;
+    const int G = a.H / a.Hkv, heads = plan.groups * a.Hkv, wk = kTreeWaves / plan.wq;
+    const uint32_t tiles = wk == 8 ? tree_unit_tiles<8>(a, plan, lane)
+                     : wk == 4 ? tree_unit_tiles<4>(a, plan, lane)
+                     : wk == 2 ? tree_unit_tiles<2>(a, plan, lane) : tree_unit_tiles<1>(a, plan, lane);
+    const int hq = blockIdx.x % a.H, bn = blockIdx.x / a.H, n = bn % a.N, b = bn / a.N;
+    const uint32_t count = tree_seq_units(a, b, tiles);
+    if (count == 1) return;   // written by its unit
+    uint32_t first = 0;       // units of the sequences before b
+    for (int x = lane; x < b; x += 64) first += tree_seq_units(a, x, tiles);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) first += __shfl_xor(first, off, 64);
+    const int h = hq / G, row = n * G + hq - h * G, rg = row / (32 * plan.wq), rr = row - rg * 32 * plan.wq;
+    const int64_t per = (int64_t)32 * plan.wq * (D + 2);
+    const float* base = a.work + ((int64_t)first * heads + rg * a.Hkv + h) * per;
+    const int st = threadIdx.x / LPR, c = (threadIdx.x % LPR) * 4;
+    float M = kTreeNegInf, L = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t u = st; u < count; u += NS) {
+        const float* p = base + (int64_t)u * heads * per;
+        const float2 z = *reinterpret_cast<const float2*>(p + 32 * plan.wq * D + 2 * rr);
+        const float4 x = *reinterpret_cast<const float4*>(p + rr * D + c);
+        const float mn = fmaxf(M, z.x), mu = mn == kTreeNegInf ? 0.f : mn;
+        const float f = exp2_fast(M - mu), fx = exp2_fast(z.x - mu);
+        L = L * f + z.y * fx;
+        o.x = o.x * f + x.x * fx;
+        o.y = o.y * f + x.y * fx;
+        o.z = o.z * f + x.z * fx;
+        o.w = o.w * f + x.w * fx;
+        M = mn;
+    }
+    if (c == 0) sm[st] = M, sl[st] = L;
+    *reinterpret_cast<float4*>(&so[st][c]) = o;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    M = kTreeNegInf;
+#pragma unroll
+    for (int x = 0; x < NS; ++x) M = fmaxf(M, sm[x]);
+    const float mu = M == kTreeNegInf ? 0.f : M;
+    float O = 0.f;
+    L = 0.f;
+#pragma unroll
+    for (int x = 0; x < NS; ++x) {
+        const float f = exp2_fast(sm[x] - mu);
+        L += sl[x] * f;
+        O += so[x][d] * f;
+    }
+    const bool none = L == 0.f || !((a.tree[b * a.treeb + n * a.treen] >> (a.first + n)) & 1);
+    a.o[(int64_t)blockIdx.x * D + d] = f32_to_bf16(none ? 0.f : O / L);
+    if (a.lse && d == 0) a.lse[blockIdx.x] = none ? kTreeNegInf : (M + log2_fast(L)) * kLn2;
+}
+
+// Launch shape.  One workgroup a CU is resident (its registers), so R = CUs of them run at once.
+// Key heads (with row groups) that fill R by themselves are not split, nor are caches of a few
+// steps of a workgroup; else the units are what R leaves over, so that all of them run at once.
+static TreePlan tree_plan(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t Tmax) {
+    TreePlan p{};
+    const int rows = N * (H / Hkv);
+    p.wq = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+    p.groups = (rows + 32 * p.wq - 1) / (32 * p.wq);
+    const int64_t pairs = (int64_t)B * Hkv * p.groups, cus = device_cus();
+    const int wk = kTreeWaves / p.wq;
+    p.least = 2 * wk;
+    const int64_t tiles = (Tmax + kTreeTile - 1) / kTreeTile;
+    if (pairs >= cus / 2 || tiles <= 4 * wk) return p;
+    p.units = (int32_t)(cus - pairs);
+    return p;
+}
+
+static int64_t tree_grid(const TreePlan& p, int32_t B, int32_t Hkv) {
+    const int64_t heads = (int64_t)p.groups * Hkv;
+    // sum over sequences of ceil(tiles / unit) heads <= units + B heads, in whole multiples of heads
+    return p.units == 0 ? B * heads : (p.units + B * heads) / heads * heads;
+}
+
+int64_t tree_attention_workspace(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t Tmax, int32_t D) {
+    if (B < 1 || N < 1 || Hkv < 1 || H < Hkv || H % Hkv || Tmax < 1 || (D != 64 && D != 128)) return 0;
+    const TreePlan p = tree_plan(B, N, H, Hkv, Tmax);
+    return p.units == 0 ? 0 : tree_grid(p, B, Hkv) * 32 * p.wq * (D + 2) * (int64_t)sizeof(float);
+}
+
+template <int D>
+static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)tree_grid(p, a.B, a.Hkv)), block(kTreeThreads);
+    switch (p.wq) {
+        case 1: hipLaunchKernelGGL((tree_attn_kernel<D, 1>), grid, block, 0, st, a, p); break;
+        case 2: hipLaunchKernelGGL((tree_attn_kernel<D, 2>), grid, block, 0, st, a, p); break;
+        case 4: hipLaunchKernelGGL((tree_attn_kernel<D, 4>), grid, block, 0, st, a, p); break;
+        default: hipLaunchKernelGGL((tree_attn_kernel<D, 8>), grid, block, 0, st, a, p); break;
+    }
+    if (int e = check_launch("tree_attention")) return e;
+    if (p.units == 0) return 0;
+    hipLaunchKernelGGL((tree_join_kernel<D>), dim3((unsigned)(a.B * a.N * a.H)), dim3(256), 0, st, a, p);
+    return check_launch("tree_attention_join");
+}
+
+int tree_attention(const TreeArgs& a, void* stream) {
+    FX_REQUIRE(a.D == 64 || a.D == 128, "tree_attention: head_dim %d not supported (64 or 128)", a.D);
+    FX_REQUIRE(a.B >= 1 && a.N >= 1 && a.Tmax >= 1 && a.Hkv >= 1 && a.H >= a.Hkv && a.H % a.Hkv == 0,
+               "tree_attention: bad shape B=%d N=%d H=%d Hkv=%d Tmax=%d", a.B, a.N, a.H, a.Hkv, a.Tmax);
+    FX_REQUIRE(a.first >= 0 && a.first <= 63 && a.first + a.N <= 64, "tree_attention: %d nodes behind %d: a tree has 64 at most", a.N, a.first);
+    FX_REQUIRE(a.Tmax <= 0x7fffffff - 128, "tree_attention: Tmax=%d too large", a.Tmax);
+    FX_REQUIRE(a.q && a.k && a.v && a.ctx && a.tree && a.o, "tree_attention: null pointer");
+    FX_REQUIRE((a.knew == nullptr) == (a.vnew == nullptr), "tree_attention: knew and vnew go together");
+    FX_REQUIRE(a.scale > 0.f && a.scale < __builtin_huge_valf(), "tree_attention: scale %g must be positive and finite", (double)a.scale);
+    const int64_t s[] = {a.qb, a.qn, a.qh, a.kb, a.kt, a.kh, a.vb, a.vt, a.vh, a.knb, a.knn, a.knh, a.vnb, a.vnn, a.vnh};
+    for (int64_t x : s) FX_REQUIRE(x % 8 == 0, "tree_attention: strides must be multiples of 8 elements");
+    FX_REQUIRE((((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o | (uintptr_t)a.work | (uintptr_t)a.knew |
+                 (uintptr_t)a.vnew) & 15) == 0,
+               "tree_attention: q, k, v, o, work, knew and vnew must be 16-byte aligned");
+    const TreePlan p = tree_plan(a.B, a.N, a.H, a.Hkv, a.Tmax);
+    const int64_t tiles = (int64_t)a.B * p.groups * a.Hkv * ((a.Tmax + kTreeTile - 1) / kTreeTile);
+    FX_REQUIRE(tiles < 0x7fffffffLL && (int64_t)a.B * a.N * a.H < 0x7fffffffLL, "tree_attention: grid too large");
+    FX_REQUIRE(p.units == 0 || a.work, "tree_attention: null workspace");
+    return a.D == 64 ? tree_launch<64>(a, p, (hipStream_t)stream) : tree_launch<128>(a, p, (hipStream_t)stream);
+}
+
+}  // namespace fx

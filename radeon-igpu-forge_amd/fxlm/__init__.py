@@ -5,6 +5,8 @@ Hand-written HIP kernels behind the reference's Python surface
   - flash attention fwd/bwd (bf16 I/O, fp32 softmax, MFMA)
   - fused cross-entropy and linear cross-entropy
   - fused RMSNorm
+  - drafted decoding: tree attention over the KV cache, sampling probabilities, draft
+    verification, cache compaction
   - FlatAdamW (fp32 master + bf16 params + dynamic loss scale)
 
 Lazy exports: ``from fxlm.env import setup_lm_env`` does not import torch.
@@ -21,6 +23,10 @@ __all__ = [
     "FlatAdamW",
     "GPT",
     "GPTConfig",
+    "tree_attention",
+    "sampling_probs",
+    "verify_draft",
+    "compact_cache",
 ]
 
 
@@ -28,7 +34,7 @@ def __getattr__(name):
     if name in ("setup_lm_env", "require_gpu"):
         from . import env as _m
         return getattr(_m, name)
-    if name in ("flash_attention", "flash_attention_qkv"):
+    if name in ("flash_attention", "flash_attention_qkv", "tree_attention"):
         from . import attention as _m
         return getattr(_m, name)
     if name in ("fused_cross_entropy", "linear_cross_entropy"):
@@ -40,6 +46,9 @@ def __getattr__(name):
     if name == "FlatAdamW":
         from .optim import FlatAdamW
         return FlatAdamW
+    if name in ("sampling_probs", "verify_draft", "compact_cache"):
+        from . import speculative as _m
+        return getattr(_m, name)
     if name in ("GPT", "GPTConfig"):
         from . import model as _m
         return getattr(_m, name)

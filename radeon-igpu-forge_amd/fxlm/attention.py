@@ -195,3 +195,70 @@ def decode_attention(q, k_cache, v_cache, lens, scale=None, return_lse=False, k_
         a.vnb, a.vnh = v_new.stride(0), v_new.stride(1)
     call("fx_attn_decode", ctypes.byref(a), stream_of(q))
     return (o, lse) if return_lse else o
+
+
+def tree_attention(q, k_cache, v_cache, ctx, tree, first=0, scale=None, return_lse=False, k_new=None, v_new=None):
+    """Attention of a tree of drafted tokens over a KV cache and over each other (inference).
+
+    q (B, N, H, Dh) bf16: the tokens at nodes first .. first + N - 1 of each sequence's tree;
+    k_cache, v_cache (B, Tmax, Hkv, Dh) bf16, H a multiple of Hkv (query head h reads key head
+    h // (H // Hkv)); Dh 64 or 128, unit stride along Dh, the other strides multiples of 8.
+    ctx (B,) int32 cuda: the cached keys below the tree, whose node j has cache row ctx[b] + j.
+    tree (B, N) or (N,) int64 cuda: bit j of tree[b, i] says that query i sees node j; at most 64
+    nodes (first + N <= 64).  Query i sees every row below ctx[b] besides.  A query whose own bit
+    (first + i) is clear is padding: zeros come out, and its row is nobody's key.
+    k_new, v_new (B, N, Hkv, Dh), both or neither: the queries' own keys and values, which the
+    kernel uses and writes into the caches (padding's are not written); without them, the caches
+    hold them already.  Rows past Tmax are neither read nor written.
+    Returns o (B, N, H, Dh) bf16 and, if asked, the fp32 logsumexp (B, N, H) (-inf where a query
+    sees no key).
+    """
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if tree.dim() == 1:
+        tree = tree.expand(q.shape[0], -1)
+    if k_new is not None:
+        for nm, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+            if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                raise ValueError(f"{nm}: an expanded cache cannot take k_new and v_new")
+    r = host.tree_attention(q, k_cache, v_cache, ctx, tree, int(first), float(scale), return_lse, k_new, v_new)
+    if r is None:
+        _check_tree(q, k_cache, v_cache, ctx, tree, first, k_new, v_new)
+        r = host.tree_attention(q, k_cache, v_cache, ctx.contiguous(), tree, int(first), float(scale), return_lse, k_new, v_new)
+    return r if return_lse else r[0]
+
+
+def _check_tree(q, k_cache, v_cache, ctx, tree, first, k_new, v_new):
+    """Raise for what tree_attention does not take."""
+    if q.dim() != 4 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"q (B,N,H,Dh) and caches (B,Tmax,Hkv,Dh): {tuple(q.shape)} "
+                         f"{tuple(k_cache.shape)} {tuple(v_cache.shape)}")
+    B, N, H, Dh = q.shape
+    Tmax, Hkv = k_cache.shape[1:3]
+    if k_cache.shape[0] != B or k_cache.shape[3] != Dh or Hkv < 1 or H % Hkv or H < 1:
+        raise ValueError(f"q {tuple(q.shape)} does not match the cache {tuple(k_cache.shape)}")
+    if Dh not in (64, 128):
+        raise ValueError(f"head_dim {Dh} not supported (must be 64 or 128)")
+    if B < 1 or N < 1 or Tmax < 1 or Tmax > 2 ** 31 - 129:
+        raise ValueError(f"invalid shape: {tuple(q.shape)} over {tuple(k_cache.shape)}")
+    if first < 0 or first + N > 64:
+        raise ValueError(f"{N} nodes behind {first}: a tree has 64 nodes at most")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    for nm, t in (("k_new", k_new), ("v_new", v_new)):
+        if t is not None and tuple(t.shape) != (B, N, Hkv, Dh):
+            raise ValueError(f"{nm} {tuple(t.shape)} must be (B, N, Hkv, Dh) = {(B, N, Hkv, Dh)}")
+    for nm, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_new", k_new), ("v_new", v_new)):
+        if t is None:
+            continue
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{nm} must be bfloat16, got {t.dtype}")
+        if not t.is_cuda:
+            raise TypeError(f"{nm} must be a cuda tensor")
+        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+            raise ValueError(f"{nm}: last dim must be contiguous, other strides multiples of 8 "
+                             "elements and the base 16-byte aligned")
+    if ctx.dtype != torch.int32 or not ctx.is_cuda or ctx.shape != (B,):
+        raise TypeError(f"ctx must be an int32 cuda tensor of shape ({B},)")
+    if tree.dtype != torch.int64 or not tree.is_cuda or tree.shape != (B, N):
+        raise TypeError(f"tree must be an int64 cuda tensor of shape ({B}, {N}) or ({N},)")

@@ -1,0 +1,424 @@
+"""Drafted decoding on the GPU against the 64-bit oracle (oracle/drafting.py).
+
+Tolerances.  Tree attention: an output is rounded once (2^-8 of it, bf16's half step) and each p
+is rounded to bf16 before its product (2^-8 of the sum of p |v|); scores, exponentials and sums are
+fp32: a score's error is at most (D + 8) 2^-24 of the sum of |q k| scale, which moves every p by that
+much relatively, and 2^-18 covers the exponentials and the sums of up to 64 partial ones.
+Probabilities (fp32): a difference from the maximum is rounded once and multiplied by 1 / T, so p is
+2^-24 (l - m) / T off besides the exponential's and the sum's few steps (128 of 2^-24).
+Tokens, paths and moved rows are exact."""
+import math
+
+import pytest
+import torch
+
+from oracle import drafting as od
+
+pytestmark = pytest.mark.gpu
+
+
+def _parents(g, N, branch, count):
+    p = [-1]
+    for i in range(1, N):
+        p.append(max(0, (i - 1) // branch - int(torch.randint(0, 2, (1,), generator=g))) if i < count else -1)
+    return p
+
+
+def _tree_case(B, N, H, Hkv, D, T, ctx, first=0, branch=2, seed=0, ragged=False):
+    g = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g).bfloat16()   # noqa: E731
+    tree = torch.stack([od.ancestors(_parents(g, first + N, branch, first + N - (b % N if ragged else 0)))[first:] for b in range(B)])
+    return {"q": rn(B, N, H, D), "k": rn(B, T, Hkv, D), "v": rn(B, T, Hkv, D), "ctx": torch.tensor(ctx, dtype=torch.int32),
+            "tree": tree, "first": first, "kn": rn(B, N, Hkv, D), "vn": rn(B, N, Hkv, D)}
+
+
+def _check_tree(dev, c, new=True, o_nan_ok=False):
+    from fxlm import tree_attention
+    kn, vn = (c["kn"], c["vn"]) if new else (None, None)
+    ro, rl, size, rk, rv = od.tree_attention(c["q"], c["k"], c["v"], c["ctx"], c["tree"], c["first"], k_new=kn, v_new=vn)
+    d = {n: t.to(dev) if torch.is_tensor(t) else t for n, t in c.items()}
+    o, l = tree_attention(d["q"], d["k"], d["v"], d["ctx"], d["tree"], first=c["first"], return_lse=True,   # noqa: E741
+                          k_new=d["kn"] if new else None, v_new=d["vn"] if new else None)
+    D = c["q"].shape[-1]
+    # the largest sum of |q k| scale that any score can have
+    mag = float(c["q"].double().norm(dim=-1).max() * max(rk.double().norm(dim=-1).nan_to_num(0, 0, 0).max(), 0.0)) / math.sqrt(D)
+    score = (D + 8) * 2.0 ** -24 * mag
+    fin = torch.isfinite(ro)
+    tol = 2.0 ** -8 * (ro.abs() + size) + (2 * score + 2.0 ** -18) * size
+    oc = o.double().cpu()
+    assert torch.equal(torch.isfinite(oc), fin)
+    assert ((oc - ro).abs() <= tol)[fin].all(), float(((oc - ro).abs() - tol)[fin].max())
+    assert torch.equal(oc.isnan(), ro.isnan()) and torch.equal(oc[oc.isinf()], ro[ro.isinf()])
+    lc = l.double().cpu()
+    fl = torch.isfinite(rl)
+    assert torch.equal(lc[~fl].nan_to_num(7.0, 9.0, -9.0), rl[~fl].nan_to_num(7.0, 9.0, -9.0))
+    assert ((lc - rl).abs() <= score + 2.0 ** -18 + 2.0 ** -22 * rl.abs())[fl].all()
+    same = lambda x, y: torch.equal(x.view(torch.int16), y.view(torch.int16))   # noqa: E731
+    assert same(d["k"].cpu(), rk) and same(d["v"].cpu(), rv)
+    return d, o, l
+
+
+# rows of a key head: up to 32, 64, 128, 256 and past 256; caches that are split (long, few heads) and not;
+# contexts of nothing, of one key, ending inside a tile and at its end
+@pytest.mark.parametrize("new", [True, False])
+@pytest.mark.parametrize("B,N,H,Hkv,D,T,ctx,first", [
+    (1, 1, 1, 1, 64, 1, [0], 0),
+    (1, 1, 1, 1, 128, 70, [64], 0),
+    (2, 8, 3, 3, 64, 300, [217, 0], 0),
+    (3, 16, 4, 2, 64, 1200, [1000, 31, 32], 0),
+    (2, 16, 4, 2, 64, 2500, [2400, 1], 0),            # split
+    (1, 5, 2, 1, 128, 5000, [4900], 0),               # split, one key head
+    (3, 1, 2, 2, 64, 3000, [2990, 5, 0], 7),          # one token behind seven
+    (2, 33, 4, 4, 128, 700, [600, 64], 0),            # 33 rows
+    (2, 64, 2, 1, 64, 4200, [4100, 63], 0),           # 128 rows, split, 64 nodes
+    (1, 57, 6, 2, 128, 2300, [2200], 3),              # 171 rows, split
+    (1, 64, 5, 1, 64, 2100, [1999], 0),               # 320 rows: two groups, split
+    (2, 64, 8, 1, 128, 500, [77, 400], 0),            # 512 rows: two groups
+    (70, 2, 1, 1, 64, 1700, [(37 * i) % 1600 for i in range(70)], 0),   # more sequences than lanes
+])
+def test_tree_attention(dev, B, N, H, Hkv, D, T, ctx, first, new):
+    for branch, ragged in ((1, False), (3, first == 0)):
+        _check_tree(dev, _tree_case(B, N, H, Hkv, D, T, ctx, first, branch, seed=B * N + D, ragged=ragged), new)
+
+
+def test_tree_attention_at_the_end_of_the_cache(dev):
+    # nodes whose rows lie past the cache are nobody's key and not written; a context past it is the cache's
+    for T, ctx, first in ((70, [66, 70], 0), (70, [64, 69], 3), (70, [71, 500], 0), (70, [-3, 5], 0)):
+        for new in (True, False):
+            _check_tree(dev, _tree_case(2, 9, 2, 1, 64, T, ctx, first, 2, seed=T + ctx[0]), new)
+
+
+def test_tree_attention_strided_views(dev):
+    # q, k_new and v_new out of one projection; caches with room between heads and sequences; a shared tree
+    from fxlm import tree_attention
+    B, N, H, Hkv, D, T = 2, 12, 6, 2, 64, 1500
+    g = torch.Generator(device=dev).manual_seed(5)
+    qkv = torch.randn(B, N, H + 2 * Hkv, D, device=dev, generator=g).bfloat16()
+    both = torch.randn(T, 2, B, Hkv + 1, D + 8, device=dev, generator=g).bfloat16()
+    k, v = (both[:, i, :, :Hkv, :D].transpose(0, 1) for i in range(2))
+    kept = both.clone()
+    q, kn, vn = qkv.split([H, Hkv, Hkv], dim=2)
+    ctx = torch.tensor([1400, 333], dtype=torch.int32, device=dev)
+    tree = od.ancestors([-1] + [i // 2 for i in range(N - 1)]).to(dev)
+    o, l = tree_attention(q, k, v, ctx, tree, return_lse=True, k_new=kn, v_new=vn)   # noqa: E741
+    o2, l2 = tree_attention(q.contiguous(), k.contiguous(), v.contiguous(), ctx.repeat_interleave(2)[::2],
+                            tree.expand(B, -1).contiguous(), return_lse=True)
+    assert torch.equal(o, o2) and torch.equal(l, l2)
+    for b in range(B):
+        kept[int(ctx[b]):int(ctx[b]) + N, 0, b, :Hkv, :D] = kn[b]
+        kept[int(ctx[b]):int(ctx[b]) + N, 1, b, :Hkv, :D] = vn[b]
+    assert torch.equal(both, kept)        # the rows of the tree, and nothing between them
+
+
+@pytest.mark.parametrize("T", [300, 3000])   # one unit a sequence, and split
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_tree_attention_values_that_are_not_finite(dev, bad, T):
+    # stale rows behind the tree and padding's rows may hold anything; a node's own row reaches the queries
+    # that see it alone
+    c = _tree_case(2, 10, 2, 2, 64, T, [T - 100, 40], 0, 2, seed=9)
+    c["tree"][0, 7] = 0
+    for t in ("k", "v"):
+        c[t][0, T - 100 + 10:] = bad
+        c[t][1, 50:] = bad
+        c[t][0, T - 93] = bad       # the padding's
+    c["kn"][0, 7] = bad
+    c["vn"][0, 7] = bad
+    _check_tree(dev, c)
+    c["vn"][0, 3, :, 5] = bad       # single elements of a value; every element of another
+    c["vn"][1, 2] = bad
+    _, o, _ = _check_tree(dev, c)
+    seen = [(int(c["tree"][0, i]) >> 3) & 1 for i in range(10)]
+    assert any(seen) and not all(seen)
+    assert [bool((~torch.isfinite(o[0, i])).any()) for i in range(10)] == [bool(s) for s in seen]
+    c["kn"][1, 4, 0] = math.nan     # and of a key
+    c["k"][1, 44, 0] = math.nan
+    from fxlm import tree_attention
+    d = {n: t.to(dev) if torch.is_tensor(t) else t for n, t in c.items()}
+    o = tree_attention(d["q"], d["k"], d["v"], d["ctx"], d["tree"], k_new=d["kn"], v_new=d["vn"])
+    for i in range(10):
+        if (int(c["tree"][1, i]) >> 4) & 1:
+            assert o[1, i, 0].isnan().all()
+        elif not (int(c["tree"][1, i]) >> 2) & 1:
+            assert torch.isfinite(o[1, i]).all()
+
+
+def test_tree_attention_agrees_with_decode_attention(dev):
+    # one node, its key in place: the decode step's softmax over lens = ctx + 1 keys
+    from fxlm import tree_attention
+    from fxlm.attention import decode_attention
+    g = torch.Generator(device=dev).manual_seed(2)
+    B, H, D, T = 3, 4, 64, 2000
+    q = torch.randn(B, H, D, device=dev, generator=g).bfloat16()
+    k, v = (torch.randn(B, T, H, D, device=dev, generator=g).bfloat16() for _ in range(2))
+    ctx = torch.tensor([1999, 0, 700], dtype=torch.int32, device=dev)
+    a, la = decode_attention(q, k, v, ctx + 1, return_lse=True)
+    o, l = tree_attention(q[:, None], k, v, ctx, torch.ones(B, 1, dtype=torch.int64, device=dev), return_lse=True)   # noqa: E741
+    assert ((a.double() - o[:, 0].double()).abs() <= 2.0 ** -7 * a.double().abs() + 2.0 ** -8).all()
+    assert ((la - l[:, 0]).abs() <= 1e-4).all()
+
+
+def test_tree_attention_of_far_rows(dev):
+    # rows behind element 2^31 of a cache: 2 sequences of 1,100,000 rows of 8 heads of 128
+    from fxlm import tree_attention
+    B, T, H, D, N = 2, 1100000, 8, 128, 4
+    k = torch.zeros(B, T, H, D, device=dev, dtype=torch.bfloat16)
+    v = torch.zeros_like(k)
+    g = torch.Generator(device=dev).manual_seed(4)
+    at = T - 100
+    k[1, at:], v[1, at:] = (torch.randn(T - at, H, D, device=dev, generator=g).bfloat16() for _ in range(2))
+    k[1, :at, :, 0] = -60.0          # scores far below the tail's
+    q = torch.randn(B, N, H, D, device=dev, generator=g).bfloat16()
+    q[..., 0] = 40.0
+    kn, vn = (torch.randn(B, N, H, D, device=dev, generator=g).bfloat16() for _ in range(2))
+    tree = od.ancestors([-1, 0, 0, 2]).expand(B, -1)
+    ctx = torch.tensor([3, T - 9], dtype=torch.int32, device=dev)
+    o = tree_attention(q, k, v, ctx, tree.to(dev), k_new=kn, v_new=vn)
+    assert torch.equal(k[1, T - 9:T - 5], kn[1]) and torch.equal(v[1, T - 9:T - 5], vn[1])
+    ro, _, size, _, _ = od.tree_attention(q[1:].cpu(), k[1:, at:].cpu(), v[1:, at:].cpu(), [T - 9 - at], tree[1:], k_new=kn[1:].cpu(), v_new=vn[1:].cpu())
+    assert ((o[1:].double().cpu() - ro).abs() <= 2.0 ** -8 * (ro.abs() + size) + 1e-3 * size).all()
+
+
+# ---- probabilities ---------------------------------------------------------------------------
+
+
+def _check_probs(dev, x, T, k):
+    from fxlm import sampling_probs
+    p = sampling_probs(x.to(dev), T, k)
+    ref = od.sampling_probs(x, T, k)
+    assert p.dtype == torch.float32 and p.shape == x.shape
+    pc = p.double().cpu()
+    m = x.double().amax(-1, keepdim=True)
+    far = ((m - x.double()) / T).nan_to_num(0, 0, 0).clamp_max(200)
+    assert torch.equal(pc > 0, ref > 1.2e-38) or ((pc > 0) != (ref > 1.2e-38)).logical_and(ref > 3e-38).sum() == 0
+    err = (pc - ref).abs() - (2.0 ** -24 * (128 + 2 * far) * ref + 1.2e-38)
+    assert (err <= 0).all(), float(err.max())
+    return p
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,k", [((1,), 0), ((3, 1), 5), ((2, 7), 3), ((5, 255), 0), ((2, 3, 1000), 50), ((4, 4097), 4096), ((3, 50304), 50),
+                                     ((2, 50304), 1), ((2, 50303), 0), ((3, 131071), 200), ((2, 131071), 20000), ((1, 300001), 50)])
+def test_sampling_probs(dev, shape, k, dtype):
+    g = torch.Generator().manual_seed(len(shape) + k)
+    x = (torch.randn(*shape, generator=g) * 3).to(dtype)
+    for T in (0.7, 1.0):
+        _check_probs(dev, x, T, k)
+
+
+def test_sampling_probs_orders_and_ties(dev):
+    V = 9000
+    up = torch.arange(V).float() / 500
+    x = torch.stack([up, up.flip(0), torch.zeros(V), torch.cat([torch.full((V - 70,), -1.0), torch.full((70,), 2.0)]),
+                     torch.where(torch.arange(V) % 2 == 0, 0.0, -0.0), up.roll(V // 2)])
+    for k in (1, 49, 50, 64, 70, 71, 1024, 1025, 8999):
+        p = _check_probs(dev, x, 0.9, k)
+        assert (p[2] > 0).all() and (p[4] > 0).all()                     # equals of the last kept stay: both zeros alike
+        assert int((p[3] > 0).sum()) == (70 if k <= 70 else V)
+        assert int((p[0] > 0).sum()) == k
+    # a row that one thread's stride holds the largest of
+    y = torch.randn(V, generator=torch.Generator().manual_seed(1))
+    y[::1024] += 30
+    y[4::4096] += 30
+    _check_probs(dev, y[None], 1.0, 50)
+
+
+def test_sampling_probs_masked_and_not_finite(dev):
+    from fxlm import sampling_probs
+    x = torch.randn(6, 5001, generator=torch.Generator().manual_seed(7))
+    x[0, 100:] = -math.inf
+    x[1, :] = -math.inf
+    x[2, 77] = math.nan
+    x[3, 5000] = math.inf
+    x[4, 1:] = torch.finfo(torch.float32).min     # masks of the type's lowest value
+    x[5, :] = torch.finfo(torch.float32).min
+    for k in (0, 50, 200):
+        p = sampling_probs(x.to(dev), 0.5, k).cpu()
+        assert torch.equal(p[0] > 0, od.sampling_probs(x[:1], 0.5, k)[0] > 0) and abs(float(p[0].sum()) - 1) < 1e-5
+        assert not p[1].any() and p[2].isnan().all() and p[3].isnan().all()
+        assert float(p[4, 0]) == 1.0 and not p[4, 1:].any()
+        assert ((p[5] - 1 / 5001).abs() <= 2.0 ** -20 / 5001).all()
+    # a slice of positions, rows at an odd address
+    y = torch.randn(3, 5, 1003, generator=torch.Generator().manual_seed(8)).to(dev)
+    assert torch.equal(sampling_probs(y[:, -1], 0.8, 20), sampling_probs(y[:, -1].clone(), 0.8, 20))
+    flat = y.flatten()[1:1 + 4 * 1001].view(4, 1001)
+    assert torch.equal(sampling_probs(flat, 0.8, 20), sampling_probs(flat.clone(), 0.8, 20))
+    assert sampling_probs(y[:0]).shape == (0, 5, 1003)
+
+
+# ---- verification ----------------------------------------------------------------------------
+
+
+def _draft_case(B, N, V, branch, seed, ragged, drafted, k=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, N, V, generator=g) * 2
+    p = od.sampling_probs(x, 0.8, k).float()
+    q = od.sampling_probs(x * 0.9 + 0.7 * torch.randn(B, N, V, generator=g), 0.8, k).float()
+    par = torch.tensor([_parents(g, N, branch, N - (b % N if ragged else 0)) for b in range(B)], dtype=torch.int32)
+    tok = torch.zeros(B, N, dtype=torch.int64)
+    for b in range(B):
+        for i in range(N):
+            tok[b, i] = torch.multinomial(q[b, max(int(par[b, i]), 0)], 1, generator=g)
+    return p, tok, par, torch.rand(B, N, generator=g), q if drafted else None
+
+
+def _check_verify(dev, p, tok, par, u, q):
+    from fxlm import verify_draft
+    got = verify_draft(*(t.to(dev) for t in (p, tok, par, u)), draft_probs=None if q is None else q.to(dev))
+    ref = od.verify_draft(p, tok, par, u, q)
+    for a, r, name in zip(got, ref, ("tokens", "path", "counts")):
+        assert torch.equal(a.cpu(), r), name
+    return got
+
+
+@pytest.mark.parametrize("drafted", [True, False])
+@pytest.mark.parametrize("B,N,V,branch,k", [(1, 1, 1, 1, 0), (3, 2, 2, 1, 0), (5, 6, 257, 1, 0), (40, 8, 100, 2, 0), (30, 16, 1000, 3, 20),
+                                            (9, 64, 513, 4, 0), (12, 7, 50304, 6, 0), (3, 5, 131071, 4, 50), (200, 4, 33, 3, 0)])
+def test_verify_draft(dev, B, N, V, branch, k, drafted):
+    for seed in range(3):
+        _check_verify(dev, *_draft_case(B, N, V, branch, 100 * seed + N, seed == 1, drafted, k))
+
+
+def test_verify_draft_edges(dev):
+    # ids outside the vocabulary, parents that are none, numbers at the ends, rows without mass, duplicates
+    p, tok, par, u, q = _draft_case(16, 12, 300, 3, 5, False, True)
+    tok[0, 1:4], tok[1, 1], par[2, 3], par[3, 5], par[4, 1] = 300, -7, 3, 9, -5
+    u[5], u[6], u[7, 0] = 0.0, 1.0 - 2.0 ** -24, 1.0 - 2.0 ** -24
+    p[8], p[9, 0, 5:] = 0.0, 0.0
+    tok[10, 1:] = tok[10, 1]
+    q[11] = p[11]                    # the draft is the target: every first child is accepted
+    q[12], p[13, :, ::2] = 0.0, 0.0
+    for d in (q, None):
+        out, path, n = _check_verify(dev, p, tok, par, u, d)
+        assert int(out[8, 0]) == -1 and int(n[8]) == 1
+        assert int((out[9, 0] < 5)) or int(n[9]) > 1
+    # NaN is no mass: refused, and a row of it gives -1
+    p[:], u[:] = math.nan, 0.5
+    from fxlm import verify_draft
+    out, path, n = verify_draft(*(t.to(dev) for t in (p, tok, par, u)), draft_probs=q.to(dev))
+    assert (n == 1).all() and (out == -1).all() and (path[:, 0] == 0).all() and (path[:, 1:] == -1).all()
+
+
+def test_verified_tokens_are_distributed_as_the_target(dev):
+    # 200,000 sequences, 5 standard deviations: the first token, and the second after each first
+    from fxlm import verify_draft
+    g = torch.Generator(device=dev).manual_seed(11)
+    B, N, V = 200000, 6, 6
+    p = torch.softmax(torch.randn(N, V, device=dev, generator=g), -1)
+    q = torch.softmax(torch.randn(N, V, device=dev, generator=g), -1)
+    # children of the root 1 and 2, of 1: 3 and 4, of 2: 5; a node's distribution hangs on its token: here each has its own
+    par = torch.tensor([-1, 0, 0, 1, 1, 2], dtype=torch.int32, device=dev).expand(B, N).contiguous()
+    tok = torch.stack([torch.multinomial(q[max(i, 0)], B, replacement=True, generator=g) for i in (-1, 0, 0, 1, 1, 2)], 1)
+    # a distribution by token, so that the law of (first, second) is a product: rows of p and q by the parent's token
+    P = torch.softmax(torch.randn(V, V, device=dev, generator=g), -1)
+    pr = p[None].expand(B, N, V).clone()
+    pr[:, 1:] = P[tok[:, 1:]]
+    qr = q[None].expand(B, N, V).contiguous()
+    out, path, n = verify_draft(pr, tok, par, torch.rand(B, N, device=dev, generator=g), draft_probs=qr)
+    f = torch.bincount(out[:, 0], minlength=V).double() / B
+    p0 = p[0].double()
+    assert ((f - p0).abs() <= 5 * (p0 * (1 - p0) / B).sqrt()).all()
+    two = n >= 2
+    for x in range(V):
+        s = out[two & (out[:, 0] == x), 1]
+        if len(s) > 1000:
+            f, px = torch.bincount(s, minlength=V).double() / len(s), P[x].double()
+            assert ((f - px).abs() <= 5 * (px * (1 - px) / len(s)).sqrt()).all()
+
+
+# ---- compaction ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("L,B,N,H,D,T", [(1, 1, 1, 1, 64, 2), (3, 4, 9, 2, 64, 50), (2, 3, 64, 12, 64, 200), (40, 2, 5, 1, 128, 20), (33, 1100, 3, 1, 8, 6)])
+def test_compact_cache(dev, L, B, N, H, D, T):
+    from fxlm import compact_cache
+    g = torch.Generator().manual_seed(L + N)
+    cache = [tuple(torch.randint(-30000, 30000, (B, T, H, D), generator=g, dtype=torch.int16).view(torch.bfloat16) for _ in range(2)) for _ in range(L)]
+    counts = torch.tensor([1 + (5 * b) % N for b in range(B)], dtype=torch.int32)
+    ctx = torch.tensor([(7 * b) % (T - N + 1) for b in range(B)], dtype=torch.int32)
+    path = torch.full((B, N), -1, dtype=torch.int32)
+    for b in range(B):
+        path[b, :counts[b]] = torch.cat([torch.zeros(1), 1 + torch.randperm(N - 1, generator=g)[:counts[b] - 1].sort().values]).int()
+    ref, rctx = od.compact_cache(cache, ctx, path, counts)
+    mine = [(k.to(dev), v.transpose(1, 2).contiguous().to(dev).transpose(1, 2)) for k, v in cache]     # two layouts
+    got = compact_cache(mine, ctx.to(dev), path.to(dev), counts.to(dev))
+    assert torch.equal(got.cpu(), rctx)
+    for t, r in zip((t for kv in mine for t in kv), ref):
+        assert torch.equal(t.cpu().view(torch.int16), r.contiguous().view(torch.int16))
+
+
+def test_compact_cache_passes_over_what_is_outside(dev):
+    from fxlm import compact_cache
+    k = torch.arange(2 * 12 * 8).view(2, 12, 1, 8).bfloat16().to(dev)
+    v = k + 1
+    k0 = k.clone()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+    got = compact_cache([(k, v)], i32(10, -4), i32([0, 5, 900], [0, 2, 3]), i32(3, 3))      # past the cache; a negative context
+    assert torch.equal(k, k0) and got.tolist() == [13, -1]
+    got = compact_cache([(k, v)], i32(2, 2), i32([-1, -1, -1], [0, 3, 3]), i32(-5, 9))      # counts outside: none, all
+    k0[1, 3], k0[1, 4] = k0[1, 5].clone(), k0[1, 5].clone()
+    assert torch.equal(k, k0) and torch.equal(v, k0 + 1) and got.tolist() == [2, 5]
+
+
+# ---- together --------------------------------------------------------------------------------
+
+
+def test_operators_in_a_row_on_another_stream_and_in_a_graph(dev):
+    # attention over the drafted tree, probabilities, verification, compaction: eager on the current stream,
+    # on another one, and captured twice and replayed with new inputs
+    from fxlm import compact_cache, sampling_probs, tree_attention, verify_draft
+    B, N, H, D, T, V = 3, 9, 4, 64, 4000, 700
+    g = torch.Generator().manual_seed(21)
+    head = (torch.randn(V, H * D, generator=g) * 0.3).to(dev)
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        rn = lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev)   # noqa: E731
+        par = [_parents(g, N, 2, N) for _ in range(B)]
+        return {"q": rn(B, N, H, D), "kn": rn(B, N, H, D), "vn": rn(B, N, H, D), "k": rn(B, T, H, D), "v": rn(B, T, H, D),
+                "ctx": torch.tensor([3000, 40 + seed, 1111], dtype=torch.int32, device=dev), "tree": torch.stack([od.ancestors(p) for p in par]).to(dev),
+                "par": torch.tensor(par, dtype=torch.int32, device=dev), "tok": torch.randint(0, V, (B, N), generator=g).to(dev),
+                "u": torch.rand(B, N, generator=g).to(dev) * 0.02}
+
+    def step(s):
+        o = tree_attention(s["q"], s["k"], s["v"], s["ctx"], s["tree"], k_new=s["kn"], v_new=s["vn"])
+        p = sampling_probs(torch.mm(o.view(B * N, -1).float(), head.t()).view(B, N, V), 0.9, 40)
+        out, path, n = verify_draft(p, s["tok"], s["par"], s["u"])
+        ctx = compact_cache([(s["k"], s["v"])], s["ctx"], path, n)
+        return o, p, out, path, n, ctx
+
+    want = {}
+    for seed in (1, 2, 3):
+        s = inputs(seed)
+        want[seed] = [t.clone() for t in step(s)] + [s["k"].clone(), s["v"].clone()]
+        for b in range(B):   # what verification saw, by the oracle
+            r = od.verify_draft(want[seed][1].cpu(), s["tok"].cpu(), s["par"].cpu(), s["u"].cpu())
+            assert all(torch.equal(a.cpu(), x) for a, x in zip(want[seed][2:5], r))
+    side = torch.cuda.Stream()
+    s = inputs(1)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = list(step(s))
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got + [s["k"], s["v"]], want[1]))
+    graphs = []
+    for _ in range(2):
+        s = inputs(1)
+        with torch.cuda.stream(side):
+            step(s)
+        torch.cuda.current_stream().wait_stream(side)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = step(s)
+        graphs.append((gr, s, got))
+    for seed in (2, 1, 3, 3):
+        for gr, s, got in graphs:
+            for n, t in inputs(seed).items():
+                s[n].copy_(t)
+        for gr, s, got in graphs:       # two graphs, one behind the other
+            gr.replay()
+        torch.cuda.synchronize()
+        for gr, s, got in graphs:
+            for a, b in zip(list(got) + [s["k"], s["v"]], want[seed]):
+                assert torch.equal(a, b), seed
+        x = inputs(seed)                # eager work between the replays
+        assert all(torch.equal(a, b) for a, b in zip(step(x), want[seed]))
