@@ -97,13 +97,6 @@ __device__ __forceinline__ uint64_t tree_live(const TreeArgs& a, int b, int ctx,
 }
 
 __device__ __forceinline__ bool bf16_not_finite(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
-__device__ __forceinline__ bool any_not_finite(const uint4& v) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= bf16_not_finite(w[i]) || bf16_not_finite(w[i] >> 16);
-    return bad;
-}
 
 // A wave's LDS operations are done in the order of its instructions; this keeps the compiler from moving
 // them past each other where lanes read what other lanes wrote.
@@ -112,25 +105,53 @@ __device__ __forceinline__ void tree_wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// A kernel argument's value in registers: a select between two arguments is otherwise one between their
+// addresses, with a load behind it in the loop
+__device__ __forceinline__ int64_t pinned(int64_t x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
+// Rows of one kind (keys or values) of a key head, as this lane loads them: cached ones, and the queries' own
+struct TreeRows {
+    const uint16_t *cached, *fresh;
+    int64_t st, stn;
+    // row j, clamped to the sequence's last
+    __device__ __forceinline__ const uint16_t* at(int j, int end, int newrow) const {
+        j = min(j, end - 1);
+        const bool nw = j >= newrow;
+        return (nw ? fresh : cached) + (j - (nw ? newrow : 0)) * (nw ? stn : st);
+    }
+};
+
 // Workgroup: WQ groups of 32 query rows x WK = 8 / WQ streams of keys; wave (wq, wk) takes the unit's
-// tiles wk, wk + WK, ...  Per tile S^T = K Q^T (a lane holds 16 of the 32 keys of one query), the
-// softmax, and O^T += V^T P^T with V read transposed from the wave's own LDS (fx_mfma.h has the
-// layouts); the next tile's keys and values are in flight in registers meanwhile, no barrier in the
-// loop.  The WK streams of a row join through LDS.
+// tiles wk, wk + WK, ... of 32 keys.  Per tile S^T = K Q^T (a lane holds 16 of the 32 keys of one
+// query), the softmax, and O^T += V^T P^T with V read transposed (fx_mfma.h has the layouts).  Keys and
+// values go through LDS in whole rows (16 lanes a 256-byte row: an operand's own pattern, 32 bytes of
+// 32 rows, took the address unit 4 times as long and bound the kernel); the next tile is in flight
+// in registers meanwhile.  One row group: each wave has a tile of its own and no barrier.  More: the WQ waves
+// of a stream load a tile together (each loading it for itself kept the address unit 90% busy),
+// into one of two buffers, with a barrier a tile.  The WK streams of a row join through LDS.
 template <int D, int WQ>
 __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, TreePlan plan) {
     constexpr int WK = kTreeWaves / WQ;
     constexpr int LPR = D / 8;        // lanes of a row in 16-byte loads
     constexpr int RPI = 64 / LPR;     // rows of a wave-wide load
     constexpr int NV = kTreeTile / RPI;
+    constexpr int PW = 2 * NV / WQ;   // loads of a wave: of one row group keys, then values; else of one kind
     constexpr int KS = D / 16;        // steps of the score product
     constexpr int DT = D / 32;
-    constexpr int VLD = D + 32;       // LDS row of V: 4 rows of a transposed read fall in distinct banks
+    constexpr int KLD = D + 8;        // LDS row of K: 16 rows of an operand read cover all banks
+    constexpr int VLD = D + 32;       // and of V: 4 rows of a transposed read fall in distinct banks
     constexpr int OLD = D + 4;        // LDS row of a wave's fp32 output
-    constexpr int kVBytes = kTreeWaves * kTreeTile * VLD * 2;
+    constexpr int kTile = kTreeTile * (KLD + VLD);   // elements
+    constexpr int kBufs = WQ == 1 ? 1 : 2;
+    constexpr int kTBytes = kBufs * WK * kTile * 2;
     constexpr int kOBytes = kTreeWaves * kTreeTile * OLD * 4;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kVBytes > kOBytes ? kVBytes : kOBytes];
+    static_assert(PW >= 1 && (WQ == 1 || PW * (WQ / 2) == NV), "a tile's loads over its waves");
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kTBytes > kOBytes ? kTBytes : kOBytes];
     __shared__ float2 ml[kTreeWaves][kTreeTile];
+    __shared__ int odd[kBufs][kTreeWaves];   // the wave loaded an infinity or a NaN
 
     const int lane = threadIdx.x & 63, ln = lane & 31, g = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -149,13 +170,13 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
         hr = blockIdx.x - u * heads;
         uint32_t first;
         if (!tree_find(a, u, tiles, lane, b, first, count)) return;
-        t0 = (u - first) * tiles;
-        t1 = t0 + tiles;
+        t0 = __builtin_amdgcn_readfirstlane((u - first) * tiles);
+        t1 = __builtin_amdgcn_readfirstlane(t0 + tiles);
     }
     const int h = hr % a.Hkv, rg = hr / a.Hkv;
     int ctx = __builtin_amdgcn_readfirstlane(a.ctx[b]);
     ctx = ctx < 0 ? 0 : (ctx > a.Tmax ? a.Tmax : ctx);
-    const int end = tree_len(a, b);
+    const int end = __builtin_amdgcn_readfirstlane(tree_len(a, b));
     t1 = min(t1, (uint32_t)((end + kTreeTile - 1) / kTreeTile));
     const uint64_t live = tree_live(a, b, ctx, lane);
     const int newrow = a.knew ? ctx + a.first : a.Tmax;   // rows from here on come from knew / vnew
@@ -174,30 +195,69 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
         for (int s = 0; s < KS; ++s) qf[s] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * s));
     }
 
-    uint16_t* vt = reinterpret_cast<uint16_t*>(lds) + w * kTreeTile * VLD;
-    const int vr = lane / LPR, vc = (lane % LPR) * 8;   // V: this lane's row of a load and its column
-    const uint16_t* kb = a.k + b * a.kb + h * a.kh + 8 * g;
-    const uint16_t* vb = a.v + b * a.vb + h * a.vh + vc;
-    const uint16_t* kn = a.knew + b * a.knb + h * a.knh + 8 * g;
-    const uint16_t* vn = a.vnew + b * a.vnb + h * a.vnh + vc;
+    uint16_t* const tile0 = reinterpret_cast<uint16_t*>(lds) + wk * kTile;   // of buffer 0
+    const int lr = lane / LPR, lc = (lane % LPR) * 8;   // this lane's row of a load and its column
+    const TreeRows ck = {a.k + b * a.kb + h * a.kh + lc, a.knew + b * a.knb + h * a.knh + lc, pinned(a.kt), pinned(a.knn)};
+    const TreeRows cv = {a.v + b * a.vb + h * a.vh + lc, a.vnew + b * a.vnb + h * a.vnh + lc, pinned(a.vt), pinned(a.vnn)};
+    const bool values = WQ > 1 && wq >= WQ / 2;         // this wave loads values, of a stream's several
+    const TreeRows mine = values ? cv : ck;
+    const int part = WQ > 1 ? (wq % (WQ > 1 ? WQ / 2 : 1)) * PW : 0;   // its first load of the tile's NV of that kind
 
-    bf16x8 kf[KS];
-    uint4 vf[NV];
-    auto load_k = [&](int j0) {
-        const int j = min(j0 + ln, end - 1);
-        const uint16_t* p = j >= newrow ? kn + (j - newrow) * a.knn : kb + (int64_t)j * a.kt;
+    uint4 st[PW];
+    // Tiles of the context alone take their rows as they lie; the tree's (at most three a sequence) clamp
+    // the row to the last one.
+    auto load_rows = [&](const TreeRows& c, int j0, int first, int n, uint4* to) {
+        if (j0 + kTreeTile <= ctx) {
+            const uint16_t* p = c.cached + (j0 + first * RPI + lr) * c.st;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) kf[s] = __builtin_bit_cast(bf16x8, ld16(p + 16 * s));
-    };
-    auto load_v = [&](int j0) {
+            for (int i = 0; i < n; ++i) to[i] = ld16(p + i * RPI * c.st);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = j0 + i * RPI + vr;
-            // a row that is nobody's key may hold anything: zeros
-            const bool ok = j < ctx || (j < end && ((live >> (j - ctx)) & 1));
-            const uint16_t* p = j >= newrow ? vn + (j - newrow) * a.vnn : vb + (int64_t)j * a.vt;
-            vf[i] = ok ? ld16(p) : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < n; ++i) to[i] = ld16(c.at(j0 + (first + i) * RPI + lr, end, newrow));
         }
+    };
+    auto load = [&](int j0) {
+        if constexpr (WQ == 1) {
+            load_rows(ck, j0, 0, NV, st);
+            load_rows(cv, j0, 0, NV, st + NV);
+        } else {
+            load_rows(mine, j0, part, PW, st);
+        }
+    };
+    // Loaded values into LDS.  In the tree's tiles, values of rows that are nobody's key are zeros, whatever
+    // they hold, and so are infinities and NaN: the queries that see them add them by themselves.
+    auto put_values = [&](uint16_t* vt, int j0, int first, int n, uint4* from, int* flag) {
+        if (j0 + kTreeTile > ctx) {
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const int j = j0 + (first + i) * RPI + lr;
+                const bool key = j < ctx || (j < end && ((live >> (j - ctx)) & 1));
+                const uint32_t keep = key ? 0xffffffffu : 0u;
+                uint32_t x[4] = {from[i].x & keep, from[i].y & keep, from[i].z & keep, from[i].w & keep};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool lo = bf16_not_finite(x[e]), hi = bf16_not_finite(x[e] >> 16);
+                    bad |= lo || hi;
+                    x[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                }
+                from[i] = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+            const uint64_t any = __ballot(bad);
+            if (lane == 0) *flag = any != 0;
+        }
+#pragma unroll
+        for (int i = 0; i < n; ++i) st16(vt + ((first + i) * RPI + lr) * VLD + lc, from[i]);
+    };
+    auto put = [&](int j0, int buf) {
+        uint16_t* ks = tile0 + buf * WK * kTile;
+        uint16_t* vt = ks + kTreeTile * KLD;
+        if (WQ == 1 || !values) {
+#pragma unroll
+            for (int i = 0; i < (WQ == 1 ? NV : PW); ++i) st16(ks + ((part + i) * RPI + lr) * KLD + lc, st[i]);
+        }
+        if (WQ == 1) put_values(vt, j0, 0, NV, st + (WQ == 1 ? NV : 0), &odd[0][w]);
+        else if (values) put_values(vt, j0, part, PW, st, &odd[buf][w]);
     };
 
     const float sc = a.scale * kLog2e;
@@ -208,30 +268,16 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
-    uint32_t t = t0 + wk;
-    if (t < t1) {
-        load_k((int)t * kTreeTile);
-        load_v((int)t * kTreeTile);
-    }
-    for (; t < t1; t += WK) {
-        const int j0 = (int)t * kTreeTile;
-        const bool more = t + WK < t1;
+    auto compute = [&](int j0, int buf) {
+        const uint16_t* ks = tile0 + buf * WK * kTile;
+        const uint16_t* vt = ks + kTreeTile * KLD;
+        const bool tail = j0 + kTreeTile > ctx;
         f32x16 s;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < KS; ++c) s = mfma32(kf[c], qf[c], s);
-        if (more) load_k(j0 + WK * kTreeTile);
-        bool odd_v = false;
-        if (j0 + kTreeTile > ctx)
-#pragma unroll
-            for (int i = 0; i < NV; ++i) odd_v |= any_not_finite(vf[i]);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) st16(vt + (i * RPI + vr) * VLD + vc, vf[i]);
-        tree_wave_order();
-        if (more) load_v(j0 + WK * kTreeTile);
-
-        if (j0 + kTreeTile > ctx) {   // the tree's rows: one bit a key
+        for (int c = 0; c < KS; ++c) s = mfma32(lds_op_row(ks, KLD, 0, 16 * c, lane), qf[c], s);
+        if (tail) {   // the tree's rows: one bit a key
             const uint32_t see = j0 < ctx ? (uint32_t)(bits << (ctx - j0)) | ((1u << (ctx - j0)) - 1u)
                                           : (j0 - ctx < 64 ? (uint32_t)(bits >> (j0 - ctx)) : 0u);
 #pragma unroll
@@ -259,43 +305,96 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
             s[i] = exp2_fast(fmaf(s[i], sc, -ms));
             l += s[i];
         }
-        if (__ballot(odd_v)) {
-            // An infinity or a NaN among the tree's values belongs to the queries that see its row
-            // alone, and a product with the others' zeros would give them a NaN: such values are
-            // added here, row by row, and leave the tile.
-            for (int j = 0; j < kTreeTile; ++j) {
-                float p = 0.f;
+        if (tail) {
+            int any = 0;
+            if (WQ == 1) any = odd[0][w];
+            else
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (8 * (i >> 2) + (i & 3) == (j & ~4)) p = s[i];
-                p = __shfl(p, ln + 32 * ((j >> 2) & 1), 64);
+                for (int x = WQ / 2; x < WQ; ++x) any |= odd[buf][wk * WQ + x];
+            if (__ballot(any)) {
+                // An infinity or a NaN among the tree's values belongs to the queries that see its row alone (a
+                // product with the others' zeros would give them a NaN): added here, row by row.
+                for (int j = 0; j < kTreeTile && j0 + j < end; ++j) {
+                    if (j0 + j >= ctx && !((live >> (j0 + j - ctx)) & 1)) continue;
+                    float p = 0.f;
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
+                    for (int i = 0; i < 16; ++i)
+                        if (8 * (i >> 2) + (i & 3) == (j & ~4)) p = s[i];
+                    p = __shfl(p, ln + 32 * ((j >> 2) & 1), 64);
+                    const uint16_t* row = cv.at(j0 + j, end, newrow) - lc + 4 * g;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const uint32_t x = vt[j * VLD + 32 * d + 8 * (e >> 2) + 4 * g + (e & 3)];
-                        if (bf16_not_finite(x) && p > 0.f) acc[d][e] += p * bf16_to_f32((uint16_t)x);
+                    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint32_t x = row[32 * d + 8 * (e >> 2) + (e & 3)];
+                            if (bf16_not_finite(x) && p > 0.f) acc[d][e] += p * bf16_to_f32((uint16_t)x);
+                        }
+                        asm volatile("" ::: "memory");   // 32 columns' loads at a time: registers
                     }
+                }
             }
-            tree_wave_order();
-            for (int i = 0; i < NV * 8; ++i) {
-                uint16_t* x = vt + ((i >> 3) * RPI + vr) * VLD + vc + (i & 7);
-                if (bf16_not_finite(*x)) *x = 0;
-            }
-            tree_wave_order();
         }
+        bf16x8 vo[DT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vo[d] = lds_op_t(vt, VLD, 0, 32 * d, lane);
         bf16x8 pf[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const f32x8 x = c == 0 ? __builtin_shufflevector(s, s, 0, 1, 2, 3, 4, 5, 6, 7)
                                    : __builtin_shufflevector(s, s, 8, 9, 10, 11, 12, 13, 14, 15);
-            pf[c] = __builtin_convertvector(x, bf16x8);   // p <= 2^8 in bf16, 2^-9 off at most; the sums take it unrounded
+            pf[c] = __builtin_convertvector(x, bf16x8);   // p <= 2^8 in bf16, 2^-8 off at most; the sums take it unrounded
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int d = 0; d < DT; ++d) {
+            acc[d] = mfma32(vo[d], pf[0], acc[d]);
+            vo[d] = lds_op_t(vt, VLD, 16, 32 * d, lane);
+        }
 #pragma unroll
-            for (int d = 0; d < DT; ++d) acc[d] = mfma32(lds_op_t(vt, VLD, 16 * c, 32 * d, lane), pf[c], acc[d]);
-        tree_wave_order();   // before the next tile's values are written over this one's
+        for (int d = 0; d < DT; ++d) acc[d] = mfma32(vo[d], pf[1], acc[d]);
+    };
+
+    // The loop has all of a step's loads in every turn (the last step is its own): the waits for older loads
+    // count the younger.  The queries have to be here before it: a wait for them inside would be
+    // one for the tile's loads behind them, every time.
+    uint32_t t = t0 + wk;
+    auto queries_here = [&] {
+#pragma unroll
+        for (int c = 0; c < KS; ++c) asm volatile("" : "+v"(qf[c]));
+    };
+    if constexpr (WQ == 1) {
+        if (t < t1) {
+            load((int)t * kTreeTile);
+            queries_here();
+            for (;; t += WK) {
+                const int j0 = (int)t * kTreeTile;
+                put(j0, 0);
+                tree_wave_order();
+                if (t + WK >= t1) break;
+                load(j0 + WK * kTreeTile);
+                compute(j0, 0);
+                tree_wave_order();   // before the next tile is written over this one
+            }
+            compute((int)t * kTreeTile, 0);
+        }
+    } else {
+        // every stream takes the steps of the first, for the barriers; a tile past the last one is the last
+        // one's rows again, not counted
+        const int steps = (int)((t1 - t0 + WK - 1) / WK);
+        if (steps > 0) {
+            load((int)t * kTreeTile);
+            queries_here();
+            int s = 0;
+            for (; s < steps - 1; ++s, t += WK) {
+                const int j0 = (int)t * kTreeTile;
+                put(j0, s & 1);
+                load(j0 + WK * kTreeTile);
+                __syncthreads();
+                compute(j0, s & 1);
+            }
+            put((int)t * kTreeTile, s & 1);
+            __syncthreads();
+            if (t < t1) compute((int)t * kTreeTile, s & 1);
+        }
     }
 
     // join the WK streams of a row
@@ -314,23 +413,23 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
     }
     __syncthreads();
     const int64_t per = (int64_t)32 * WQ * (D + 2);   // floats of a unit's partial
-    float* part = a.work + (int64_t)blockIdx.x * per;
+    float* unit = a.work + (int64_t)blockIdx.x * per;
     for (int i = threadIdx.x; i < 32 * WQ * LPR; i += kTreeThreads) {
         const int rr = i / LPR, c = (i % LPR) * 8;      // row of the unit, columns c..c+7
         const int row = rg * WQ * kTreeTile + rr;
         if (row >= rows) continue;
-        const int wr = rr >> 5, lr = rr & 31;
+        const int wr = rr >> 5, rl = rr & 31;
         float M = kTreeNegInf;
 #pragma unroll
-        for (int x = 0; x < WK; ++x) M = fmaxf(M, ml[x * WQ + wr][lr].x);
+        for (int x = 0; x < WK; ++x) M = fmaxf(M, ml[x * WQ + wr][rl].x);
         const float mu = M == kTreeNegInf ? 0.f : M;
         float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < WK; ++x) {
-            const float2 z = ml[x * WQ + wr][lr];
+            const float2 z = ml[x * WQ + wr][rl];
             const float f = exp2_fast(z.x - mu);
             L += z.y * f;
-            const float* op = reinterpret_cast<const float*>(lds) + ((x * WQ + wr) * kTreeTile + lr) * OLD + c;
+            const float* op = reinterpret_cast<const float*>(lds) + ((x * WQ + wr) * kTreeTile + rl) * OLD + c;
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] += op[e] * f;
         }
@@ -346,8 +445,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e += 4)
-                *reinterpret_cast<float4*>(part + rr * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            if (c == 0) *reinterpret_cast<float2*>(part + 32 * WQ * D + 2 * rr) = make_float2(M, L);
+                *reinterpret_cast<float4*>(unit + rr * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            if (c == 0) *reinterpret_cast<float2*>(unit + 32 * WQ * D + 2 * rr) = make_float2(M, L);
         }
     }
     // the new rows into the cache, by the sequence's last unit
@@ -356,8 +455,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
             const int n = i / LPR, c = (i % LPR) * 8;
             if (!((live >> (a.first + n)) & 1)) continue;
             const int64_t j = newrow + n;
-            st16(const_cast<uint16_t*>(a.k) + b * a.kb + h * a.kh + j * a.kt + c, ld16(kn - 8 * g + n * a.knn + c));
-            st16(const_cast<uint16_t*>(a.v) + b * a.vb + h * a.vh + j * a.vt + c, ld16(vn - vc + n * a.vnn + c));
+            st16(const_cast<uint16_t*>(ck.cached) - lc + j * a.kt + c, ld16(ck.fresh - lc + n * a.knn + c));
+            st16(const_cast<uint16_t*>(cv.cached) - lc + j * a.vt + c, ld16(cv.fresh - lc + n * a.vnn + c));
         }
     }
 }
