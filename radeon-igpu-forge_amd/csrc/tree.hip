@@ -35,62 +35,64 @@ struct TreePlan {
     int32_t units, least, groups, wq;
 };
 
-__device__ __forceinline__ int tree_len(const TreeArgs& a, int b) {
-    const int c = a.ctx[b];
+// keys of a sequence with its context `c` (as the caller gave it): its tree's rows included
+__device__ __forceinline__ int tree_len(const TreeArgs& a, int c) {
     const int64_t e = (int64_t)(c < 0 ? 0 : c) + a.first + a.N;
     return (int)(e < a.Tmax ? e : a.Tmax);
 }
+__device__ __forceinline__ uint32_t tree_tiles(const TreeArgs& a, int c) { return (uint32_t)((tree_len(a, c) + kTreeTile - 1) / kTreeTile); }
 
-// Tiles of a unit: as many as let all sequences' tiles fit the units, in whole steps of the
-// workgroup.  Every wave computes it by itself, 64 sequences at a time.
-template <int WK>
-__device__ __forceinline__ uint32_t tree_unit_tiles(const TreeArgs& a, const TreePlan& p, int lane) {
-    uint32_t sum = 0;
-    for (int b = lane; b < a.B; b += 64) sum += (uint32_t)((tree_len(a, b) + kTreeTile - 1) / kTreeTile);
+// The units of a launch, found by every wave by itself, 64 sequences at a time: `tiles` of a unit (as many as let
+// all sequences' fit the launch's units, in whole steps of the workgroup's `wk` streams).  `mine`: the
+// context of sequence `lane`, loaded once.
+struct TreeUnits {
+    uint32_t tiles;
+    int mine;
+    __device__ __forceinline__ void init(const TreeArgs& a, const TreePlan& p, uint32_t wk, int lane) {
+        mine = lane < a.B ? a.ctx[lane] : 0;
+        uint32_t sum = lane < a.B ? tree_tiles(a, mine) : 0u;
+        for (int b = lane + 64; b < a.B; b += 64) sum += tree_tiles(a, a.ctx[b]);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    sum *= (uint32_t)(p.groups * a.Hkv);
-    const uint32_t t = max((sum + p.units - 1) / (uint32_t)p.units, (uint32_t)p.least);
-    return (t + WK - 1) / WK * WK;
-}
-
-__device__ __forceinline__ uint32_t tree_seq_units(const TreeArgs& a, int b, uint32_t tiles) {
-    const uint32_t n = (uint32_t)((tree_len(a, b) + kTreeTile - 1) / kTreeTile);
-    return max(1u, (n + tiles - 1) / tiles);
-}
-
-// The sequence that holds unit u of those counted a sequence at a time (u in units of one key head
-// and row group), its first unit and its number of units; false past the last sequence.
-__device__ __forceinline__ bool tree_find(const TreeArgs& a, uint32_t u, uint32_t tiles, int lane, int& b, uint32_t& first,
-                                          uint32_t& count) {
-    uint32_t before = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const uint32_t n = b0 + lane < a.B ? tree_seq_units(a, b0 + lane, tiles) : 0u;
-        uint32_t up = n;   // inclusive scan
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t o = __shfl_up(up, off, 64);
-            if (lane >= off) up += o;
-        }
-        const uint64_t past = __ballot(before + up > u);
-        if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            b = __builtin_amdgcn_readfirstlane(b0 + l);
-            count = __builtin_amdgcn_readfirstlane(__shfl(n, l, 64));
-            first = __builtin_amdgcn_readfirstlane(before + __shfl(up, l, 64)) - count;
-            return true;
-        }
-        before += __shfl(up, 63, 64);
+        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        sum *= (uint32_t)(p.groups * a.Hkv);
+        const uint32_t t = max((sum + p.units - 1) / (uint32_t)p.units, (uint32_t)p.least);
+        tiles = (t + wk - 1) / wk * wk;
     }
-    return false;
-}
+    __device__ __forceinline__ uint32_t count(const TreeArgs& a, int c) const { return max(1u, (tree_tiles(a, c) + tiles - 1) / tiles); }
+    // The sequence with unit u (counted a sequence at a time, in units of one key head and row group), its first
+    // unit, their number and its context; false past the last sequence.
+    __device__ __forceinline__ bool find(const TreeArgs& a, uint32_t u, int lane, int& b, uint32_t& first, uint32_t& n, int& c) const {
+        uint32_t before = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
+            const bool in = b0 + lane < a.B;
+            const int x = b0 == 0 ? mine : in ? a.ctx[b0 + lane] : 0;
+            const uint32_t k = in ? count(a, x) : 0u;
+            uint32_t up = k;   // inclusive scan
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t o = __shfl_up(up, off, 64);
+                if (lane >= off) up += o;
+            }
+            const uint64_t past = __ballot(before + up > u);
+            if (past) {
+                const int l = __ffsll((unsigned long long)past) - 1;
+                b = __builtin_amdgcn_readfirstlane(b0 + l);
+                n = (uint32_t)__builtin_amdgcn_readlane((int)k, l);
+                first = before + (uint32_t)__builtin_amdgcn_readlane((int)up, l) - n;
+                c = __builtin_amdgcn_readlane(x, l);
+                return true;
+            }
+            before += (uint32_t)__builtin_amdgcn_readlane((int)up, 63);
+        }
+        return false;
+    }
+};
 
 // bits of the tree's nodes that are keys: drafted before this call (below `first`), or queries of it
 // that are no padding, and inside the cache
-__device__ __forceinline__ uint64_t tree_live(const TreeArgs& a, int b, int ctx, int lane) {
-    bool real = false;
-    if (lane < a.N) real = (a.tree[b * a.treeb + lane * a.treen] >> (a.first + lane)) & 1;
-    uint64_t live = (uint64_t)__ballot(real);
+// (`word`: the bit set of query `lane`)
+__device__ __forceinline__ uint64_t tree_live(const TreeArgs& a, uint64_t word, int ctx, int lane) {
+    uint64_t live = (uint64_t)__ballot(lane < a.N && ((word >> ((a.first + lane) & 63)) & 1));
     live = a.first ? (live << a.first) | ((1ull << a.first) - 1) : live;
     const int room = a.Tmax - ctx;
     return room >= 64 ? live : live & ((1ull << (room > 0 ? room : 0)) - 1);
@@ -159,41 +161,40 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
     const int G = a.H / a.Hkv, heads = plan.groups * a.Hkv;
 
     // the unit: sequence, key head, row group, tiles [t0, t1)
-    int b, hr;
+    int b, hr, ctx;
     uint32_t count = 1, t0 = 0, t1 = 0xffffffffu;
     if (plan.units == 0) {
         b = blockIdx.x / heads;
         hr = blockIdx.x - b * heads;
+        ctx = a.ctx[b];
     } else {
-        const uint32_t tiles = tree_unit_tiles<WK>(a, plan, lane);
+        TreeUnits units;
+        units.init(a, plan, WK, lane);
         const uint32_t u = blockIdx.x / heads;
         hr = blockIdx.x - u * heads;
         uint32_t first;
-        if (!tree_find(a, u, tiles, lane, b, first, count)) return;
-        t0 = __builtin_amdgcn_readfirstlane((u - first) * tiles);
-        t1 = __builtin_amdgcn_readfirstlane(t0 + tiles);
+        if (!units.find(a, u, lane, b, first, count, ctx)) return;
+        t0 = __builtin_amdgcn_readfirstlane((u - first) * units.tiles);
+        t1 = __builtin_amdgcn_readfirstlane(t0 + units.tiles);
     }
     const int h = hr % a.Hkv, rg = hr / a.Hkv;
-    int ctx = __builtin_amdgcn_readfirstlane(a.ctx[b]);
-    ctx = ctx < 0 ? 0 : (ctx > a.Tmax ? a.Tmax : ctx);
-    const int end = __builtin_amdgcn_readfirstlane(tree_len(a, b));
-    t1 = min(t1, (uint32_t)((end + kTreeTile - 1) / kTreeTile));
-    const uint64_t live = tree_live(a, b, ctx, lane);
-    const int newrow = a.knew ? ctx + a.first : a.Tmax;   // rows from here on come from knew / vnew
 
-    // this lane's query row: node and head
+    // this lane's query row: node and head; and the tree's word of query `lane`
     const int rows = a.N * G;
     const int r = (rg * WQ + wq) * kTreeTile + ln;
     const int node = r < rows ? r / G : 0;
-    uint64_t bits = r < rows ? (uint64_t)a.tree[b * a.treeb + node * a.treen] : 0ull;
-    if (!((bits >> (a.first + node)) & 1)) bits = 0;
-    bits &= live;
+    uint64_t bits = (uint64_t)a.tree[b * a.treeb + node * a.treen];
+    const uint64_t word = (uint64_t)a.tree[b * a.treeb + min(lane, a.N - 1) * a.treen];
     bf16x8 qf[KS];
     {
         const uint16_t* qp = a.q + b * a.qb + node * a.qn + (int64_t)(h * G + (r < rows ? r - node * G : 0)) * a.qh + 8 * g;
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = __builtin_bit_cast(bf16x8, ld16(qp + 16 * s));
     }
+    const int end = __builtin_amdgcn_readfirstlane(tree_len(a, ctx));
+    ctx = __builtin_amdgcn_readfirstlane(ctx < 0 ? 0 : (ctx > a.Tmax ? a.Tmax : ctx));
+    t1 = min(t1, (uint32_t)((end + kTreeTile - 1) / kTreeTile));
+    const int newrow = a.knew ? ctx + a.first : a.Tmax;   // rows from here on come from knew / vnew
 
     uint16_t* const tile0 = reinterpret_cast<uint16_t*>(lds) + wk * kTile;   // of buffer 0
     const int lr = lane / LPR, lc = (lane % LPR) * 8;   // this lane's row of a load and its column
@@ -203,6 +204,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
     const TreeRows mine = values ? cv : ck;
     const int part = WQ > 1 ? (wq % (WQ > 1 ? WQ / 2 : 1)) * PW : 0;   // its first load of the tile's NV of that kind
 
+    uint64_t live = 0;   // set once the first loads are under way
     uint4 st[PW];
     // Tiles of the context alone take their rows as they lie; the tree's (at most three a sequence) clamp
     // the row to the last one.
@@ -222,6 +224,15 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
             load_rows(cv, j0, 0, NV, st + NV);
         } else {
             load_rows(mine, j0, part, PW, st);
+        }
+    };
+    // New rows into the cache, out of the registers of the wave that loaded them (for the first row group)
+    auto keep_rows = [&](const TreeRows& c, int j0, int first, int n, const uint4* from) {
+        if (rg != 0 || j0 + kTreeTile <= newrow) return;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const int j = j0 + (first + i) * RPI + lr;
+            if (j >= newrow && j < end && ((live >> (j - ctx)) & 1)) st16(const_cast<uint16_t*>(c.cached) + j * c.st, from[i]);
         }
     };
     // Loaded values into LDS.  In the tree's tiles, values of rows that are nobody's key are zeros, whatever
@@ -253,11 +264,15 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
         uint16_t* ks = tile0 + buf * WK * kTile;
         uint16_t* vt = ks + kTreeTile * KLD;
         if (WQ == 1 || !values) {
+            keep_rows(ck, j0, part, WQ == 1 ? NV : PW, st);
 #pragma unroll
             for (int i = 0; i < (WQ == 1 ? NV : PW); ++i) st16(ks + ((part + i) * RPI + lr) * KLD + lc, st[i]);
         }
-        if (WQ == 1) put_values(vt, j0, 0, NV, st + (WQ == 1 ? NV : 0), &odd[0][w]);
-        else if (values) put_values(vt, j0, part, PW, st, &odd[buf][w]);
+        if (WQ == 1 || values) {
+            uint4* v = st + (WQ == 1 ? NV : 0);
+            keep_rows(cv, j0, part, WQ == 1 ? NV : PW, v);
+            put_values(vt, j0, part, WQ == 1 ? NV : PW, v, &odd[buf][w]);
+        }
     };
 
     const float sc = a.scale * kLog2e;
@@ -360,6 +375,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
     auto queries_here = [&] {
 #pragma unroll
         for (int c = 0; c < KS; ++c) asm volatile("" : "+v"(qf[c]));
+        live = tree_live(a, word, ctx, lane);
+        bits = r < rows && ((bits >> (a.first + node)) & 1) ? bits & live : 0ull;
     };
     if constexpr (WQ == 1) {
         if (t < t1) {
@@ -449,75 +466,79 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
             if (c == 0) *reinterpret_cast<float2*>(unit + 32 * WQ * D + 2 * rr) = make_float2(M, L);
         }
     }
-    // the new rows into the cache, by the sequence's last unit
-    if (a.knew && rg == 0 && t1 * kTreeTile >= (uint32_t)end) {
-        for (int i = threadIdx.x; i < a.N * LPR; i += kTreeThreads) {
-            const int n = i / LPR, c = (i % LPR) * 8;
-            if (!((live >> (a.first + n)) & 1)) continue;
-            const int64_t j = newrow + n;
-            st16(const_cast<uint16_t*>(ck.cached) - lc + j * a.kt + c, ld16(ck.fresh - lc + n * a.knn + c));
-            st16(const_cast<uint16_t*>(cv.cached) - lc + j * a.vt + c, ld16(cv.fresh - lc + n * a.vnn + c));
-        }
-    }
 }
 
-// Join the units of one query row: a workgroup a row, D / 4 lanes for a unit's row of D floats.
-template <int D>
+// Join the units of query rows: WPR waves a row (1, or 4 where a row has many units), D / 4 lanes of them for a
+// unit's row of D floats.
+template <int D, int WPR>
 __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, TreePlan plan) {
-    constexpr int LPR = D / 4, NS = 256 / LPR;   // units read side by side
-    __shared__ float sm[NS], sl[NS];
-    __shared__ __attribute__((aligned(16))) float so[NS][D];
-    const int lane = threadIdx.x & 63;
-    const int G = a.H / a.Hkv, heads = plan.groups * a.Hkv, wk = kTreeWaves / plan.wq;
-    const uint32_t tiles = wk == 8 ? tree_unit_tiles<8>(a, plan, lane)
-                     : wk == 4 ? tree_unit_tiles<4>(a, plan, lane)
-                     : wk == 2 ? tree_unit_tiles<2>(a, plan, lane) : tree_unit_tiles<1>(a, plan, lane);
-    const int hq = blockIdx.x % a.H, bn = blockIdx.x / a.H, n = bn % a.N, b = bn / a.N;
-    const uint32_t count = tree_seq_units(a, b, tiles);
+    constexpr int LPR = D / 4, NS = WPR * 64 / LPR;   // units read side by side
+    __shared__ float2 sml[WPR];
+    __shared__ __attribute__((aligned(16))) float so[WPR][D];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int G = a.H / a.Hkv, heads = plan.groups * a.Hkv;
+    const int row = WPR == 1 ? blockIdx.x * 4 + w : blockIdx.x;
+    if (row >= a.B * a.N * a.H) return;
+    TreeUnits units;
+    units.init(a, plan, kTreeWaves / plan.wq, lane);
+    const int hq = row % a.H, bn = row / a.H, n = bn % a.N, b = bn / a.N;
+    const uint32_t count = units.count(a, a.ctx[b]);
     if (count == 1) return;   // written by its unit
-    uint32_t first = 0;       // units of the sequences before b
-    for (int x = lane; x < b; x += 64) first += tree_seq_units(a, x, tiles);
+    const uint64_t bits = (uint64_t)a.tree[b * a.treeb + n * a.treen];
+    uint32_t first = lane < b ? units.count(a, units.mine) : 0u;   // units of the sequences before b
+    for (int x = lane + 64; x < b; x += 64) first += units.count(a, a.ctx[x]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) first += __shfl_xor(first, off, 64);
-    const int h = hq / G, row = n * G + hq - h * G, rg = row / (32 * plan.wq), rr = row - rg * 32 * plan.wq;
-    const int64_t per = (int64_t)32 * plan.wq * (D + 2);
+    const int h = hq / G, rq = n * G + hq - h * G, rg = rq / (32 * plan.wq), rr = rq - rg * 32 * plan.wq;
+    const int64_t per = (int64_t)32 * plan.wq * (D + 2), step = heads * per;
     const float* base = a.work + ((int64_t)first * heads + rg * a.Hkv + h) * per;
-    const int st = threadIdx.x / LPR, c = (threadIdx.x % LPR) * 4;
+    const int st = (WPR == 1 ? lane : (int)threadIdx.x) / LPR, c = (lane % LPR) * 4;
     float M = kTreeNegInf, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t u = st; u < count; u += NS) {
-        const float* p = base + (int64_t)u * heads * per;
-        const float2 z = *reinterpret_cast<const float2*>(p + 32 * plan.wq * D + 2 * rr);
-        const float4 x = *reinterpret_cast<const float4*>(p + rr * D + c);
-        const float mn = fmaxf(M, z.x), mu = mn == kTreeNegInf ? 0.f : mn;
-        const float f = exp2_fast(M - mu), fx = exp2_fast(z.x - mu);
-        L = L * f + z.y * fx;
+    auto join = [&](float m, float l, const float4& x) {
+        const float mn = fmaxf(M, m), mu = mn == kTreeNegInf ? 0.f : mn;
+        const float f = exp2_fast(M - mu), fx = exp2_fast(m - mu);
+        L = L * f + l * fx;
         o.x = o.x * f + x.x * fx;
         o.y = o.y * f + x.y * fx;
         o.z = o.z * f + x.z * fx;
         o.w = o.w * f + x.w * fx;
         M = mn;
-    }
-    if (c == 0) sm[st] = M, sl[st] = L;
-    *reinterpret_cast<float4*>(&so[st][c]) = o;
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= D) return;
-    M = kTreeNegInf;
+    };
+    constexpr int U = 4;   // units of a lane in flight
+    for (uint32_t u = st; u < count; u += NS * U) {
+        float2 z[U];
+        float4 x[U];
 #pragma unroll
-    for (int x = 0; x < NS; ++x) M = fmaxf(M, sm[x]);
-    const float mu = M == kTreeNegInf ? 0.f : M;
-    float O = 0.f;
-    L = 0.f;
+        for (int i = 0; i < U; ++i) {
+            const float* p = base + (int64_t)min(u + i * NS, count - 1) * step;
+            z[i] = *reinterpret_cast<const float2*>(p + 32 * plan.wq * D + 2 * rr);
+            x[i] = *reinterpret_cast<const float4*>(p + rr * D + c);
+        }
 #pragma unroll
-    for (int x = 0; x < NS; ++x) {
-        const float f = exp2_fast(sm[x] - mu);
-        L += sl[x] * f;
-        O += so[x][d] * f;
+        for (int i = 0; i < U; ++i)
+            if (u + i * NS < count) join(z[i].x, z[i].y, x[i]);
     }
-    const bool none = L == 0.f || !((a.tree[b * a.treeb + n * a.treen] >> (a.first + n)) & 1);
-    a.o[(int64_t)blockIdx.x * D + d] = f32_to_bf16(none ? 0.f : O / L);
-    if (a.lse && d == 0) a.lse[blockIdx.x] = none ? kTreeNegInf : (M + log2_fast(L)) * kLn2;
+#pragma unroll
+    for (int off = LPR; off < 64; off <<= 1)
+        join(__shfl_xor(M, off, 64), __shfl_xor(L, off, 64),
+             make_float4(__shfl_xor(o.x, off, 64), __shfl_xor(o.y, off, 64), __shfl_xor(o.z, off, 64), __shfl_xor(o.w, off, 64)));
+    if (WPR > 1) {
+        if (lane < LPR) *reinterpret_cast<float4*>(&so[w % WPR][c]) = o;
+        if (lane == 0) sml[w % WPR] = make_float2(M, L);
+        __syncthreads();
+        if (w != 0) return;
+#pragma unroll
+        for (int x = 1; x < WPR; ++x) join(sml[x].x, sml[x].y, *reinterpret_cast<const float4*>(&so[x][c]));
+    }
+    if (lane >= LPR) return;
+    const bool none = L == 0.f || !((bits >> (a.first + n)) & 1);
+    const float inv = none ? 0.f : 1.f / L;
+    uint2 out;
+    out.x = none ? 0u : pack_bf16x2(o.x * inv, o.y * inv);
+    out.y = none ? 0u : pack_bf16x2(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(a.o + (int64_t)row * D + c) = out;
+    if (a.lse && lane == 0) a.lse[row] = none ? kTreeNegInf : (M + log2_fast(L)) * kLn2;
 }
 
 // Launch shape.  One workgroup a CU is resident (its registers), so R = CUs of them run at once.
@@ -526,7 +547,10 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, TreePlan pla
 static TreePlan tree_plan(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t Tmax) {
     TreePlan p{};
     const int rows = N * (H / Hkv);
-    p.wq = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+    // row groups: one workgroup's while the keys' bytes bound it (8 tiles of 32 rows at most), else of whichever
+    // size pads fewer rows
+    const int tiles32 = (rows + 31) / 32;
+    p.wq = tiles32 == 1 ? 1 : tiles32 == 2 ? 2 : tiles32 <= 4 ? 4 : tiles32 <= 8 || (tiles32 + 3) / 4 % 2 == 0 ? 8 : 4;
     p.groups = (rows + 32 * p.wq - 1) / (32 * p.wq);
     const int64_t pairs = (int64_t)B * Hkv * p.groups, cus = device_cus();
     const int wk = kTreeWaves / p.wq;
@@ -560,7 +584,11 @@ static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
     }
     if (int e = check_launch("tree_attention")) return e;
     if (p.units == 0) return 0;
-    hipLaunchKernelGGL((tree_join_kernel<D>), dim3((unsigned)(a.B * a.N * a.H)), dim3(256), 0, st, a, p);
+    const int64_t rows = (int64_t)a.B * a.N * a.H;
+    if (p.units > 16 * a.B * p.groups * a.Hkv)   // over 16 units a row
+        hipLaunchKernelGGL((tree_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, p);
+    else
+        hipLaunchKernelGGL((tree_join_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p);
     return check_launch("tree_attention_join");
 }
 
