@@ -12,9 +12,21 @@ namespace fx {
 //
 // p_v = exp((l_v - m) / T) / sum over the kept u of exp((l_u - m) / T), m the row's maximum, kept: the
 // top_k largest logits and the equals of the last of them (GPT.generate's rule).  HBM-bound: a row is
-// read once and written once.  One workgroup a row.
+// read once and written once.  One workgroup a row, which holds the row in registers (what does
+// not fit is read again, from the caches): the maximum, the selection, the sum and the output are
+// passes over registers.
+//
+// The selection.  The top_k-th largest of the threads' own maxima is at most the top_k-th largest
+// logit, and few logits lie above it: those are listed, and the exact bound found among them.  Both
+// searches are one wave's, halving an interval of order-preserving integer keys until the keys at or above
+// its lower end are few enough, or top_k.  Where the list is too small for the logits above the first bound
+// (a sorted row, a thousand equals) the bound is found a bit at a time over the registers, and where
+// top_k is beyond half the threads by another kernel, eleven bits at a time: three passes that count the
+// keys of what is settled of it.
 
 constexpr int kProbThreads = 1024, kProbWaves = kProbThreads / 64;
+constexpr int kProbList = kProbThreads;   // logits of the list
+constexpr int kProbBins = 2048;
 constexpr float kDraftNegInf = -__builtin_huge_valf();
 
 // a logit's bits in an order that unsigned comparison keeps, both zeros alike
@@ -52,70 +64,312 @@ struct JoinCount {
     static __device__ __forceinline__ int join(int a, int b) { return a + b; }
 };
 
-// A row of V values from flat index i0 of a 16-byte aligned tensor, NP a 16-byte load: f(value, v) for
-// every v of this thread's, the row's ragged ends by single loads
+// A wave's search among n keys in LDS (n <= 64 R): a bound with at least `want` keys at or above it, and at most
+// `most`, or, where equals prevent that, the want-th largest key itself (the largest bound with `want`).
+template <int R>
+__device__ __forceinline__ uint32_t wave_bound(const uint32_t* keys, int n, int want, int most, int lane) {
+    uint32_t k[R], lo = 0xffffffffu, hi = 0u;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int j = i * 64 + lane;
+        k[i] = j < n ? keys[j] : 0u;
+        if (j < n) lo = min(lo, k[i]), hi = max(hi, k[i]);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        lo = min(lo, (uint32_t)__shfl_xor((int)lo, off, 64));
+        hi = max(hi, (uint32_t)__shfl_xor((int)hi, off, 64));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    // all keys are at or above lo; keys above hi: none.  (A slot past n holds 0, the least key, below any mid.)
+    int have = n;
+    while (lo < hi && have > most) {
+        const uint32_t mid = lo + (hi - lo) / 2 + 1;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) c += __popcll(__ballot(k[i] >= mid));
+        if (c >= want) lo = mid, have = c;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// f(logit, place) for this thread's of a row of V from flat index i0 of a 16-byte aligned tensor: 16-byte loads, the ragged
+// ends by single ones
 template <bool BF, typename Fn>
 __device__ __forceinline__ void each_logit(const void* base, int64_t i0, int64_t V, Fn f) {
     constexpr int NP = BF ? 8 : 4;
     const int64_t head = min(V, (NP - i0 % NP) % NP), body = (V - head) / NP;
     auto one = [&](int64_t v) { return BF ? bf16_to_f32(static_cast<const uint16_t*>(base)[i0 + v]) : static_cast<const float*>(base)[i0 + v]; };
+#pragma unroll 2
     for (int64_t i = threadIdx.x; i < body; i += kProbThreads) {
-        const int64_t v = head + i * NP;
+        const uint4 u = ld16(static_cast<const char*>(base) + (i0 + head + i * NP) * (BF ? 2 : 4));
         float x[NP];
-        const uint4 u = ld16(static_cast<const char*>(base) + (i0 + v) * (BF ? 2 : 4));
-        if constexpr (BF) {
-            unpack8(u, x);
-        } else {
-            x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
-        }
+        if constexpr (BF) unpack8(u, x);
+        else x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
 #pragma unroll
-        for (int e = 0; e < NP; ++e) f(x[e], v + e);
+        for (int e = 0; e < NP; ++e) f(x[e], head + i * NP + e);
     }
     if ((int64_t)threadIdx.x < head) f(one(threadIdx.x), (int64_t)threadIdx.x);
     const int64_t v = head + body * NP + threadIdx.x;
     if (v < V) f(one(v), v);
 }
 
+// The want-th largest key of a row, 11, 11 and 10 bits at a time: the bins of the keys that share the bits above.
 template <bool BF>
-__global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits, float* probs, int64_t V, double temperature, int64_t top_k) {
+__device__ __forceinline__ uint32_t radix_bound(const void* logits, int64_t i0, int64_t V, int want, uint32_t* hist) {
+    __shared__ uint32_t digit;
+    __shared__ int above;
+    const int lane = threadIdx.x & 63;
+    uint32_t key = 0, settled = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kProbBins; i += kProbThreads) hist[i] = 0;
+        __syncthreads();
+        each_logit<BF>(logits, i0, V, [&](float x, int64_t) {
+            const uint32_t k = order_key(x);
+            if ((k & settled) == key) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+        });
+        __syncthreads();
+        if (threadIdx.x < 64) {   // bins from the top: 32 a lane (half of them empty in the last pass)
+            constexpr int PL = kProbBins / 64;
+            const int top = kProbBins - 1 - lane * PL;
+            int sum = 0;
+            for (int i = 0; i < PL; ++i) sum += (int)hist[top - i];
+            int up = sum;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int o = __shfl_up(up, off, 64);
+                if (lane >= off) up += o;
+            }
+            const uint64_t past = __ballot(up >= want);
+            if (lane == __ffsll((unsigned long long)past) - 1) {   // the want-th lies in this lane's bins
+                int run = up - sum, i = 0;
+                for (; i < PL - 1 && run + (int)hist[top - i] < want; ++i) run += (int)hist[top - i];
+                digit = (uint32_t)(top - i);
+                above = run;
+            }
+        }
+        __syncthreads();
+        key |= digit << shift;
+        settled |= ((1u << bits) - 1) << shift;
+        want -= above;
+    }
+    return key;
+}
+
+// V logits from flat index i0 of a 16-byte aligned tensor, as the threads of a workgroup hold them: NR 16-byte vectors
+// each, vectors past those read again at every pass, and the row's ragged ends (fewer than two vectors'
+// values, one a thread)
+template <bool BF, int NR>
+struct LogitRow {
+    static constexpr int NP = BF ? 8 : 4;
+    uint4 x[NR];
+    float edge;
+    int64_t edge_at;   // -1: none
+    const char* base;  // the first whole vector
+    int64_t head;
+    int body;
+
+    __device__ __forceinline__ static void unpack(const uint4& u, float* f) {
+        if constexpr (BF) unpack8(u, f);
+        else f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+    }
+    __device__ __forceinline__ void load(const void* logits, int64_t i0, int64_t V) {
+        head = min(V, (NP - i0 % NP) % NP);
+        body = (int)((V - head) / NP);
+        base = static_cast<const char*>(logits) + (i0 + head) * (BF ? 2 : 4);
+        // what lies behind the row's end is -inf: nothing counts it
+        const uint32_t ninf = BF ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            x[i] = (int)threadIdx.x < body - i * kProbThreads ? ld16(base + threadIdx.x * 16 + i * kProbThreads * 16)
+                                                              : make_uint4(ninf, ninf, ninf, ninf);
+        }
+        const int64_t tail = head + (int64_t)body * NP, t = threadIdx.x;
+        edge_at = t < head ? t : t - head < V - tail ? tail + t - head : -1;
+        edge = kDraftNegInf;
+        if (edge_at >= 0)
+            edge = BF ? bf16_to_f32(static_cast<const uint16_t*>(logits)[i0 + edge_at]) : static_cast<const float*>(logits)[i0 + edge_at];
+    }
+    // f(four values, the vector's place in the row or -1, its values' offset) for every four; then the edge by itself
+    template <typename Fn>
+    __device__ __forceinline__ void each(Fn f) const {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            // a copy that the compiler cannot see through: what a pass makes of a vector is not kept in registers
+            // for the next pass, nor made before its turn
+            uint4 u;
+            asm volatile("v_mov_b32 %0, %4\n\tv_mov_b32 %1, %5\n\tv_mov_b32 %2, %6\n\tv_mov_b32 %3, %7"
+                         : "=&v"(u.x), "=&v"(u.y), "=&v"(u.z), "=&v"(u.w)
+                         : "v"(x[i].x), "v"(x[i].y), "v"(x[i].z), "v"(x[i].w));
+            float y[NP];
+            unpack(u, y);
+            const bool in = (int)threadIdx.x < body - i * kProbThreads;
+#pragma unroll
+            for (int e = 0; e < NP; e += 4) f(y + e, in ? head + (int64_t)threadIdx.x * NP + (i * kProbThreads * NP + e) : -1);
+            __builtin_amdgcn_sched_barrier(0);   // a vector after the other: registers
+        }
+        for (int j = NR * kProbThreads + threadIdx.x; j < body; j += kProbThreads) {
+            float y[NP];
+            unpack(ld16(base + (int64_t)j * 16), y);
+#pragma unroll
+            for (int e = 0; e < NP; e += 4) f(y + e, head + (int64_t)j * NP + e);
+        }
+    }
+    // the same for passes that need no places, one value at a time
+    template <typename Fn>
+    __device__ __forceinline__ void each_value(Fn f) const {
+        each([&](const float* y, int64_t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(y[e]);
+        });
+        f(edge);
+    }
+};
+
+// exp((l - m) / T) as 2^((l - m) log2(e) / T), 0 for keys below `key`: the difference is rounded once, the factor
+// is held in two parts
+struct ProbVal {
+    float m, hi, lo;
+    uint32_t key;
+    __device__ __forceinline__ ProbVal(float m, double temperature, uint32_t key) : m(m), key(key) {
+        const double f = 1.4426950408889634 / temperature;
+        hi = (float)f;
+        lo = (float)(f - (double)hi);
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        const float d = x - m, y = d * hi;
+        const float v = exp2_fast(y) * (1.f + kLn2 * (fmaf(d, hi, -y) + d * lo));
+        return y < -200.f || order_key(x) < key ? 0.f : v;   // -inf among the first
+    }
+};
+
+// zeros or NaN for a row that has no probabilities: of -inf alone, or with a NaN or +inf
+__device__ __forceinline__ bool no_probs(float m, bool nan, float* out, int64_t V) {
+    const bool empty = !nan && m == kDraftNegInf;
+    if (!nan && !empty && m != __builtin_huge_valf()) return false;
+    const float v = empty ? 0.f : __builtin_nanf("");
+    for (int64_t i = threadIdx.x; i < V; i += kProbThreads) out[i] = v;
+    return true;
+}
+
+// Any top_k: every step a pass over memory (the first from HBM, the others from the caches)
+template <bool BF>
+__global__ void __launch_bounds__(kProbThreads) probs_passes_kernel(const void* logits, float* probs, int64_t V, double temperature, int top_k) {
     __shared__ float shf[kProbWaves];
-    __shared__ int shi[kProbWaves];
+    __shared__ uint32_t hist[kProbBins];
     const int64_t i0 = (int64_t)blockIdx.x * V;
+    float* out = probs + i0;
     float m = kDraftNegInf;
     bool nan = false;
     each_logit<BF>(logits, i0, V, [&](float x, int64_t) { m = fmaxf(m, x), nan |= x != x; });
     m = block_reduce<JoinMax>(m, shf);
     nan = __syncthreads_or(nan);
-    float* out = probs + i0;
-    if (nan || m == kDraftNegInf || m == __builtin_huge_valf()) {   // no probabilities
-        const float v = !nan && m == kDraftNegInf ? 0.f : __builtin_nanf("");
-        for (int64_t i = threadIdx.x; i < V; i += kProbThreads) out[i] = v;
-        return;
-    }
-    uint32_t key = 0;   // logits from this key on are kept
-    if (top_k > 0 && top_k < V) {
-        // the largest key with top_k keys at or above it, a bit at a time
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t t = key | (1u << bit);
-            int n = 0;
-            each_logit<BF>(logits, i0, V, [&](float x, int64_t) { n += order_key(x) >= t; });
-            if (block_reduce<JoinCount>(n, shi) >= top_k) key = t;
-        }
-    }
-    // 2^((l - m) log2(e) / T): the difference is rounded once, the factor is held in two parts
-    const double f = 1.4426950408889634 / temperature;
-    const float hi = (float)f, lo = (float)(f - (double)hi);
-    auto val = [&](float x) {
-        const float d = x - m;
-        const float y = d * hi;
-        if (y < -200.f) return 0.f;   // -inf among them
-        return exp2_fast(y) * (1.f + kLn2 * (fmaf(d, hi, -y) + d * lo));
-    };
+    if (no_probs(m, nan, out, V)) return;
+    const ProbVal val(m, temperature, radix_bound<BF>(logits, i0, V, top_k, hist));
     float s = 0.f;
-    each_logit<BF>(logits, i0, V, [&](float x, int64_t) { s += order_key(x) >= key ? val(x) : 0.f; });
+    each_logit<BF>(logits, i0, V, [&](float x, int64_t) { s += val(x); });
     s = block_reduce<JoinSum>(s, shf);
     const float inv = 1.f / s;
-    each_logit<BF>(logits, i0, V, [&](float x, int64_t v) { out[v] = order_key(x) >= key ? val(x) * inv : 0.f; });
+    each_logit<BF>(logits, i0, V, [&](float x, int64_t v) { out[v] = val(x) * inv; });
+}
+
+// TOP: with top_k (at most half the threads), else over the whole row
+template <bool BF, int NR, bool TOP>
+__global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits, float* probs, int64_t V, double temperature, int top_k) {
+    __shared__ float shf[kProbWaves];
+    __shared__ int shi[kProbWaves], listed;
+    __shared__ uint32_t keys[TOP ? kProbThreads : 1], bound;   // the threads' maxima, then the list
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t i0 = (int64_t)blockIdx.x * V;
+    float* out = probs + i0;
+    LogitRow<BF, NR> row;
+    row.load(logits, i0, V);
+    float own = kDraftNegInf;   // this thread's maximum
+    bool nan = false;
+    row.each_value([&](float x) {
+        own = fmaxf(own, x), nan |= x != x;
+        asm volatile("" : "+v"(own));
+    });
+    if constexpr (TOP) {
+        if (threadIdx.x == 0) listed = 0;
+        keys[threadIdx.x] = order_key(own);
+    }
+    const float m = block_reduce<JoinMax>(own, shf);
+    nan = __syncthreads_or(nan);
+    if (no_probs(m, nan, out, V)) return;
+    uint32_t key = 0;   // logits from this key on are kept
+    if constexpr (TOP) {
+        if (w == 0) {
+            const uint32_t t = wave_bound<kProbWaves>(keys, kProbThreads, top_k, top_k + top_k / 4 + 8, lane);
+            if (lane == 0) bound = t;
+        }
+        __syncthreads();
+        const uint32_t t = bound;
+        row.each_value([&](float x) {
+            if (order_key(x) >= t) {
+                const int at = atomicAdd(&listed, 1);   // in any order: the list is only searched
+                if (at < kProbList) keys[at] = order_key(x);
+            }
+        });
+        __syncthreads();
+        const int n = listed;
+        if (n <= kProbList) {
+            if (w == 0) {
+                const uint32_t t2 = n <= 256 ? wave_bound<4>(keys, n, top_k, top_k, lane) : wave_bound<kProbWaves>(keys, n, top_k, top_k, lane);
+                if (lane == 0) bound = t2;
+            }
+            __syncthreads();
+            key = bound;
+        } else {
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t t2 = key | (1u << bit);
+                int c = 0;
+                row.each_value([&](float x) {
+                    c += order_key(x) >= t2;
+                    asm volatile("" : "+v"(c));
+                });
+                if (block_reduce<JoinCount>(c, shi) >= top_k) key = t2;
+            }
+        }
+    }
+    const ProbVal val(m, temperature, key);
+    float s = 0.f;
+    row.each_value([&](float x) {
+        s += val(x);
+        asm volatile("" : "+v"(s));
+    });
+    s = block_reduce<JoinSum>(s, shf);
+    const float inv = 1.f / s;
+    row.each([&](const float* y, int64_t v) {
+        if (v >= 0) *reinterpret_cast<float4*>(out + v) = make_float4(val(y[0]) * inv, val(y[1]) * inv, val(y[2]) * inv, val(y[3]) * inv);
+    });
+    if (row.edge_at >= 0) out[row.edge_at] = val(row.edge) * inv;
+}
+
+template <bool BF>
+static void probs_launch(const void* logits, float* probs, int64_t rows, int64_t V, double temperature, int64_t top_k, hipStream_t st) {
+    constexpr int NP = BF ? 8 : 4;
+    const int64_t vectors = (V / NP + kProbThreads - 1) / kProbThreads;   // a thread's, of a row
+    const bool top = top_k > 0 && top_k < V;
+    const dim3 grid((unsigned)rows), block(kProbThreads);
+    if (top && top_k > kProbThreads / 2) {
+        hipLaunchKernelGGL((probs_passes_kernel<BF>), grid, block, 0, st, logits, probs, V, temperature, (int)top_k);
+        return;
+    }
+#define FX_PROBS(NR)                                                                                                                \
+    if (top) hipLaunchKernelGGL((probs_kernel<BF, NR, true>), grid, block, 0, st, logits, probs, V, temperature, (int)top_k);       \
+    else hipLaunchKernelGGL((probs_kernel<BF, NR, false>), grid, block, 0, st, logits, probs, V, temperature, 0)
+    if (vectors <= 1) { FX_PROBS(1); }
+    else if (vectors <= 4) { FX_PROBS(4); }
+    else if (vectors <= 8) { FX_PROBS(8); }
+    else if (vectors <= 13) { FX_PROBS(13); }
+    else { FX_PROBS(16); }
+#undef FX_PROBS
 }
 
 int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, int64_t V, double temperature, int64_t top_k, void* stream) {
@@ -123,10 +377,8 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
     FX_REQUIRE(temperature > 0.f && temperature < __builtin_huge_val(), "sampling_probs: temperature %g must be positive and finite", temperature);
     if (rows == 0) return 0;
     FX_REQUIRE(logits && probs && (((uintptr_t)logits | (uintptr_t)probs) & 15) == 0, "sampling_probs: logits and probs must be 16-byte aligned");
-    if (bf16)
-        hipLaunchKernelGGL((probs_kernel<true>), dim3((unsigned)rows), dim3(kProbThreads), 0, (hipStream_t)stream, logits, probs, V, temperature, top_k);
-    else
-        hipLaunchKernelGGL((probs_kernel<false>), dim3((unsigned)rows), dim3(kProbThreads), 0, (hipStream_t)stream, logits, probs, V, temperature, top_k);
+    if (bf16) probs_launch<true>(logits, probs, rows, V, temperature, top_k, (hipStream_t)stream);
+    else probs_launch<false>(logits, probs, rows, V, temperature, top_k, (hipStream_t)stream);
     return check_launch("sampling_probs");
 }
 
@@ -141,17 +393,77 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
 // there, and a rejection takes x out of p.  The last token is drawn from what is left of the last
 // row by its running sum.  Sums and tests are in 64 bits: the tokens do not hang on a summation order.
 
+//
+// One workgroup a sequence; bound by what one CU takes from the caches (64 bytes a cycle), so rows are read in 16-byte
+// vectors, several in flight.  The draw halves nothing: the row's sum is taken in 16 regions, a wave each, then
+// the region that the running sum passes `at` in by itself, down to what one wave scans.
+
 constexpr int kVerNodes = 64;
-constexpr int kVerSeg = 256;                      // values of a segment of the running sum
 constexpr int64_t kVerMaxV = 1 << 20;
-constexpr int kVerSegs = (int)(kVerMaxV / kVerSeg);
+constexpr int kVerScan = 512;   // values that a wave scans
+constexpr int kVerVecs = 4;     // 16-byte vectors of each row in flight a thread
+
+// what rejections leave of a row: p, or max(p - c q, 0), or p without the dropped tokens
+struct Left {
+    const float *p, *q;   // the rows; q null: no draft rows
+    const int64_t* tok;   // the nodes' tokens (LDS)
+    uint64_t drop;        // nodes whose tokens are out (no draft rows)
+    double c;
+    int64_t V;
+    int off;              // values of the row's first 16-byte vector before the row
+
+    __device__ __forceinline__ double weigh(float x, float y, int64_t v) const {
+        if (q) return fmax((double)x - c * (double)y, 0.0);
+        for (uint64_t d = drop; d; d &= d - 1)
+            if (tok[__ffsll((unsigned long long)d) - 1] == v) return 0.0;
+        return (double)fmaxf(x, 0.f);
+    }
+    __device__ __forceinline__ double at(int64_t v) const { return v < 0 || v >= V ? 0.0 : weigh(p[v], q ? q[v] : 0.f, v); }
+    // a thread's share of the sum over vectors [lo, hi) (vector i: values 4 i - off ...), threads `stride` apart
+    __device__ __forceinline__ double sum(int64_t lo, int64_t hi, int first, int stride) const {
+        double s = 0.0;
+        int64_t i = lo + first;
+        for (; i < hi; i += (int64_t)kVerVecs * stride) {
+            float4 x[kVerVecs], y[kVerVecs];
+#pragma unroll
+            for (int u = 0; u < kVerVecs; ++u) {
+                const int64_t j = i + (int64_t)u * stride, v = 4 * j - off;
+                x[u] = y[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (j >= hi) continue;
+                if (v >= 0 && v + 4 <= V) {
+                    x[u] = *reinterpret_cast<const float4*>(p + v);
+                    if (q) y[u] = *reinterpret_cast<const float4*>(q + v);
+                } else {   // a ragged end
+                    float* xe = &x[u].x;
+                    float* ye = &y[u].x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (v + e >= 0 && v + e < V) xe[e] = p[v + e], ye[e] = q ? q[v + e] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kVerVecs; ++u) {
+                const int64_t v = 4 * (i + (int64_t)u * stride) - off;
+                s += weigh(x[u].x, y[u].x, v) + weigh(x[u].y, y[u].y, v + 1) + weigh(x[u].z, y[u].z, v + 2) + weigh(x[u].w, y[u].w, v + 3);
+            }
+        }
+        return s;
+    }
+    __device__ __forceinline__ int64_t vectors() const { return (V + off + 3) / 4; }
+};
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
 
 __global__ void __launch_bounds__(kProbThreads) verify_kernel(const float* probs, const float* draft, const int64_t* tokens, const int32_t* parents,
                                                               const float* uniform, int64_t* out, int32_t* path, int32_t* counts, int32_t N, int64_t V) {
     __shared__ int64_t tok[kVerNodes];
     __shared__ int par[kVerNodes], spath[kVerNodes];
     __shared__ float un[kVerNodes], pt[kVerNodes], qt[kVerNodes];
-    __shared__ double seg[kVerSegs + 1], shd[kProbWaves];
+    __shared__ double shd[kProbWaves], reg[2][kProbWaves];
     __shared__ int64_t last;
     const int64_t b = blockIdx.x;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -170,130 +482,114 @@ __global__ void __launch_bounds__(kProbThreads) verify_kernel(const float* probs
     }
     __syncthreads();
 
+    Left left{P, Q, tok, 0, 0.0, V, (int)((b * N * V) & 3)};
     int cur = 0, n = 0;
-    uint64_t drop = 0;    // rejected children of cur (no draft rows)
-    double c = 0.0, S = 1.0;
+    double S = 1.0;
     bool stale = false;   // c has moved since S was formed
-    auto weight = [&](int64_t v) {
-        const float p = P[cur * V + v];
-        if (Q) return fmax((double)p - c * (double)Q[cur * V + v], 0.0);
-        for (uint64_t d = drop; d; d &= d - 1)
-            if (tok[__ffsll((unsigned long long)d) - 1] == v) return 0.0;
-        return (double)fmaxf(p, 0.f);
-    };
-    auto row_sum = [&] {
-        double s = 0.0;
-        for (int64_t v = threadIdx.x; v < V; v += kProbThreads) s += weight(v);
-        return block_reduce<JoinSumD>(s, shd);
-    };
     if (threadIdx.x == 0) spath[0] = 0;
     for (int i = 1; i < N; ++i) {
         if (par[i] != cur) continue;
-        double left = (double)pt[i];
+        double x = (double)pt[i];
         if (Q) {
-            if (stale) S = row_sum(), stale = false;
-            left = fmax(left - c * (double)qt[i], 0.0);
+            if (stale) S = block_reduce<JoinSumD>(left.sum(0, left.vectors(), threadIdx.x, kProbThreads), shd), stale = false;
+            x = fmax(x - left.c * (double)qt[i], 0.0);
         } else {
-            for (uint64_t d = drop; d; d &= d - 1)
-                if (tok[__ffsll((unsigned long long)d) - 1] == tok[i]) left = 0.0;
+            for (uint64_t d = left.drop; d; d &= d - 1)
+                if (tok[__ffsll((unsigned long long)d) - 1] == tok[i]) x = 0.0;
         }
-        if ((double)un[i] * S * (double)qt[i] < left) {
-            cur = i, c = 0.0, S = 1.0, drop = 0, stale = false;
+        if ((double)un[i] * S * (double)qt[i] < x) {
+            cur = i;
+            const int64_t at = (int64_t)i * V;
+            left = Left{P + at, Q ? Q + at : nullptr, tok, 0, 0.0, V, (int)((b * N * V + at) & 3)};
+            S = 1.0, stale = false;
             if (threadIdx.x == 0) spath[n + 1] = i;
             ++n;
         } else if (Q) {
-            c += S;
+            left.c += S;
             stale = true;
         } else {
-            S -= left;
-            drop |= 1ull << i;
+            S -= x;
+            left.drop |= 1ull << i;
         }
     }
-    // segment sums of what is left, then of the row itself where nothing is
-    const int64_t nseg = (V + kVerSeg - 1) / kVerSeg;
-    double W = 0.0;
-    for (int round = 0; round < 2; ++round) {
-        for (int64_t s = w; s < nseg; s += kProbWaves) {
-            double x = 0.0;
-#pragma unroll
-            for (int e = 0; e < kVerSeg / 64; ++e) {
-                const int64_t v = s * kVerSeg + e * 64 + lane;
-                if (v < V) x += weight(v);
-            }
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-            if (lane == 0) seg[s] = x;
-        }
-        double x = 0.0;
+
+    // the last token, from what is left; from the row itself where nothing is
+    int64_t lo = 0, hi = left.vectors(), got = -1;
+    double at = 0.0, base = 0.0;   // the sum before vector lo
+    bool any = true;
+    for (int level = 0, round = 0;;) {
+        if (level > 0 && (hi - lo) * 4 <= kVerScan) break;
+        const int64_t part = (hi - lo + kProbWaves - 1) / kProbWaves, l = lo + part * w;
+        const double s = wave_sum_d(left.sum(min(l, hi), min(l + part, hi), lane, 64));
+        if (lane == 0) reg[level & 1][w] = s;   // two, in turn: one barrier a level
         __syncthreads();
-        for (int64_t s = threadIdx.x; s < nseg; s += kProbThreads) x += seg[s];
-        W = block_reduce<JoinSumD>(x, shd);
-        if (W > 0.0) break;
-        c = 0.0, drop = 0;
-        __syncthreads();
+        double run = base, from = base, some_from = base;
+        int pick = -1, some = -1;
+        if (level == 0) {
+            double W = 0.0;
+            for (int x = 0; x < kProbWaves; ++x) W += reg[0][x];
+            if (!(W > 0.0) && round == 0) {
+                left.c = 0.0, left.drop = 0, round = 1;
+                __syncthreads();
+                continue;
+            }
+            if (!(W > 0.0) || W == __builtin_huge_val()) {
+                any = false;
+                break;
+            }
+            at = (double)un[0] * W;
+        }
+        for (int x = 0; x < kProbWaves; ++x) {
+            const double z = reg[level & 1][x];
+            if (z > 0.0) {
+                some = x, some_from = run;
+                if (pick < 0 && run + z > at) pick = x, from = run;
+            }
+            run += z;
+        }
+        if (pick < 0) pick = some, from = some_from;   // by rounding none may pass: the last with weight
+        if (pick < 0) {   // a region's sum that its parts do not have: not reached
+            any = false;
+            break;
+        }
+        const int64_t l2 = lo + part * pick;
+        hi = min(l2 + part, hi);
+        lo = l2;
+        base = from;
+        ++level;
     }
-    if (w == 0) {
-        int64_t got = -1;
-        if (W > 0.0 && W < __builtin_huge_val()) {
-            const double at = (double)un[0] * W;
-            // the first segment whose running sum passes `at`; by rounding none may: the last with weight
-            double before = 0.0, base = 0.0;
-            int64_t pick = -1, some = -1;
-            double some_base = 0.0;
-            for (int64_t s0 = 0; s0 < nseg && pick < 0; s0 += 64) {
-                const double x = s0 + lane < nseg ? seg[s0 + lane] : 0.0;
-                double up = x;
+    if (any && w == 0) {
+        constexpr int E = kVerScan / 64;
+        double x[E], sum = 0.0;
+        const int64_t v0 = 4 * lo - left.off + (int64_t)lane * E, v1 = min(V, 4 * hi - left.off);
 #pragma unroll
-                for (int off = 1; off < 64; off <<= 1) {
-                    const double o = __shfl_up(up, off, 64);
-                    if (lane >= off) up += o;
-                }
-                const uint64_t past = __ballot(x > 0.0 && before + up > at), has = __ballot(x > 0.0);
-                if (has) {
-                    const int l = 63 - __clzll((long long)has);
-                    some = s0 + l;
-                    some_base = before + __shfl(up, l, 64) - __shfl(x, l, 64);
-                }
-                if (past) {
-                    const int l = __ffsll((unsigned long long)past) - 1;
-                    pick = s0 + l;
-                    base = before + __shfl(up, l, 64) - __shfl(x, l, 64);
-                }
-                before += __shfl(up, 63, 64);
-            }
-            if (pick < 0) pick = some, base = some_base;
-            // and the value within it, four of each lane's
-            double x[kVerSeg / 64], sum = 0.0;
-            const int64_t v0 = pick * kVerSeg + lane * (kVerSeg / 64);
+        for (int e = 0; e < E; ++e) x[e] = v0 + e < v1 ? left.at(v0 + e) : 0.0, sum += x[e];
+        double up = sum;
 #pragma unroll
-            for (int e = 0; e < kVerSeg / 64; ++e) x[e] = v0 + e < V ? weight(v0 + e) : 0.0, sum += x[e];
-            double up = sum;
+        for (int off = 1; off < 64; off <<= 1) {
+            const double o = __shfl_up(up, off, 64);
+            if (lane >= off) up += o;
+        }
+        double run = base + (up - sum);
+        int hit = -1, has = -1;
 #pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const double o = __shfl_up(up, off, 64);
-                if (lane >= off) up += o;
-            }
-            double run = base + (up - sum);
-            int hit = -1, any = -1;
-#pragma unroll
-            for (int e = 0; e < kVerSeg / 64; ++e) {
-                run += x[e];
-                if (x[e] > 0.0) {
-                    any = e;
-                    if (hit < 0 && run > at) hit = e;
-                }
-            }
-            const uint64_t hits = __ballot(hit >= 0), anys = __ballot(any >= 0);
-            if (hits) {
-                const int l = __ffsll((unsigned long long)hits) - 1;
-                got = pick * kVerSeg + l * (kVerSeg / 64) + __shfl(hit, l, 64);
-            } else if (anys) {
-                const int l = 63 - __clzll((long long)anys);
-                got = pick * kVerSeg + l * (kVerSeg / 64) + __shfl(any, l, 64);
+        for (int e = 0; e < E; ++e) {
+            run += x[e];
+            if (x[e] > 0.0) {
+                has = e;
+                if (hit < 0 && run > at) hit = e;
             }
         }
-        if (lane == 0) last = got;
+        const uint64_t hits = __ballot(hit >= 0), some = __ballot(has >= 0);
+        if (hits) {
+            const int l = __ffsll((unsigned long long)hits) - 1;
+            got = 4 * lo - left.off + l * E + __shfl(hit, l, 64);
+        } else if (some) {
+            const int l = 63 - __clzll((long long)some);
+            got = 4 * lo - left.off + l * E + __shfl(has, l, 64);
+        }
     }
+    if (threadIdx.x == 0) last = got;
     __syncthreads();
     if ((int)threadIdx.x < N) {
         const int d = threadIdx.x;
@@ -309,6 +605,7 @@ int verify_draft(const float* probs, const float* draft, const int64_t* tokens, 
                B, N, kVerNodes, (long long)V, (long long)kVerMaxV);
     if (B == 0) return 0;
     FX_REQUIRE(probs && tokens && parents && uniform && out && path && counts, "verify_draft: null pointer");
+    FX_REQUIRE((((uintptr_t)probs | (uintptr_t)draft) & 15) == 0, "verify_draft: probs and draft_probs must be 16-byte aligned");
     hipLaunchKernelGGL(verify_kernel, dim3((unsigned)B), dim3(kProbThreads), 0, (hipStream_t)stream, probs, draft, tokens, parents, uniform, out,
                        path, counts, N, V);
     return check_launch("verify_draft");
@@ -317,8 +614,10 @@ int verify_draft(const float* probs, const float* draft, const int64_t* tokens, 
 // ---- accepted rows together --------------------------------------------------------------
 //
 // Bound by the moved rows' bytes, read and written once.  A thread owns 16 bytes of a (tensor,
-// sequence)'s row and moves them for every d: the path ascends, so a row that is written
-// (ctx + d <= ctx + path[d]) is never one that is still to be read.
+// sequence)'s row and moves them for every d, eight rows in flight: the path ascends, so a row that is
+// written (ctx + d <= ctx + path[d]) is never one that is still to be read.
+
+constexpr int kCompactRows = 8;
 
 __global__ void __launch_bounds__(256) compact_kernel(CompactArgs a) {
     const int y = blockIdx.y, b = y % a.B, ten = y / a.B;
@@ -326,15 +625,25 @@ __global__ void __launch_bounds__(256) compact_kernel(CompactArgs a) {
     int n = a.counts[b];
     n = n < 0 ? 0 : (n > a.N ? a.N : n);
     if (a.ctx_out && ten == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.ctx_out[b] = ctx + n;
-    const int i = blockIdx.x * 256 + threadIdx.x, cpr = a.D / 8;
+    const int i = blockIdx.x * blockDim.x + threadIdx.x, cpr = a.D / 8;
     if (i >= a.H * cpr || ctx < 0) return;
     const int h = i / cpr, col = (i - h * cpr) * 8;
-    uint16_t* p = a.at[ten] + b * a.sb[ten] + h * a.sh[ten] + col;
     const int64_t st = a.st[ten];
-    for (int d = 0; d < n; ++d) {
-        const int s = a.path[(int64_t)b * a.N + d];
-        if (s <= d || s >= a.T - ctx) continue;   // in its place already, or no row of the cache
-        st16(p + (int64_t)(ctx + d) * st, ld16(p + (int64_t)(ctx + s) * st));
+    uint16_t* p = a.at[ten] + b * a.sb[ten] + h * a.sh[ten] + ctx * st + col;
+    const int32_t* path = a.path + (int64_t)b * a.N;
+    const int room = a.T - ctx;   // rows of the cache behind the context
+    for (int d0 = 0; d0 < n; d0 += kCompactRows) {
+        uint4 x[kCompactRows];
+        bool move[kCompactRows];
+#pragma unroll
+        for (int u = 0; u < kCompactRows; ++u) {
+            const int s = path[min(d0 + u, n - 1)];
+            move[u] = d0 + u < n && s > d0 + u && s < room;   // else in its place already, or no row of the cache
+            if (move[u]) x[u] = ld16(p + s * st);
+        }
+#pragma unroll
+        for (int u = 0; u < kCompactRows; ++u)
+            if (move[u]) st16(p + (d0 + u) * st, x[u]);
     }
 }
 
@@ -346,8 +655,8 @@ int compact_cache(const CompactArgs& a, void* stream) {
     for (int i = 0; i < a.count; ++i)
         FX_REQUIRE(a.at[i] && ((uintptr_t)a.at[i] & 15) == 0 && a.sb[i] % 8 == 0 && a.st[i] % 8 == 0 && a.sh[i] % 8 == 0,
                    "compact_cache: caches must be 16-byte aligned with strides of multiples of 8 elements");
-    const unsigned chunks = (unsigned)((a.H * (a.D / 8) + 255) / 256);
-    hipLaunchKernelGGL(compact_kernel, dim3(chunks, (unsigned)(a.count * a.B)), dim3(256), 0, (hipStream_t)stream, a);
+    const unsigned chunks = (unsigned)(a.H * (a.D / 8)), threads = chunks < 256 ? (chunks + 63) / 64 * 64 : 256;
+    hipLaunchKernelGGL(compact_kernel, dim3((chunks + threads - 1) / threads, (unsigned)(a.count * a.B)), dim3(threads), 0, (hipStream_t)stream, a);
     return check_launch("compact_cache");
 }
 

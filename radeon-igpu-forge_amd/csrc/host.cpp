@@ -539,6 +539,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> verify_draft(const Tensor& pro
         if (t->dim() != 2 || t->size(0) != B || t->size(1) != N || !t->is_cuda() || !t->is_contiguous()) return std::nullopt;
     for (const Tensor* t : {&probs, &uniform, draft.has_value() ? &*draft : &probs})
         if (t->scalar_type() != at::kFloat || !t->is_cuda() || !t->is_contiguous()) return std::nullopt;
+    if (!aligned(probs) || (draft.has_value() && !aligned(*draft))) return std::nullopt;
     same_gpu(probs, tokens, parents, uniform, draft);
     const c10::DeviceGuard guard(probs.device());
     Tensor out = at::empty({B, N}, tokens.options()), path = at::empty({B, N}, parents.options()),
@@ -566,6 +567,8 @@ OptT compact_cache(const std::vector<Tensor>& caches, const Tensor& ctx, const T
         if (t->scalar_type() != at::kInt || !t->is_cuda() || !t->is_contiguous()) return std::nullopt;
     for (const Tensor& t : caches) {
         if (!rows16(t, 4) || t.sizes() != c.sizes()) return std::nullopt;
+        for (int64_t i = 0; i < 3; ++i)
+            if (t.stride(i) == 0 && t.size(i) > 1) return std::nullopt;   // one row in many places
         same_gpu(c, t);
     }
     same_gpu(c, ctx, path, counts);

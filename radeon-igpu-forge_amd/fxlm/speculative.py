@@ -72,8 +72,9 @@ def verify_draft(probs, tokens, parents, uniform, draft_probs=None):
                 raise TypeError(f"{nm} must be a cuda tensor")
             if tuple(t.shape) != shape:
                 raise ValueError(f"{nm} must be {shape}, got {tuple(t.shape)}")
-        r = host.verify_draft(probs.contiguous(), tokens.contiguous(), parents.contiguous(), uniform.contiguous(),
-                              None if draft_probs is None else draft_probs.contiguous())
+        p, q = (None if t is None else t.contiguous() if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+                for t in (probs, draft_probs))
+        r = host.verify_draft(p, tokens.contiguous(), parents.contiguous(), uniform.contiguous(), q)
     return r
 
 
@@ -84,15 +85,14 @@ def compact_cache(cache, ctx, path, counts):
     (verify_draft's); entries outside the cache are passed over.  In place; returns ctx + counts,
     the new lengths.  Rows past them keep what they held."""
     flat = [t for kv in cache for t in kv]
-    for t in flat:
-        if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-            raise ValueError("an expanded cache cannot be compacted")
     r = host.compact_cache(flat, ctx, path, counts)
     if r is None:
         if not flat:
             raise ValueError("cache holds no tensors")
         s = flat[0].shape
         for t in flat:
+            if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                raise ValueError("an expanded cache cannot be compacted")
             if t.dtype != torch.bfloat16 or not t.is_cuda:
                 raise TypeError("caches must be bfloat16 cuda tensors")
             if t.dim() != 4 or t.shape != s or min(s) < 1 or s[3] % 8 or s[0] > 65535:
