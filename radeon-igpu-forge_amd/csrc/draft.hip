@@ -29,11 +29,12 @@ constexpr int kProbList = kProbThreads;   // logits of the list
 constexpr int kProbBins = 2048;
 constexpr float kDraftNegInf = -__builtin_huge_valf();
 
-// a logit's bits in an order that unsigned comparison keeps, both zeros alike
+// a logit's bits in an order that unsigned comparison keeps, both zeros alike, and the logit of such a key
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
     return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
 template <typename F>
 __device__ __forceinline__ auto block_reduce(decltype(F::zero()) v, decltype(F::zero()) * sh) {
@@ -195,23 +196,29 @@ struct LogitRow {
         if (edge_at >= 0)
             edge = BF ? bf16_to_f32(static_cast<const uint16_t*>(logits)[i0 + edge_at]) : static_cast<const float*>(logits)[i0 + edge_at];
     }
-    // f(four values, the vector's place in the row or -1, its values' offset) for every four; then the edge by itself
-    template <typename Fn>
-    __device__ __forceinline__ void each(Fn f) const {
+    // f(four values, their place in the row) for every four of the row's vectors.  What a pass makes of
+    // a vector must not be kept in registers for the next pass, nor made before its turn: the vectors go
+    // through an empty statement that the compiler cannot see through (LOOP: a copy of them does, since a loop
+    // would otherwise hold the vectors twice).
+    template <bool LOOP, typename Fn>
+    __device__ __forceinline__ void each(Fn f) {
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            // a copy that the compiler cannot see through: what a pass makes of a vector is not kept in registers
-            // for the next pass, nor made before its turn
             uint4 u;
-            asm volatile("v_mov_b32 %0, %4\n\tv_mov_b32 %1, %5\n\tv_mov_b32 %2, %6\n\tv_mov_b32 %3, %7"
-                         : "=&v"(u.x), "=&v"(u.y), "=&v"(u.z), "=&v"(u.w)
-                         : "v"(x[i].x), "v"(x[i].y), "v"(x[i].z), "v"(x[i].w));
+            if constexpr (LOOP) {
+                asm volatile("v_mov_b32 %0, %4\n\tv_mov_b32 %1, %5\n\tv_mov_b32 %2, %6\n\tv_mov_b32 %3, %7"
+                             : "=&v"(u.x), "=&v"(u.y), "=&v"(u.z), "=&v"(u.w)
+                             : "v"(x[i].x), "v"(x[i].y), "v"(x[i].z), "v"(x[i].w));
+            } else {
+                asm volatile("" : "+v"(x[i].x), "+v"(x[i].y), "+v"(x[i].z), "+v"(x[i].w));
+                u = x[i];
+            }
             float y[NP];
             unpack(u, y);
-            const bool in = (int)threadIdx.x < body - i * kProbThreads;
+            const bool in = (int)threadIdx.x < body - i * kProbThreads;   // else -inf, and of no place
 #pragma unroll
             for (int e = 0; e < NP; e += 4) f(y + e, in ? head + (int64_t)threadIdx.x * NP + (i * kProbThreads * NP + e) : -1);
-            __builtin_amdgcn_sched_barrier(0);   // a vector after the other: registers
+            __builtin_amdgcn_sched_barrier(0);
         }
         for (int j = NR * kProbThreads + threadIdx.x; j < body; j += kProbThreads) {
             float y[NP];
@@ -220,31 +227,20 @@ struct LogitRow {
             for (int e = 0; e < NP; e += 4) f(y + e, head + (int64_t)j * NP + e);
         }
     }
-    // the same for passes that need no places, one value at a time
-    template <typename Fn>
-    __device__ __forceinline__ void each_value(Fn f) const {
-        each([&](const float* y, int64_t) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f(y[e]);
-        });
-        f(edge);
-    }
 };
 
-// exp((l - m) / T) as 2^((l - m) log2(e) / T), 0 for keys below `key`: the difference is rounded once, the factor
-// is held in two parts
+// exp((l - m) / T) as 2^((l - m) log2(e) / T): the difference is rounded once, the factor is held in two parts
 struct ProbVal {
-    float m, hi, lo;
-    uint32_t key;
-    __device__ __forceinline__ ProbVal(float m, double temperature, uint32_t key) : m(m), key(key) {
+    float m, hi, lo, least;
+    __device__ __forceinline__ ProbVal(float m, double temperature) : m(m) {
         const double f = 1.4426950408889634 / temperature;
         hi = (float)f;
         lo = (float)(f - (double)hi);
+        least = -200.f / hi;   // 2^-200 is 0; -inf is no number to multiply
     }
     __device__ __forceinline__ float operator()(float x) const {
-        const float d = x - m, y = d * hi;
-        const float v = exp2_fast(y) * (1.f + kLn2 * (fmaf(d, hi, -y) + d * lo));
-        return y < -200.f || order_key(x) < key ? 0.f : v;   // -inf among the first
+        const float d = fmaxf(x - m, least), y = d * hi;
+        return exp2_fast(y) * fmaf(kLn2, fmaf(d, lo, fmaf(d, hi, -y)), 1.f);
     }
 };
 
@@ -270,12 +266,13 @@ __global__ void __launch_bounds__(kProbThreads) probs_passes_kernel(const void* 
     m = block_reduce<JoinMax>(m, shf);
     nan = __syncthreads_or(nan);
     if (no_probs(m, nan, out, V)) return;
-    const ProbVal val(m, temperature, radix_bound<BF>(logits, i0, V, top_k, hist));
+    const float least = key_value(radix_bound<BF>(logits, i0, V, top_k, hist));   // logits from here on are kept
+    const ProbVal val(m, temperature);
     float s = 0.f;
-    each_logit<BF>(logits, i0, V, [&](float x, int64_t) { s += val(x); });
+    each_logit<BF>(logits, i0, V, [&](float x, int64_t) { s += x >= least ? val(x) : 0.f; });
     s = block_reduce<JoinSum>(s, shf);
     const float inv = 1.f / s;
-    each_logit<BF>(logits, i0, V, [&](float x, int64_t v) { out[v] = val(x) * inv; });
+    each_logit<BF>(logits, i0, V, [&](float x, int64_t v) { out[v] = x >= least ? val(x) * inv : 0.f; });
 }
 
 // TOP: with top_k (at most half the threads), else over the whole row
@@ -289,10 +286,11 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
     float* out = probs + i0;
     LogitRow<BF, NR> row;
     row.load(logits, i0, V);
-    float own = kDraftNegInf;   // this thread's maximum
-    bool nan = false;
-    row.each_value([&](float x) {
-        own = fmaxf(own, x), nan |= x != x;
+    float own = row.edge;   // this thread's maximum
+    bool nan = row.edge != row.edge;
+    row.template each<false>([&](const float* y, int64_t) {
+        own = fmaxf(fmaxf(fmaxf(own, y[0]), fmaxf(y[1], y[2])), y[3]);
+        nan |= __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]);
         asm volatile("" : "+v"(own));
     });
     if constexpr (TOP) {
@@ -302,20 +300,24 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
     const float m = block_reduce<JoinMax>(own, shf);
     nan = __syncthreads_or(nan);
     if (no_probs(m, nan, out, V)) return;
-    uint32_t key = 0;   // logits from this key on are kept
+    float least = kDraftNegInf;   // logits from here on are kept
     if constexpr (TOP) {
         if (w == 0) {
             const uint32_t t = wave_bound<kProbWaves>(keys, kProbThreads, top_k, top_k + top_k / 4 + 8, lane);
             if (lane == 0) bound = t;
         }
         __syncthreads();
-        const uint32_t t = bound;
-        row.each_value([&](float x) {
-            if (order_key(x) >= t) {
+        const float t = key_value(bound);
+        auto list = [&](float x) {
+            if (x >= t) {
                 const int at = atomicAdd(&listed, 1);   // in any order: the list is only searched
                 if (at < kProbList) keys[at] = order_key(x);
             }
+        };
+        row.template each<false>([&](const float* y, int64_t) {
+            if (fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= t) list(y[0]), list(y[1]), list(y[2]), list(y[3]);
         });
+        list(row.edge);
         __syncthreads();
         const int n = listed;
         if (n <= kProbList) {
@@ -324,31 +326,41 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
                 if (lane == 0) bound = t2;
             }
             __syncthreads();
-            key = bound;
+            least = key_value(bound);
         } else {
+            uint32_t key = 0;
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t t2 = key | (1u << bit);
-                int c = 0;
-                row.each_value([&](float x) {
-                    c += order_key(x) >= t2;
+                int c = order_key(row.edge) >= t2;
+                row.template each<true>([&](const float* y, int64_t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c += order_key(y[e]) >= t2;
                     asm volatile("" : "+v"(c));
                 });
                 if (block_reduce<JoinCount>(c, shi) >= top_k) key = t2;
             }
+            least = key_value(key);
         }
     }
-    const ProbVal val(m, temperature, key);
-    float s = 0.f;
-    row.each_value([&](float x) {
-        s += val(x);
+    const ProbVal val(m, temperature);
+    float s = row.edge >= least ? val(row.edge) : 0.f;
+    row.template each<false>([&](const float* y, int64_t) {
+        if (TOP && !(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += !TOP || y[e] >= least ? val(y[e]) : 0.f;
         asm volatile("" : "+v"(s));
     });
     s = block_reduce<JoinSum>(s, shf);
     const float inv = 1.f / s;
-    row.each([&](const float* y, int64_t v) {
-        if (v >= 0) *reinterpret_cast<float4*>(out + v) = make_float4(val(y[0]) * inv, val(y[1]) * inv, val(y[2]) * inv, val(y[3]) * inv);
+    row.template each<false>([&](const float* y, int64_t v) {
+        float z[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!TOP || fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = !TOP || y[e] >= least ? val(y[e]) * inv : 0.f;
+        }
+        if (v >= 0) *reinterpret_cast<float4*>(out + v) = make_float4(z[0], z[1], z[2], z[3]);
     });
-    if (row.edge_at >= 0) out[row.edge_at] = val(row.edge) * inv;
+    if (row.edge_at >= 0) out[row.edge_at] = row.edge >= least ? val(row.edge) * inv : 0.f;
 }
 
 template <bool BF>
