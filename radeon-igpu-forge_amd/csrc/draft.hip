@@ -180,7 +180,7 @@ struct LogitRow {
         else f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
     }
     __device__ __forceinline__ void load(const void* logits, int64_t i0, int64_t V) {
-        head = min(V, (NP - i0 % NP) % NP);
+        head = min(V, (32 - i0 % 32) % 32);   // the output's 128-byte lines, each a wave's own
         body = (int)((V - head) / NP);
         base = static_cast<const char*>(logits) + (i0 + head) * (BF ? 2 : 4);
         // what lies behind the row's end is -inf: nothing counts it
@@ -196,7 +196,7 @@ struct LogitRow {
         if (edge_at >= 0)
             edge = BF ? bf16_to_f32(static_cast<const uint16_t*>(logits)[i0 + edge_at]) : static_cast<const float*>(logits)[i0 + edge_at];
     }
-    // f(four values, their place in the row) for every four of the row's vectors.  What a pass makes of
+    // f(four values) for every four of the row's vectors.  What a pass makes of
     // a vector must not be kept in registers for the next pass, nor made before its turn: the vectors go
     // through an empty statement that the compiler cannot see through (LOOP: a copy of them does, since a loop
     // would otherwise hold the vectors twice).
@@ -215,32 +215,72 @@ struct LogitRow {
             }
             float y[NP];
             unpack(u, y);
-            const bool in = (int)threadIdx.x < body - i * kProbThreads;   // else -inf, and of no place
 #pragma unroll
-            for (int e = 0; e < NP; e += 4) f(y + e, in ? head + (int64_t)threadIdx.x * NP + (i * kProbThreads * NP + e) : -1);
+            for (int e = 0; e < NP; e += 4) f(y + e);
             __builtin_amdgcn_sched_barrier(0);
         }
         for (int j = NR * kProbThreads + threadIdx.x; j < body; j += kProbThreads) {
             float y[NP];
             unpack(ld16(base + (int64_t)j * 16), y);
 #pragma unroll
-            for (int e = 0; e < NP; e += 4) f(y + e, head + (int64_t)j * NP + e);
+            for (int e = 0; e < NP; e += 4) f(y + e);
+        }
+    }
+
+    // out[place] = f(value) over the row's vectors, four values a store that its neighbours' follow: a bf16 vector's
+    // eight would be two stores with gaps between the lanes, so a pair of lanes exchanges halves first.
+    template <typename Fn>
+    __device__ __forceinline__ void write(float* out, Fn f) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            asm volatile("" : "+v"(x[i].x), "+v"(x[i].y), "+v"(x[i].z), "+v"(x[i].w));
+            put(x[i], i * kProbThreads + (int)threadIdx.x, out, f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        for (int j = NR * kProbThreads + threadIdx.x; (j & ~1) < body; j += kProbThreads)   // pairs of lanes stay together
+            put(ld16(base + (int64_t)min(j, body - 1) * 16), j, out, f);
+    }
+    template <typename Fn>
+    __device__ __forceinline__ void put(const uint4& u, int j, float* out, Fn f) const {
+        float y[NP];
+        unpack(u, y);
+#pragma unroll
+        for (int e = 0; e < NP; e += 4) f(y + e);
+        if constexpr (!BF) {
+            if (j < body) *reinterpret_cast<float4*>(out + head + (int64_t)j * 4) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+            const bool odd = threadIdx.x & 1;
+            const int first = j & ~1;   // the pair's
+            auto other = [](float v) {   // lane ^ 1's
+                return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0xb1, 0xf, 0xf, true));
+            };
+            float a[4], b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float low = other(y[e]), high = other(y[4 + e]);
+                a[e] = odd ? high : y[e];
+                b[e] = odd ? y[4 + e] : low;
+            }
+            float* p = out + head + (int64_t)first * 8 + (odd ? 4 : 0);
+            if (first < body) *reinterpret_cast<float4*>(p) = make_float4(a[0], a[1], a[2], a[3]);
+            if (first + 1 < body) *reinterpret_cast<float4*>(p + 8) = make_float4(b[0], b[1], b[2], b[3]);
         }
     }
 };
 
-// exp((l - m) / T) as 2^((l - m) log2(e) / T): the difference is rounded once, the factor is held in two parts
+// exp((l - m) / T) as 2^((l - m) f), f = log2(e) / T in two parts: the difference and the product are rounded, once each.
+// The first part is below f, so that -inf times the second is -inf too, and its power 0.
 struct ProbVal {
-    float m, hi, lo, least;
+    float m, hi, lo;
     __device__ __forceinline__ ProbVal(float m, double temperature) : m(m) {
         const double f = 1.4426950408889634 / temperature;
         hi = (float)f;
+        if ((double)hi >= f) hi = __uint_as_float(__float_as_uint(hi) - 1);
         lo = (float)(f - (double)hi);
-        least = -200.f / hi;   // 2^-200 is 0; -inf is no number to multiply
     }
     __device__ __forceinline__ float operator()(float x) const {
-        const float d = fmaxf(x - m, least), y = d * hi;
-        return exp2_fast(y) * fmaf(kLn2, fmaf(d, lo, fmaf(d, hi, -y)), 1.f);
+        const float d = x - m;
+        return exp2_fast(fmaf(d, hi, d * lo));
     }
 };
 
@@ -288,7 +328,7 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
     row.load(logits, i0, V);
     float own = row.edge;   // this thread's maximum
     bool nan = row.edge != row.edge;
-    row.template each<false>([&](const float* y, int64_t) {
+    row.template each<false>([&](const float* y) {
         own = fmaxf(fmaxf(fmaxf(own, y[0]), fmaxf(y[1], y[2])), y[3]);
         nan |= __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]);
         asm volatile("" : "+v"(own));
@@ -314,7 +354,7 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
                 if (at < kProbList) keys[at] = order_key(x);
             }
         };
-        row.template each<false>([&](const float* y, int64_t) {
+        row.template each<false>([&](const float* y) {
             if (fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= t) list(y[0]), list(y[1]), list(y[2]), list(y[3]);
         });
         list(row.edge);
@@ -332,7 +372,7 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t t2 = key | (1u << bit);
                 int c = order_key(row.edge) >= t2;
-                row.template each<true>([&](const float* y, int64_t) {
+                row.template each<true>([&](const float* y) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) c += order_key(y[e]) >= t2;
                     asm volatile("" : "+v"(c));
@@ -344,7 +384,7 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
     }
     const ProbVal val(m, temperature);
     float s = row.edge >= least ? val(row.edge) : 0.f;
-    row.template each<false>([&](const float* y, int64_t) {
+    row.template each<false>([&](const float* y) {
         if (TOP && !(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) return;
 #pragma unroll
         for (int e = 0; e < 4; ++e) s += !TOP || y[e] >= least ? val(y[e]) : 0.f;
@@ -352,13 +392,13 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
     });
     s = block_reduce<JoinSum>(s, shf);
     const float inv = 1.f / s;
-    row.template each<false>([&](const float* y, int64_t v) {
-        float z[4] = {0.f, 0.f, 0.f, 0.f};
-        if (!TOP || fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = !TOP || y[e] >= least ? val(y[e]) * inv : 0.f;
+    row.write(out, [&](float* y) {
+        if (TOP && !(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) {
+            y[0] = y[1] = y[2] = y[3] = 0.f;
+            return;
         }
-        if (v >= 0) *reinterpret_cast<float4*>(out + v) = make_float4(z[0], z[1], z[2], z[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = !TOP || y[e] >= least ? val(y[e]) * inv : 0.f;
     });
     if (row.edge_at >= 0) out[row.edge_at] = row.edge >= least ? val(row.edge) * inv : 0.f;
 }

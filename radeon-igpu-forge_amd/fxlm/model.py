@@ -19,10 +19,11 @@ from torch import nn
 from fxgpu.abi import host
 from fxgpu.fused_linear import FEW_ROWS, fused_linear, fused_mlp, linear, linear_ex
 
-from .attention import decode_attention, flash_attention_qkv
+from .attention import decode_attention, flash_attention_qkv, tree_attention
 from .cross_entropy import linear_cross_entropy
 from .embedding import token_embedding
 from .norm import add_pre_norm, pre_norm, rms_norm
+from .speculative import compact_cache, sampling_probs, verify_draft
 
 
 @dataclass
@@ -149,6 +150,24 @@ class Block(nn.Module):
         x = x + self._lin(y.reshape(B, 1, D), self.proj)
         return self._mlp(x)
 
+    def tree_step(self, x, kv, ctx, tree, first):
+        """The tokens of a drafted tree, x (B, N, D) at nodes first .. first + N - 1: step() with
+        tree_attention over the cache and the tree; the tree's keys and values go into the
+        caches' rows behind ctx."""
+        B, N, D = x.shape
+        fused = self._fused_step(B * N)
+        if fused:
+            qkv = linear_ex(x, self.qkv.weight, norm_weight=self.ln1_w, eps=self.eps)
+        else:
+            qkv = self._lin(self._norm(x, self.ln1_w), self.qkv)
+        q, k, v = qkv.view(B, N, 3, self.n_head, self.head_dim).unbind(2)
+        y = tree_attention(q, kv[0], kv[1], ctx, tree, first=first, k_new=k, v_new=v).view(B, N, D)
+        if fused:
+            x = linear_ex(y, self.proj.weight, residual=x)
+            u = linear_ex(x, self.fc.weight, norm_weight=self.ln2_w, eps=self.eps, activation="gelu_tanh")
+            return linear_ex(u, self.fc2.weight, residual=x)
+        return self._mlp(x + self._lin(y, self.proj))
+
     def _fused_step(self, rows):
         return (self.norm_impl == "fused" and self.linear_impl == "fused" and self.mlp_impl == "fused"
                 and rows <= FEW_ROWS)
@@ -249,8 +268,11 @@ class GPT(nn.Module):
 
     def init_cache(self, batch, max_len=None):
         """Per-layer (k, v) caches (batch, max_len, H, Dh) bf16 on the model's device."""
+        T = self.cfg.seq_len if max_len is None else min(int(max_len), self.cfg.seq_len)
+        return self._new_cache(batch, T)
+
+    def _new_cache(self, batch, T):
         cfg = self.cfg
-        T = cfg.seq_len if max_len is None else min(int(max_len), cfg.seq_len)
         H, Dh = cfg.n_head, cfg.d_model // cfg.n_head
         dev = self.pos_emb.device
         return [(torch.empty(batch, T, H, Dh, device=dev, dtype=torch.bfloat16),
@@ -302,6 +324,27 @@ class GPT(nn.Module):
         lens = torch.full((B,), pos + 1, dtype=torch.int32, device=tok.device)
         return self._decode(tok, cache, p, lens)
 
+    @torch.no_grad()
+    def tree_step(self, tok, depth, cache, ctx, tree, first=0):
+        """Logits (B, N, V) fp32 of the tokens tok (B, N) int64 at nodes first .. first + N - 1 of
+        drafted trees behind each sequence's ctx (B,) int32 cached tokens: tree (B, N) or (N,)
+        int64 ancestor bits (fxlm.tree_attention), depth (B, N) or (N,) a node's tokens below ctx
+        (the root's 0).  The tree's keys and values go into the caches' rows ctx + node, where
+        compact_cache takes the accepted ones from.  ctx + depth has to be a position of the
+        model (a position past them is taken as the last)."""
+        if self.cfg.attn_impl != "flash":
+            raise ValueError("cached inference needs attn_impl='flash'")
+        if tok.dim() != 2 or ctx.shape != tok.shape[:1]:
+            raise ValueError(f"tok (B, N) and ctx (B,): {tuple(tok.shape)} {tuple(ctx.shape)}")
+        B, N = tok.shape
+        pos = (ctx[:, None] + depth).clamp_(0, self.pos_emb.shape[0] - 1)
+        x = self.tok_emb(tok) + self.pos_emb[pos]
+        for blk, kv in zip(self.blocks, cache):
+            x = blk.tree_step(x, kv, ctx, tree, first)
+        if self.blocks and self.blocks[0]._fused_step(B * N):
+            return linear_ex(x, self._head_w(), norm_weight=self.lnf_w, eps=self.cfg.eps).float()
+        return self._head(self._norm_f(x)).float()
+
     def decode_graph(self, cache, batch):
         """A HIP graph of one cached step for `cache` (the launches of ~14 ops per layer
         otherwise cost more host time than the step's GPU work).  Call the returned
@@ -340,6 +383,78 @@ class GPT(nn.Module):
                 break
             logits = step(nxt[:, 0], pos) if step is not None and pos < cache[0][0].shape[1] else None
         return torch.cat(out, dim=1) if out else idx.new_zeros(B, 0)
+
+
+    @torch.no_grad()
+    def speculate(self, idx, max_new, draft, branches=(2, 2, 1), temperature=0.8, top_k=50, generator=None, proposals="sampled"):
+        """generate() with a draft model: max_new tokens after idx (B, T), distributed as
+        generate's samples, several of them a pass of this model.  `draft`, a GPT over the same
+        vocabulary, proposes a tree behind each sequence, branches[d] tokens after every node of
+        depth d ("sampled": drawn from its distribution; "likeliest": its top ones); one
+        tree_step of this model checks it (verify_draft).  T + max_new tokens have to fit both
+        models' seq_len.  Returns (B, max_new) int64."""
+        B, T = idx.shape
+        if draft.cfg.vocab_size != self.cfg.vocab_size:
+            raise ValueError(f"the draft's vocabulary ({draft.cfg.vocab_size}) is not the model's ({self.cfg.vocab_size})")
+        if proposals not in ("sampled", "likeliest"):
+            raise ValueError(f"proposals {proposals!r} not in ('sampled', 'likeliest')")
+        for m in (self, draft):
+            if T + max_new > m.cfg.seq_len:
+                raise ValueError(f"{T} + {max_new} tokens > seq_len={m.cfg.seq_len}")
+        levels, parents, depth = [range(1)], [-1], [0]
+        for d, n in enumerate(branches):
+            if n < 1 or n > self.cfg.vocab_size:
+                raise ValueError(f"branches {tuple(branches)}: at least one token and at most the vocabulary")
+            for p in levels[-1]:
+                parents += [p] * n
+                depth += [d + 1] * n
+            levels.append(range(levels[-1].stop, len(parents)))
+        N = len(parents)
+        if N > 64:
+            raise ValueError(f"branches {tuple(branches)}: a tree of {N} nodes (64 at most)")
+        if max_new < 1 or B < 1:
+            return idx.new_zeros(B, 0)
+        dev = idx.device
+        bits = [1]
+        for i in range(1, N):
+            bits.append(bits[parents[i]] | 1 << i)
+        whole = torch.tensor([b - (1 << 64) if b >> 63 else b for b in bits], device=dev)
+        parents = torch.tensor(parents, dtype=torch.int32, device=dev).expand(B, N).contiguous()
+        depth = torch.tensor(depth, dtype=torch.int32, device=dev)
+        sample = dict(temperature=max(temperature, 1e-5), top_k=top_k)
+        caches = [m._new_cache(B, T + max_new + N) for m in (self, draft)]
+        draft.prefill(idx, caches[1])
+        p = sampling_probs(self.prefill(idx, caches[0]), **sample)
+        tok = torch.zeros(B, N, dtype=torch.int64, device=dev)
+        tok[:, :1] = torch.multinomial(p, 1, generator=generator)
+        out = [[t] for t in tok[:, 0].tolist()]
+        ctx = torch.full((B,), T, dtype=torch.int32, device=dev)
+        q = torch.empty(B, N, self.cfg.vocab_size, device=dev) if proposals == "sampled" else None
+        while min(len(o) for o in out) < max_new:
+            # a finished sequence's tree is padding: nothing of it is written or moved
+            going = torch.tensor([len(o) < max_new for o in out], device=dev)
+            tree = torch.where(going[:, None], whole, 0)
+            for level, below in zip(levels, levels[1:] + [None]):
+                a, b = level.start, level.stop
+                lg = draft.tree_step(tok[:, a:b], depth[a:b], caches[1], ctx, tree[:, a:b], first=a)
+                if below is None:
+                    break    # the last level's pass is for its keys
+                n = len(below) // len(level)
+                if q is None:
+                    tok[:, below.start:below.stop] = lg.topk(n).indices.view(B, -1)
+                else:
+                    q[:, a:b] = sampling_probs(lg, **sample)
+                    tok[:, below.start:below.stop] = torch.multinomial(q[:, a:b].reshape(B * (b - a), -1), n, replacement=True,
+                                                                       generator=generator).view(B, -1)
+            p = sampling_probs(self.tree_step(tok, depth, caches[0], ctx, tree), **sample)
+            got, path, n = verify_draft(p, tok, parents, torch.rand(B, N, device=dev, generator=generator), draft_probs=q)
+            n = torch.where(going, n, 0)
+            compact_cache(caches[1], ctx, path, n)
+            ctx = compact_cache(caches[0], ctx, path, n)
+            tok[:, 0] = got.gather(1, (n.long()[:, None] - 1).clamp_min(0))[:, 0]
+            for o, row, k in zip(out, got.tolist(), n.tolist()):
+                o += row[:k]
+        return torch.tensor([o[:max_new] for o in out], dtype=torch.int64, device=dev)
 
 
 def _check_pos(pos, cache_len, positions):

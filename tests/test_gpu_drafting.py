@@ -422,3 +422,98 @@ def test_operators_in_a_row_on_another_stream_and_in_a_graph(dev):
                 assert torch.equal(a, b), seed
         x = inputs(seed)                # eager work between the replays
         assert all(torch.equal(a, b) for a, b in zip(step(x), want[seed]))
+
+
+# ---- the model's steps -----------------------------------------------------------------------
+
+
+def _model(dev, seed=0, seq_len=160, n_layer=2, **kw):
+    from fxlm.model import GPT, GPTConfig
+    torch.manual_seed(seed)
+    m = GPT(GPTConfig(vocab_size=256, seq_len=seq_len, n_layer=n_layer, n_head=2, d_model=128, **kw)).to(dev).bfloat16().eval()
+    for blk in m.blocks:
+        torch.nn.init.normal_(blk.proj.weight, std=0.05)
+        torch.nn.init.normal_(blk.fc2.weight, std=0.05)
+    return m
+
+
+@pytest.mark.parametrize("B,kw", [(2, {}), (9, {}), (2, dict(norm_impl="torch", mlp_impl="torch", linear_impl="torch"))])
+def test_tree_step_logits_are_the_full_forwards(dev, B, kw):
+    # every node of a tree against a full forward over its own prefix (9 x 8 rows: past the few-row kernels);
+    # the bound of the cached step's test
+    m = _model(dev, **kw)
+    g = torch.Generator(device=dev).manual_seed(3)
+    T, parents = 37, [-1, 0, 0, 1, 1, 2, 4, 6]
+    N, depth = len(parents), [0, 1, 1, 2, 2, 2, 3, 4]
+    idx = torch.randint(0, 256, (B, T), device=dev, generator=g)
+    tok = torch.randint(0, 256, (B, N), device=dev, generator=g)
+    cache = m._new_cache(B, T + N)
+    m.prefill(idx, cache)
+    ctx = torch.full((B,), T, dtype=torch.int32, device=dev)
+    bits, dep = od.ancestors(parents).to(dev), torch.tensor(depth, device=dev)
+    lg = m.tree_step(tok, dep, cache, ctx, bits)
+    again = m._new_cache(B, T + N)
+    m.prefill(idx, again)
+    parts = [m.tree_step(tok[:, a:b], dep[a:b], again, ctx, bits[a:b], first=a) for a, b in ((0, 1), (1, 3), (3, 6), (6, 8))]
+    with torch.no_grad():
+        for i in range(N):
+            chain = []
+            j = i
+            while j >= 0:
+                chain.append(j)
+                j = parents[j]
+            ref = m(torch.cat([idx, tok[:, chain[::-1]]], 1))[:, -1].float()
+            scale = max(1.0, float(ref.abs().max()))
+            assert float((lg[:, i] - ref).abs().max()) <= 3e-2 * scale
+            assert float((torch.cat(parts, 1)[:, i] - ref).abs().max()) <= 3e-2 * scale
+
+
+@pytest.mark.parametrize("proposals,branches", [("sampled", (2, 2, 1)), ("likeliest", (3, 1)), ("sampled", (1, 1, 1, 1))])
+def test_speculate_greedy_is_the_models_own(dev, proposals, branches):
+    # top_k = 1: whatever the draft proposes, each token is the model's own choice within the rounding of its logits
+    m, d = _model(dev, n_layer=3), _model(dev, seed=5, n_layer=1)
+    g = torch.Generator(device=dev).manual_seed(6)
+    idx = torch.randint(0, 256, (3, 20), device=dev, generator=g)
+    for draft in (d, m):
+        out = m.speculate(idx, 33, draft, branches=branches, temperature=1.0, top_k=1, generator=g, proposals=proposals)
+        assert out.shape == (3, 33) and out.dtype == torch.int64
+        x = torch.cat([idx, out], 1)
+        with torch.no_grad():
+            lg = m(x[:, :-1])[:, 19:].float()
+        gap = lg.max(-1).values - lg.gather(2, out[:, :, None])[:, :, 0]
+        assert bool((gap <= 3e-2 * lg.abs().amax(-1).clamp_min(1.0)).all())
+
+
+def test_speculate_samples_as_generate_does(dev):
+    # the second token's law over 6,000 sequences of one prompt, against the model's own probabilities given
+    # the first: 5 standard deviations
+    m, d = _model(dev, n_layer=1, seq_len=16), _model(dev, seed=5, n_layer=1, seq_len=16)
+    g = torch.Generator(device=dev).manual_seed(8)
+    B = 6000
+    idx = torch.randint(0, 256, (1, 5), device=dev, generator=g).expand(B, -1).contiguous()
+    out = m.speculate(idx, 3, d, branches=(2, 1), temperature=0.9, top_k=4, generator=g)
+    assert out.shape == (B, 3) and int(out.min()) >= 0
+    first, count = out[:, 0].unique(return_counts=True)
+    x = first[count.argmax()]
+    rows = out[out[:, 0] == x]
+    with torch.no_grad():
+        p = od.sampling_probs(m(torch.cat([idx[:1], x.view(1, 1)], 1))[0, -1].float().cpu(), 0.9, 4)
+    f = torch.bincount(rows[:, 1].cpu(), minlength=256).double() / len(rows)
+    # the logits of a batched bf16 pass differ by roundings: 2 % of a probability besides
+    assert ((f - p).abs() <= 5 * (p * (1 - p) / len(rows)).sqrt() + 0.02 * p).all()
+    assert set(f.nonzero()[:, 0].tolist()) <= set((p > 0).nonzero()[:, 0].tolist())
+
+
+def test_speculate_ends_and_refuses(dev):
+    m, d = _model(dev, seq_len=40), _model(dev, seed=2, seq_len=40, n_layer=1)
+    idx = torch.randint(0, 256, (2, 30), device=dev)
+    g = torch.Generator(device=dev).manual_seed(1)
+    for n in (0, 1, 2, 10):          # 10: to the last position
+        out = m.speculate(idx, n, d, generator=g)
+        assert out.shape == (2, n) and (n == 0 or 0 <= int(out.min()) <= int(out.max()) < 256)
+    for kw in ({"max_new": 11}, {"branches": (4, 4, 3)}, {"branches": (0,)}, {"proposals": "best"}):
+        with pytest.raises(ValueError):
+            m.speculate(idx, **{"max_new": 4, "draft": d, **kw})
+    with pytest.raises(ValueError):
+        m.tree_step(idx[:, 0], torch.zeros(1, dtype=torch.int32, device=dev), m._new_cache(2, 40), torch.zeros(2, dtype=torch.int32, device=dev),
+                    torch.ones(1, dtype=torch.int64, device=dev))
