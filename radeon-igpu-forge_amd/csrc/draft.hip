@@ -446,14 +446,15 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
 // row by its running sum.  Sums and tests are in 64 bits: the tokens do not hang on a summation order.
 
 //
-// One workgroup a sequence; bound by what one CU takes from the caches (64 bytes a cycle), so rows are read in 16-byte
-// vectors, several in flight.  The draw halves nothing: the row's sum is taken in 16 regions, a wave each, then
-// the region that the running sum passes `at` in by itself, down to what one wave scans.
+// One workgroup a sequence; bound by what one CU takes from the caches (64 bytes a cycle) and by its latency, so rows are
+// read in 16-byte vectors, several in flight and the next ones behind them.  The draw: the row's sum is taken in
+// 16 regions, a wave each, then the region that the running sum passes the drawn point in by itself, down to
+// what one wave scans.
 
 constexpr int kVerNodes = 64;
 constexpr int64_t kVerMaxV = 1 << 20;
 constexpr int kVerScan = 512;   // values that a wave scans
-constexpr int kVerVecs = 4;     // 16-byte vectors of each row in flight a thread
+constexpr int kVerVecs = 4;     // 16-byte vectors of each row that a thread has in flight, twice
 
 // what rejections leave of a row: p, or max(p - c q, 0), or p without the dropped tokens
 struct Left {
@@ -461,47 +462,97 @@ struct Left {
     const int64_t* tok;   // the nodes' tokens (LDS)
     uint64_t drop;        // nodes whose tokens are out (no draft rows)
     double c;
-    int64_t V;
-    int off;              // values of the row's first 16-byte vector before the row
+    int V;
+    int off;              // values of the row's first 16-byte vector that lie before the row: vector i has values 4 i - off ..
 
-    __device__ __forceinline__ double weigh(float x, float y, int64_t v) const {
-        if (q) return fmax((double)x - c * (double)y, 0.0);
+    __device__ __forceinline__ void row(const float* probs, const float* draft, int64_t at) {
+        p = probs + at;
+        q = draft ? draft + at : nullptr;
+        drop = 0;
+        c = 0.0;
+        off = (int)(at & 3);
+    }
+    __device__ __forceinline__ int vectors() const { return (V + off + 3) / 4; }
+    __device__ __forceinline__ double at(int v) const {
+        if (v < 0 || v >= V) return 0.0;
+        if (q) return fmax(fma(-c, (double)q[v], (double)p[v]), 0.0);
         for (uint64_t d = drop; d; d &= d - 1)
             if (tok[__ffsll((unsigned long long)d) - 1] == v) return 0.0;
-        return (double)fmaxf(x, 0.f);
+        return (double)fmaxf(p[v], 0.f);
     }
-    __device__ __forceinline__ double at(int64_t v) const { return v < 0 || v >= V ? 0.0 : weigh(p[v], q ? q[v] : 0.f, v); }
-    // a thread's share of the sum over vectors [lo, hi) (vector i: values 4 i - off ...), threads `stride` apart
-    __device__ __forceinline__ double sum(int64_t lo, int64_t hi, int first, int stride) const {
+    template <bool Q>
+    __device__ __forceinline__ double four(const float4& x, const float4& y, int i) const {
+        if constexpr (Q) {
+            return (fmax(fma(-c, (double)y.x, (double)x.x), 0.0) + fmax(fma(-c, (double)y.y, (double)x.y), 0.0)) +
+                   (fmax(fma(-c, (double)y.z, (double)x.z), 0.0) + fmax(fma(-c, (double)y.w, (double)x.w), 0.0));
+        } else {
+            float z[4] = {fmaxf(x.x, 0.f), fmaxf(x.y, 0.f), fmaxf(x.z, 0.f), fmaxf(x.w, 0.f)};
+            for (uint64_t d = drop; d; d &= d - 1) {
+                const int64_t e = tok[__ffsll((unsigned long long)d) - 1] - (4 * (int64_t)i - off);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (e == k) z[k] = 0.f;
+            }
+            return ((double)z[0] + (double)z[1]) + ((double)z[2] + (double)z[3]);
+        }
+    }
+    // thread `first` of `stride`'s share of the sum over vectors [lo, hi)
+    template <bool Q>
+    __device__ __forceinline__ double share(int lo, int hi, int first, int stride) const {
+        const float4* p4 = reinterpret_cast<const float4*>(p - off);
+        const float4* q4 = reinterpret_cast<const float4*>((Q ? q : p) - off);
         double s = 0.0;
-        int64_t i = lo + first;
-        for (; i < hi; i += (int64_t)kVerVecs * stride) {
-            float4 x[kVerVecs], y[kVerVecs];
+        // the row's ragged vectors, value by value
+        const int whole = (V + off) / 4;   // vectors from here on end behind the row
+        if (first == 0) {
+            if (lo == 0 && off && hi > 0)
+                for (int e = 0; e < 4; ++e) s += at(e - off);
+            if (hi > whole && whole >= lo && (whole > 0 || !off))
+                for (int e = 0; e < 4; ++e) s += at(4 * whole - off + e);
+        }
+        if (lo == 0 && off) lo = 1;
+        hi = min(hi, whole);
+        float4 x[kVerVecs], y[kVerVecs];
+        const int step = kVerVecs * stride, turns = hi > lo ? (hi - lo) / step : 0;   // of whole steps, the same for every thread
+        int i = lo + first;
+        if (turns > 0) {
 #pragma unroll
             for (int u = 0; u < kVerVecs; ++u) {
-                const int64_t j = i + (int64_t)u * stride, v = 4 * j - off;
-                x[u] = y[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (j >= hi) continue;
-                if (v >= 0 && v + 4 <= V) {
-                    x[u] = *reinterpret_cast<const float4*>(p + v);
-                    if (q) y[u] = *reinterpret_cast<const float4*>(q + v);
-                } else {   // a ragged end
-                    float* xe = &x[u].x;
-                    float* ye = &y[u].x;
+                x[u] = p4[i + u * stride];
+                if constexpr (Q) y[u] = q4[i + u * stride];
+            }
+            for (int t = 1; t < turns; ++t, i += step) {
+                float4 nx[kVerVecs], ny[kVerVecs];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (v + e >= 0 && v + e < V) xe[e] = p[v + e], ye[e] = q ? q[v + e] : 0.f;
+                for (int u = 0; u < kVerVecs; ++u) {
+                    nx[u] = p4[i + step + u * stride];
+                    if constexpr (Q) ny[u] = q4[i + step + u * stride];
+                }
+#pragma unroll
+                for (int u = 0; u < kVerVecs; ++u) {
+                    s += four<Q>(x[u], y[u], i + u * stride);
+                    x[u] = nx[u];
+                    if constexpr (Q) y[u] = ny[u];
                 }
             }
 #pragma unroll
-            for (int u = 0; u < kVerVecs; ++u) {
-                const int64_t v = 4 * (i + (int64_t)u * stride) - off;
-                s += weigh(x[u].x, y[u].x, v) + weigh(x[u].y, y[u].y, v + 1) + weigh(x[u].z, y[u].z, v + 2) + weigh(x[u].w, y[u].w, v + 3);
-            }
+            for (int u = 0; u < kVerVecs; ++u) s += four<Q>(x[u], y[u], i + u * stride);
+            i += step;
         }
+#pragma unroll
+        for (int u = 0; u < kVerVecs; ++u) {
+            if (i + u * stride >= hi) continue;
+            x[u] = p4[i + u * stride];
+            if constexpr (Q) y[u] = q4[i + u * stride];
+        }
+#pragma unroll
+        for (int u = 0; u < kVerVecs; ++u)
+            if (i + u * stride < hi) s += four<Q>(x[u], y[u], i + u * stride);
         return s;
     }
-    __device__ __forceinline__ int64_t vectors() const { return (V + off + 3) / 4; }
+    __device__ __forceinline__ double sum(int lo, int hi, int first, int stride) const {
+        return q ? share<true>(lo, hi, first, stride) : share<false>(lo, hi, first, stride);
+    }
 };
 
 __device__ __forceinline__ double wave_sum_d(double v) {
@@ -534,7 +585,10 @@ __global__ void __launch_bounds__(kProbThreads) verify_kernel(const float* probs
     }
     __syncthreads();
 
-    Left left{P, Q, tok, 0, 0.0, V, (int)((b * N * V) & 3)};
+    Left left;
+    left.tok = tok;
+    left.V = (int)V;
+    left.row(probs, draft, b * N * V);
     int cur = 0, n = 0;
     double S = 1.0;
     bool stale = false;   // c has moved since S was formed
@@ -551,8 +605,7 @@ __global__ void __launch_bounds__(kProbThreads) verify_kernel(const float* probs
         }
         if ((double)un[i] * S * (double)qt[i] < x) {
             cur = i;
-            const int64_t at = (int64_t)i * V;
-            left = Left{P + at, Q ? Q + at : nullptr, tok, 0, 0.0, V, (int)((b * N * V + at) & 3)};
+            left.row(probs, draft, (b * N + i) * V);
             S = 1.0, stale = false;
             if (threadIdx.x == 0) spath[n + 1] = i;
             ++n;
@@ -566,12 +619,12 @@ __global__ void __launch_bounds__(kProbThreads) verify_kernel(const float* probs
     }
 
     // the last token, from what is left; from the row itself where nothing is
-    int64_t lo = 0, hi = left.vectors(), got = -1;
+    int lo = 0, hi = left.vectors(), got = -1;
     double at = 0.0, base = 0.0;   // the sum before vector lo
     bool any = true;
     for (int level = 0, round = 0;;) {
         if (level > 0 && (hi - lo) * 4 <= kVerScan) break;
-        const int64_t part = (hi - lo + kProbWaves - 1) / kProbWaves, l = lo + part * w;
+        const int part = (hi - lo + kProbWaves - 1) / kProbWaves, l = lo + part * w;
         const double s = wave_sum_d(left.sum(min(l, hi), min(l + part, hi), lane, 64));
         if (lane == 0) reg[level & 1][w] = s;   // two, in turn: one barrier a level
         __syncthreads();
@@ -604,7 +657,7 @@ __global__ void __launch_bounds__(kProbThreads) verify_kernel(const float* probs
             any = false;
             break;
         }
-        const int64_t l2 = lo + part * pick;
+        const int l2 = lo + part * pick;
         hi = min(l2 + part, hi);
         lo = l2;
         base = from;
@@ -613,7 +666,7 @@ __global__ void __launch_bounds__(kProbThreads) verify_kernel(const float* probs
     if (any && w == 0) {
         constexpr int E = kVerScan / 64;
         double x[E], sum = 0.0;
-        const int64_t v0 = 4 * lo - left.off + (int64_t)lane * E, v1 = min(V, 4 * hi - left.off);
+        const int v0 = 4 * lo - left.off + lane * E, v1 = min(left.V, 4 * hi - left.off);
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = v0 + e < v1 ? left.at(v0 + e) : 0.0, sum += x[e];
         double up = sum;

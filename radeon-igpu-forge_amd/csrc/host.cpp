@@ -14,6 +14,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <array>
 #include <initializer_list>
 #include <tuple>
 #include <vector>
@@ -468,6 +469,13 @@ bool rows16(const Tensor& t, int64_t dims) {
     return true;
 }
 
+// an expanded tensor: what is written to one place shows in others
+bool one_row_many(const Tensor& t) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.stride(i) == 0 && t.size(i) > 1) return true;
+    return false;
+}
+
 // (o, lse or None) of checked tensors, or None when a check fails
 std::optional<std::tuple<Tensor, OptT>> tree_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ctx,
                                                        const Tensor& tree, int64_t first, double scale, bool want_lse,
@@ -481,9 +489,11 @@ std::optional<std::tuple<Tensor, OptT>> tree_attention(const Tensor& q, const Te
     if (ctx.dim() != 1 || ctx.size(0) != B || ctx.scalar_type() != at::kInt || !ctx.is_cuda() || !ctx.is_contiguous() ||
         tree.dim() != 2 || tree.size(0) != B || tree.size(1) != N || tree.scalar_type() != at::kLong || !tree.is_cuda())
         return std::nullopt;
-    if (knew.has_value())
+    if (knew.has_value()) {
         for (const Tensor* t : {&*knew, &*vnew})
             if (!rows16(*t, 4) || t->size(0) != B || t->size(1) != N || t->size(2) != Hkv || t->size(3) != D) return std::nullopt;
+        if (one_row_many(k) || one_row_many(v)) return std::nullopt;
+    }
     same_gpu(q, k, v, ctx, tree, knew, vnew);
     const c10::DeviceGuard guard(q.device());   // launches and the allocations below go to q's GPU
     fx::TreeArgs a{};
@@ -553,9 +563,9 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> verify_draft(const Tensor& pro
 }
 
 // ctx + counts, or None when a check fails; the caches' rows moved in place
-OptT compact_cache(const std::vector<Tensor>& caches, const Tensor& ctx, const Tensor& path, const Tensor& counts) {
-    if (caches.empty() || path.dim() != 2 || path.size(1) < 1) return std::nullopt;
-    const Tensor& c = caches[0];
+OptT compact_cache(const std::vector<std::array<Tensor, 2>>& cache, const Tensor& ctx, const Tensor& path, const Tensor& counts) {
+    if (cache.empty() || path.dim() != 2 || path.size(1) < 1) return std::nullopt;
+    const Tensor& c = cache[0][0];
     if (c.dim() != 4) return std::nullopt;
     const int64_t B = c.size(0), T = c.size(1), H = c.size(2), D = c.size(3);
     if (B < 1 || B > 65535 || T < 1 || T > 0x7fffffff || H < 1 || D < 8 || D % 8 || H * D > 0x7fffffff || path.size(0) != B ||
@@ -565,12 +575,11 @@ OptT compact_cache(const std::vector<Tensor>& caches, const Tensor& ctx, const T
         if (t->dim() != 1 || t->size(0) != B) return std::nullopt;
     for (const Tensor* t : {&ctx, &path, &counts})
         if (t->scalar_type() != at::kInt || !t->is_cuda() || !t->is_contiguous()) return std::nullopt;
-    for (const Tensor& t : caches) {
-        if (!rows16(t, 4) || t.sizes() != c.sizes()) return std::nullopt;
-        for (int64_t i = 0; i < 3; ++i)
-            if (t.stride(i) == 0 && t.size(i) > 1) return std::nullopt;   // one row in many places
-        same_gpu(c, t);
-    }
+    for (const auto& kv : cache)
+        for (const Tensor& t : kv) {
+            if (!rows16(t, 4) || t.sizes() != c.sizes() || one_row_many(t)) return std::nullopt;
+            same_gpu(c, t);
+        }
     same_gpu(c, ctx, path, counts);
     const c10::DeviceGuard guard(c.device());
     Tensor out = at::empty({B}, ctx.options());
@@ -579,12 +588,12 @@ OptT compact_cache(const std::vector<Tensor>& caches, const Tensor& ctx, const T
     a.path = static_cast<int32_t*>(path.data_ptr());
     a.counts = static_cast<int32_t*>(counts.data_ptr());
     a.B = (int32_t)B, a.T = (int32_t)T, a.H = (int32_t)H, a.D = (int32_t)D, a.N = (int32_t)path.size(1);
-    const size_t most = std::min<size_t>(fx::kCompactTensors, 65535 / (size_t)B);
-    for (size_t i = 0; i < caches.size(); i += most) {
-        a.count = (int32_t)std::min(most, caches.size() - i);
+    const size_t total = 2 * cache.size(), most = std::min<size_t>(fx::kCompactTensors, 65535 / (size_t)B);
+    for (size_t i = 0; i < total; i += most) {
+        a.count = (int32_t)std::min(most, total - i);
         a.ctx_out = i == 0 ? static_cast<int32_t*>(out.data_ptr()) : nullptr;
         for (int32_t j = 0; j < a.count; ++j) {
-            const Tensor& t = caches[i + j];
+            const Tensor& t = cache[(i + j) / 2][(i + j) % 2];
             a.at[j] = bf(t);
             a.sb[j] = t.stride(0), a.st[j] = t.stride(1), a.sh[j] = t.stride(2);
         }

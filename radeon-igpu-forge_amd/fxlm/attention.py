@@ -217,10 +217,6 @@ def tree_attention(q, k_cache, v_cache, ctx, tree, first=0, scale=None, return_l
         scale = 1.0 / math.sqrt(q.shape[-1])
     if tree.dim() == 1:
         tree = tree.expand(q.shape[0], -1)
-    if k_new is not None:
-        for nm, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-            if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-                raise ValueError(f"{nm}: an expanded cache cannot take k_new and v_new")
     r = host.tree_attention(q, k_cache, v_cache, ctx, tree, int(first), float(scale), return_lse, k_new, v_new)
     if r is None:
         _check_tree(q, k_cache, v_cache, ctx, tree, first, k_new, v_new)
@@ -245,6 +241,9 @@ def _check_tree(q, k_cache, v_cache, ctx, tree, first, k_new, v_new):
         raise ValueError(f"{N} nodes behind {first}: a tree has 64 nodes at most")
     if (k_new is None) != (v_new is None):
         raise ValueError("k_new and v_new go together")
+    for nm, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if k_new is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{nm}: an expanded cache cannot take k_new and v_new")
     for nm, t in (("k_new", k_new), ("v_new", v_new)):
         if t is not None and tuple(t.shape) != (B, N, Hkv, Dh):
             raise ValueError(f"{nm} {tuple(t.shape)} must be (B, N, Hkv, Dh) = {(B, N, Hkv, Dh)}")

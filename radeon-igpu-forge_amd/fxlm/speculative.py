@@ -84,9 +84,9 @@ def compact_cache(cache, ctx, path, counts):
     for d < counts[b].  ctx, counts (B,) and path (B, N) int32 cuda, a path ascending
     (verify_draft's); entries outside the cache are passed over.  In place; returns ctx + counts,
     the new lengths.  Rows past them keep what they held."""
-    flat = [t for kv in cache for t in kv]
-    r = host.compact_cache(flat, ctx, path, counts)
+    r = host.compact_cache(cache, ctx, path, counts)
     if r is None:
+        flat = [t for kv in cache for t in kv]
         if not flat:
             raise ValueError("cache holds no tensors")
         s = flat[0].shape
@@ -105,5 +105,5 @@ def compact_cache(cache, ctx, path, counts):
                 raise TypeError(f"{nm} must be an int32 cuda tensor")
         if tuple(ctx.shape) != (s[0],) or tuple(counts.shape) != (s[0],) or path.dim() != 2 or path.shape[0] != s[0] or path.shape[1] < 1:
             raise ValueError(f"ctx and counts ({s[0]},), path ({s[0]}, N): {tuple(ctx.shape)} {tuple(counts.shape)} {tuple(path.shape)}")
-        r = host.compact_cache(flat, ctx.contiguous(), path.contiguous(), counts.contiguous())
+        r = host.compact_cache(cache, ctx.contiguous(), path.contiguous(), counts.contiguous())
     return r

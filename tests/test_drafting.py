@@ -98,5 +98,5 @@ def test_host_module_returns_nothing_off_the_gpu():
     assert host.tree_attention(q, k, k, c, t, 0, 0.125, True, None, None) is None
     assert host.sampling_probs(torch.zeros(2, 8), 1.0, 0) is None
     assert host.verify_draft(torch.zeros(1, 2, 8), t, t.int(), torch.zeros(1, 2), None) is None
-    assert host.compact_cache([k, k], c, t.int(), c) is None
+    assert host.compact_cache([(k, k)], c, t.int(), c) is None
     assert host.compact_cache([], c, t.int(), c) is None
