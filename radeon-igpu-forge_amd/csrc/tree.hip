@@ -32,7 +32,7 @@ constexpr float kTreeLazy = 8.f;   // the running maximum moves only past this (
 // what a kernel needs besides the arguments: units a launch aims at (0: keys are not split), the
 // fewest tiles of a unit, query row groups of a key head
 struct TreePlan {
-    int32_t units, least, groups, wq;
+    int32_t units, least, groups, wq, grid;
 };
 
 // keys of a sequence with its context `c` (as the caller gave it): its tree's rows included
@@ -87,6 +87,11 @@ struct TreeUnits {
         return false;
     }
 };
+
+// where the join finds a sequence's units: (first, count), behind the units' partials
+__device__ __forceinline__ uint2* tree_places(const TreeArgs& a, const TreePlan& p) {
+    return reinterpret_cast<uint2*>(a.work + (int64_t)p.grid * 32 * p.wq * (a.D + 2));
+}
 
 // bits of the tree's nodes that are keys: drafted before this call (below `first`), or queries of it
 // that are no padding, and inside the cache
@@ -174,6 +179,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
         hr = blockIdx.x - u * heads;
         uint32_t first;
         if (!units.find(a, u, lane, b, first, count, ctx)) return;
+        if (u == first && hr == 0 && threadIdx.x == 0) tree_places(a, plan)[b] = make_uint2(first, count);
         t0 = __builtin_amdgcn_readfirstlane((u - first) * units.tiles);
         t1 = __builtin_amdgcn_readfirstlane(t0 + units.tiles);
     }
@@ -479,16 +485,11 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, TreePlan pla
     const int G = a.H / a.Hkv, heads = plan.groups * a.Hkv;
     const int row = WPR == 1 ? blockIdx.x * 4 + w : blockIdx.x;
     if (row >= a.B * a.N * a.H) return;
-    TreeUnits units;
-    units.init(a, plan, kTreeWaves / plan.wq, lane);
     const int hq = row % a.H, bn = row / a.H, n = bn % a.N, b = bn / a.N;
-    const uint32_t count = units.count(a, a.ctx[b]);
-    if (count == 1) return;   // written by its unit
+    const uint2 place = tree_places(a, plan)[b];
     const uint64_t bits = (uint64_t)a.tree[b * a.treeb + n * a.treen];
-    uint32_t first = lane < b ? units.count(a, units.mine) : 0u;   // units of the sequences before b
-    for (int x = lane + 64; x < b; x += 64) first += units.count(a, a.ctx[x]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) first += __shfl_xor(first, off, 64);
+    const uint32_t first = place.x, count = place.y;
+    if (count == 1) return;   // written by its unit
     const int h = hq / G, rq = n * G + hq - h * G, rg = rq / (32 * plan.wq), rr = rq - rg * 32 * plan.wq;
     const int64_t per = (int64_t)32 * plan.wq * (D + 2), step = heads * per;
     const float* base = a.work + ((int64_t)first * heads + rg * a.Hkv + h) * per;
@@ -556,26 +557,24 @@ static TreePlan tree_plan(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t 
     const int wk = kTreeWaves / p.wq;
     p.least = 2 * wk;
     const int64_t tiles = (Tmax + kTreeTile - 1) / kTreeTile;
+    p.grid = (int32_t)pairs;
     if (pairs >= cus / 2 || tiles <= 4 * wk) return p;
     p.units = (int32_t)(cus - pairs);
-    return p;
-}
-
-static int64_t tree_grid(const TreePlan& p, int32_t B, int32_t Hkv) {
-    const int64_t heads = (int64_t)p.groups * Hkv;
     // sum over sequences of ceil(tiles / unit) heads <= units + B heads, in whole multiples of heads
-    return p.units == 0 ? B * heads : (p.units + B * heads) / heads * heads;
+    const int32_t heads = p.groups * Hkv;
+    p.grid = (int32_t)((p.units + pairs) / heads * heads);
+    return p;
 }
 
 int64_t tree_attention_workspace(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t Tmax, int32_t D) {
     if (B < 1 || N < 1 || Hkv < 1 || H < Hkv || H % Hkv || Tmax < 1 || (D != 64 && D != 128)) return 0;
     const TreePlan p = tree_plan(B, N, H, Hkv, Tmax);
-    return p.units == 0 ? 0 : tree_grid(p, B, Hkv) * 32 * p.wq * (D + 2) * (int64_t)sizeof(float);
+    return p.units == 0 ? 0 : (int64_t)p.grid * 32 * p.wq * (D + 2) * (int64_t)sizeof(float) + B * (int64_t)sizeof(uint2);
 }
 
 template <int D>
 static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
-    const dim3 grid((unsigned)tree_grid(p, a.B, a.Hkv)), block(kTreeThreads);
+    const dim3 grid((unsigned)p.grid), block(kTreeThreads);
     switch (p.wq) {
         case 1: hipLaunchKernelGGL((tree_attn_kernel<D, 1>), grid, block, 0, st, a, p); break;
         case 2: hipLaunchKernelGGL((tree_attn_kernel<D, 2>), grid, block, 0, st, a, p); break;
