@@ -337,6 +337,17 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
         if (threadIdx.x == 0) listed = 0;
         keys[threadIdx.x] = order_key(own);
     }
+    float s = 0.f;
+    if constexpr (!TOP) {
+        // the sum above the thread's own maximum, before the workgroup waits for the slowest of its loads
+        const ProbVal val(own == kDraftNegInf ? 0.f : own, temperature);
+        s = val(row.edge);
+        row.template each<false>([&](const float* y) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += val(y[e]);
+            asm volatile("" : "+v"(s));
+        });
+    }
     const float m = block_reduce<JoinMax>(own, shf);
     nan = __syncthreads_or(nan);
     if (no_probs(m, nan, out, V)) return;
@@ -383,13 +394,17 @@ __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits,
         }
     }
     const ProbVal val(m, temperature);
-    float s = row.edge >= least ? val(row.edge) : 0.f;
-    row.template each<false>([&](const float* y) {
-        if (TOP && !(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) return;
+    if constexpr (TOP) {
+        s = row.edge >= least ? val(row.edge) : 0.f;
+        row.template each<false>([&](const float* y) {
+            if (!(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) return;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s += !TOP || y[e] >= least ? val(y[e]) : 0.f;
-        asm volatile("" : "+v"(s));
-    });
+            for (int e = 0; e < 4; ++e) s += y[e] >= least ? val(y[e]) : 0.f;
+            asm volatile("" : "+v"(s));
+        });
+    } else {
+        s *= val(own);   // from the thread's maximum to the row's
+    }
     s = block_reduce<JoinSum>(s, shf);
     const float inv = 1.f / s;
     row.write(out, [&](float* y) {
