@@ -588,12 +588,26 @@ OptT compact_cache(const std::vector<std::array<Tensor, 2>>& cache, const Tensor
     a.path = static_cast<int32_t*>(path.data_ptr());
     a.counts = static_cast<int32_t*>(counts.data_ptr());
     a.B = (int32_t)B, a.T = (int32_t)T, a.H = (int32_t)H, a.D = (int32_t)D, a.N = (int32_t)path.size(1);
-    const size_t total = 2 * cache.size(), most = std::min<size_t>(fx::kCompactTensors, 65535 / (size_t)B);
+    // each once: layers may share a tensor, and to move a moved row again is another result
+    std::vector<const Tensor*> once;
+    once.reserve(2 * cache.size());
+    for (const auto& kv : cache)
+        for (const Tensor& t : kv) once.push_back(&t);
+    std::vector<uint16_t*> seen;
+    for (const Tensor* t : once) seen.push_back(bf(*t));
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) {
+        std::vector<const Tensor*> all;
+        all.swap(once);
+        for (const Tensor* t : all)
+            if (std::none_of(once.begin(), once.end(), [&](const Tensor* o) { return bf(*o) == bf(*t); })) once.push_back(t);
+    }
+    const size_t total = once.size(), most = std::min<size_t>(fx::kCompactTensors, 65535 / (size_t)B);
     for (size_t i = 0; i < total; i += most) {
         a.count = (int32_t)std::min(most, total - i);
         a.ctx_out = i == 0 ? static_cast<int32_t*>(out.data_ptr()) : nullptr;
         for (int32_t j = 0; j < a.count; ++j) {
-            const Tensor& t = cache[(i + j) / 2][(i + j) % 2];
+            const Tensor& t = *once[i + j];
             a.at[j] = bf(t);
             a.sb[j] = t.stride(0), a.st[j] = t.stride(1), a.sh[j] = t.stride(2);
         }

@@ -424,7 +424,7 @@ class GPT(nn.Module):
         sample = dict(temperature=max(temperature, 1e-5), top_k=top_k)
         caches = [m._new_cache(B, T + max_new + N) for m in (self, draft)]
         draft.prefill(idx, caches[1])
-        p = sampling_probs(self.prefill(idx, caches[0]), **sample)
+        p = _with_mass(sampling_probs(self.prefill(idx, caches[0]), **sample))
         tok = torch.zeros(B, N, dtype=torch.int64, device=dev)
         tok[:, :1] = torch.multinomial(p, 1, generator=generator)
         out = [[t] for t in tok[:, 0].tolist()]
@@ -443,7 +443,7 @@ class GPT(nn.Module):
                 if q is None:
                     tok[:, below.start:below.stop] = lg.topk(n).indices.view(B, -1)
                 else:
-                    q[:, a:b] = sampling_probs(lg, **sample)
+                    q[:, a:b] = _with_mass(sampling_probs(lg, **sample))
                     tok[:, below.start:below.stop] = torch.multinomial(q[:, a:b].reshape(B * (b - a), -1), n, replacement=True,
                                                                        generator=generator).view(B, -1)
             p = sampling_probs(self.tree_step(tok, depth, caches[0], ctx, tree), **sample)
@@ -453,8 +453,17 @@ class GPT(nn.Module):
             ctx = compact_cache(caches[0], ctx, path, n)
             tok[:, 0] = got.gather(1, (n.long()[:, None] - 1).clamp_min(0))[:, 0]
             for o, row, k in zip(out, got.tolist(), n.tolist()):
+                if -1 in row[:k]:
+                    raise RuntimeError("the model's logits are not finite: there is no next token to draw")
                 o += row[:k]
         return torch.tensor([o[:max_new] for o in out], dtype=torch.int64, device=dev)
+
+
+def _with_mass(p):
+    """p, probabilities that are about to be drawn from; a row of logits that were not finite has none."""
+    if not bool((p.sum(-1) > 0.5).all()):
+        raise RuntimeError("the model's logits are not finite: there is no next token to draw")
+    return p
 
 
 def _check_pos(pos, cache_len, positions):

@@ -82,8 +82,9 @@ def compact_cache(cache, ctx, path, counts):
     """Move each sequence's accepted rows together: in every tensor of cache, a list of (k, v)
     pairs (B, Tmax, Hkv, Dh) bf16 (GPT.init_cache's), row ctx[b] + path[b, d] to row ctx[b] + d
     for d < counts[b].  ctx, counts (B,) and path (B, N) int32 cuda, a path ascending
-    (verify_draft's); entries outside the cache are passed over.  In place; returns ctx + counts,
-    the new lengths.  Rows past them keep what they held."""
+    (verify_draft's); entries outside the cache are passed over.  A tensor that is in the list more
+    than once (layers that share one) is compacted once.  In place; returns ctx + counts, the new
+    lengths.  Rows past them keep what they held."""
     r = host.compact_cache(cache, ctx, path, counts)
     if r is None:
         flat = [t for kv in cache for t in kv]

@@ -359,6 +359,15 @@ def test_compact_cache_passes_over_what_is_outside(dev):
     assert torch.equal(k, k0) and torch.equal(v, k0 + 1) and got.tolist() == [2, 5]
 
 
+def test_compact_cache_moves_a_shared_tensor_once(dev):
+    from fxlm import compact_cache
+    k, v = (torch.randn(2, 20, 1, 64, device=dev).bfloat16() for _ in range(2))
+    ctx, path, n = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([3, 4], [[0, 2, 3, 7], [0, 1, 4, 5]], [4, 4]))
+    ref, _ = od.compact_cache([(k.cpu(), v.cpu())], ctx.cpu(), path.cpu(), n.cpu())
+    compact_cache([(k, v), (k, v), (v, k)], ctx, path, n)
+    assert torch.equal(k.cpu(), ref[0]) and torch.equal(v.cpu(), ref[1])
+
+
 # ---- together --------------------------------------------------------------------------------
 
 
@@ -502,6 +511,40 @@ def test_speculate_samples_as_generate_does(dev):
     # the logits of a batched bf16 pass differ by roundings: 2 % of a probability besides
     assert ((f - p).abs() <= 5 * (p * (1 - p) / len(rows)).sqrt() + 0.02 * p).all()
     assert set(f.nonzero()[:, 0].tolist()) <= set((p > 0).nonzero()[:, 0].tolist())
+
+
+def test_speculate_without_finite_logits(dev):
+    m, d = _model(dev, seq_len=40), _model(dev, seed=2, seq_len=40, n_layer=1)
+    idx = torch.randint(0, 256, (2, 30), device=dev)
+    with torch.no_grad():
+        d.lnf_w[3] = math.nan
+    with pytest.raises(RuntimeError, match="not finite"):
+        m.speculate(idx, 4, d)
+    with pytest.raises(RuntimeError, match="not finite"):
+        d.speculate(idx, 4, m)
+
+
+def test_operators_on_two_streams_at_once(dev):
+    # each call has a workspace of its own: two streams' calls, none waiting for the other, against the same calls in turn
+    from fxlm import sampling_probs, tree_attention, verify_draft
+    cases = [{n: t.to(dev) if torch.is_tensor(t) else t for n, t in _tree_case(2, 16, 4, 2, 64, 9000, [8900, 70 + s], seed=s).items()} for s in range(2)]
+    drafts = [[t.to(dev) for t in _draft_case(6, 9, 3000, 2, s, False, True)] for s in range(2)]
+
+    def calls(i):
+        c, (p, tok, par, u, q) = cases[i], drafts[i]
+        r = [tree_attention(c["q"], c["k"], c["v"], c["ctx"], c["tree"], return_lse=True, k_new=c["kn"], v_new=c["vn"]) for _ in range(8)][-1]
+        return list(r) + [sampling_probs(p * 50, 0.7, 40)] + list(verify_draft(p, tok, par, u, draft_probs=q))
+
+    want = [calls(0), calls(1)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(3):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i] = calls(i)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_speculate_ends_and_refuses(dev):
