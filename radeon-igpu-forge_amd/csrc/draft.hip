@@ -12,20 +12,26 @@ namespace fx {
 //
 // p_v = exp((l_v - m) / T) / sum over the kept u of exp((l_u - m) / T), m the row's maximum, kept: the
 // top_k largest logits and the equals of the last of them (GPT.generate's rule).  HBM-bound: a row is
-// read once and written once.  One workgroup a row, which holds the row in registers (what does
-// not fit is read again, from the caches): the maximum, the selection, the sum and the output are
-// passes over registers.
+// read once and written once.  One workgroup a row, which holds the row in registers (up to 65,536 fp32
+// or 131,072 bf16 logits; what does not fit is read again, from the caches): the maximum, the selection,
+// the sum and the output are passes over registers.  256 rows of 50,304 with top-k 50 take 23 us
+// (4.5 TB/s), a single row 12; 768 rows of 131,071 bf16, all kept, 160 us (3.8 TB/s: with one
+// workgroup a CU, its loads, sums and stores follow one another; half rows in registers and two
+// workgroups a CU, or none and four, took 160 to 183).
 //
 // The selection.  The top_k-th largest of the threads' own maxima is at most the top_k-th largest
-// logit, and few logits lie above it: those are listed, and the exact bound found among them.  Both
-// searches are one wave's, halving an interval of order-preserving integer keys until the keys at or above
-// its lower end are few enough, or top_k.  Where the list is too small for the logits above the first bound
-// (a sorted row, a thousand equals) the bound is found a bit at a time over the registers, and where
-// top_k is beyond half the threads by another kernel, eleven bits at a time: three passes that count the
-// keys of what is settled of it.
+// logit, and few logits lie above it (of random ones -1024 ln(1 - k / 1024) for the k-th of 1024 maxima): those
+// are listed, and the exact bound found among them.  Both searches are one wave's, halving an interval of
+// order-preserving integer keys until the keys at or above its lower end are few enough, or top_k.
+// Where the list is too small for the logits above the first bound (a sorted row, a thousand equals) the
+// bound is found a bit at a time over the registers.  A top_k above 3/8 of the threads, whose list
+// would near its 1024 places, goes to another kernel that finds the bound eleven bits at a time, three
+// passes over memory that count the keys of what is settled of it: 256 rows, top-k 384 30 us against 52,
+// top-k 512 105 (most lists full) against 52.
 
 constexpr int kProbThreads = 1024, kProbWaves = kProbThreads / 64;
 constexpr int kProbList = kProbThreads;   // logits of the list
+constexpr int kProbTop = kProbThreads * 3 / 8;   // the largest top_k of the list
 constexpr int kProbBins = 2048;
 constexpr float kDraftNegInf = -__builtin_huge_valf();
 
@@ -315,7 +321,7 @@ __global__ void __launch_bounds__(kProbThreads) probs_passes_kernel(const void* 
     each_logit<BF>(logits, i0, V, [&](float x, int64_t v) { out[v] = x >= least ? val(x) * inv : 0.f; });
 }
 
-// TOP: with top_k (at most half the threads), else over the whole row
+// TOP: with top_k (up to kProbTop), else over the whole row
 template <bool BF, int NR, bool TOP>
 __global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits, float* probs, int64_t V, double temperature, int top_k) {
     __shared__ float shf[kProbWaves];
@@ -424,7 +430,7 @@ static void probs_launch(const void* logits, float* probs, int64_t rows, int64_t
     const int64_t vectors = (V / NP + kProbThreads - 1) / kProbThreads;   // a thread's, of a row
     const bool top = top_k > 0 && top_k < V;
     const dim3 grid((unsigned)rows), block(kProbThreads);
-    if (top && top_k > kProbThreads / 2) {
+    if (top && top_k > kProbTop) {
         hipLaunchKernelGGL((probs_passes_kernel<BF>), grid, block, 0, st, logits, probs, V, temperature, (int)top_k);
         return;
     }
@@ -461,10 +467,14 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
 // row by its running sum.  Sums and tests are in 64 bits: the tokens do not hang on a summation order.
 
 //
-// One workgroup a sequence; bound by what one CU takes from the caches (64 bytes a cycle) and by its latency, so rows are
-// read in 16-byte vectors, several in flight and the next ones behind them.  The draw: the row's sum is taken in
-// 16 regions, a wave each, then the region that the running sum passes the drawn point in by itself, down to
-// what one wave scans.
+// One workgroup a sequence, every step of the walk in it: bound by what one CU takes from memory (about 80 GB/s here) and
+// by the walk's round trips, so rows are read in 16-byte vectors, several in flight and the next ones behind
+// them.  64 trees of 24 nodes over 131,072 ids take 70 to 80 us by the seed (two passes a sequence on
+// average, five or so in the longest walk), a chain of five over 50,304 12.  Launches that share a pass over
+// several workgroups a sequence, and walk again from the start, took longer (84 us for four such launches, 101
+// for six); 32-bit sums 71 for 77, and would let the order of a sum choose tokens.
+// The draw: the row's sum is taken in 16 regions, a wave each, then the region that the running sum passes
+// the drawn point in by itself, down to what one wave scans.
 
 constexpr int kVerNodes = 64;
 constexpr int64_t kVerMaxV = 1 << 20;
@@ -733,9 +743,11 @@ int verify_draft(const float* probs, const float* draft, const int64_t* tokens, 
 
 // ---- accepted rows together --------------------------------------------------------------
 //
-// Bound by the moved rows' bytes, read and written once.  A thread owns 16 bytes of a (tensor,
-// sequence)'s row and moves them for every d, eight rows in flight: the path ascends, so a row that is
-// written (ctx + d <= ctx + path[d]) is never one that is still to be read.
+// Bound by the moved rows' bytes, read and written once, from pages all over the caches: 60 tensors of 48
+// sequences, 112 MB, take 30 us cold (3.7 TB/s; 16 rows in flight 39, two to eight the same), a 12-layer cache's
+// 1.8 MB 4.  A thread owns 16 bytes of a (tensor, sequence)'s row and moves them for every d, eight rows in
+// flight: the path ascends, so a row that is written (ctx + d <= ctx + path[d]) is never one that is still to be
+// read.
 
 constexpr int kCompactRows = 8;
 

@@ -16,6 +16,11 @@
 // A unit's length comes from the sequences' own lengths on the device, so a long sequence among
 // short ones gets more units and the cache's size costs nothing; a second kernel joins the units
 // of a row by their maxima and sums.  See the launch shape below for when keys are not split.
+//
+// 32 nodes of 4 query heads a key head, 4 sequences of 16,001 to 32,768 keys, 8 key heads of 128: 403 MB in 98 us (95 of
+// them this kernel, 4.3 TB/s); one token over up to 65,011 keys of 16 heads of 64: 430 MB in 95 us (89, 4.8 TB/s).  Two
+// tiles a step, or a second one in flight behind it, change neither: memory bounds them.  Short contexts
+// are bounded by their chain of round trips (context, keys, sums): 225 keys of 12 heads take 7 us.
 #include <math.h>
 
 #include "fx_internal.h"
@@ -543,13 +548,16 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, TreePlan pla
 }
 
 // Launch shape.  One workgroup a CU is resident (its registers), so R = CUs of them run at once.
-// Key heads (with row groups) that fill R by themselves are not split, nor are caches of a few
-// steps of a workgroup; else the units are what R leaves over, so that all of them run at once.
+// Key heads (with row groups) that fill half of R by themselves are not split (192 of them over 8,000 keys 73 us against 76
+// split, over 500 to 8,000 keys 42 against 45; only 128 of such unlike lengths gain, 38 to 33), nor are caches of up to six
+// steps of a workgroup: 12 key heads over 1,000 keys 9.8 us against 12.3 for two launches, over 1,500 12.0 / 12.4,
+// over 2,000 14.2 / 12.4; 32 over 350 keys in four row groups 15.8 / 16.1.  Else the units are what R leaves over, so
+// that all of them run at once.
 static TreePlan tree_plan(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t Tmax) {
     TreePlan p{};
     const int rows = N * (H / Hkv);
     // row groups: one workgroup's while the keys' bytes bound it (8 tiles of 32 rows at most), else of whichever
-    // size pads fewer rows
+    // size pads fewer rows (305 rows as three groups of four tiles 33 us, as two of eight 39)
     const int tiles32 = (rows + 31) / 32;
     p.wq = tiles32 == 1 ? 1 : tiles32 == 2 ? 2 : tiles32 <= 4 ? 4 : tiles32 <= 8 || (tiles32 + 3) / 4 % 2 == 0 ? 8 : 4;
     p.groups = (rows + 32 * p.wq - 1) / (32 * p.wq);
@@ -558,7 +566,7 @@ static TreePlan tree_plan(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t 
     p.least = 2 * wk;
     const int64_t tiles = (Tmax + kTreeTile - 1) / kTreeTile;
     p.grid = (int32_t)pairs;
-    if (pairs >= cus / 2 || tiles <= 4 * wk) return p;
+    if (pairs >= cus / 2 || tiles <= 6 * wk) return p;
     p.units = (int32_t)(cus - pairs);
     // sum over sequences of ceil(tiles / unit) heads <= units + B heads, in whole multiples of heads
     const int32_t heads = p.groups * Hkv;
@@ -584,7 +592,9 @@ static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
     if (int e = check_launch("tree_attention")) return e;
     if (p.units == 0) return 0;
     const int64_t rows = (int64_t)a.B * a.N * a.H;
-    if (p.units > 16 * a.B * p.groups * a.Hkv)   // over 16 units a row
+    // Over 16 units a row, four waves of them: with 255 units 26 us against 46, with 31 27.0 / 27.6; with 7 a wave a row
+    // is the better, 18 us against 25.
+    if (p.units > 16 * a.B * p.groups * a.Hkv)
         hipLaunchKernelGGL((tree_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, p);
     else
         hipLaunchKernelGGL((tree_join_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p);
