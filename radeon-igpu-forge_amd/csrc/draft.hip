@@ -472,7 +472,7 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
 // them.  64 trees of 24 nodes over 131,072 ids take 70 to 80 us by the seed (two passes a sequence on
 // average, five or so in the longest walk), a chain of five over 50,304 12.  Launches that share a pass over
 // several workgroups a sequence, and walk again from the start, took longer (84 us for four such launches, 101
-// for six); 32-bit sums 71 for 77, and would let the order of a sum choose tokens.
+// for six).
 // The draw: the row's sum is taken in 16 regions, a wave each, then the region that the running sum passes
 // the drawn point in by itself, down to what one wave scans.
 
