@@ -447,7 +447,7 @@ static void probs_launch(const void* logits, float* probs, int64_t rows, int64_t
 
 int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, int64_t V, double temperature, int64_t top_k, void* stream) {
     FX_REQUIRE(rows >= 0 && rows < 0x7fffffffLL && V >= 1 && V < 0x7fffffffLL, "sampling_probs: bad shape rows=%lld V=%lld", (long long)rows, (long long)V);
-    FX_REQUIRE(temperature > 0.f && temperature < __builtin_huge_val(), "sampling_probs: temperature %g must be positive and finite", temperature);
+    FX_REQUIRE(temperature >= 1e-30 && temperature <= 1e30, "sampling_probs: temperature %g must lie in [1e-30, 1e30]", temperature);
     if (rows == 0) return 0;
     FX_REQUIRE(logits && probs && (((uintptr_t)logits | (uintptr_t)probs) & 15) == 0, "sampling_probs: logits and probs must be 16-byte aligned");
     if (bf16) probs_launch<true>(logits, probs, rows, V, temperature, top_k, (hipStream_t)stream);

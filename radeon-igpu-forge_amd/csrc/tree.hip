@@ -548,11 +548,13 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, TreePlan pla
 }
 
 // Launch shape.  One workgroup a CU is resident (its registers), so R = CUs of them run at once.
-// Key heads (with row groups) that fill half of R by themselves are not split (192 of them over 8,000 keys 73 us against 76
-// split, over 500 to 8,000 keys 42 against 45; only 128 of such unlike lengths gain, 38 to 33), nor are caches of up to six
-// steps of a workgroup: 12 key heads over 1,000 keys 9.8 us against 12.3 for two launches, over 1,500 12.0 / 12.4,
-// over 2,000 14.2 / 12.4; 32 over 350 keys in four row groups 15.8 / 16.1.  Else the units are what R leaves over, so
-// that all of them run at once.
+// Caches of up to six steps of a workgroup are not split: 12 key heads over 1,000 keys 9.8 us against 12.3 for two
+// launches, over 1,500 12.0 / 12.4, over 2,000 14.2 / 12.4; 32 over 350 keys in four row groups 15.8 / 16.1.  Key
+// heads (with row groups) below half of R are split into units that R leaves over, so that all of them run at once.
+// More of them are split for unlike sequences alone, at twice the mean length, where a cache may hold 64 steps of a
+// workgroup or more: one sequence of 19,000 keys among 63 of 500 (8 key heads) 31 us against 81, of 60,000
+// 42 / 241, at the cost of a join that finds nothing: 192 of 18,000 keys each 162 / 159, 64 sequences
+// of 500 24 / 19.5; in caches of 8,192 rows such splits lost 3 to 11 % on mixed lengths and are not made.
 static TreePlan tree_plan(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t Tmax) {
     TreePlan p{};
     const int rows = N * (H / Hkv);
@@ -566,8 +568,10 @@ static TreePlan tree_plan(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t 
     p.least = 2 * wk;
     const int64_t tiles = (Tmax + kTreeTile - 1) / kTreeTile;
     p.grid = (int32_t)pairs;
-    if (pairs >= cus / 2 || tiles <= 6 * wk) return p;
-    p.units = (int32_t)(cus - pairs);
+    if (tiles <= 6 * wk) return p;
+    if (pairs < cus / 2) p.units = (int32_t)(cus - pairs);
+    else if (pairs <= 8 * cus && tiles >= 64 * wk) p.units = (int32_t)(pairs / 2);
+    else return p;
     // sum over sequences of ceil(tiles / unit) heads <= units + B heads, in whole multiples of heads
     const int32_t heads = p.groups * Hkv;
     p.grid = (int32_t)((p.units + pairs) / heads * heads);

@@ -221,6 +221,8 @@ def tree_attention(q, k_cache, v_cache, ctx, tree, first=0, scale=None, return_l
     if r is None:
         _check_tree(q, k_cache, v_cache, ctx, tree, first, k_new, v_new)
         r = host.tree_attention(q, k_cache, v_cache, ctx.contiguous(), tree, int(first), float(scale), return_lse, k_new, v_new)
+        if r is None:
+            raise ValueError(f"tree_attention: sizes that it does not take: {tuple(q.shape)} over {tuple(k_cache.shape)}")
     return r if return_lse else r[0]
 
 

@@ -16,12 +16,19 @@ import torch
 from fxgpu.abi import host
 
 
+def _taken(r, name):
+    """r, what the host module returned, which is None for what none of the checks names"""
+    if r is None:
+        raise ValueError(f"{name}: tensors of a layout or size that it does not take")
+    return r
+
+
 def sampling_probs(logits, temperature=1.0, top_k=0):
     """logits (..., V) fp32 or bf16 -> probabilities (..., V) fp32: softmax(logits / temperature)
     over each row's top_k largest logits and the equals of the last of them (over all for
     top_k <= 0), as GPT.generate samples.  A row of -inf gives zeros; NaN or +inf gives NaN."""
-    if not 0.0 < float(temperature) < float("inf"):
-        raise ValueError(f"temperature {temperature} must be positive and finite")
+    if not 1e-30 <= float(temperature) <= 1e30:
+        raise ValueError(f"temperature {temperature} must lie in [1e-30, 1e30]")
     r = host.sampling_probs(logits, float(temperature), int(top_k))
     if r is None:
         if logits.dtype not in (torch.float32, torch.bfloat16):
@@ -32,7 +39,7 @@ def sampling_probs(logits, temperature=1.0, top_k=0):
             raise ValueError(f"logits must be (..., V), got {tuple(logits.shape)}")
         x = logits.contiguous()   # a slice of positions, or rows at an odd address
         r = host.sampling_probs(x if x.data_ptr() % 16 == 0 else x.clone(), float(temperature), int(top_k))
-    return r
+    return _taken(r, "sampling_probs")
 
 
 def verify_draft(probs, tokens, parents, uniform, draft_probs=None):
@@ -75,7 +82,7 @@ def verify_draft(probs, tokens, parents, uniform, draft_probs=None):
         p, q = (None if t is None else t.contiguous() if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
                 for t in (probs, draft_probs))
         r = host.verify_draft(p, tokens.contiguous(), parents.contiguous(), uniform.contiguous(), q)
-    return r
+    return _taken(r, "verify_draft")
 
 
 def compact_cache(cache, ctx, path, counts):
@@ -107,4 +114,4 @@ def compact_cache(cache, ctx, path, counts):
         if tuple(ctx.shape) != (s[0],) or tuple(counts.shape) != (s[0],) or path.dim() != 2 or path.shape[0] != s[0] or path.shape[1] < 1:
             raise ValueError(f"ctx and counts ({s[0]},), path ({s[0]}, N): {tuple(ctx.shape)} {tuple(counts.shape)} {tuple(path.shape)}")
         r = host.compact_cache(cache, ctx.contiguous(), path.contiguous(), counts.contiguous())
-    return r
+    return _taken(r, "compact_cache")

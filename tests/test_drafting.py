@@ -73,7 +73,8 @@ def test_wrappers_refuse():
             pytest.fail(f"not refused: {kw} {[tuple(a.shape) for a in args]}")
     x = torch.zeros(2, 10)
     for err, args, kw in [(TypeError, (x,), {}), (TypeError, (x.half(),), {}), (ValueError, (x,), {"temperature": 0.0}),
-                          (ValueError, (x,), {"temperature": math.inf}), (ValueError, (x,), {"temperature": math.nan})]:
+                          (ValueError, (x,), {"temperature": math.inf}), (ValueError, (x,), {"temperature": math.nan}),
+                          (ValueError, (x,), {"temperature": 1e-31}), (ValueError, (x,), {"temperature": 1e31})]:
         with pytest.raises(err):
             sampling_probs(*args, **kw)
     p, tok, par, u = torch.zeros(2, 3, 10), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, 3)

@@ -75,6 +75,7 @@ def _check_tree(dev, c, new=True, o_nan_ok=False):
     (1, 64, 5, 1, 64, 2100, [1999], 0),               # 320 rows: two groups, split
     (2, 64, 8, 1, 128, 500, [77, 400], 0),            # 512 rows: two groups
     (70, 2, 1, 1, 64, 1700, [(37 * i) % 1600 for i in range(70)], 0),   # more sequences than lanes
+    (16, 17, 32, 8, 64, 4200, [40 + 9 * i for i in range(11)] + [4100, 0, 1100, 31, 7], 0),   # many key heads, split for the long one
 ])
 def test_tree_attention(dev, B, N, H, Hkv, D, T, ctx, first, new):
     for branch, ragged in ((1, False), (3, first == 0)):
@@ -237,6 +238,11 @@ def test_sampling_probs_masked_and_not_finite(dev):
         assert not p[1].any() and p[2].isnan().all() and p[3].isnan().all()
         assert float(p[4, 0]) == 1.0 and not p[4, 1:].any()
         assert ((p[5] - 1 / 5001).abs() <= 2.0 ** -20 / 5001).all()
+    # temperatures at the ends: the largest alone, and all that are not masked alike
+    p = sampling_probs(x[:1].to(dev), 1e-30).cpu()
+    assert float(p[0, x[0].argmax()]) == 1.0 and int((p > 0).sum()) == 1
+    p = sampling_probs(x[:1].to(dev), 1e30).cpu()
+    assert ((p[0, :100] - 0.01).abs() <= 2.0 ** -20 / 100).all() and not p[0, 100:].any()
     # a slice of positions, rows at an odd address
     y = torch.randn(3, 5, 1003, generator=torch.Generator().manual_seed(8)).to(dev)
     assert torch.equal(sampling_probs(y[:, -1], 0.8, 20), sampling_probs(y[:, -1].clone(), 0.8, 20))
