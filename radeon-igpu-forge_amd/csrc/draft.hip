@@ -469,10 +469,11 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
 //
 // One workgroup a sequence, every step of the walk in it: bound by what one CU takes from memory (about 80 GB/s here) and
 // by the walk's round trips, so rows are read in 16-byte vectors, several in flight and the next ones behind
-// them.  64 trees of 24 nodes over 131,072 ids take 70 to 80 us by the seed (two passes a sequence on
-// average, five or so in the longest walk), a chain of five over 50,304 12.  Launches that share a pass over
+// them.  64 trees of 24 nodes over 131,072 ids take 62 to 74 us by the seed (two passes a sequence on
+// average, five or so in the longest walk; with the draft's row read at a leaf too 74 to 78), a chain of
+// five over 50,304 12.6.  Launches that share a pass over
 // several workgroups a sequence, and walk again from the start, took longer (84 us for four such launches, 101
-// for six).
+// for six, against 70 to 80 then).
 // The draw: the row's sum is taken in 16 regions, a wave each, then the region that the running sum passes
 // the drawn point in by itself, down to what one wave scans.
 
@@ -486,7 +487,7 @@ struct Left {
     const float *p, *q;   // the rows; q null: no draft rows
     const int64_t* tok;   // the nodes' tokens (LDS)
     uint64_t drop;        // nodes whose tokens are out (no draft rows)
-    double c;
+    double c;             // zero while nothing is refused: the draft row is not read then (a leaf's may hold anything)
     int V;
     int off;              // values of the row's first 16-byte vector that lie before the row: vector i has values 4 i - off ..
 
@@ -500,7 +501,7 @@ struct Left {
     __device__ __forceinline__ int vectors() const { return (V + off + 3) / 4; }
     __device__ __forceinline__ double at(int v) const {
         if (v < 0 || v >= V) return 0.0;
-        if (q) return fmax(fma(-c, (double)q[v], (double)p[v]), 0.0);
+        if (c != 0.0) return fmax(fma(-c, (double)q[v], (double)p[v]), 0.0);
         for (uint64_t d = drop; d; d &= d - 1)
             if (tok[__ffsll((unsigned long long)d) - 1] == v) return 0.0;
         return (double)fmaxf(p[v], 0.f);
@@ -576,7 +577,7 @@ struct Left {
         return s;
     }
     __device__ __forceinline__ double sum(int lo, int hi, int first, int stride) const {
-        return q ? share<true>(lo, hi, first, stride) : share<false>(lo, hi, first, stride);
+        return c != 0.0 ? share<true>(lo, hi, first, stride) : share<false>(lo, hi, first, stride);
     }
 };
 

@@ -48,8 +48,9 @@ def verify_draft(probs, tokens, parents, uniform, draft_probs=None):
     probs (B, N, V) fp32: row i is the target's distribution after node i.  tokens (B, N) int64,
     parents (B, N) int32 cuda: the tree.  uniform (B, N) fp32: independent numbers of [0, 1), one
     a node (the root's draws the last token).  draft_probs (B, N, V) fp32: row i is the
-    distribution that node i's children were drawn from, independently; None: proposals without
-    one (looked up, or the likeliest), each certain of its token.  N <= 64, V <= 1,048,576.
+    distribution that node i's children were drawn from, independently (the row of a node without
+    children may hold anything); None: proposals without one (looked up, or the likeliest), each
+    certain of its token.  N <= 64, V <= 1,048,576.
 
     From the root, the children of the node that is reached are asked in their order.  One with
     token x is accepted with probability min(1, p(x) / q(x)); a refusal leaves

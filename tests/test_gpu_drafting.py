@@ -304,6 +304,20 @@ def test_verify_draft_edges(dev):
     assert (n == 1).all() and (out == -1).all() and (path[:, 0] == 0).all() and (path[:, 1:] == -1).all()
 
 
+@pytest.mark.parametrize("V", [5, 700, 20001])
+def test_verify_draft_rows_that_nothing_was_drawn_from(dev, V):
+    # a leaf's draft row is nobody's distribution: whatever it holds, the last token comes from the target's row
+    p, tok, par, u, q = _draft_case(24, 9, V, 2, 3, False, True)
+    q = (q + 3 * p) / 4              # near the target: walks that reach the leaves
+    leaf = torch.ones(24, 9, dtype=torch.bool)
+    leaf.scatter_(1, par.clamp_min(0).long(), False)
+    for bad in (math.nan, math.inf, -math.inf, 1e38):
+        q[leaf] = bad
+        _, path, n = _check_verify(dev, p, tok, par, u, q)
+        end = path.cpu().gather(1, n.cpu().long()[:, None] - 1)[:, 0].long()
+        assert bool(leaf[torch.arange(24), end].any())
+
+
 def test_verified_tokens_are_distributed_as_the_target(dev):
     # 200,000 sequences, 5 standard deviations: the first token, and the second after each first
     from fxlm import verify_draft
