@@ -331,14 +331,15 @@ class GPT(nn.Module):
         int64 ancestor bits (fxlm.tree_attention), depth (B, N) or (N,) a node's tokens below ctx
         (the root's 0).  The tree's keys and values go into the caches' rows ctx + node, where
         compact_cache takes the accepted ones from.  ctx + depth has to be a position of the
-        model (a position past them is taken as the last)."""
+        model (a position past them is taken as the last); a padding node's token may be anything
+        (what is no id is looked up as the nearest)."""
         if self.cfg.attn_impl != "flash":
             raise ValueError("cached inference needs attn_impl='flash'")
         if tok.dim() != 2 or ctx.shape != tok.shape[:1]:
             raise ValueError(f"tok (B, N) and ctx (B,): {tuple(tok.shape)} {tuple(ctx.shape)}")
         B, N = tok.shape
         pos = (ctx[:, None] + depth).clamp_(0, self.pos_emb.shape[0] - 1)
-        x = self.tok_emb(tok) + self.pos_emb[pos]
+        x = self.tok_emb(tok.clamp(0, self.tok_emb.num_embeddings - 1)) + self.pos_emb[pos]
         for blk, kv in zip(self.blocks, cache):
             x = blk.tree_step(x, kv, ctx, tree, first)
         if self.blocks and self.blocks[0]._fused_step(B * N):

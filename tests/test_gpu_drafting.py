@@ -497,6 +497,23 @@ def test_tree_step_logits_are_the_full_forwards(dev, B, kw):
             assert float((torch.cat(parts, 1)[:, i] - ref).abs().max()) <= 3e-2 * scale
 
 
+def test_tree_step_of_padding_with_tokens_that_are_no_ids(dev):
+    # what verify_draft returns behind the last token is -1: nodes that are padding, and no node sees them
+    m = _model(dev)
+    idx = torch.randint(0, 256, (2, 11), device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+    ctx = torch.full((2,), 11, dtype=torch.int32, device=dev)
+    dep = torch.tensor([0, 1, 2, 2, 1], dtype=torch.int32, device=dev)
+    bits = od.ancestors([-1, 0, 1, -1, -1]).to(dev)
+    res = []
+    for t3, t4 in ((7, 9), (-1, 256), (2 ** 62, -2 ** 62)):
+        cache = m._new_cache(2, 20)
+        m.prefill(idx, cache)
+        tok = torch.tensor([[1, 2, 3, t3, t4]] * 2, device=dev)
+        res.append((m.tree_step(tok, dep, cache, ctx, bits)[:, :3], [t[:, :14].clone() for kv in cache for t in kv]))
+    for lg, rows in res[1:]:
+        assert torch.equal(lg, res[0][0]) and all(torch.equal(a, b) for a, b in zip(rows, res[0][1]))
+
+
 @pytest.mark.parametrize("proposals,branches", [("sampled", (2, 2, 1)), ("likeliest", (3, 1)), ("sampled", (1, 1, 1, 1))])
 def test_speculate_greedy_is_the_models_own(dev, proposals, branches):
     # top_k = 1: whatever the draft proposes, each token is the model's own choice within the rounding of its logits
