@@ -450,8 +450,14 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
     FX_REQUIRE(temperature >= 1e-30 && temperature <= 1e30, "sampling_probs: temperature %g must lie in [1e-30, 1e30]", temperature);
     if (rows == 0) return 0;
     FX_REQUIRE(logits && probs && (((uintptr_t)logits | (uintptr_t)probs) & 15) == 0, "sampling_probs: logits and probs must be 16-byte aligned");
-    if (bf16) probs_launch<true>(logits, probs, rows, V, temperature, top_k, (hipStream_t)stream);
-    else probs_launch<false>(logits, probs, rows, V, temperature, top_k, (hipStream_t)stream);
+    // a launch has less than 2^32 work items; a multiple of 8 rows keeps the alignment
+    constexpr int64_t most = (1ll << 31) / kProbThreads;
+    for (int64_t r = 0; r < rows; r += most) {
+        const int64_t n = rows - r < most ? rows - r : most;
+        const char* x = static_cast<const char*>(logits) + r * V * (bf16 ? 2 : 4);
+        if (bf16) probs_launch<true>(x, probs + r * V, n, V, temperature, top_k, (hipStream_t)stream);
+        else probs_launch<false>(x, probs + r * V, n, V, temperature, top_k, (hipStream_t)stream);
+    }
     return check_launch("sampling_probs");
 }
 
@@ -734,6 +740,7 @@ int verify_draft(const float* probs, const float* draft, const int64_t* tokens, 
                  int64_t* out, int32_t* path, int32_t* counts, int32_t B, int32_t N, int64_t V, void* stream) {
     FX_REQUIRE(B >= 0 && N >= 1 && N <= kVerNodes && V >= 1 && V <= kVerMaxV, "verify_draft: bad shape B=%d N=%d (up to %d) V=%lld (up to %lld)",
                B, N, kVerNodes, (long long)V, (long long)kVerMaxV);
+    FX_REQUIRE(B <= 0xffffffffu / kProbThreads, "verify_draft: grid too large (B=%d)", B);
     if (B == 0) return 0;
     FX_REQUIRE(probs && tokens && parents && uniform && out && path && counts, "verify_draft: null pointer");
     FX_REQUIRE((((uintptr_t)probs | (uintptr_t)draft) & 15) == 0, "verify_draft: probs and draft_probs must be 16-byte aligned");

@@ -620,8 +620,9 @@ int tree_attention(const TreeArgs& a, void* stream) {
                  (uintptr_t)a.vnew) & 15) == 0,
                "tree_attention: q, k, v, o, work, knew and vnew must be 16-byte aligned");
     const TreePlan p = tree_plan(a.B, a.N, a.H, a.Hkv, a.Tmax);
-    const int64_t tiles = (int64_t)a.B * p.groups * a.Hkv * ((a.Tmax + kTreeTile - 1) / kTreeTile);
-    FX_REQUIRE(tiles < 0x7fffffffLL && (int64_t)a.B * a.N * a.H < 0x7fffffffLL, "tree_attention: grid too large");
+    const int64_t pairs = (int64_t)a.B * p.groups * a.Hkv, tiles = pairs * ((a.Tmax + kTreeTile - 1) / kTreeTile);
+    FX_REQUIRE(tiles < 0x7fffffffLL && (int64_t)a.B * a.N * a.H < 0x7fffffffLL && pairs <= 0xffffffffu / kTreeThreads,
+               "tree_attention: grid too large");   // a launch has less than 2^32 work items (units are made of few pairs alone)
     FX_REQUIRE(p.units == 0 || a.work, "tree_attention: null workspace");
     return a.D == 64 ? tree_launch<64>(a, p, (hipStream_t)stream) : tree_launch<128>(a, p, (hipStream_t)stream);
 }

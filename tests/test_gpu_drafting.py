@@ -251,6 +251,31 @@ def test_sampling_probs_masked_and_not_finite(dev):
     assert sampling_probs(y[:0]).shape == (0, 5, 1003)
 
 
+def test_sampling_probs_of_more_rows_than_a_launch_has(dev):
+    from fxlm import sampling_probs
+    n = 2 ** 22 + 13                 # workgroups of 1,024 threads: past 2^32 work items
+    x = torch.randn(16, 5, generator=torch.Generator().manual_seed(3))
+    for dtype in (torch.float32, torch.bfloat16):
+        r = x.to(dtype).to(dev)
+        want = sampling_probs(r, 0.7, 3)
+        got = sampling_probs(r.repeat(n // 16 + 1, 1)[:n].contiguous(), 0.7, 3)
+        assert torch.equal(got[:n // 16 * 16].view(-1, 16, 5), want.expand(n // 16, 16, 5)) and torch.equal(got[n // 16 * 16:], want[:n % 16])
+
+
+def test_batches_past_a_launch_are_refused(dev):
+    from fxlm import tree_attention, verify_draft
+    n = 2 ** 22
+    one = torch.ones(n, 1, 1, device=dev)
+    zero = torch.zeros(n, 1, dtype=torch.int64, device=dev)
+    with pytest.raises(ValueError, match="grid too large"):
+        verify_draft(one, zero, zero.int() - 1, one[..., 0] * 0)
+    B = 2 ** 17                      # 64 key heads each: 2^23 workgroups of 512 threads
+    q = torch.zeros(1, 1, 64, 64, dtype=torch.bfloat16, device=dev).expand(B, -1, -1, -1)
+    kv = torch.zeros(1, 1, 64, 64, dtype=torch.bfloat16, device=dev).expand(B, -1, -1, -1)
+    with pytest.raises(ValueError, match="grid too large"):
+        tree_attention(q, kv, kv, torch.zeros(B, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int64, device=dev))
+
+
 # ---- verification ----------------------------------------------------------------------------
 
 
