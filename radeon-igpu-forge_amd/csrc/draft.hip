@@ -15,9 +15,15 @@ namespace fx {
 // read once and written once.  One workgroup a row, which holds the row in registers (up to 65,536 fp32
 // or 131,072 bf16 logits; what does not fit is read again, from the caches): the maximum, the selection,
 // the sum and the output are passes over registers.  256 rows of 50,304 with top-k 50 take 23 us
-// (4.5 TB/s), a single row 12; 768 rows of 131,071 bf16, all kept, 160 us (3.8 TB/s: with one
-// workgroup a CU, its loads, sums and stores follow one another; half rows in registers and two
-// workgroups a CU, or none and four, took 160 to 183).
+// (4.5 TB/s), a single row 12; 768 rows of 131,071 bf16, all kept, 150 us (4.0 TB/s; half rows in
+// registers and two workgroups a CU, or none and four, took 160 to 183).
+//
+// Rows of up to four vectors a thread leave room for two workgroups a CU (64 registers: 2,000 rows of 16,384
+// fp32 with top-k 50 58 us against 90 with 66), and one's loads run beside the other's stores.  Longer rows
+// are a workgroup's alone, so there it walks over several: a vector's registers take the next row's as
+// soon as it is stored.  Against a workgroup for each row: 2,000 rows of 24,576 fp32 83 us / 92, 768 of
+// 50,176 60 / 71, of 61,440 82 / 89, 768 bf16 rows of 131,071 150 / 160 (300 rows of 122,880 69 / 68);
+// below eight vectors it would be the slower, by the registers it takes (2,000 of 16,384 56 / 48).
 //
 // The selection.  The top_k-th largest of the threads' own maxima is at most the top_k-th largest
 // logit, and few logits lie above it (of random ones -1024 ln(1 - k / 1024) for the k-th of 1024 maxima): those
@@ -33,6 +39,7 @@ constexpr int kProbThreads = 1024, kProbWaves = kProbThreads / 64;
 constexpr int kProbList = kProbThreads;   // logits of the list
 constexpr int kProbTop = kProbThreads * 3 / 8;   // the largest top_k of the list
 constexpr int kProbBins = 2048;
+constexpr int kProbStream = 8;   // vectors a thread from which on a workgroup walks over rows
 constexpr float kDraftNegInf = -__builtin_huge_valf();
 
 // a logit's bits in an order that unsigned comparison keeps, both zeros alike, and the logit of such a key
@@ -168,39 +175,58 @@ __device__ __forceinline__ uint32_t radix_bound(const void* logits, int64_t i0, 
     return key;
 }
 
-// V logits from flat index i0 of a 16-byte aligned tensor, as the threads of a workgroup hold them: NR 16-byte vectors
-// each, vectors past those read again at every pass, and the row's ragged ends (fewer than two vectors'
-// values, one a thread)
-template <bool BF, int NR>
-struct LogitRow {
+// Where V logits from flat index i0 of a 16-byte aligned tensor lie: whole vectors, and the row's ragged ends (fewer than
+// two vectors' values, one a thread)
+template <bool BF>
+struct LogitPlace {
     static constexpr int NP = BF ? 8 : 4;
-    uint4 x[NR];
-    float edge;
-    int64_t edge_at;   // -1: none
     const char* base;  // the first whole vector
     int64_t head;
+    int edge_at;       // -1: none
     int body;
+    int tid;           // the thread's index
+
+    __device__ __forceinline__ void place(const void* logits, int64_t i0, int64_t V, int t) {
+        tid = t;
+        head = min(V, (32 - i0 % 32) % 32);   // the output's 128-byte lines, each a wave's own
+        body = (int)((V - head) / NP);
+        base = static_cast<const char*>(logits) + (i0 + head) * (BF ? 2 : 4);
+        const int tail = (int)head + body * NP;
+        edge_at = t < head ? t : t - head < V - tail ? tail + t - (int)head : -1;
+    }
+    // this thread's i-th vector; what lies behind the row's end is -inf: nothing counts it
+    __device__ __forceinline__ uint4 load(int i) const {
+        const uint32_t ninf = BF ? 0xff80ff80u : 0xff800000u;
+        return tid < body - i * kProbThreads ? ld16(base + (uint32_t)(tid * 16 + i * kProbThreads * 16))
+                                                          : make_uint4(ninf, ninf, ninf, ninf);
+    }
+    __device__ __forceinline__ float load_edge(const void* logits, int64_t i0) const {
+        if (edge_at < 0) return kDraftNegInf;
+        return BF ? bf16_to_f32(static_cast<const uint16_t*>(logits)[i0 + edge_at]) : static_cast<const float*>(logits)[i0 + edge_at];
+    }
+};
+
+// A row as the threads of a workgroup hold it: NR 16-byte vectors each; vectors past those are read again at every pass
+template <bool BF, int NR>
+struct LogitRow : LogitPlace<BF> {
+    using LogitPlace<BF>::NP;
+    using LogitPlace<BF>::base;
+    using LogitPlace<BF>::head;
+    using LogitPlace<BF>::edge_at;
+    using LogitPlace<BF>::body;
+    using LogitPlace<BF>::tid;
+    uint4 x[NR];
+    float edge;
 
     __device__ __forceinline__ static void unpack(const uint4& u, float* f) {
         if constexpr (BF) unpack8(u, f);
         else f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
     }
-    __device__ __forceinline__ void load(const void* logits, int64_t i0, int64_t V) {
-        head = min(V, (32 - i0 % 32) % 32);   // the output's 128-byte lines, each a wave's own
-        body = (int)((V - head) / NP);
-        base = static_cast<const char*>(logits) + (i0 + head) * (BF ? 2 : 4);
-        // what lies behind the row's end is -inf: nothing counts it
-        const uint32_t ninf = BF ? 0xff80ff80u : 0xff800000u;
+    __device__ __forceinline__ void start(const void* logits, int64_t i0, int64_t V) {
+        this->place(logits, i0, V, threadIdx.x);
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            x[i] = (int)threadIdx.x < body - i * kProbThreads ? ld16(base + threadIdx.x * 16 + i * kProbThreads * 16)
-                                                              : make_uint4(ninf, ninf, ninf, ninf);
-        }
-        const int64_t tail = head + (int64_t)body * NP, t = threadIdx.x;
-        edge_at = t < head ? t : t - head < V - tail ? tail + t - head : -1;
-        edge = kDraftNegInf;
-        if (edge_at >= 0)
-            edge = BF ? bf16_to_f32(static_cast<const uint16_t*>(logits)[i0 + edge_at]) : static_cast<const float*>(logits)[i0 + edge_at];
+        for (int i = 0; i < NR; ++i) x[i] = this->load(i);
+        edge = this->load_edge(logits, i0);
     }
     // f(four values) for every four of the row's vectors.  What a pass makes of
     // a vector must not be kept in registers for the next pass, nor made before its turn: the vectors go
@@ -235,16 +261,35 @@ struct LogitRow {
 
     // out[place] = f(value) over the row's vectors, four values a store that its neighbours' follow: a bf16 vector's
     // eight would be two stores with gaps between the lanes, so a pair of lanes exchanges halves first.
-    template <typename Fn>
-    __device__ __forceinline__ void write(float* out, Fn f) {
+    // NEXT: a vector's registers take the one of the row at `next` as soon as it is stored, so that loads run behind the
+    // stores, and this is that row then (`more`: there is one).
+    template <bool NEXT, typename Fn>
+    __device__ __forceinline__ void write(float* out, Fn f, bool more, const void* logits, int64_t next, int64_t V) {
+        LogitPlace<BF> to = *this;
+        if constexpr (NEXT) {
+            int t = threadIdx.x;
+            asm volatile("" : "+v"(t));   // anew: addresses made of it are not kept in registers from one row for the next
+            to.place(logits, next, V, t);
+            if (!more) to.body = 0, to.edge_at = -1;
+        }
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             asm volatile("" : "+v"(x[i].x), "+v"(x[i].y), "+v"(x[i].z), "+v"(x[i].w));
-            put(x[i], i * kProbThreads + (int)threadIdx.x, out, f);
+            put(x[i], i * kProbThreads + tid, out, f);
+            if constexpr (NEXT) x[i] = to.load(i);
             __builtin_amdgcn_sched_barrier(0);
         }
         for (int j = NR * kProbThreads + threadIdx.x; (j & ~1) < body; j += kProbThreads)   // pairs of lanes stay together
             put(ld16(base + (int64_t)min(j, body - 1) * 16), j, out, f);
+        if (edge_at >= 0) {
+            float y[4] = {edge, edge, edge, edge};
+            f(y);
+            out[edge_at] = y[0];
+        }
+        if constexpr (NEXT) {
+            edge = to.load_edge(logits, next);
+            static_cast<LogitPlace<BF>&>(*this) = to;
+        }
     }
     template <typename Fn>
     __device__ __forceinline__ void put(const uint4& u, int j, float* out, Fn f) const {
@@ -255,7 +300,7 @@ struct LogitRow {
         if constexpr (!BF) {
             if (j < body) *reinterpret_cast<float4*>(out + head + (int64_t)j * 4) = make_float4(y[0], y[1], y[2], y[3]);
         } else {
-            const bool odd = threadIdx.x & 1;
+            const bool odd = tid & 1;
             const int first = j & ~1;   // the pair's
             auto other = [](float v) {   // lane ^ 1's
                 return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0xb1, 0xf, 0xf, true));
@@ -323,105 +368,117 @@ __global__ void __launch_bounds__(kProbThreads) probs_passes_kernel(const void* 
 
 // TOP: with top_k (up to kProbTop), else over the whole row
 template <bool BF, int NR, bool TOP>
-__global__ void __launch_bounds__(kProbThreads) probs_kernel(const void* logits, float* probs, int64_t V, double temperature, int top_k) {
+__global__ void __launch_bounds__(kProbThreads, NR < kProbStream ? 8 : 4) probs_kernel(const void* logits, float* probs, int64_t rows, int64_t V, double temperature, int top_k) {
     __shared__ float shf[kProbWaves];
     __shared__ int shi[kProbWaves], listed;
     __shared__ uint32_t keys[TOP ? kProbThreads : 1], bound;   // the threads' maxima, then the list
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t i0 = (int64_t)blockIdx.x * V;
-    float* out = probs + i0;
+    constexpr bool STREAM = NR >= kProbStream;
     LogitRow<BF, NR> row;
-    row.load(logits, i0, V);
-    float own = row.edge;   // this thread's maximum
-    bool nan = row.edge != row.edge;
-    row.template each<false>([&](const float* y) {
-        own = fmaxf(fmaxf(fmaxf(own, y[0]), fmaxf(y[1], y[2])), y[3]);
-        nan |= __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]);
-        asm volatile("" : "+v"(own));
-    });
-    if constexpr (TOP) {
-        if (threadIdx.x == 0) listed = 0;
-        keys[threadIdx.x] = order_key(own);
-    }
-    float s = 0.f;
-    if constexpr (!TOP) {
-        // the sum above the thread's own maximum, before the workgroup waits for the slowest of its loads
-        const ProbVal val(own == kDraftNegInf ? 0.f : own, temperature);
-        s = val(row.edge);
+    const int64_t step = (int64_t)gridDim.x * V;
+    int64_t i0 = (int64_t)blockIdx.x * V;
+    row.start(logits, i0, V);
+#pragma unroll 1
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, i0 += step) {
+        float* out = probs + i0;
+        const bool more = r + gridDim.x < rows;
+        float own = row.edge;   // this thread's maximum
+        bool nan = row.edge != row.edge;
         row.template each<false>([&](const float* y) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s += val(y[e]);
-            asm volatile("" : "+v"(s));
+            own = fmaxf(fmaxf(fmaxf(own, y[0]), fmaxf(y[1], y[2])), y[3]);
+            nan |= __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]);
+            asm volatile("" : "+v"(own));
         });
-    }
-    const float m = block_reduce<JoinMax>(own, shf);
-    nan = __syncthreads_or(nan);
-    if (no_probs(m, nan, out, V)) return;
-    float least = kDraftNegInf;   // logits from here on are kept
-    if constexpr (TOP) {
-        if (w == 0) {
-            const uint32_t t = wave_bound<kProbWaves>(keys, kProbThreads, top_k, top_k + top_k / 4 + 8, lane);
-            if (lane == 0) bound = t;
+        if constexpr (TOP) {
+            if (threadIdx.x == 0) listed = 0;
+            keys[threadIdx.x] = order_key(own);
         }
-        __syncthreads();
-        const float t = key_value(bound);
-        auto list = [&](float x) {
-            if (x >= t) {
-                const int at = atomicAdd(&listed, 1);   // in any order: the list is only searched
-                if (at < kProbList) keys[at] = order_key(x);
-            }
-        };
-        row.template each<false>([&](const float* y) {
-            if (fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= t) list(y[0]), list(y[1]), list(y[2]), list(y[3]);
-        });
-        list(row.edge);
-        __syncthreads();
-        const int n = listed;
-        if (n <= kProbList) {
+        float s = 0.f;
+        if constexpr (!TOP) {
+            // the sum above the thread's own maximum, before the workgroup waits for the slowest of its loads
+            const ProbVal val(own == kDraftNegInf ? 0.f : own, temperature);
+            s = val(row.edge);
+            row.template each<false>([&](const float* y) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s += val(y[e]);
+                asm volatile("" : "+v"(s));
+            });
+        }
+        const float m = block_reduce<JoinMax>(own, shf);
+        nan = __syncthreads_or(nan);
+        // a row of -inf, with NaN or with +inf goes through the same stores (a second place that loads the next row would take
+        // registers) and is filled behind them
+        const bool none = nan || m == kDraftNegInf || m == __builtin_huge_valf();
+        float least = kDraftNegInf;   // logits from here on are kept
+        if (TOP && !none) {
             if (w == 0) {
-                const uint32_t t2 = n <= 256 ? wave_bound<4>(keys, n, top_k, top_k, lane) : wave_bound<kProbWaves>(keys, n, top_k, top_k, lane);
-                if (lane == 0) bound = t2;
+                const uint32_t t = wave_bound<kProbWaves>(keys, kProbThreads, top_k, top_k + top_k / 4 + 8, lane);
+                if (lane == 0) bound = t;
             }
             __syncthreads();
-            least = key_value(bound);
-        } else {
-            uint32_t key = 0;
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t t2 = key | (1u << bit);
-                int c = order_key(row.edge) >= t2;
-                row.template each<true>([&](const float* y) {
+            const float t = key_value(bound);
+            auto list = [&](float x) {
+                if (x >= t) {
+                    const int at = atomicAdd(&listed, 1);   // in any order: the list is only searched
+                    if (at < kProbList) keys[at] = order_key(x);
+                }
+            };
+            row.template each<false>([&](const float* y) {
+                if (fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= t) list(y[0]), list(y[1]), list(y[2]), list(y[3]);
+            });
+            list(row.edge);
+            __syncthreads();
+            const int n = listed;
+            if (n <= kProbList) {
+                if (w == 0) {
+                    const uint32_t t2 = n <= 256 ? wave_bound<4>(keys, n, top_k, top_k, lane) : wave_bound<kProbWaves>(keys, n, top_k, top_k, lane);
+                    if (lane == 0) bound = t2;
+                }
+                __syncthreads();
+                least = key_value(bound);
+            } else {
+                uint32_t key = 0;
+                for (int bit = 31; bit >= 0; --bit) {
+                    const uint32_t t2 = key | (1u << bit);
+                    int c = order_key(row.edge) >= t2;
+                    row.template each<true>([&](const float* y) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) c += order_key(y[e]) >= t2;
-                    asm volatile("" : "+v"(c));
-                });
-                if (block_reduce<JoinCount>(c, shi) >= top_k) key = t2;
+                        for (int e = 0; e < 4; ++e) c += order_key(y[e]) >= t2;
+                        asm volatile("" : "+v"(c));
+                    });
+                    if (block_reduce<JoinCount>(c, shi) >= top_k) key = t2;
+                }
+                least = key_value(key);
             }
-            least = key_value(key);
         }
-    }
-    const ProbVal val(m, temperature);
-    if constexpr (TOP) {
-        s = row.edge >= least ? val(row.edge) : 0.f;
-        row.template each<false>([&](const float* y) {
-            if (!(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) return;
+        const ProbVal val(m, temperature);
+        if constexpr (TOP) {
+            s = row.edge >= least ? val(row.edge) : 0.f;
+            row.template each<false>([&](const float* y) {
+                if (!(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) return;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += y[e] >= least ? val(y[e]) : 0.f;
-            asm volatile("" : "+v"(s));
-        });
-    } else {
-        s *= val(own);   // from the thread's maximum to the row's
-    }
-    s = block_reduce<JoinSum>(s, shf);
-    const float inv = 1.f / s;
-    row.write(out, [&](float* y) {
-        if (TOP && !(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) {
-            y[0] = y[1] = y[2] = y[3] = 0.f;
-            return;
+                for (int e = 0; e < 4; ++e) s += y[e] >= least ? val(y[e]) : 0.f;
+                asm volatile("" : "+v"(s));
+            });
+        } else {
+            s *= val(own);   // from the thread's maximum to the row's
         }
+        s = block_reduce<JoinSum>(s, shf);
+        const float inv = 1.f / s;
+        row.template write<STREAM>(out, [&](float* y) {
+            if (TOP && !(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= least)) {
+                y[0] = y[1] = y[2] = y[3] = 0.f;
+                return;
+            }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = !TOP || y[e] >= least ? val(y[e]) * inv : 0.f;
-    });
-    if (row.edge_at >= 0) out[row.edge_at] = row.edge >= least ? val(row.edge) * inv : 0.f;
+            for (int e = 0; e < 4; ++e) y[e] = !TOP || y[e] >= least ? val(y[e]) * inv : 0.f;
+        }, more, logits, i0 + step, V);
+        if (none) {
+            __syncthreads();
+            no_probs(m, nan, out, V);
+        }
+        if (!STREAM) break;
+    }
 }
 
 template <bool BF>
@@ -429,14 +486,16 @@ static void probs_launch(const void* logits, float* probs, int64_t rows, int64_t
     constexpr int NP = BF ? 8 : 4;
     const int64_t vectors = (V / NP + kProbThreads - 1) / kProbThreads;   // a thread's, of a row
     const bool top = top_k > 0 && top_k < V;
-    const dim3 grid((unsigned)rows), block(kProbThreads);
+    const int64_t cus = device_cus();
+    const dim3 grid((unsigned)rows), block(kProbThreads), resident((unsigned)(rows < cus ? rows : cus));
     if (top && top_k > kProbTop) {
         hipLaunchKernelGGL((probs_passes_kernel<BF>), grid, block, 0, st, logits, probs, V, temperature, (int)top_k);
         return;
     }
-#define FX_PROBS(NR)                                                                                                                \
-    if (top) hipLaunchKernelGGL((probs_kernel<BF, NR, true>), grid, block, 0, st, logits, probs, V, temperature, (int)top_k);       \
-    else hipLaunchKernelGGL((probs_kernel<BF, NR, false>), grid, block, 0, st, logits, probs, V, temperature, 0)
+#define FX_PROBS(NR)                                                                                               \
+    const dim3 g = NR >= kProbStream ? resident : grid;                                                            \
+    if (top) hipLaunchKernelGGL((probs_kernel<BF, NR, true>), g, block, 0, st, logits, probs, rows, V, temperature, (int)top_k); \
+    else hipLaunchKernelGGL((probs_kernel<BF, NR, false>), g, block, 0, st, logits, probs, rows, V, temperature, 0)
     if (vectors <= 1) { FX_PROBS(1); }
     else if (vectors <= 4) { FX_PROBS(4); }
     else if (vectors <= 8) { FX_PROBS(8); }

@@ -251,6 +251,31 @@ def test_sampling_probs_masked_and_not_finite(dev):
     assert sampling_probs(y[:0]).shape == (0, 5, 1003)
 
 
+@pytest.mark.parametrize("V,dtype", [(20003, torch.float32), (50304, torch.float32), (65536, torch.bfloat16), (131071, torch.bfloat16)])
+def test_sampling_probs_of_many_long_rows(dev, V, dtype):
+    # more rows than the GPU runs at once, rows without probabilities among them: each as it is alone
+    from fxlm import sampling_probs
+    n = torch.cuda.get_device_properties(dev).multi_processor_count
+    x = (torch.randn(2 * n + 3, V, device=dev, generator=torch.Generator(device=dev).manual_seed(V)) * 2).to(dtype)
+    x[1] = -math.inf
+    x[n - 1, 5] = math.nan
+    x[n] = -math.inf
+    x[n + 2, V - 1] = math.inf
+    x[2 * n + 1, :V - 1] = -math.inf
+    x[3] = 0.5                          # equals: more than the list holds
+    for k in (0, 50):
+        p = sampling_probs(x, 0.8, k)
+        assert not p[1].any() and not p[n].any() and p[n - 1].isnan().all() and p[n + 2].isnan().all()
+        for rows in torch.arange(2 * n + 3).split(64):
+            rows = torch.tensor([i for i in rows.tolist() if i not in (1, n - 1, n, n + 2)], device=dev)
+            y, pc = x[rows].double(), p[rows].double()
+            ref = od.sampling_probs(y, 0.8, k)
+            far = ((y.amax(-1, keepdim=True) - y) / 0.8).nan_to_num(0, 0, 0).clamp_max(200)
+            assert ((pc > 0) != (ref > 1.2e-38)).logical_and(ref > 3e-38).sum() == 0
+            assert ((pc - ref).abs() <= 2.0 ** -24 * (128 + 2 * far) * ref + 1.2e-38).all()   # as above
+        assert torch.equal(sampling_probs(x, 0.8, k).nan_to_num(2), p.nan_to_num(2))
+
+
 def test_sampling_probs_of_more_rows_than_a_launch_has(dev):
     from fxlm import sampling_probs
     n = 2 ** 22 + 13                 # workgroups of 1,024 threads: past 2^32 work items
