@@ -15,7 +15,7 @@ namespace fx {
 // read once and written once.  One workgroup a row, which holds the row in registers (up to 65,536 fp32
 // or 131,072 bf16 logits; what does not fit is read again, from the caches): the maximum, the selection,
 // the sum and the output are passes over registers.  256 rows of 50,304 with top-k 50 take 23 us
-// (4.5 TB/s), a single row 12; 768 rows of 131,071 bf16, all kept, 150 us (4.0 TB/s; half rows in
+// (4.5 TB/s), a single row 13; 768 rows of 131,071 bf16, all kept, 150 us (4.0 TB/s; half rows in
 // registers and two workgroups a CU, or none and four, took 160 to 183).
 //
 // Rows of up to four vectors a thread leave room for two workgroups a CU (64 registers: 2,000 rows of 16,384
