@@ -363,20 +363,27 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
         bf16x8 vo[DT];
 #pragma unroll
         for (int d = 0; d < DT; ++d) vo[d] = lds_op_t(vt, VLD, 0, 32 * d, lane);
-        bf16x8 pf[2];
+        // p <= 2^8 in bf16, 2^-8 of it off at most; the sums take it unrounded.  One row group (a single token's heads among
+        // them, whose decode attention keeps p in fp32) takes what that rounding drops as a second operand, p to 2^-16: memory
+        // or round trips bound it (225 keys of 12 heads 7.0 -> 7.1 us, 1,000 keys of 192 11.5 -> 12.1, one token over 65,011
+        // 94.5 -> 94.6).  With more row groups the products would show: 128 rows of 8 heads of 128 over 32,768 keys 98 -> 113 us,
+        // 305 rows 32.0 -> 35.5.
+        constexpr int PARTS = WQ == 1 ? 2 : 1;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const f32x8 x = c == 0 ? __builtin_shufflevector(s, s, 0, 1, 2, 3, 4, 5, 6, 7)
-                                   : __builtin_shufflevector(s, s, 8, 9, 10, 11, 12, 13, 14, 15);
-            pf[c] = __builtin_convertvector(x, bf16x8);   // p <= 2^8 in bf16, 2^-8 off at most; the sums take it unrounded
-        }
+            f32x8 x = c == 0 ? __builtin_shufflevector(s, s, 0, 1, 2, 3, 4, 5, 6, 7)
+                             : __builtin_shufflevector(s, s, 8, 9, 10, 11, 12, 13, 14, 15);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            acc[d] = mfma32(vo[d], pf[0], acc[d]);
-            vo[d] = lds_op_t(vt, VLD, 16, 32 * d, lane);
-        }
+            for (int part = 0; part < PARTS; ++part) {
+                const bf16x8 pf = __builtin_convertvector(x, bf16x8);
+                if (part + 1 < PARTS) x -= __builtin_convertvector(pf, f32x8);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = mfma32(vo[d], pf[1], acc[d]);
+                for (int d = 0; d < DT; ++d) {
+                    acc[d] = mfma32(vo[d], pf, acc[d]);
+                    if (c == 0 && part + 1 == PARTS) vo[d] = lds_op_t(vt, VLD, 16, 32 * d, lane);
+                }
+            }
+        }
     };
 
     // The loop has all of a step's loads in every turn (the last step is its own): the waits for older loads

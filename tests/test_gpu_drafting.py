@@ -82,6 +82,21 @@ def test_tree_attention(dev, B, N, H, Hkv, D, T, ctx, first, new):
         _check_tree(dev, _tree_case(B, N, H, Hkv, D, T, ctx, first, branch, seed=B * N + D, ragged=ragged), new)
 
 
+@pytest.mark.parametrize("B,N,H,Hkv,D,T,ctx", [(1, 1, 4, 4, 64, 500, [400]), (1, 8, 4, 4, 64, 300, [217]), (3, 16, 4, 2, 128, 500, [401, 0, 33]),
+                                               (2, 1, 64, 2, 64, 2500, [2400, 700]), (1, 32, 1, 1, 64, 2100, [700])])
+def test_tree_attention_of_few_rows_rounds_its_output_alone(dev, B, N, H, Hkv, D, T, ctx):
+    # up to 32 rows a key head, as in the decode attention: one rounding to bf16, the output's (2^-8 of it); p reaches its
+    # product to 2^-16, besides what the scores, exponentials and sums are off by (above)
+    from fxlm import tree_attention
+    c = _tree_case(B, N, H, Hkv, D, T, ctx, branch=2, seed=N + T)
+    ro, _, size, rk, _ = od.tree_attention(c["q"], c["k"], c["v"], c["ctx"], c["tree"], k_new=c["kn"], v_new=c["vn"])
+    o = tree_attention(*(c[n].to(dev) for n in ("q", "k", "v", "ctx", "tree")), k_new=c["kn"].to(dev), v_new=c["vn"].to(dev))
+    score = (D + 8) * 2.0 ** -24 * float(c["q"].double().norm(dim=-1).max() * rk.double().norm(dim=-1).max()) / math.sqrt(D)
+    tol = 2.0 ** -8 * ro.abs() + (2 * score + 2.0 ** -16 + 2.0 ** -18) * size
+    err = (o.double().cpu() - ro).abs()
+    assert (err <= tol).all(), float((err - tol).max())
+
+
 def test_tree_attention_at_the_end_of_the_cache(dev):
     # nodes whose rows lie past the cache are nobody's key and not written; a context past it is the cache's
     for T, ctx, first in ((70, [66, 70], 0), (70, [64, 69], 3), (70, [71, 500], 0), (70, [-3, 5], 0)):
