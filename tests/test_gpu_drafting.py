@@ -615,6 +615,28 @@ def test_speculate_samples_as_generate_does(dev):
     assert set(f.nonzero()[:, 0].tolist()) <= set((p > 0).nonzero()[:, 0].tolist())
 
 
+@pytest.mark.parametrize("proposals,branches", [("sampled", (2, 1)), ("sampled", (1, 3)), ("likeliest", (2, 2))])
+def test_speculate_samples_every_token_as_generate_does(dev, proposals, branches):
+    # each token's law given the most frequent tokens before it, over 20,000 sequences of one prompt: the second hangs on the
+    # root's draft row, the third on the rows of inner nodes, the later ones on caches compacted in rounds before
+    m, d = _model(dev, n_layer=1, seq_len=16), _model(dev, seed=5, n_layer=1, seq_len=16)
+    g = torch.Generator(device=dev).manual_seed(18)
+    B, n = 20000, 6
+    idx = torch.randint(0, 256, (1, 5), device=dev, generator=g).expand(B, -1).contiguous()
+    out = m.speculate(idx, n, d, branches=branches, temperature=0.7, top_k=3, generator=g, proposals=proposals)
+    assert out.shape == (B, n) and int(out.min()) >= 0
+    rows, x = out, idx[:1]
+    for i in range(n):
+        with torch.no_grad():
+            p = od.sampling_probs(m(x)[0, -1].float().cpu(), 0.7, 3)
+        f = torch.bincount(rows[:, i].cpu(), minlength=256).double() / len(rows)
+        # as above: 5 standard deviations, and 2 % for the roundings of the logits
+        assert ((f - p).abs() <= 5 * (p * (1 - p) / len(rows)).sqrt() + 0.02 * p).all(), i
+        best = f.argmax().to(dev)
+        rows, x = rows[rows[:, i] == best], torch.cat([x, best.view(1, 1)], 1)
+    assert len(rows) >= 20
+
+
 def test_speculate_without_finite_logits(dev):
     m, d = _model(dev, seq_len=40), _model(dev, seed=2, seq_len=40, n_layer=1)
     idx = torch.randint(0, 256, (2, 30), device=dev)
