@@ -26,6 +26,18 @@ int decode_inputs(const int64_t* tok, int64_t n, int64_t pos, int64_t* tok_out, 
 // NaN for an id or a position outside its table
 int decode_embed(const int64_t* tok, const int64_t* pos, const uint16_t* E, int64_t V, const uint16_t* P, int64_t T, uint16_t* x,
                  int64_t n, int64_t D, void* stream);
+// x (B, N, D) = bf16(E[tok] + P[ctx + depth]) of the nodes first .. first + N - 1 of drafted trees behind ctx cached
+// tokens, E (V, D) and P (L, D) contiguous; a node whose own bit is set in its tree word is a row of NaN if its token or
+// position is outside the table or its row ctx + node outside a cache of Tmax.  Strides in elements, b / n.
+struct TreeEmbedArgs {
+    const int64_t *tok, *tree;
+    const int32_t *ctx, *depth;
+    const uint16_t *E, *P;
+    uint16_t* x;
+    int64_t tokb, tokn, depthb, depthn, treeb, treen, V, L, Tmax, D;
+    int32_t N, first;
+};
+int tree_embed(const TreeEmbedArgs& a, int64_t B, void* stream);
 // out (M, N) fp32 = the bf16 values of norm(X) W^T (fx_linear_fwd_ex with the norm, M <= 64), X rows
 // ldx apart
 int few_rows_logits(const uint16_t* X, int64_t ldx, const uint16_t* W, const uint16_t* norm_w, float eps, float* out, int64_t M,

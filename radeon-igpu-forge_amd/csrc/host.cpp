@@ -445,6 +445,36 @@ OptT decode_embed(const Tensor& tok, const Tensor& pos, const Tensor& E, const T
     return x;
 }
 
+// the rows of a tree's nodes (B, N, D), or None when a check fails
+OptT tree_embed(const Tensor& tok, const Tensor& depth, const Tensor& ctx, const Tensor& tree, int64_t first, int64_t Tmax, const Tensor& E,
+                const Tensor& P) {
+    if (tok.dim() != 2 || tok.size(0) < 1 || tok.size(1) < 1 || tok.size(1) > 64 || first < 0 || first > 64 - tok.size(1) ||
+        tok.numel() >= 1 << 25 || tok.scalar_type() != at::kLong || tree.scalar_type() != at::kLong || depth.scalar_type() != at::kInt ||
+        ctx.scalar_type() != at::kInt || ctx.dim() != 1 || ctx.size(0) != tok.size(0) || !ctx.is_contiguous() || !is_bf(E) || !is_bf(P) ||
+        E.dim() != 2 || P.dim() != 2 || E.size(0) < 1 || P.size(0) < 1 || E.size(1) != P.size(1) || E.size(1) % 8 || E.size(1) < 8 ||
+        !E.is_contiguous() || !P.is_contiguous() || !aligned(E) || !aligned(P))
+        return std::nullopt;
+    for (const Tensor* t : {&tree, &depth})   // (B, N), or (N) for all sequences
+        if ((t->dim() != 1 && (t->dim() != 2 || t->size(0) != tok.size(0))) || t->size(-1) != tok.size(1)) return std::nullopt;
+    for (const Tensor* t : {&tok, &depth, &ctx, &tree, &E, &P})
+        if (!t->is_cuda()) return std::nullopt;
+    same_gpu(E, P, tok, depth, ctx, tree);
+    const c10::DeviceGuard guard(E.device());
+    fx::TreeEmbedArgs a{};
+    a.tok = static_cast<int64_t*>(tok.data_ptr()), a.tree = static_cast<int64_t*>(tree.data_ptr());
+    a.ctx = static_cast<int32_t*>(ctx.data_ptr()), a.depth = static_cast<int32_t*>(depth.data_ptr());
+    a.E = bf(E), a.P = bf(P);
+    a.tokb = tok.stride(0), a.tokn = tok.stride(1);
+    a.depthb = depth.dim() == 2 ? depth.stride(0) : 0, a.depthn = depth.stride(-1);
+    a.treeb = tree.dim() == 2 ? tree.stride(0) : 0, a.treen = tree.stride(-1);
+    a.V = E.size(0), a.L = P.size(0), a.Tmax = Tmax, a.D = E.size(1);
+    a.N = (int32_t)tok.size(1), a.first = (int32_t)first;
+    Tensor x = at::empty({tok.size(0), tok.size(1), a.D}, E.options());
+    a.x = bf(x);
+    check(fx::tree_embed(a, tok.size(0), stream_of(E)), "tree_embed");
+    return x;
+}
+
 // norm(x) W^T as fp32 for x (B, D) rows, or None when a check fails
 OptT few_rows_logits(const Tensor& x, const Tensor& w, const Tensor& norm_w, double eps) {
     if (x.dim() != 2 || w.dim() != 2 || norm_w.dim() != 1 || !is_bf(x) || !is_bf(w) || !is_bf(norm_w) || !x.is_cuda() ||
@@ -705,6 +735,7 @@ PYBIND11_MODULE(_host, m) {
     FX_DEF(column_sums);
     FX_DEF(decode_inputs);
     FX_DEF(decode_embed);
+    FX_DEF(tree_embed);
     FX_DEF(few_rows_logits);
     FX_DEF(tree_attention);
     FX_DEF(sampling_probs);

@@ -330,16 +330,24 @@ class GPT(nn.Module):
         drafted trees behind each sequence's ctx (B,) int32 cached tokens: tree (B, N) or (N,)
         int64 ancestor bits (fxlm.tree_attention), depth (B, N) or (N,) a node's tokens below ctx
         (the root's 0).  The tree's keys and values go into the caches' rows ctx + node, where
-        compact_cache takes the accepted ones from.  ctx + depth has to be a position of the
-        model (a position past them is taken as the last); a padding node's token may be anything
-        (what is no id is looked up as the nearest)."""
+        compact_cache takes the accepted ones from.  A node whose token is no id, whose position
+        ctx + depth is none of the model's or whose row the cache does not have gives NaN, and so
+        do the nodes that see it; of a padding node all of these may be anything."""
         if self.cfg.attn_impl != "flash":
             raise ValueError("cached inference needs attn_impl='flash'")
         if tok.dim() != 2 or ctx.shape != tok.shape[:1]:
             raise ValueError(f"tok (B, N) and ctx (B,): {tuple(tok.shape)} {tuple(ctx.shape)}")
         B, N = tok.shape
-        pos = (ctx[:, None] + depth).clamp_(0, self.pos_emb.shape[0] - 1)
-        x = self.tok_emb(tok.clamp(0, self.tok_emb.num_embeddings - 1)) + self.pos_emb[pos]
+        rows = cache[0][0].shape[1]
+        x = None
+        if _table_lookup(self.tok_emb):
+            x = host.tree_embed(tok, depth, ctx, tree, first, rows, self.tok_emb.weight, self.pos_emb)
+        if x is None:
+            node = torch.arange(first, first + N, device=tok.device)
+            at = ctx[:, None] + depth
+            pos, t = at.clamp(0, self.pos_emb.shape[0] - 1), tok.clamp(0, self.tok_emb.num_embeddings - 1)
+            none = ((t != tok) | (pos != at) | (ctx[:, None] + node >= rows)) & ((tree >> node & 1) == 1)
+            x = (self.tok_emb(t) + self.pos_emb[pos]).masked_fill(none[:, :, None], math.nan)
         for blk, kv in zip(self.blocks, cache):
             x = blk.tree_step(x, kv, ctx, tree, first)
         if self.blocks and self.blocks[0]._fused_step(B * N):
@@ -432,9 +440,11 @@ class GPT(nn.Module):
         ctx = torch.full((B,), T, dtype=torch.int32, device=dev)
         q = torch.empty(B, N, self.cfg.vocab_size, device=dev) if proposals == "sampled" else None
         while min(len(o) for o in out) < max_new:
-            # a finished sequence's tree is padding: nothing of it is written or moved
-            going = torch.tensor([len(o) < max_new for o in out], device=dev)
-            tree = torch.where(going[:, None], whole, 0)
+            # nodes behind the last token that is asked for are padding, and so is a finished sequence's whole tree: nothing
+            # of it is written or moved
+            have = torch.tensor([len(o) for o in out], device=dev)[:, None]
+            going = have[:, 0] < max_new
+            tree = torch.where(have + depth < max_new, whole, 0)
             for level, below in zip(levels, levels[1:] + [None]):
                 a, b = level.start, level.stop
                 lg = draft.tree_step(tok[:, a:b], depth[a:b], caches[1], ctx, tree[:, a:b], first=a)

@@ -579,6 +579,49 @@ def test_tree_step_of_padding_with_tokens_that_are_no_ids(dev):
         assert torch.equal(lg, res[0][0]) and all(torch.equal(a, b) for a, b in zip(rows, res[0][1]))
 
 
+@pytest.mark.parametrize("first,hook", [(0, False), (1, False), (0, True)])
+def test_tree_step_of_nodes_that_cannot_be(dev, first, hook):
+    # no id, no position of the model, no row of the cache: NaN for the node and those that see it, and for no other; with a
+    # hook on the embedding, which is called then, too
+    m = _model(dev, seq_len=40)
+    called = []
+    if hook:
+        m.tok_emb.register_forward_hook(lambda *a: called.append(1))
+    parents, dep = [-1, 0, 0, 1, 2, 4], torch.tensor([0, 1, 1, 2, 2, 3], dtype=torch.int32, device=dev)
+    bits = od.ancestors(parents).to(dev)
+    idx = torch.randint(0, 256, (3, 37), device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+
+    def step(ctx, tok, rows, depth=dep, bits=bits):
+        cache = m._new_cache(3, rows)
+        m.prefill(idx[:, :max(ctx)], cache)
+        ctx = torch.tensor(ctx, dtype=torch.int32, device=dev)
+        tok = torch.tensor(tok, device=dev)
+        if first:
+            m.tree_step(tok[:, :1], depth[..., :1], cache, ctx, bits[:1])
+        return m.tree_step(tok[:, first:], depth[..., first:], cache, ctx, bits[first:], first=first)
+
+    good = [[1, 2, 3, 4, 5, 6]] * 3
+    ref = step([30] * 3, good, 48)
+    assert torch.isfinite(ref).all() and bool(called) == hook
+    assert torch.equal(step([30] * 3, good, 48, depth=dep.long().expand(3, -1)), ref)
+    for bad in (256, -1, 2 ** 40):
+        lg = step([30] * 3, [good[0], [1, 2, bad, 4, 5, 6], good[0]], 48)
+        want = torch.zeros(3, 6, dtype=torch.bool, device=dev)
+        want[1, [2, 4, 5]] = True
+        assert torch.equal(lg.isnan().all(-1), want[:, first:]) and torch.equal(lg.isnan().any(-1), want[:, first:])
+        assert torch.equal(lg[~want[:, first:]], ref[~want[:, first:]])
+    # depth 3 of the second sequence is position 40 of 40
+    lg = step([36, 37, 36], good, 48)
+    assert lg.isnan().all(-1).tolist() == [[False] * (6 - first), [False] * (5 - first) + [True], [False] * (6 - first)]
+    # and of a cache of 35 rows node 5 has none, of 33 rows nodes 3 to 5 have none
+    for rows, gone in ((35, [5]), (33, [3, 4, 5])):
+        lg = step([30] * 3, good, rows)
+        assert lg.isnan().all(-1).tolist() == [[i in gone for i in range(first, 6)]] * 3
+    # padding's may lie behind the cache
+    lg = step([30] * 3, good, 48, bits=od.ancestors([-1, 0, 0, -1, -1, -1]).to(dev))
+    assert torch.equal(step([30] * 3, good, 33, bits=od.ancestors([-1, 0, 0, -1, -1, -1]).to(dev)), lg) and torch.isfinite(lg).all()
+
+
 @pytest.mark.parametrize("proposals,branches", [("sampled", (2, 2, 1)), ("likeliest", (3, 1)), ("sampled", (1, 1, 1, 1))])
 def test_speculate_greedy_is_the_models_own(dev, proposals, branches):
     # top_k = 1: whatever the draft proposes, each token is the model's own choice within the rounding of its logits
