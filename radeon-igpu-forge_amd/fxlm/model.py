@@ -433,18 +433,19 @@ class GPT(nn.Module):
         sample = dict(temperature=max(temperature, 1e-5), top_k=top_k)
         caches = [m._new_cache(B, T + max_new + N) for m in (self, draft)]
         draft.prefill(idx, caches[1])
-        p = _with_mass(sampling_probs(self.prefill(idx, caches[0]), **sample))
+        p, sure = _drawable(sampling_probs(self.prefill(idx, caches[0]), **sample))
         tok = torch.zeros(B, N, dtype=torch.int64, device=dev)
         tok[:, :1] = torch.multinomial(p, 1, generator=generator)
-        out = [[t] for t in tok[:, 0].tolist()]
+        *first, ok = torch.cat([tok[:, 0], sure]).tolist()
+        _check_finite(ok)
+        out = [[t] for t in first]
+        have = torch.ones(B, dtype=torch.int64, device=dev)   # the lengths of out
         ctx = torch.full((B,), T, dtype=torch.int32, device=dev)
         q = torch.empty(B, N, self.cfg.vocab_size, device=dev) if proposals == "sampled" else None
         while min(len(o) for o in out) < max_new:
             # nodes behind the last token that is asked for are padding, and so is a finished sequence's whole tree: nothing
             # of it is written or moved
-            have = torch.tensor([len(o) for o in out], device=dev)[:, None]
-            going = have[:, 0] < max_new
-            tree = torch.where(have + depth < max_new, whole, 0)
+            tree = torch.where(have[:, None] + depth < max_new, whole, 0)
             for level, below in zip(levels, levels[1:] + [None]):
                 a, b = level.start, level.stop
                 lg = draft.tree_step(tok[:, a:b], depth[a:b], caches[1], ctx, tree[:, a:b], first=a)
@@ -454,27 +455,34 @@ class GPT(nn.Module):
                 if q is None:
                     tok[:, below.start:below.stop] = lg.topk(n).indices.view(B, -1)
                 else:
-                    q[:, a:b] = _with_mass(sampling_probs(lg, **sample))
+                    q[:, a:b], ok = _drawable(sampling_probs(lg, **sample))
+                    sure = sure & ok
                     tok[:, below.start:below.stop] = torch.multinomial(q[:, a:b].reshape(B * (b - a), -1), n, replacement=True,
                                                                        generator=generator).view(B, -1)
             p = sampling_probs(self.tree_step(tok, depth, caches[0], ctx, tree), **sample)
             got, path, n = verify_draft(p, tok, parents, torch.rand(B, N, device=dev, generator=generator), draft_probs=q)
-            n = torch.where(going, n, 0)
+            n = torch.where(have < max_new, n, 0)
+            have = have + n
             compact_cache(caches[1], ctx, path, n)
             ctx = compact_cache(caches[0], ctx, path, n)
             tok[:, 0] = got.gather(1, (n.long()[:, None] - 1).clamp_min(0))[:, 0]
-            for o, row, k in zip(out, got.tolist(), n.tolist()):
-                if -1 in row[:k]:
-                    raise RuntimeError("the model's logits are not finite: there is no next token to draw")
+            # all that the host reads of a round
+            for o, (*row, k, ok) in zip(out, torch.cat([got, n[:, None], sure.expand(B)[:, None]], 1).tolist()):
+                _check_finite(ok and -1 not in row[:k])
                 o += row[:k]
         return torch.tensor([o[:max_new] for o in out], dtype=torch.int64, device=dev)
 
 
-def _with_mass(p):
-    """p, probabilities that are about to be drawn from; a row of logits that were not finite has none."""
-    if not bool((p.sum(-1) > 0.5).all()):
+def _drawable(p):
+    """p, probabilities that are about to be drawn from, and (1,) whether every row has them: a row of logits that were not
+    finite has none, and becomes one that can be drawn from."""
+    mass = p.sum(-1, keepdim=True) > 0.5
+    return p.masked_fill_(~mass, 1.0), mass.all().view(1)
+
+
+def _check_finite(ok):
+    if not ok:
         raise RuntimeError("the model's logits are not finite: there is no next token to draw")
-    return p
 
 
 def _check_pos(pos, cache_len, positions):

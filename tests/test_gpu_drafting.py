@@ -691,6 +691,33 @@ def test_speculate_without_finite_logits(dev):
         d.speculate(idx, 4, m)
 
 
+@pytest.mark.parametrize("proposals", ["sampled", "likeliest"])
+def test_speculate_reads_the_device_once_a_round(dev, proposals, monkeypatch):
+    import warnings
+
+    import fxlm.model as M
+    m, d = _model(dev, seq_len=40), _model(dev, seed=2, seq_len=40, n_layer=1)
+    idx = torch.randint(0, 256, (2, 5), device=dev)
+    rounds = []
+    verify = M.verify_draft
+    monkeypatch.setattr(M, "verify_draft", lambda *a, **kw: rounds.append(1) or verify(*a, **kw))
+
+    def reads(n):   # (waits for the GPU, rounds) of a call
+        rounds.clear()
+        with warnings.catch_warnings(record=True) as w:
+            warnings.simplefilter("always")
+            torch.cuda.set_sync_debug_mode("warn")
+            try:
+                m.speculate(idx, n, d, proposals=proposals, generator=torch.Generator(device=dev).manual_seed(3))
+            finally:
+                torch.cuda.set_sync_debug_mode("default")
+        return sum("synchroniz" in str(x.message) for x in w), len(rounds)
+
+    reads(3)
+    (a, ra), (b, rb) = reads(2), reads(30)
+    assert a > 0 and rb > ra and b - a == rb - ra
+
+
 def test_operators_on_two_streams_at_once(dev):
     # each call has a workspace of its own: two streams' calls, none waiting for the other, against the same calls in turn
     from fxlm import sampling_probs, tree_attention, verify_draft
