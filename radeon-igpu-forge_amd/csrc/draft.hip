@@ -29,7 +29,8 @@ namespace fx {
 // logit, and few logits lie above it (of random ones -1024 ln(1 - k / 1024) for the k-th of 1024 maxima): those
 // are listed, and the exact bound found among them.  Both searches are one wave's, halving an interval of
 // order-preserving integer keys until the keys at or above its lower end are few enough, or top_k.
-// Where the list is too small for the logits above the first bound (a sorted row, a thousand equals) the
+// Where fewer threads than top_k hold logits that are not -inf, the list is of all such logits (a row with 40 of 50,304 left,
+// top-k 50, 18 us; with 60 left 13).  Where it is too small for the logits above the first bound (a sorted row, a thousand equals) the
 // bound is found a bit at a time over the registers.  A top_k above 3/8 of the threads, whose list
 // would near its 1024 places, goes to another kernel that finds the bound eleven bits at a time, three
 // passes over memory that count the keys of what is settled of it: 256 rows, top-k 384 30 us against 52,
@@ -194,7 +195,7 @@ struct LogitPlace {
         const int tail = (int)head + body * NP;
         edge_at = t < head ? t : t - head < V - tail ? tail + t - (int)head : -1;
     }
-    // this thread's i-th vector; what lies behind the row's end is -inf: nothing counts it
+    // this thread's i-th vector; what lies behind the row's end is -inf: neither kept nor summed
     __device__ __forceinline__ uint4 load(int i) const {
         const uint32_t ninf = BF ? 0xff80ff80u : 0xff800000u;
         return tid < body - i * kProbThreads ? ld16(base + (uint32_t)(tid * 16 + i * kProbThreads * 16))
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(kProbThreads, NR < kProbStream ? 8 : 4) probs_
                 if (lane == 0) bound = t;
             }
             __syncthreads();
-            const float t = key_value(bound);
+            const float t = fmaxf(key_value(bound), -__FLT_MAX__);   // masked logits and what lies behind the row are not listed
             auto list = [&](float x) {
                 if (x >= t) {
                     const int at = atomicAdd(&listed, 1);   // in any order: the list is only searched
@@ -429,7 +430,9 @@ __global__ void __launch_bounds__(kProbThreads, NR < kProbStream ? 8 : 4) probs_
             list(row.edge);
             __syncthreads();
             const int n = listed;
-            if (n <= kProbList) {
+            if (n <= top_k) {   // every listed logit: all that are not masked, if they are fewer
+                least = t;
+            } else if (n <= kProbList) {
                 if (w == 0) {
                     const uint32_t t2 = n <= 256 ? wave_bound<4>(keys, n, top_k, top_k, lane) : wave_bound<kProbWaves>(keys, n, top_k, top_k, lane);
                     if (lane == 0) bound = t2;

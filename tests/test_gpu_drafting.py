@@ -266,6 +266,44 @@ def test_sampling_probs_masked_and_not_finite(dev):
     assert sampling_probs(y[:0]).shape == (0, 5, 1003)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,k,left", [(256, 50, None), (257, 200, None), (512, 384, None), (1000, 300, None), (2000, 300, None), (5001, 50, 40),
+                                      (5001, 50, 50), (5001, 50, 51), (5001, 384, 1030), (50304, 50, 1), (50304, 200, 199), (131071, 50, 49)])
+def test_sampling_probs_of_few_logits(dev, V, k, left, dtype):
+    # fewer threads than top_k hold logits: a short row, or one that a mask leaves few of (the rest -inf, or the lowest value)
+    g = torch.Generator().manual_seed(V + k)
+    x = (torch.randn(4, V, generator=g) * 3).to(dtype)
+    if left:
+        out = torch.ones(4, V, dtype=torch.bool).scatter_(1, torch.rand(4, V, generator=g).topk(left, -1).indices, False)
+        x[:3][out[:3]] = -math.inf
+        x[3][out[3]] = torch.finfo(dtype).min
+    _check_probs(dev, x, 0.8, k)
+
+
+def test_sampling_probs_of_a_masked_row_takes_no_counted_passes(dev):
+    # 40 logits of 50,304 with top-k 50 took 8 times what 60 did: each -inf was listed, the list ran over, and 32 passes over
+    # the row found the bound.  Four times would be that again
+    from fxlm import sampling_probs
+    x = torch.randn(50304, generator=torch.Generator().manual_seed(2))
+
+    def least(left):
+        y = x.clone()
+        y[torch.randperm(50304, generator=torch.Generator().manual_seed(left))[left:]] = -math.inf
+        y = y[None].to(dev)
+        took = []
+        for i in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(100):
+                sampling_probs(y, 0.8, 50)
+            b.record()
+            torch.cuda.synchronize()
+            took.append(a.elapsed_time(b))
+        return min(took)
+
+    assert least(40) < 4 * least(60)
+
+
 @pytest.mark.parametrize("V,dtype", [(20003, torch.float32), (50304, torch.float32), (65536, torch.bfloat16), (131071, torch.bfloat16)])
 def test_sampling_probs_of_many_long_rows(dev, V, dtype):
     # more rows than the GPU runs at once, rows without probabilities among them: each as it is alone
