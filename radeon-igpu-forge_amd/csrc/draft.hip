@@ -321,14 +321,15 @@ struct LogitRow : LogitPlace<BF> {
 };
 
 // exp((l - m) / T) as 2^((l - m) f), f = log2(e) / T in two parts: the difference and the product are rounded, once each.
-// The first part is below f, so that -inf times the second is -inf too, and its power 0.
+// The first part is below f and the second no less than the least normal number (2^-26 of the least f), so that -inf times
+// the second is -inf too, and its power 0.
 struct ProbVal {
     float m, hi, lo;
     __device__ __forceinline__ ProbVal(float m, double temperature) : m(m) {
         const double f = 1.4426950408889634 / temperature;
         hi = (float)f;
         if ((double)hi >= f) hi = __uint_as_float(__float_as_uint(hi) - 1);
-        lo = (float)(f - (double)hi);
+        lo = fmaxf((float)(f - (double)hi), __FLT_MIN__);
     }
     __device__ __forceinline__ float operator()(float x) const {
         const float d = x - m;

@@ -266,6 +266,20 @@ def test_sampling_probs_masked_and_not_finite(dev):
     assert sampling_probs(y[:0]).shape == (0, 5, 1003)
 
 
+@pytest.mark.parametrize("T", [9.999999414548473e29, 9.999999414548476e29, 9.7e29, 8.3e29, 1e29])
+def test_sampling_probs_masked_at_the_largest_temperatures(dev, T):
+    # log2(e) / T in two floats: of the first two what the first float leaves is no float at all
+    from fxlm import sampling_probs
+    x = torch.randn(2, 5001, generator=torch.Generator().manual_seed(9))
+    x[:, 100:] = -math.inf
+    x[1, 7] = -1e30
+    for k in (0, 200):
+        p = sampling_probs(x.to(dev), T, k).double().cpu()
+        ref = od.sampling_probs(x, T, k)
+        # exact differences, one rounding each of the product, the power and the quotient, and the sum's 100 terms
+        assert ((p - ref).abs() <= 2.0 ** -24 * 128 * ref).all() and not p[:, 100:].any()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V,k,left", [(256, 50, None), (257, 200, None), (512, 384, None), (1000, 300, None), (2000, 300, None), (5001, 50, 40),
                                       (5001, 50, 50), (5001, 50, 51), (5001, 384, 1030), (50304, 50, 1), (50304, 200, 199), (131071, 50, 49)])
