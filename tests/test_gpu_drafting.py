@@ -343,6 +343,25 @@ def test_sampling_probs_of_many_long_rows(dev, V, dtype):
         assert torch.equal(sampling_probs(x, 0.8, k).nan_to_num(2), p.nan_to_num(2))
 
 
+@pytest.mark.parametrize("V,dtype", [(70001, torch.float32), (140003, torch.bfloat16)])
+def test_sampling_probs_of_many_rows_past_the_registers(dev, V, dtype):
+    # rows of which a workgroup holds a part and reads the rest again, several a workgroup
+    from fxlm import sampling_probs
+    n = torch.cuda.get_device_properties(dev).multi_processor_count + 40
+    x = (torch.randn(n, V, device=dev, generator=torch.Generator(device=dev).manual_seed(V)) * 2).to(dtype)
+    x[2, V - 40000:] = -math.inf
+    x[n - 1, V - 1] = 40
+    for k in (0, 50):
+        p = sampling_probs(x, 0.8, k)
+        rows = [0, 1, 2, 39, 40, 41, n - 41, n - 40, n - 2, n - 1]
+        y, pc = x[rows].double().cpu(), p[rows].double().cpu()
+        ref = od.sampling_probs(y, 0.8, k)
+        far = ((y.amax(-1, keepdim=True) - y) / 0.8).nan_to_num(0, 0, 0).clamp_max(200)
+        assert ((pc > 0) != (ref > 1.2e-38)).logical_and(ref > 3e-38).sum() == 0
+        assert ((pc - ref).abs() <= 2.0 ** -24 * (128 + 2 * far) * ref + 1.2e-38).all()   # as above
+        assert torch.equal(sampling_probs(x, 0.8, k), p)
+
+
 def test_sampling_probs_of_more_rows_than_a_launch_has(dev):
     from fxlm import sampling_probs
     n = 2 ** 22 + 13                 # workgroups of 1,024 threads: past 2^32 work items
@@ -399,6 +418,16 @@ def _check_verify(dev, p, tok, par, u, q):
 def test_verify_draft(dev, B, N, V, branch, k, drafted):
     for seed in range(3):
         _check_verify(dev, *_draft_case(B, N, V, branch, 100 * seed + N, seed == 1, drafted, k))
+
+
+def test_verify_draft_of_the_largest_vocabulary(dev):
+    # 2^20 ids, the most that it takes; one more is refused
+    for drafted in (True, False):
+        _check_verify(dev, *_draft_case(2, 4, 2 ** 20, 2, 7, False, drafted, 0))
+    from fxlm import verify_draft
+    i = torch.zeros(1, 2, dtype=torch.int64, device=dev)
+    with pytest.raises(ValueError):
+        verify_draft(torch.zeros(1, 2, 2 ** 20 + 1, device=dev), i, i.int() - 1, torch.zeros(1, 2, device=dev))
 
 
 def test_verify_draft_edges(dev):
