@@ -21,7 +21,10 @@ namespace fx {
 // Rows of up to four vectors a thread leave room for two workgroups a CU (64 registers: 2,000 rows of 16,384
 // fp32 with top-k 50 58 us against 90 with 66), and one's loads run beside the other's stores.  Longer rows
 // are a workgroup's alone, so there it walks over several: a vector's registers take the next row's as
-// soon as it is stored.  Against a workgroup for each row: 2,000 rows of 24,576 fp32 83 us / 92, 768 of
+// soon as it is stored.  Rows of 9 to 13 vectors a thread (53,248 fp32) have a kernel of 13: what the one of 16 holds
+// beyond the row's end is still walked over (256 rows, top-k 50, of 34,000 fp32 19.1 us / 20.2, of 53,000 25.3 / 25.9, one
+// row of 34,000 13.1 / 14.4; kernels of 10, 12 and 14 instead are within 4 % of it on either side).  Against a
+// workgroup for each row: 2,000 rows of 24,576 fp32 83 us / 92, 768 of
 // 50,176 60 / 71, of 61,440 82 / 89, 768 bf16 rows of 131,071 150 / 160 (300 rows of 122,880 69 / 68);
 // below eight vectors it would be the slower, by the registers it takes (2,000 of 16,384 56 / 48).
 //
@@ -536,9 +539,10 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
 // row by its running sum.  Sums and tests are in 64 bits: the tokens do not hang on a summation order.
 
 //
-// One workgroup a sequence, every step of the walk in it: bound by what one CU takes from memory (about 80 GB/s here) and
-// by the walk's round trips, so rows are read in 16-byte vectors, several in flight and the next ones behind
-// them.  64 trees of 24 nodes over 131,072 ids take 62 to 74 us by the seed (two passes a sequence on
+// One workgroup a sequence, every step of the walk in it: bound by the longest walk's passes, one behind the other on one
+// CU.  A pass is as much 64-bit arithmetic as memory: VALU issues in 55 % of the SIMDs' cycles while they have waves, and the
+// waves wait 56 % of their time for loads and barriers (a CU takes about 80 GB/s).  Rows are read in 16-byte vectors,
+// several in flight and the next ones behind them.  64 trees of 24 nodes over 131,072 ids take 62 to 74 us by the seed (two passes a sequence on
 // average, five or so in the longest walk; with the draft's row read at a leaf too 74 to 78), a chain of
 // five over 50,304 12.6.  Launches that share a pass over
 // several workgroups a sequence, and walk again from the start, took longer (84 us for four such launches, 101

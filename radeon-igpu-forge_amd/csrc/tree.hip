@@ -14,13 +14,15 @@
 // rows of a key head stay in one workgroup, 32 to a wave's MFMA tile, and the keys are split:
 // over the workgroup's waves, and over workgroups ("units") for as many as fill the CUs at once.
 // A unit's length comes from the sequences' own lengths on the device, so a long sequence among
-// short ones gets more units and the cache's size costs nothing; a second kernel joins the units
-// of a row by their maxima and sums.  See the launch shape below for when keys are not split.
+// short ones gets more units; a second kernel joins the units of a row by their maxima and sums.
+// Whether keys are split at all goes by the cache's size, which the host knows (the launch shape
+// below): short contexts in a large cache pay for the second launch.
 //
 // 32 nodes of 4 query heads a key head, 4 sequences of 16,001 to 32,768 keys, 8 key heads of 128: 403 MB in 98 us (95 of
 // them this kernel, 4.3 TB/s); one token over up to 65,011 keys of 16 heads of 64: 430 MB in 95 us (89, 4.8 TB/s).  Two
-// tiles a step, or a second one in flight behind it, change neither: memory bounds them.  Short contexts
-// are bounded by their chain of round trips (context, keys, sums): 225 keys of 12 heads take 7 us.
+// tiles a step, or a second one in flight behind it, change neither: memory bounds the second.  The first's waves also wait
+// for one another: MFMA is busy in 32 % of the SIMDs' cycles, VALU in 37 %, LDS in 26 %, and half again as many MFMA would
+// add 15 us.  Short contexts are bounded by their chain of round trips (context, keys, sums): 225 keys of 12 heads take 7 us.
 #include <math.h>
 
 #include "fx_internal.h"
@@ -364,10 +366,10 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeArgs a, Tre
 #pragma unroll
         for (int d = 0; d < DT; ++d) vo[d] = lds_op_t(vt, VLD, 0, 32 * d, lane);
         // p <= 2^8 in bf16, 2^-8 of it off at most; the sums take it unrounded.  One row group (a single token's heads among
-        // them, whose decode attention keeps p in fp32) takes what that rounding drops as a second operand, p to 2^-16: memory
-        // or round trips bound it (225 keys of 12 heads 7.0 -> 7.1 us, 1,000 keys of 192 11.5 -> 12.1, one token over 65,011
-        // 94.5 -> 94.6).  With more row groups the products would show: 128 rows of 8 heads of 128 over 32,768 keys 98 -> 113 us,
-        // 305 rows 32.0 -> 35.5.
+        // them, whose decode attention keeps p in fp32) takes what that rounding drops as a second operand, p to 2^-16: 225 keys
+        // of 12 heads 7.0 -> 7.1 us, 1,000 keys 9.8 -> 10.7 (a chain that nothing hides), 1,000 keys of 192 heads 11.4 -> 12.1,
+        // one token over 65,011 95.1 both.  More row groups keep the one rounding: 128 rows of 8 heads of 128 over 32,768 keys
+        // would go 98 -> 113 us, 305 rows 32.0 -> 35.5.
         constexpr int PARTS = WQ == 1 ? 2 : 1;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -555,13 +557,15 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, TreePlan pla
 }
 
 // Launch shape.  One workgroup a CU is resident (its registers), so R = CUs of them run at once.
-// Caches of up to six steps of a workgroup are not split: 12 key heads over 1,000 keys 9.8 us against 12.3 for two
-// launches, over 1,500 12.0 / 12.4, over 2,000 14.2 / 12.4; 32 over 350 keys in four row groups 15.8 / 16.1.  Key
+// Caches of up to six steps of a workgroup are not split: 12 key heads over 1,000 keys 10.7 us against 12.7 for two
+// launches, over 1,500 13.1 / 12.9, over 2,000 15.6 / 12.7; 32 over 350 keys in four row groups 15.8 / 16.1.  Key
 // heads (with row groups) below half of R are split into units that R leaves over, so that all of them run at once.
 // More of them are split for unlike sequences alone, at twice the mean length, where a cache may hold 64 steps of a
-// workgroup or more: one sequence of 19,000 keys among 63 of 500 (8 key heads) 31 us against 81, of 60,000
-// 42 / 241, at the cost of a join that finds nothing: 192 of 18,000 keys each 162 / 159, 64 sequences
-// of 500 24 / 19.5; in caches of 8,192 rows such splits lost 3 to 11 % on mixed lengths and are not made.
+// workgroup or more: one sequence of 19,000 keys among 63 of 500 (8 key heads) 32 us against 93, of 60,000
+// 43 / 276, at the cost of a join that finds nothing: 192 of 18,000 keys each 162 / 159, 64 sequences
+// of 500 24.6 / 19.9; in caches of 8,192 rows such splits lost 3 to 11 % on mixed lengths and are not made.
+// Equal long sequences pay for a last round that is not full: 18,000 keys a head of 128 take 4.7 to 4.9 TB/s for 112 to
+// 136 key heads (no step at half of R), 6.0 for 256, 4.2 for 264 and 6.0 for 512.
 static TreePlan tree_plan(int32_t B, int32_t N, int32_t H, int32_t Hkv, int32_t Tmax) {
     TreePlan p{};
     const int rows = N * (H / Hkv);

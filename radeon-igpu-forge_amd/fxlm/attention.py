@@ -209,9 +209,10 @@ def tree_attention(q, k_cache, v_cache, ctx, tree, first=0, scale=None, return_l
     (first + i) is clear is padding: zeros come out, and its row is nobody's key.
     k_new, v_new (B, N, Hkv, Dh), both or neither: the queries' own keys and values, which the
     kernel uses and writes into the caches (padding's are not written); without them, the caches
-    hold them already.  Rows past Tmax are neither read nor written.
+    hold them already.  Rows past Tmax are neither read nor written: a node whose row is past it is
+    nobody's key, its own query's neither.  scale (1 / sqrt(Dh) by default) is positive and finite.
     Returns o (B, N, H, Dh) bf16 and, if asked, the fp32 logsumexp (B, N, H) (-inf where a query
-    sees no key).
+    sees no key), without gradients.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])

@@ -5,7 +5,8 @@ in one pass (GPT.tree_step), ``sampling_probs`` turns its logits into the probab
 GPT.generate would sample from, ``verify_draft`` accepts a path of the tree so that the accepted
 tokens and the one after them are distributed as the target's own samples, and ``compact_cache``
 moves the path's keys and values together in every layer's cache.  The reference has no drafting
-(its ml/fxlm/sample.py:62-73 samples one token a pass).
+(its ml/fxlm/sample.py:62-73 samples one token a pass).  All of it is inference: what these functions
+return has no gradient, whatever their inputs require.
 
 A tree is two (B, N) tensors: tokens, and parents (a node's parent lies below it).  Node 0 is the
 root, the sequence's last token, whose key is not in the cache yet; a node with a parent of -1 is
@@ -26,7 +27,8 @@ def _taken(r, name):
 def sampling_probs(logits, temperature=1.0, top_k=0):
     """logits (..., V) fp32 or bf16 -> probabilities (..., V) fp32: softmax(logits / temperature)
     over each row's top_k largest logits and the equals of the last of them (over all for
-    top_k <= 0), as GPT.generate samples.  A row of -inf gives zeros; NaN or +inf gives NaN."""
+    top_k <= 0), as GPT.generate samples.  A row of -inf gives zeros; NaN or +inf gives NaN.  Without
+    a gradient (inference)."""
     if not 1e-30 <= float(temperature) <= 1e30:
         raise ValueError(f"temperature {temperature} must lie in [1e-30, 1e30]")
     r = host.sampling_probs(logits, float(temperature), int(top_k))
@@ -92,7 +94,7 @@ def compact_cache(cache, ctx, path, counts):
     for d < counts[b].  ctx, counts (B,) and path (B, N) int32 cuda, a path ascending
     (verify_draft's); entries outside the cache are passed over.  A tensor that is in the list more
     than once (layers that share one) is compacted once.  In place; returns ctx + counts, the new
-    lengths.  Rows past them keep what they held."""
+    lengths, which count the entries that are passed over.  Rows past them keep what they held."""
     r = host.compact_cache(cache, ctx, path, counts)
     if r is None:
         flat = [t for kv in cache for t in kv]
