@@ -542,7 +542,7 @@ int sampling_probs(const void* logits, bool bf16, float* probs, int64_t rows, in
 // One workgroup a sequence, every step of the walk in it: bound by the longest walk's passes, one behind the other on one
 // CU.  A pass is as much 64-bit arithmetic as memory: VALU issues in 55 % of the SIMDs' cycles while they have waves, and the
 // waves wait 56 % of their time for loads and barriers (a CU takes about 80 GB/s).  Rows are read in 16-byte vectors,
-// several in flight and the next ones behind them.  64 trees of 24 nodes over 131,072 ids take 62 to 74 us by the seed (two passes a sequence on
+// several in flight and the next ones behind them.  64 trees of 24 nodes over 131,072 ids take 59 to 74 us by the seed (two passes a sequence on
 // average, five or so in the longest walk; with the draft's row read at a leaf too 74 to 78), a chain of
 // five over 50,304 12.6.  Launches that share a pass over
 // several workgroups a sequence, and walk again from the start, took longer (84 us for four such launches, 101
