@@ -83,4 +83,88 @@ struct CompactArgs {
 };
 int compact_cache(const CompactArgs& a, void* stream);
 
+// ---- paged cache ----
+// Pools (N, P, Hkv, D), P = 2^shift rows a page, strides p / t / h; a row's pages are the first of its line of `table`
+// (R, M), lines `tab` apart; a page's uses count the rows that hold it.
+
+// Attention of one new token a row over its pages (paged.hip): q (R, H, D), o (R, H, D) and lse (R, H) contiguous.
+// Strides in elements, r / h.  A table entry that is no page: its keys are nobody's.
+struct PagedArgs {
+    const uint16_t *q, *knew, *vnew;
+    uint16_t *k, *v;
+    const int32_t *table, *lens;
+    uint16_t* o;
+    float *lse, *work;
+    int64_t qr, qh, kp, kt, kh, vp, vt, vh, knr, knh, vnr, vnh, tab;
+    int32_t R, H, Hkv, N, shift, M, D;
+    float scale;
+};
+int64_t paged_attention_workspace(int32_t R, int32_t H, int32_t Hkv, int32_t M, int32_t shift, int32_t D);
+int paged_attention(const PagedArgs& a, void* stream);
+
+// Pages and slots for tokens to be added (pages.hip).  slots (R, most) int64, out (R) int32 the lengths after it;
+// `work`: extend_pages_workspace bytes, whose first R int4 are each row's copy: (page, to page, rows, 0), rows 0 for none.
+constexpr int kPagesRows = 8192;   // rows of a table, at most
+struct ExtendArgs {
+    int32_t *table, *uses;
+    const int32_t *lens, *add;
+    int64_t* slots;
+    int32_t *out, *work;
+    int64_t tab;
+    int32_t R, M, N, shift, most;
+    bool copies;   // false: rows whose open page others hold get nothing
+};
+int64_t extend_pages_workspace(int32_t R, int32_t M, int32_t N, int32_t shift, int32_t most);
+int extend_pages(const ExtendArgs& a, void* stream);
+// the copies of extend_pages in up to kCopyTensors pools of one shape
+constexpr int kCopyTensors = 64;
+struct CopyPagesArgs {
+    uint16_t* at[kCopyTensors];
+    int64_t sp[kCopyTensors], st[kCopyTensors], sh[kCopyTensors];
+    const int32_t* copies;
+    int32_t count, R, H, D;
+};
+int copy_pages(const CopyPagesArgs& a, void* stream);
+
+// Rows k, v (R, T, H, D) to slots (R, T) int64 of the pools; a slot outside them is passed over.  Strides r / t / h.
+struct StorePagesArgs {
+    const uint16_t *k, *v;
+    const int64_t* slots;
+    uint16_t *kp, *vp;
+    int64_t kr, kt, kh, vr, vt, vh, sr, st, kpp, kpt, kph, vpp, vpt, vph;
+    int64_t N;
+    int32_t R, T, H, D, shift;
+};
+int store_pages(const StorePagesArgs& a, void* stream);
+
+// Row r becomes row parents[r], or ends where that is no row; out (R) the lengths after it.
+struct ReorderArgs {
+    int32_t *table, *uses;
+    const int32_t *lens, *parents;
+    int32_t* out;
+    int64_t tab;
+    int32_t R, M, N, shift;
+};
+int reorder_pages(const ReorderArgs& a, void* stream);
+
+// The best K continuations of each sequence's K beams (beam.hip): logits (B, K, V) contiguous, fp32 or (bf16) bfloat16;
+// scores, weight (B, K) fp32 and done (B, K) bytes contiguous, weight and done may be null; out (B, K) fp32, rows (B, K)
+// int32, tokens (B, K) int64.  `work`: beam_select_workspace bytes.
+constexpr int kBeamMost = 32;             // beams
+constexpr int64_t kBeamVocab = 1 << 20;   // logits of a row
+struct BeamArgs {
+    const void* logits;
+    const float *scores, *weight;
+    const uint8_t* done;
+    float* out;
+    int32_t* rows;
+    int64_t* tokens;
+    void* work;
+    int64_t V, fill;
+    int32_t B, K;
+    bool bf16;
+};
+int64_t beam_select_workspace(int32_t B, int32_t K, int64_t V, bool bf16);
+int beam_select(const BeamArgs& a, void* stream);
+
 }  // namespace fx

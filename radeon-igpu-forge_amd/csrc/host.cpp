@@ -646,6 +646,183 @@ OptT compact_cache(const std::vector<std::array<Tensor, 2>>& cache, const Tensor
     return out;
 }
 
+// ---- paged cache -------------------------------------------------------------------------
+
+bool ints(const Tensor& t, int64_t n) {
+    return t.scalar_type() == at::kInt && t.is_cuda() && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+// log2 of a page's rows, a power of two from 16 to 1024; -1 for others
+int page_shift(int64_t P) {
+    for (int s = 4; s <= 10; ++s)
+        if (P == int64_t(1) << s) return s;
+    return -1;
+}
+bool table_ok(const Tensor& t, bool written) {
+    return t.dim() == 2 && t.scalar_type() == at::kInt && t.is_cuda() && t.size(0) >= 1 && t.size(1) >= 1 && t.size(0) <= 0x7fffffff &&
+           t.size(1) <= 0x7fffffff && (t.stride(1) == 1 || t.size(1) == 1) && t.stride(0) >= 0 &&
+           (!written || t.size(0) == 1 || t.stride(0) >= t.size(1));
+}
+bool pool_ok(const Tensor& t) {
+    return rows16(t, 4) && t.size(0) >= 1 && t.size(0) <= 0x7fffffff && page_shift(t.size(1)) >= 0 && t.size(2) >= 1 && t.size(2) <= 0x7fffffff;
+}
+int32_t* i32(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+// (o, lse or None), or None when a check fails
+std::optional<std::tuple<Tensor, OptT>> paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table,
+                                                        const Tensor& lens, double scale, bool want_lse, const OptT& knew, const OptT& vnew) {
+    if (!rows16(q, 3) || !pool_ok(k) || !pool_ok(v) || v.sizes() != k.sizes() || !table_ok(table, false) || knew.has_value() != vnew.has_value())
+        return std::nullopt;
+    const int64_t R = q.size(0), H = q.size(1), D = q.size(2), Hkv = k.size(2);
+    if ((D != 64 && D != 128) || k.size(3) != D || H < 1 || H > 0x7fffffff || H % Hkv || table.size(0) != R || !ints(lens, R)) return std::nullopt;
+    if (knew.has_value()) {
+        for (const Tensor* t : {&*knew, &*vnew})
+            if (!rows16(*t, 3) || t->size(0) != R || t->size(1) != Hkv || t->size(2) != D) return std::nullopt;
+        if (one_row_many(k) || one_row_many(v)) return std::nullopt;
+    }
+    same_gpu(q, k, v, table, lens, knew, vnew);
+    const c10::DeviceGuard guard(q.device());   // launches and the allocations below go to q's GPU
+    fx::PagedArgs a{};
+    a.q = bf(q), a.k = bf(k), a.v = bf(v), a.knew = bf(knew), a.vnew = bf(vnew);
+    a.table = i32(table), a.lens = i32(lens);
+    a.qr = q.stride(0), a.qh = q.stride(1);
+    a.kp = k.stride(0), a.kt = k.stride(1), a.kh = k.stride(2);
+    a.vp = v.stride(0), a.vt = v.stride(1), a.vh = v.stride(2);
+    if (knew.has_value()) {
+        a.knr = knew->stride(0), a.knh = knew->stride(1);
+        a.vnr = vnew->stride(0), a.vnh = vnew->stride(1);
+    }
+    a.tab = table.stride(0);
+    a.R = (int32_t)R, a.H = (int32_t)H, a.Hkv = (int32_t)Hkv, a.N = (int32_t)k.size(0), a.shift = page_shift(k.size(1));
+    a.M = (int32_t)table.size(1), a.D = (int32_t)D;
+    a.scale = (float)scale;
+    Tensor o = at::empty({R, H, D}, q.options()), work;
+    OptT lse;
+    if (want_lse) lse = at::empty({R, H}, as_f32(q));
+    a.o = bf(o);
+    a.lse = want_lse ? f32(*lse) : nullptr;
+    const int64_t nbytes = fx::paged_attention_workspace(a.R, a.H, a.Hkv, a.M, a.shift, a.D);
+    if (nbytes) work = at::empty({nbytes / 4}, as_f32(q));
+    a.work = nbytes ? f32(work) : nullptr;
+    check(fx::paged_attention(a, stream_of(q)), "paged_attention");
+    return std::make_tuple(o, lse);
+}
+
+// (slots, lengths), or None when a check fails; table, uses and the caches' pages changed in place
+std::optional<std::tuple<Tensor, Tensor>> extend_pages(const Tensor& table, const Tensor& lens, const Tensor& add, const Tensor& uses, int64_t page,
+                                                       int64_t most, const std::optional<std::vector<std::array<Tensor, 2>>>& cache) {
+    const int shift = page_shift(page);
+    if (!table_ok(table, true) || shift < 0 || most < 1 || most > 0x7fffffff) return std::nullopt;
+    const int64_t R = table.size(0), M = table.size(1), N = uses.numel();
+    if (R > fx::kPagesRows || N < 1 || N > 0x7fffffff || !ints(lens, R) || !ints(add, R) || !ints(uses, N)) return std::nullopt;
+    same_gpu(table, lens, add, uses);
+    if (cache.has_value()) {
+        if (cache->empty()) return std::nullopt;
+        const Tensor& c = (*cache)[0][0];
+        for (const auto& kv : *cache)
+            for (const Tensor& t : kv) {
+                if (!pool_ok(t) || t.sizes() != c.sizes() || t.size(0) != N || t.size(1) != page || t.size(3) < 8 || t.size(3) % 8 || one_row_many(t))
+                    return std::nullopt;
+                same_gpu(table, t);
+            }
+        if (page * c.size(2) * (c.size(3) / 8) > 0x7fffffff) return std::nullopt;
+    }
+    const c10::DeviceGuard guard(table.device());
+    fx::ExtendArgs a{};
+    a.table = i32(table), a.uses = i32(uses), a.lens = i32(lens), a.add = i32(add);
+    a.tab = table.stride(0);
+    a.R = (int32_t)R, a.M = (int32_t)M, a.N = (int32_t)N, a.shift = shift, a.most = (int32_t)most;
+    a.copies = cache.has_value();
+    Tensor slots = at::empty({R, most}, table.options().dtype(at::kLong)), out = at::empty({R}, lens.options());
+    Tensor work = at::empty({fx::extend_pages_workspace(a.R, a.M, a.N, a.shift, a.most) / 4}, lens.options());
+    a.slots = static_cast<int64_t*>(slots.data_ptr()), a.out = i32(out), a.work = i32(work);
+    check(fx::extend_pages(a, stream_of(table)), "extend_pages");
+    if (cache.has_value()) {
+        fx::CopyPagesArgs c{};
+        c.copies = a.work, c.R = a.R, c.H = (int32_t)(*cache)[0][0].size(2), c.D = (int32_t)(*cache)[0][0].size(3);
+        for (const auto& kv : *cache)
+            for (const Tensor& t : kv) {
+                c.at[c.count] = bf(t);
+                c.sp[c.count] = t.stride(0), c.st[c.count] = t.stride(1), c.sh[c.count] = t.stride(2);
+                if (++c.count == fx::kCopyTensors) {
+                    check(fx::copy_pages(c, stream_of(table)), "extend_pages");
+                    c.count = 0;
+                }
+            }
+        if (c.count) check(fx::copy_pages(c, stream_of(table)), "extend_pages");
+    }
+    return std::make_tuple(slots, out);
+}
+
+// whether the rows were written; false when a check fails
+bool store_pages(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& kp, const Tensor& vp) {
+    if (!rows16(k, 4) || !rows16(v, 4) || v.sizes() != k.sizes() || !pool_ok(kp) || !pool_ok(vp) || vp.sizes() != kp.sizes() || one_row_many(kp) ||
+        one_row_many(vp))
+        return false;
+    const int64_t R = k.size(0), T = k.size(1), H = k.size(2), D = k.size(3);
+    if (R < 1 || T < 1 || R > 0x7fffffff || T > 0x7fffffff || kp.size(2) != H || kp.size(3) != D || D < 8 || D % 8 || slots.dim() != 2 ||
+        slots.size(0) != R || slots.size(1) != T || slots.scalar_type() != at::kLong || !slots.is_cuda() || D > 0x7fffffff)
+        return false;
+    same_gpu(k, v, slots, kp, vp);
+    const c10::DeviceGuard guard(k.device());
+    fx::StorePagesArgs a{};
+    a.k = bf(k), a.v = bf(v), a.kp = bf(kp), a.vp = bf(vp);
+    a.slots = static_cast<int64_t*>(slots.data_ptr());
+    a.kr = k.stride(0), a.kt = k.stride(1), a.kh = k.stride(2);
+    a.vr = v.stride(0), a.vt = v.stride(1), a.vh = v.stride(2);
+    a.sr = slots.stride(0), a.st = slots.stride(1);
+    a.kpp = kp.stride(0), a.kpt = kp.stride(1), a.kph = kp.stride(2);
+    a.vpp = vp.stride(0), a.vpt = vp.stride(1), a.vph = vp.stride(2);
+    a.N = kp.size(0);
+    a.R = (int32_t)R, a.T = (int32_t)T, a.H = (int32_t)H, a.D = (int32_t)D, a.shift = page_shift(kp.size(1));
+    check(fx::store_pages(a, stream_of(k)), "store_pages");
+    return true;
+}
+
+// the lengths after it, or None when a check fails; table and uses changed in place
+OptT reorder_pages(const Tensor& table, const Tensor& lens, const Tensor& parents, const Tensor& uses, int64_t page) {
+    const int shift = page_shift(page);
+    if (!table_ok(table, true) || shift < 0) return std::nullopt;
+    const int64_t R = table.size(0), N = uses.numel();
+    if (R > fx::kPagesRows || N < 1 || N > 0x7fffffff || !ints(lens, R) || !ints(parents, R) || !ints(uses, N)) return std::nullopt;
+    same_gpu(table, lens, parents, uses);
+    const c10::DeviceGuard guard(table.device());
+    fx::ReorderArgs a{};
+    a.table = i32(table), a.uses = i32(uses), a.lens = i32(lens), a.parents = i32(parents);
+    a.tab = table.stride(0);
+    a.R = (int32_t)R, a.M = (int32_t)table.size(1), a.N = (int32_t)N, a.shift = shift;
+    Tensor out = at::empty({R}, lens.options());
+    a.out = i32(out);
+    check(fx::reorder_pages(a, stream_of(table)), "reorder_pages");
+    return out;
+}
+
+// (scores, rows, tokens), or None when a check fails
+std::optional<std::tuple<Tensor, Tensor, Tensor>> beam_select(const Tensor& logits, const Tensor& scores, const OptT& done, int64_t fill,
+                                                              const OptT& weight) {
+    const bool b = is_bf(logits);
+    if ((!b && logits.scalar_type() != at::kFloat) || !logits.is_cuda() || logits.dim() != 3 || !logits.is_contiguous() || !aligned(logits))
+        return std::nullopt;
+    const int64_t B = logits.size(0), K = logits.size(1), V = logits.size(2);
+    if (B < 1 || K < 1 || K > fx::kBeamMost || V < 1 || V > fx::kBeamVocab || B * K > 0x7fffffff) return std::nullopt;
+    auto beams = [&](const Tensor& t, at::ScalarType want) {
+        return t.scalar_type() == want && t.is_cuda() && t.dim() == 2 && t.size(0) == B && t.size(1) == K && t.is_contiguous();
+    };
+    if (!beams(scores, at::kFloat) || (weight.has_value() && !beams(*weight, at::kFloat)) || (done.has_value() && !beams(*done, at::kBool)))
+        return std::nullopt;
+    same_gpu(logits, scores, done, weight);
+    const c10::DeviceGuard guard(logits.device());
+    fx::BeamArgs a{};
+    a.logits = logits.data_ptr(), a.scores = f32(scores), a.weight = weight.has_value() ? f32(*weight) : nullptr;
+    a.done = done.has_value() ? static_cast<uint8_t*>(done->data_ptr()) : nullptr;
+    a.V = V, a.fill = fill, a.B = (int32_t)B, a.K = (int32_t)K, a.bf16 = b;
+    Tensor out = at::empty({B, K}, scores.options()), rows = at::empty({B, K}, scores.options().dtype(at::kInt)),
+           tokens = at::empty({B, K}, scores.options().dtype(at::kLong));
+    Tensor work = at::empty({fx::beam_select_workspace(a.B, a.K, V, b) / 8}, tokens.options());
+    a.out = f32(out), a.rows = i32(rows), a.tokens = static_cast<int64_t*>(tokens.data_ptr()), a.work = work.data_ptr();
+    check(fx::beam_select(a, stream_of(logits)), "beam_select");
+    return std::make_tuple(out, rows, tokens);
+}
+
 // ---- optimiser -------------------------------------------------------------------------
 
 // The flat layout of FlatAdamW: per parameter its offset, size and weight-decay flag.
@@ -741,6 +918,11 @@ PYBIND11_MODULE(_host, m) {
     FX_DEF(sampling_probs);
     FX_DEF(verify_draft);
     FX_DEF(compact_cache);
+    FX_DEF(paged_attention);
+    FX_DEF(extend_pages);
+    FX_DEF(store_pages);
+    FX_DEF(reorder_pages);
+    FX_DEF(beam_select);
     FX_DEF(ce_inv_nvalid);
     FX_DEF(ce_rows);
     FX_DEF(ce_finalize);

@@ -7,6 +7,8 @@ Hand-written HIP kernels behind the reference's Python surface
   - fused RMSNorm
   - drafted decoding: tree attention over the KV cache, sampling probabilities, draft
     verification, cache compaction
+  - a paged KV cache: page tables and slots, stores, reordering, attention over pages; beam
+    selection
   - FlatAdamW (fp32 master + bf16 params + dynamic loss scale)
 
 Lazy exports: ``from fxlm.env import setup_lm_env`` does not import torch.
@@ -27,6 +29,12 @@ __all__ = [
     "sampling_probs",
     "verify_draft",
     "compact_cache",
+    "paged_attention",
+    "extend_pages",
+    "store_pages",
+    "reorder_pages",
+    "PagedCache",
+    "beam_select",
 ]
 
 
@@ -34,7 +42,7 @@ def __getattr__(name):
     if name in ("setup_lm_env", "require_gpu"):
         from . import env as _m
         return getattr(_m, name)
-    if name in ("flash_attention", "flash_attention_qkv", "tree_attention"):
+    if name in ("flash_attention", "flash_attention_qkv", "tree_attention", "paged_attention"):
         from . import attention as _m
         return getattr(_m, name)
     if name in ("fused_cross_entropy", "linear_cross_entropy"):
@@ -49,6 +57,12 @@ def __getattr__(name):
     if name in ("sampling_probs", "verify_draft", "compact_cache"):
         from . import speculative as _m
         return getattr(_m, name)
+    if name in ("extend_pages", "store_pages", "reorder_pages", "PagedCache"):
+        from . import paged as _m
+        return getattr(_m, name)
+    if name == "beam_select":
+        from .beam import beam_select
+        return beam_select
     if name in ("GPT", "GPTConfig"):
         from . import model as _m
         return getattr(_m, name)

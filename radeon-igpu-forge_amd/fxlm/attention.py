@@ -264,3 +264,73 @@ def _check_tree(q, k_cache, v_cache, ctx, tree, first, k_new, v_new):
         raise TypeError(f"ctx must be an int32 cuda tensor of shape ({B},)")
     if tree.dtype != torch.int64 or not tree.is_cuda or tree.shape != (B, N):
         raise TypeError(f"tree must be an int64 cuda tensor of shape ({B}, {N}) or ({N},)")
+
+
+def paged_attention(q, k_pages, v_pages, table, lens, scale=None, return_lse=False, k_new=None, v_new=None):
+    """One new query per (row, head) over a paged KV cache (inference).
+
+    q (R, H, Dh) bf16; k_pages, v_pages (N, P, Hkv, Dh) bf16, H a multiple of Hkv (query head h reads
+    key head h // (H // Hkv)); P a power of two from 16 to 1024, Dh 64 or 128, unit stride along Dh, the
+    other strides multiples of 8 (a page's rows less than 2^23 elements apart).  table (R, M) int32
+    cuda, unit stride along M: row r's pages in order, key j in page table[r, j // P] at j % P; lens
+    (R,) int32 cuda: the keys of each row, the new token's own included (at most M P).  Entries behind
+    a row's pages may be anything; the keys of an entry that is no page of the N are nobody's.
+    Returns o (R, H, Dh) bf16 = softmax(scale q K^T) V over the row's keys, zeros for a row without
+    any, and, if asked, the fp32 logsumexp (R, H) (-inf for such a row).  Rows may share pages.
+    k_new, v_new (R, Hkv, Dh), both or neither: the new tokens' keys and values, which the kernel uses
+    as key lens[r] - 1 and writes to its page (which no other row may hold: extend_pages sees to that);
+    without them the pages hold it already.  scale (1 / sqrt(Dh) by default) is positive and finite.
+    """
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    r = host.paged_attention(q, k_pages, v_pages, table, lens, float(scale), return_lse, k_new, v_new)
+    if r is None:
+        _check_paged(q, k_pages, v_pages, table, lens, k_new, v_new)
+        r = host.paged_attention(q, k_pages, v_pages, table if table.stride(1) == 1 else table.contiguous(), lens.contiguous(), float(scale),
+                                 return_lse, k_new, v_new)
+        if r is None:
+            raise ValueError(f"paged_attention: sizes that it does not take: {tuple(q.shape)} over {tuple(k_pages.shape)}")
+    return r if return_lse else r[0]
+
+
+def _check_paged(q, k_pages, v_pages, table, lens, k_new, v_new):
+    """Raise for what paged_attention does not take."""
+    if q.dim() != 3 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError(f"q (R,H,Dh) and pages (N,P,Hkv,Dh): {tuple(q.shape)} {tuple(k_pages.shape)} {tuple(v_pages.shape)}")
+    R, H, Dh = q.shape
+    N, P, Hkv = k_pages.shape[:3]
+    if k_pages.shape[3] != Dh or Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError(f"q {tuple(q.shape)} does not match the pages {tuple(k_pages.shape)}")
+    if Dh not in (64, 128):
+        raise ValueError(f"head_dim {Dh} not supported (must be 64 or 128)")
+    check_page(P)
+    if R < 1 or N < 1:
+        raise ValueError(f"invalid shape: {tuple(q.shape)} over {tuple(k_pages.shape)}")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    for nm, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if k_new is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{nm}: expanded pages cannot take k_new and v_new")
+    for nm, t in (("k_new", k_new), ("v_new", v_new)):
+        if t is not None and tuple(t.shape) != (R, Hkv, Dh):
+            raise ValueError(f"{nm} {tuple(t.shape)} must be (R, Hkv, Dh) = {(R, Hkv, Dh)}")
+    for nm, t in (("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("k_new", k_new), ("v_new", v_new)):
+        if t is None:
+            continue
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{nm} must be bfloat16, got {t.dtype}")
+        if not t.is_cuda:
+            raise TypeError(f"{nm} must be a cuda tensor")
+        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+            raise ValueError(f"{nm}: last dim must be contiguous, other strides multiples of 8 "
+                             "elements and the base 16-byte aligned")
+    if table.dtype != torch.int32 or not table.is_cuda or table.dim() != 2 or table.shape[0] != R or table.shape[1] < 1:
+        raise TypeError(f"table must be an int32 cuda tensor of shape ({R}, M)")
+    if lens.dtype != torch.int32 or not lens.is_cuda or lens.shape != (R,):
+        raise TypeError(f"lens must be an int32 cuda tensor of shape ({R},)")
+
+
+def check_page(page):
+    """Raise for what no page's number of rows can be."""
+    if page not in (16, 32, 64, 128, 256, 512, 1024):
+        raise ValueError(f"pages of {page} rows (must be a power of two from 16 to 1024)")

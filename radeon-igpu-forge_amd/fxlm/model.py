@@ -19,10 +19,12 @@ from torch import nn
 from fxgpu.abi import host
 from fxgpu.fused_linear import FEW_ROWS, fused_linear, fused_mlp, linear, linear_ex
 
-from .attention import decode_attention, flash_attention_qkv, tree_attention
+from .attention import decode_attention, flash_attention_qkv, paged_attention, tree_attention
+from .beam import beam_select
 from .cross_entropy import linear_cross_entropy
 from .embedding import token_embedding
 from .norm import add_pre_norm, pre_norm, rms_norm
+from .paged import PagedCache, store_pages
 from .speculative import compact_cache, sampling_probs, verify_draft
 
 
@@ -99,13 +101,14 @@ class Block(nn.Module):
         x = x + r
         return x, self._norm(x, w)
 
-    def forward(self, x, kv=None):
+    def forward(self, x, kv=None, slots=None):
         """kv: optional (k_cache, v_cache) (B, Tmax, H, Dh) that receive this block's
-        keys and values at positions 0..T-1 (the prompt of a cached generation)."""
-        x, out = self.forward_pair(x, None, kv)
+        keys and values at positions 0..T-1 (the prompt of a cached generation); with
+        slots (B, T), a paged cache's pools, which receive them there."""
+        x, out = self.forward_pair(x, None, kv, slots)
         return x + out
 
-    def forward_pair(self, x, branch=None, kv=None):
+    def forward_pair(self, x, branch=None, kv=None, slots=None):
         """(x', out) with the block's output x' + out (ml/fxlm/model.py:58-72), the last
         residual sum left to the next norm that reads it; `branch`, the previous block's
         `out`, is added to x inside this block's first norm."""
@@ -115,7 +118,9 @@ class Block(nn.Module):
         else:
             x, h = self._add_prenorm(x, branch, self.ln1_w)
         qkv = self._lin(h, self.qkv).view(B, T, 3, self.n_head, self.head_dim)
-        if kv is not None:
+        if slots is not None:
+            store_pages(qkv[:, :, 1], qkv[:, :, 2], slots, kv[0], kv[1])
+        elif kv is not None:
             kv[0][:, :T].copy_(qkv[:, :, 1])
             kv[1][:, :T].copy_(qkv[:, :, 2])
         if self.attn_impl == "flash":
@@ -162,6 +167,23 @@ class Block(nn.Module):
             qkv = self._lin(self._norm(x, self.ln1_w), self.qkv)
         q, k, v = qkv.view(B, N, 3, self.n_head, self.head_dim).unbind(2)
         y = tree_attention(q, kv[0], kv[1], ctx, tree, first=first, k_new=k, v_new=v).view(B, N, D)
+        if fused:
+            x = linear_ex(y, self.proj.weight, residual=x)
+            u = linear_ex(x, self.fc.weight, norm_weight=self.ln2_w, eps=self.eps, activation="gelu_tanh")
+            return linear_ex(u, self.fc2.weight, residual=x)
+        return self._mlp(x + self._lin(y, self.proj))
+
+    def paged_step(self, x, kv, table, lens):
+        """One new token a row, x (R, 1, D): step() over a paged cache's pools, each row at the position
+        lens[r] - 1 of its own."""
+        R, _, D = x.shape
+        fused = self._fused_step(R)
+        if fused:
+            qkv = linear_ex(x, self.qkv.weight, norm_weight=self.ln1_w, eps=self.eps)
+        else:
+            qkv = self._lin(self._norm(x, self.ln1_w), self.qkv)
+        q, k, v = qkv.view(R, 3, self.n_head, self.head_dim).unbind(1)
+        y = paged_attention(q, kv[0], kv[1], table, lens, k_new=k, v_new=v).view(R, 1, D)
         if fused:
             x = linear_ex(y, self.proj.weight, residual=x)
             u = linear_ex(x, self.fc.weight, norm_weight=self.ln2_w, eps=self.eps, activation="gelu_tanh")
@@ -361,13 +383,130 @@ class GPT(nn.Module):
         the next call."""
         return _DecodeGraph(self, cache, batch)
 
+    # -- a paged cache: rows of unlike lengths, and beams that share their prompt -----------
+
+    def paged_cache(self, rows, pages, page=16, max_len=None):
+        """A cache of `pages` pages of `page` rows for `rows` rows of up to max_len (seq_len) tokens each
+        (fxlm.PagedCache)."""
+        cfg = self.cfg
+        T = cfg.seq_len if max_len is None else min(int(max_len), cfg.seq_len)
+        return PagedCache(rows, pages, page, -(-T // page), cfg.n_layer, cfg.n_head, cfg.d_model // cfg.n_head, self.pos_emb.device)
+
     @torch.no_grad()
-    def generate(self, idx, max_new, temperature=0.8, top_k=50, generator=None, graph=True):
+    def paged_prefill(self, idx, lens, cache, rows=None):
+        """Run prompts idx (B, T) int64, of lens (B,) int32 tokens each and padding of any kind behind them,
+        into rows (B,) of a paged cache (an int64 tensor of unlike rows; by default its first B); what
+        these held ends.  Returns the logits (B, V) fp32 after each prompt, NaN for one that is empty or
+        that the cache has no pages for."""
+        if self.cfg.attn_impl != "flash":
+            raise ValueError("cached inference needs attn_impl='flash'")
+        B, T = idx.shape
+        if lens.shape != (B,) or B > cache.lens.numel() or (rows is not None and rows.shape != (B,)):
+            raise ValueError(f"lens and rows ({B},) of a cache of {cache.lens.numel()} rows: {tuple(lens.shape)} {None if rows is None else tuple(rows.shape)}")
+        if T > self.cfg.seq_len:
+            raise ValueError(f"T={T} > seq_len={self.cfg.seq_len}")
+        if rows is None:
+            rows = torch.arange(B, device=idx.device)
+        cache.end(rows)
+        add = torch.zeros_like(cache.lens)
+        add[rows] = lens.to(add.dtype)
+        slots = cache.extend(add, T)[rows]
+        x = self.tok_emb(torch.where(slots >= 0, idx, 0)) + self.pos_emb[:T]
+        for blk, kv in zip(self.blocks, cache.kv):
+            x = blk(x, kv, slots)
+        have = cache.lens[rows].long()
+        x = x[torch.arange(B, device=idx.device), (have - 1).clamp_min(0)]
+        x = self._head(self._norm_f(x.contiguous())).float()
+        return x.masked_fill((have == 0)[:, None], math.nan)
+
+    @torch.no_grad()
+    def paged_step(self, tok, cache, on=None):
+        """One token more for each row of a paged cache that has some (and whose on (R,) bool is true):
+        tok (R,) int64 at each row's own position; returns the logits (R, V) fp32, NaN for the other rows
+        and for those without a page, a position or an id for the token (the cache of the last is
+        longer by a token of NaN)."""
+        R = cache.lens.numel()
+        if tok.shape != (R,):
+            raise ValueError(f"tok must be ({R},), got {tuple(tok.shape)}")
+        L = self.pos_emb.shape[0]
+        add = (cache.lens > 0) & (cache.lens < L)
+        if on is not None:
+            add &= on
+        served = cache.extend(add.int())[:, 0] >= 0
+        lens = torch.where(served, cache.lens, 0)
+        at = torch.where(served, cache.lens - 1, L)   # a row of NaN for the others
+        x = None
+        if _table_lookup(self.tok_emb):
+            x = host.tree_embed(tok[:, None], cache.lens.new_zeros(1), at, tok.new_ones(1), 0, L + 1, self.tok_emb.weight, self.pos_emb)
+        if x is None:
+            t = tok.clamp(0, self.tok_emb.num_embeddings - 1)
+            x = self.tok_emb(t[:, None]) + self.pos_emb[at.clamp_max(L - 1)][:, None]
+            x = x.masked_fill(((t != tok) | (at == L))[:, None, None], math.nan)
+        for blk, kv in zip(self.blocks, cache.kv):
+            x = blk.paged_step(x, kv, cache.table, lens)
+        if self.blocks and self.blocks[0]._fused_step(R):
+            logits = host.few_rows_logits(x[:, 0], self._head_w(), self.lnf_w, self.cfg.eps)
+            if logits is None:
+                logits = linear_ex(x[:, 0], self._head_w(), norm_weight=self.lnf_w, eps=self.cfg.eps).float()
+            return logits
+        return self._head(self._norm_f(x)[:, 0]).float()
+
+    @torch.no_grad()
+    def beam_search(self, idx, max_new, beams=4, lens=None, eos=None, length_penalty=0.0, page=16, graph=True):
+        """The `beams` likeliest continuations by max_new tokens that a beam search finds after each of the
+        prompts idx (B, T), of lens (B,) int32 tokens (T by default).  A beam that draws the token `eos` is
+        done and goes on by it without cost.  Beams are ranked by their log-probability over their length
+        to the power length_penalty.  Returns tokens (B, beams, max_new) int64 and log-probabilities
+        (B, beams) fp32, best first; a beam that does not exist (fewer than `beams` continuations) has
+        -inf.  The beams of a prompt share its pages; a step is replayed from a HIP graph when `graph`."""
+        B, T = idx.shape
+        K, L = int(beams), self.cfg.seq_len
+        if T + max_new > L:
+            raise ValueError(f"{T} + {max_new} tokens > seq_len={L}")
+        if not 1 <= K <= 32:
+            raise ValueError(f"{beams} beams (1 to 32)")
+        dev, R = idx.device, B * K
+        if lens is not None:
+            _check_prompts(lens, T)
+        if max_new < 1 or B < 1:
+            return idx.new_zeros(B, K, max(max_new, 0)), torch.zeros(B, K, device=dev)
+        # each prompt's pages, and for each beam those behind the prompt's full ones
+        cache = self.paged_cache(R, B * -(-T // page) + R * (-(-(T + max_new) // page) - (T if lens is None else 0) // page), page, T + max_new)
+        if lens is None:
+            lens = torch.full((B,), T, dtype=torch.int32, device=dev)
+        first = torch.arange(0, R, K, device=dev)
+        logits = torch.empty(B, K, self.cfg.vocab_size, device=dev)
+        logits[:, 0] = self.paged_prefill(idx, lens, cache, first)
+        s = _Beams(self, cache, K, eos, length_penalty)
+        s.scores[:, 0] = 0.0
+        s.choose(logits)
+        step = (lambda: s.choose(self.paged_step(s.tok, cache, ~s.done.view(-1)).view(B, K, -1)))
+        if graph and max_new > 2:
+            step = s.graph(step)
+        toks, parents = [s.tok.clone()], [s.parents.clone()]
+        for _ in range(max_new - 1):
+            step()
+            toks.append(s.tok.clone())
+            parents.append(s.parents.clone())
+        # back from each beam's last token to its first
+        toks, parents, scores = torch.stack(toks).cpu(), torch.stack(parents).cpu().long(), s.scores.cpu()
+        _check_finite(not bool(scores.isnan().any()))
+        row, out = torch.arange(R), torch.empty(R, max_new, dtype=torch.int64)
+        for t in range(max_new - 1, -1, -1):
+            out[:, t] = toks[t, row]
+            row = parents[t, row].clamp_min(0)
+        return out.view(B, K, max_new).to(dev), s.scores.clone()
+
+    @torch.no_grad()
+    def generate(self, idx, max_new, temperature=0.8, top_k=50, generator=None, graph=True, lens=None):
         """Sample max_new tokens after idx (B, T) as ml/fxlm/sample.py:62-73 does
         (temperature, top-k, multinomial); returns (B, max_new) int64.  While the
         context fits seq_len each token is one cached step (replayed from a HIP graph
         when `graph`); past it, as in the reference, the model re-runs the last seq_len
-        tokens."""
+        tokens.  lens (B,) int32: prompts of unlike lengths, padding of any kind behind
+        them; they go through a paged cache, and T + max_new tokens have to fit seq_len."""
+        if lens is not None:
+            return self._generate_paged(idx, max_new, temperature, top_k, generator, graph, lens)
         x = idx
         B = idx.shape[0]
         L = self.cfg.seq_len
@@ -380,11 +519,7 @@ class GPT(nn.Module):
         for _ in range(max_new):
             if logits is None:  # context beyond seq_len: re-run the cropped window
                 logits = self(x[:, -L:])[:, -1, :].float()
-            logits = logits / max(temperature, 1e-5)
-            if top_k > 0:
-                v, _ = torch.topk(logits, min(top_k, logits.shape[-1]))
-                logits = logits.masked_fill(logits < v[:, -1:], -float("inf"))
-            nxt = torch.multinomial(torch.softmax(logits, dim=-1), 1, generator=generator)
+            nxt = _sample(logits, temperature, top_k, generator)
             out.append(nxt)
             x = torch.cat([x, nxt], dim=1)
             pos = x.shape[1] - 1
@@ -393,6 +528,26 @@ class GPT(nn.Module):
             logits = step(nxt[:, 0], pos) if step is not None and pos < cache[0][0].shape[1] else None
         return torch.cat(out, dim=1) if out else idx.new_zeros(B, 0)
 
+    def _generate_paged(self, idx, max_new, temperature, top_k, generator, graph, lens):
+        B, T = idx.shape
+        if T + max_new > self.cfg.seq_len:
+            raise ValueError(f"{T} + {max_new} tokens > seq_len={self.cfg.seq_len}")
+        if max_new < 1 or B < 1:
+            return idx.new_zeros(B, 0)
+        _check_prompts(lens, T)
+        cache = self.paged_cache(B, B * -(-(T + max_new) // 16), 16, T + max_new)
+        logits = self.paged_prefill(idx, lens, cache)
+        tok = idx.new_zeros(B)
+        step = (lambda: self.paged_step(tok, cache))
+        if graph and max_new > 2:
+            step = _captured(step, [tok, cache.table, cache.lens, cache.uses])
+        out = []
+        for i in range(max_new):
+            out.append(_sample(logits, temperature, top_k, generator))
+            if i + 1 < max_new:
+                tok.copy_(out[-1][:, 0])
+                logits = step()
+        return torch.cat(out, dim=1)
 
     @torch.no_grad()
     def speculate(self, idx, max_new, draft, branches=(2, 2, 1), temperature=0.8, top_k=50, generator=None, proposals="sampled"):
@@ -473,6 +628,69 @@ class GPT(nn.Module):
         return torch.tensor([o[:max_new] for o in out], dtype=torch.int64, device=dev)
 
 
+def _sample(logits, temperature, top_k, generator):
+    """A token (B, 1) for each row of logits (B, V) (ml/fxlm/sample.py:66-71)"""
+    logits = logits / max(temperature, 1e-5)
+    if top_k > 0:
+        v, _ = torch.topk(logits, min(top_k, logits.shape[-1]))
+        logits = logits.masked_fill(logits < v[:, -1:], -float("inf"))
+    return torch.multinomial(torch.softmax(logits, dim=-1), 1, generator=generator)
+
+
+def _captured(step, state):
+    """step, a function of tensors that it keeps in place, as a HIP graph to replay; `state` are the tensors that the warm-up
+    must leave as they are.  What step returns is reused by the next replay."""
+    saved = [t.clone() for t in state]
+    dev = state[0].device
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step()
+            for t, old in zip(state, saved):
+                t.copy_(old)
+    torch.cuda.current_stream(dev).wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+
+    def replay():
+        g.replay()
+        return out
+    return replay
+
+
+class _Beams:
+    """What a beam search's step changes, in place: the beams' scores, last tokens and parents, who is done, their lengths, and
+    the rows of the cache that they go on from."""
+
+    def __init__(self, model, cache, K, eos, length_penalty):
+        R, dev = cache.lens.numel(), cache.lens.device
+        self.cache, self.eos, self.penalty = cache, -1 if eos is None else int(eos), float(length_penalty)
+        self.scores = torch.full((R // K, K), -math.inf, device=dev)
+        self.done = torch.zeros(R // K, K, dtype=torch.bool, device=dev)
+        self.length = torch.zeros(R // K, K, device=dev)
+        self.tok = torch.zeros(R, dtype=torch.int64, device=dev)
+        self.parents = torch.zeros(R, dtype=torch.int32, device=dev)
+
+    def choose(self, logits):
+        """The best continuations by logits (B, K, V): the beams from here on."""
+        length = self.length + (~self.done)
+        weight = length.clamp_min(1).pow(-self.penalty) if self.penalty else None
+        scores, parents, tok = beam_select(logits, self.scores, self.done, max(self.eos, 0), weight)
+        row = parents.view(-1).clamp_min(0).long()
+        self.scores.copy_(scores)
+        self.parents.copy_(parents.view(-1))
+        self.tok.copy_(tok.view(-1))
+        self.length.view(-1).copy_(length.view(-1)[row])
+        self.done.view(-1).copy_(self.done.view(-1)[row] | (self.tok == self.eos))
+        self.cache.reorder(self.parents)
+
+    def graph(self, step):
+        c = self.cache
+        return _captured(step, [self.scores, self.done, self.length, self.tok, self.parents, c.table, c.lens, c.uses])
+
+
 def _drawable(p):
     """p, probabilities that are about to be drawn from, and (1,) whether every row has them: a row of logits that were not
     finite has none, and becomes one that can be drawn from."""
@@ -483,6 +701,12 @@ def _drawable(p):
 def _check_finite(ok):
     if not ok:
         raise RuntimeError("the model's logits are not finite: there is no next token to draw")
+
+
+def _check_prompts(lens, T):
+    """Refuse lengths of prompts that a batch padded to T does not have (one read of device values)."""
+    if bool(((lens < 1) | (lens > T)).any()):
+        raise ValueError(f"prompts of {lens.tolist()} tokens (1 to {T})")
 
 
 def _check_pos(pos, cache_len, positions):
