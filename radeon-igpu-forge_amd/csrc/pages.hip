@@ -241,21 +241,44 @@ int copy_pages(const CopyPagesArgs& a, void* stream) {
 
 // ---- store -------------------------------------------------------------------------------
 //
-// HBM-bound: every new row is read once and written once, 16 bytes a lane.
+// HBM-bound: every new row is read once and written once, 16 bytes a lane.  A workgroup takes some tokens of a row of
+// the batch, a thread four pieces of them at a time.
 
-__global__ void __launch_bounds__(256) store_pages_kernel(StorePagesArgs a) {
-    const int per = a.D / 8;
-    const int64_t n = (int64_t)a.R * a.T * a.H * per, step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-        const int d = (int)(i % per);
-        const int64_t x = i / per, rt = x / a.H;
-        const int h = (int)(x - rt * a.H), r = (int)(rt / a.T), t = (int)(rt - (int64_t)r * a.T);
-        const int64_t slot = a.slots[r * a.sr + t * a.st];
-        if (slot < 0 || slot >= a.N << a.shift) continue;
-        const int64_t page = slot >> a.shift, j = slot & ((1 << a.shift) - 1);
-        const uint4 k = ld16(a.k + r * a.kr + t * a.kt + h * a.kh + d * 8), v = ld16(a.v + r * a.vr + t * a.vt + h * a.vh + d * 8);
-        st16(a.kp + page * a.kpp + j * a.kpt + h * a.kph + d * 8, k);
-        st16(a.vp + page * a.vpp + j * a.vpt + h * a.vph + d * 8, v);
+struct StorePlan {
+    int32_t tokens, units;   // of a workgroup; 16-byte pieces of a token
+};
+
+__global__ void __launch_bounds__(256) store_pages_kernel(StorePagesArgs a, StorePlan p) {
+    const int r = blockIdx.y, t0 = blockIdx.x * p.tokens, n = min(p.tokens, a.T - t0) * p.units, per = a.D / 8;
+    const int64_t* slots = a.slots + r * a.sr;
+    const uint16_t *k = a.k + r * a.kr, *v = a.v + r * a.vr;
+    constexpr int U = 4;
+    for (int i0 = threadIdx.x; i0 < n; i0 += 256 * U) {
+        int64_t slot[U];
+        uint4 x[U], y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 256 * u, t = t0 + i / p.units;
+            slot[u] = i < n ? slots[t * a.st] : -1;
+            if (slot[u] >= a.N << a.shift) slot[u] = -1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 256 * u, tt = i / p.units, e = i - tt * p.units, h = e / per, d = (e - h * per) * 8;
+            if (slot[u] >= 0) {
+                x[u] = ld16_nt(k + (t0 + tt) * a.kt + h * a.kh + d);
+                y[u] = ld16_nt(v + (t0 + tt) * a.vt + h * a.vh + d);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 256 * u, tt = i / p.units, e = i - tt * p.units, h = e / per, d = (e - h * per) * 8;
+            if (slot[u] >= 0) {
+                const int64_t page = slot[u] >> a.shift, j = slot[u] & ((1 << a.shift) - 1);
+                st16(a.kp + page * a.kpp + j * a.kpt + h * a.kph + d, x[u]);
+                st16(a.vp + page * a.vpp + j * a.vpt + h * a.vph + d, y[u]);
+            }
+        }
     }
 }
 
@@ -266,8 +289,13 @@ int store_pages(const StorePagesArgs& a, void* stream) {
     const int64_t s[] = {a.kr, a.kt, a.kh, a.vr, a.vt, a.vh, a.kpp, a.kpt, a.kph, a.vpp, a.vpt, a.vph};
     for (int64_t x : s) FX_REQUIRE(x % 8 == 0, "store_pages: strides must be multiples of 8 elements");
     FX_REQUIRE((((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15) == 0, "store_pages: 16-byte aligned tensors");
-    const int64_t n = (int64_t)a.R * a.T * a.H * (a.D / 8), blocks = (n + 255) / 256, most = 16 * (int64_t)device_cus();
-    hipLaunchKernelGGL(store_pages_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, (hipStream_t)stream, a);
+    FX_REQUIRE((int64_t)a.H * (a.D / 8) < (1 << 24) && a.R <= 65535, "store_pages: %d rows of %d x %d are too many or too wide", a.R, a.H, a.D);
+    StorePlan p{};
+    p.units = a.H * (a.D / 8);
+    p.tokens = p.units >= 2048 ? 1 : 2048 / p.units;   // two turns of a thread
+    const dim3 grid((unsigned)((a.T + p.tokens - 1) / p.tokens), (unsigned)a.R);
+    FX_REQUIRE((int64_t)grid.x * 256 <= 0xffffffffLL, "store_pages: %d tokens are too many", a.T);
+    hipLaunchKernelGGL(store_pages_kernel, grid, dim3(256), 0, (hipStream_t)stream, a, p);
     return check_launch("store_pages");
 }
 
@@ -275,47 +303,50 @@ int store_pages(const StorePagesArgs& a, void* stream) {
 //
 // A workgroup a few columns of the table, for all rows at once: what the rows held is in LDS before
 // any of it is overwritten, so it is done in place.  A page that row p held is now held by as many rows as went on from
-// p: its uses change by one less than that.
+// p: its uses change by one less than that.  Bounded by its chain of round trips (lengths, entries, and
+// what is written) up to some megabytes of table.
 
-__global__ void __launch_bounds__(256) reorder_kernel(ReorderArgs a, int C) {
-    extern __shared__ int32_t lds[];
-    int32_t *children = lds, *was = lds + a.R;
-    const int c0 = blockIdx.x * C;
-    auto length = [&](int r) { return pages_len(a.lens[r], a.M, a.shift); };
-    auto parent = [&](int r) {
-        const int p = a.parents[r];
-        return (uint32_t)p < (uint32_t)a.R ? p : -1;
-    };
+constexpr int kReorderLds = 32768;   // ints: two a row, and its columns
+
+__global__ void __launch_bounds__(kPagesThreads) reorder_kernel(ReorderArgs a, int cols) {
+    __shared__ int32_t lds[kReorderLds];
+    int32_t *parent = lds, *state = lds + a.R, *was = state + a.R;   // state: the row's columns here, and 64 times the rows that go on from it
+    const int C = 1 << cols, c0 = blockIdx.x * C, threads = blockDim.x;
     bool any = false;
-    for (int r = threadIdx.x; r < a.R; r += 256) {
-        children[r] = 0;
-        any |= pages_of(length(r), a.shift) > c0;
+    for (int r = threadIdx.x; r < a.R; r += threads) {
+        const int p = a.parents[r], n = min(max(pages_of(pages_len(a.lens[r], a.M, a.shift), a.shift) - c0, 0), C);
+        parent[r] = (uint32_t)p < (uint32_t)a.R ? p : -1;
+        state[r] = n;
+        any |= n > 0;
+        if (blockIdx.x == 0) a.out[r] = (uint32_t)p < (uint32_t)a.R ? pages_len(a.lens[p], a.M, a.shift) : 0;
     }
-    const bool mine = __syncthreads_or(any);
+    any = __syncthreads_or(any);
+    if (!any) return;   // no row has a page here
     __syncthreads();
-    if (blockIdx.x == 0)
-        for (int r = threadIdx.x; r < a.R; r += 256) {
-            const int p = parent(r);
-            a.out[r] = p < 0 ? 0 : length(p);
+    for (int r = threadIdx.x; r < a.R; r += threads)
+        if (parent[r] >= 0) atomicAdd(&state[parent[r]], 64);
+    const int n = a.R << cols;
+    constexpr int U = 4;
+    for (int i0 = threadIdx.x; i0 < n; i0 += threads * U) {
+        int x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * threads, r = i >> cols, c = i & (C - 1);
+            x[u] = i < n && c < (state[r] & 63) ? a.table[(int64_t)r * a.tab + c0 + c] : -1;
         }
-    if (!mine) return;   // no row has a page here
-    for (int r = threadIdx.x; r < a.R; r += 256) {
-        const int p = parent(r);
-        if (p >= 0) atomicAdd(&children[p], 1);
-    }
-    for (int i = threadIdx.x; i < a.R * C; i += 256) {
-        const int r = i / C, c = i - r * C;
-        if (c0 + c < pages_of(length(r), a.shift)) was[i] = a.table[(int64_t)r * a.tab + c0 + c];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * threads < n) was[i0 + u * threads] = x[u];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < a.R * C; i += 256) {
-        const int r = i / C, c = i - r * C;
-        if (c0 + c < pages_of(length(r), a.shift)) {
-            const int p = was[i], d = children[r] - 1;
-            if (d != 0 && (uint32_t)p < (uint32_t)a.N) atomicAdd(&a.uses[p], d);
+    for (int i = threadIdx.x; i < n; i += threads) {
+        const int r = i >> cols, c = i & (C - 1), s = state[r];
+        if (c < (s & 63) && s >> 6 != 1) {
+            const int p = was[i];
+            if ((uint32_t)p < (uint32_t)a.N) atomicAdd(&a.uses[p], (s >> 6) - 1);
         }
-        const int from = parent(r);
-        if (from >= 0 && from != r && c0 + c < pages_of(length(from), a.shift)) a.table[(int64_t)r * a.tab + c0 + c] = was[from * C + c];
+        const int from = parent[r];
+        if (from >= 0 && from != r && c < (state[from] & 63)) a.table[(int64_t)r * a.tab + c0 + c] = was[(from << cols) + c];
     }
 }
 
@@ -324,9 +355,10 @@ int reorder_pages(const ReorderArgs& a, void* stream) {
     FX_REQUIRE(a.M >= 1 && a.N >= 1 && a.shift >= 0 && a.shift <= 20 && ((int64_t)a.M << a.shift) <= 0x7fffffff - 128,
                "reorder_pages: bad shape M=%d N=%d shift=%d", a.M, a.N, a.shift);
     FX_REQUIRE(a.table && a.uses && a.lens && a.parents && a.out, "reorder_pages: null pointer");
-    int C = 16;
-    while (C > 1 && (int64_t)a.R * (C + 1) * 4 > 65536) C /= 2;
-    hipLaunchKernelGGL(reorder_kernel, dim3((unsigned)((a.M + C - 1) / C)), dim3(256), (size_t)a.R * (C + 1) * 4, (hipStream_t)stream, a, C);
+    int cols = 3;
+    while ((int64_t)a.R * ((1 << cols) + 2) > kReorderLds) --cols;
+    const int64_t n = (int64_t)a.R << cols;
+    hipLaunchKernelGGL(reorder_kernel, dim3((unsigned)((a.M + (1 << cols) - 1) >> cols)), dim3(n <= 512 ? 256 : kPagesThreads), 0, (hipStream_t)stream, a, cols);
     return check_launch("reorder_pages");
 }
 
