@@ -50,6 +50,7 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
 // chunks of a row, and logits of each (a whole number of vectors; the last is shorter)
 struct BeamPlan {
     int32_t chunks, length;
+    bool few;   // short chunks
 };
 
 // the workspace: of each row and chunk the best K (logit's key, complement of the token; 0: none), then the maximum and sum
@@ -63,115 +64,143 @@ __device__ __forceinline__ bool beam_goes_on(const BeamArgs& a, int64_t row) {
     return !(a.done && a.done[row]) && s == s && s != kBeamNegInf;
 }
 
+// A thread's part of a chunk: NR vectors of 16 bytes, as they lie in memory.  What a pass makes of a vector is not kept for the next.
 template <bool BF, int NR>
-__global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a, BeamPlan plan) {
+struct BeamChunk {
+    static constexpr int NP = BF ? 8 : 4;
+    uint4 raw[NR];
+    float edge;           // one logit of the ragged ends
+    int tok0, edge_tok;   // the tokens of the first vector's first value (below 0: of the row before) and of the edge
+
+    __device__ __forceinline__ static void unpack(const uint4& u, float* f) {
+        if constexpr (BF) unpack8(u, f);
+        else f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+    }
+    // flat places [i0, i1) of the logits, in a row that begins at `row`; what is not theirs is -inf: neither listed nor summed
+    __device__ __forceinline__ void load(const void* logits, int64_t i0, int64_t i1, int64_t row) {
+        const int64_t f0 = i0 / NP * NP;
+        const char* base = static_cast<const char*>(logits) + f0 * (BF ? 2 : 4);
+        const int lo = (int)(i0 - f0), hi = (int)(i1 - f0), tid = threadIdx.x, whole = hi / NP;   // places from f0 on; whole vectors end here
+        const uint32_t ninf = BF ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int v = tid + i * kBeamThreads;
+            raw[i] = make_uint4(ninf, ninf, ninf, ninf);
+            if (v < whole && (v > 0 || lo == 0)) raw[i] = ld16(base + (uint32_t)v * 16u);
+        }
+        // the first vector's, where it is not whole, by the first threads; the last one's by the next
+        const int at = tid < NP ? tid : whole * NP + tid - NP;
+        const bool mine = tid < NP ? (lo > 0 || whole == 0) && at >= lo && at < hi : tid < 2 * NP && whole > 0 && at < hi;
+        edge = kBeamNegInf;
+        if (mine) edge = BF ? bf16_to_f32(reinterpret_cast<const uint16_t*>(base)[at]) : reinterpret_cast<const float*>(base)[at];
+        tok0 = (int)(f0 - row) + tid * NP;
+        edge_tok = (int)(f0 - row) + at;
+    }
+    // f(its number, its values, the first value's token) of every vector
+    template <typename Fn>
+    __device__ __forceinline__ void each(Fn f) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            asm volatile("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z), "+v"(raw[i].w));
+            float x[NP];
+            unpack(raw[i], x);
+            f(i, x, (uint32_t)(tok0 + i * kBeamThreads * NP));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+__device__ __forceinline__ uint64_t beam_entry(float x, uint32_t tok) { return (uint64_t)beam_key(x) << 32 | (0xffffffffu - tok); }
+
+template <bool BF, int NR>
+__global__ void __launch_bounds__(kBeamThreads, 8) beam_chunk_kernel(BeamArgs a, BeamPlan plan) {
     constexpr int NP = BF ? 8 : 4;
-    __shared__ float gmax[kBeamWaves][64], shm[kBeamWaves], shs[kBeamWaves];
-    __shared__ uint32_t bound;
+    __shared__ float gmax[kBeamWaves][64], shs[kBeamWaves];
     __shared__ int listed;
     __shared__ uint64_t list[kBeamList];
     const int64_t row = blockIdx.x / plan.chunks;
     const int chunk = (int)(blockIdx.x - row * plan.chunks);
     if (!beam_goes_on(a, row)) return;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    // flat places: the chunk's first and last, and the first vector
-    const int64_t i0 = row * a.V + (int64_t)chunk * plan.length;
-    const int64_t i1 = min(i0 + plan.length, (row + 1) * a.V), f0 = i0 / NP * NP;
-
-    float x[NR][NP];
-    uint4 raw[NR];
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-        const int64_t f = f0 + (int64_t)(i * kBeamThreads + tid) * NP;
-        const uint32_t ninf = BF ? 0xff80ff80u : 0xff800000u;
-        raw[i] = make_uint4(ninf, ninf, ninf, ninf);
-        if (f >= i0 && f + NP <= i1) raw[i] = ld16(static_cast<const char*>(a.logits) + f * (BF ? 2 : 4));
-    }
-    float own = kBeamNegInf;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-        const int64_t f = f0 + (int64_t)(i * kBeamThreads + tid) * NP;
-        if constexpr (BF) unpack8(raw[i], x[i]);
-        else x[i][0] = __uint_as_float(raw[i].x), x[i][1] = __uint_as_float(raw[i].y), x[i][2] = __uint_as_float(raw[i].z), x[i][3] = __uint_as_float(raw[i].w);
-        if (f < i1 && f + NP > i0 && !(f >= i0 && f + NP <= i1)) {   // the chunk's ragged ends
-#pragma unroll
-            for (int e = 0; e < NP; ++e)
-                if (f + e >= i0 && f + e < i1)
-                    x[i][e] = BF ? bf16_to_f32(static_cast<const uint16_t*>(a.logits)[f + e]) : static_cast<const float*>(a.logits)[f + e];
-        }
-#pragma unroll
-        for (int e = 0; e < NP; e += 2) {
-            own = fmaxf(own, fmaxf(x[i][e], x[i][e + 1]));
-            nan |= __builtin_isunordered(x[i][e], x[i][e + 1]);
-        }
-    }
-    // the sum above the thread's own maximum, before the workgroup waits for the slowest of its loads
-    const float mine = own == kBeamNegInf ? 0.f : own;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NR; ++i)
-#pragma unroll
-        for (int e = 0; e < NP; ++e) s += exp2_fast((x[i][e] - mine) * kLog2e);
-
+    const int64_t i0 = row * a.V + (int64_t)chunk * plan.length, i1 = min(i0 + plan.length, (row + 1) * a.V);
+    BeamChunk<BF, NR> c;
+    c.load(a.logits, i0, i1, row * a.V);
     if (tid == 0) listed = 0;
-    gmax[w][lane] = own;
-    nan = __syncthreads_or(nan);
-    __syncthreads();
-    float m = kBeamNegInf;
-    if (w == 0) {
-        float g = gmax[0][lane];
+    float own = c.edge, most[NR];   // the thread's largest, and each vector's
+    c.each([&](int i, const float* x, uint32_t) {
+        most[i] = fmaxf(x[0], x[1]);
 #pragma unroll
-        for (int i = 1; i < kBeamWaves; ++i) g = fmaxf(g, gmax[i][lane]);
-        const uint32_t k = beam_key(g);
-        uint32_t lo = k, hi = k;
+        for (int e = 2; e < NP; e += 2) most[i] = fmaxf(most[i], fmaxf(x[e], x[e + 1]));
+        own = fmaxf(own, most[i]);
+    });
+    // The sum above the thread's own maximum, before the workgroup waits for the slowest of its loads: the exponent x log2 e - c is
+    // rounded once, and what c, the maximum's, is rounded by is taken from the sum.  A NaN or +inf makes it NaN.
+    const float mine = own == kBeamNegInf ? 0.f : own, ref = mine * kLog2e;
+    float s;
+    if (fabsf(mine) < 1e38f) {
+        s = exp2_fast(fmaf(c.edge, kLog2e, -ref));
+        c.each([&](int, const float* x, uint32_t) {
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            lo = min(lo, (uint32_t)__shfl_xor((int)lo, off, 64));
-            hi = max(hi, (uint32_t)__shfl_xor((int)hi, off, 64));
-        }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = __builtin_amdgcn_readfirstlane(hi);
-        if (lane == 0) shm[0] = beam_logit(hi);
-        // a bound with K or a few more group maxima at or above it
-        int have = 64;
-        while (lo < hi && have > a.K + a.K / 4) {
-            const uint32_t mid = lo + (hi - lo) / 2 + 1;
-            const int c = __popcll(__ballot(k >= mid));
-            if (c >= a.K) lo = mid, have = c;
-            else hi = mid - 1;
-        }
-        if (lane == 0) bound = lo;
+            for (int e = 0; e < NP; ++e) s += exp2_fast(fmaf(x[e], kLog2e, -ref));
+            asm volatile("" : "+v"(s));
+        });
+        s *= exp2_fast(-fmaf(mine, kLog2e, -ref));
+    } else {   // c would be past the type's range (masks of its lowest value)
+        s = exp2_fast((c.edge - mine) * kLog2e);
+        c.each([&](int, const float* x, uint32_t) {
+#pragma unroll
+            for (int e = 0; e < NP; ++e) s += exp2_fast((x[e] - mine) * kLog2e);
+            asm volatile("" : "+v"(s));
+        });
     }
+    gmax[w][lane] = s != s ? s : own;
     __syncthreads();
-    m = shm[0];
-    const float least = beam_logit(bound);
+    // every wave by itself: the chunk's maximum, and a bound with K or a few more group maxima at or above it
+    float g = gmax[0][lane];
+    bool bad = g != g;
+#pragma unroll
+    for (int i = 1; i < kBeamWaves; ++i) bad |= gmax[i][lane] != gmax[i][lane], g = fmaxf(g, gmax[i][lane]);
+    const float m = group_max<64>(g);
     const int64_t place = row * plan.chunks + chunk;
     uint64_t* out = beam_lists(a) + place * a.K;
     float2* stat = beam_stats(a, plan) + place;
-    if (nan || m == __builtin_huge_valf()) {   // no sum: the beam's score is NaN
+    if (__ballot(bad)) {   // no sum: the beam's score is NaN
         if (tid == 0) *stat = make_float2(__builtin_nanf(""), 0.f);
         for (int i = tid; i < a.K; i += kBeamThreads) out[i] = 0;
         return;
     }
-    s *= exp2_fast((mine - m) * kLog2e);   // a thread without logits: mine is 0 and s 0
-    if (own == kBeamNegInf) s = 0.f;
+    const uint32_t k = beam_key(g), top = beam_key(m);
+    // (logits of -inf continue nothing)
+    uint32_t lo = beam_key(kBeamNegInf) + 1, hi = top;
+    int have = __popcll(__ballot(k >= lo));
+    if (have > a.K) {
+        // the search begins above the least of the maxima
+        const uint32_t least = beam_key(-group_max<64>(k >= lo ? -g : kBeamNegInf));
+        lo = __builtin_amdgcn_readfirstlane(least);
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        while (lo < hi && have > a.K + a.K / 4) {
+            const uint32_t mid = lo + (hi - lo) / 2 + 1;
+            const int n = __popcll(__ballot(k >= mid));
+            if (n >= a.K) lo = mid, have = n;
+            else hi = mid - 1;
+        }
+    }
+    s = own == kBeamNegInf ? 0.f : s * exp2_fast((mine - m) * kLog2e);
     s = group_sum<64>(s);
     if (lane == 0) shs[w] = s;
-
-    auto key = [&](int i, int e) {
-        const uint32_t tok = (uint32_t)(f0 + (int64_t)(i * kBeamThreads + tid) * NP + e - row * a.V);
-        return (uint64_t)beam_key(x[i][e]) << 32 | (0xffffffffu - tok);
+    const float least = beam_logit(lo);
+    auto put = [&](float x, uint32_t tok) {
+        const int at = atomicAdd(&listed, 1);
+        if (at < kBeamList) list[at] = beam_entry(x, tok);
     };
-    if (own >= least && own > kBeamNegInf) {
+    if (own >= least) {
+        c.each([&](int i, const float* x, uint32_t tok) {
+            if (most[i] >= least)
 #pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int e = 0; e < NP; ++e)
-                if (x[i][e] >= least && x[i][e] > kBeamNegInf) {
-                    const int at = atomicAdd(&listed, 1);
-                    if (at < kBeamList) list[at] = key(i, e);
-                }
+                for (int e = 0; e < NP; ++e)
+                    if (x[e] >= least) put(x[e], tok + e);
+        });
+        if (c.edge >= least) put(c.edge, c.edge_tok);
     }
     __syncthreads();
     if (tid == 0) {
@@ -183,25 +212,23 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a, Be
     const int n = listed;
     if (n <= kBeamList) {
         for (int i = tid; i < n; i += kBeamThreads) {
-            const uint64_t k = list[i];
+            const uint64_t x = list[i];
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += list[j] > k;
-            if (rank < a.K) out[rank] = k;
+            for (int j = 0; j < n; ++j) rank += list[j] > x;
+            if (rank < a.K) out[rank] = x;
         }
         for (int i = n + tid; i < a.K; i += kBeamThreads) out[i] = 0;
         return;
     }
-    // many equals: the best one by one, each below the last
+    // many equals: the best one by one, each below the last, from memory
     uint64_t last = ~0ull;
     for (int j = 0; j < a.K; ++j) {
         uint64_t best = 0;
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int e = 0; e < NP; ++e) {
-                const uint64_t k = x[i][e] > kBeamNegInf ? key(i, e) : 0;
-                if (k < last && k > best) best = k;
-            }
+        for (int64_t f = i0 + tid; f < i1; f += kBeamThreads) {
+            const float x = BF ? bf16_to_f32(static_cast<const uint16_t*>(a.logits)[f]) : static_cast<const float*>(a.logits)[f];
+            const uint64_t y = x > kBeamNegInf ? beam_entry(x, (uint32_t)(f - row * a.V)) : 0;
+            if (y < last && y > best) best = y;
+        }
         best = wave_max64(best);
         __syncthreads();   // the last round's are read
         if (lane == 0) list[w] = best;
@@ -214,102 +241,177 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a, Be
     }
 }
 
-// A workgroup a sequence.  A wave a row at a time: the sum of its chunks' exponentials, and its best K of the
-// chunks' lists, which are sorted: a lane holds the head of a list.  Then one wave merges the rows' lists the same way.
-__global__ void __launch_bounds__(1024) beam_join_kernel(BeamArgs a, BeamPlan plan) {
-    __shared__ uint64_t best[kBeamMost][kBeamMost];
-    __shared__ float top[kBeamMost];      // a row's largest logit, and the logarithm of its sum
-    __shared__ double logs[kBeamMost];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int64_t row0 = (int64_t)blockIdx.x * a.K;
-    for (int k = w; k < a.K; k += waves) {
+// A continuation as it is ranked: its rank's key, then one of the beam, the logit and the token
+struct BeamRank {
+    uint64_t rank, rest;
+    __device__ __forceinline__ bool above(const BeamRank& o) const { return rank > o.rank || (rank == o.rank && rest > o.rest); }
+};
+
+// A workgroup a sequence.  The chunks' lists are sorted, so of a set of lists the best K continuations lie in the K with the best
+// heads: first of each row's lists, then of all rows'; the continuations of these K that are not below the last of their heads are
+// ranked.  All ranking is by counting, of a few threads for each.
+constexpr int kBeamJoin = 1024, kBeamChunks = 130;
+constexpr int kBeamStage = kBeamMost * kBeamChunks;   // entries in LDS
+
+struct BeamJoin {
+    uint64_t stage[kBeamStage];                 // the lists, or their heads
+    BeamRank cand[kBeamMost * kBeamMost];       // the rows' best heads, then the last lists' continuations
+    uint64_t entry[kBeamMost * kBeamMost];      // and their entries
+    int from[kBeamMost * kBeamMost];            // the heads' lists, the continuations' rows
+    int some[kBeamMost * kBeamMost];            // which of the heads may be among the best
+    int chosen[kBeamMost], kind[kBeamMost], n, m, last;
+    float top[kBeamMost], score[kBeamMost];     // a row's largest logit, its score
+    double logs[kBeamMost], weight[kBeamMost];  // the logarithm of its sum, its weight
+};
+
+__global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPlan plan) {
+    __shared__ BeamJoin j;
+    enum { kNone, kLogits, kItself, kNaN };     // a row's continuations: none, those of its logits, itself, itself as NaN
+    constexpr int kParts = (kBeamChunks + 63) / 64;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, threads = blockDim.x, S = plan.chunks, K = a.K;
+    const int64_t row0 = (int64_t)blockIdx.x * K;
+    const uint64_t* lists = beam_lists(a) + row0 * S * K;
+    const int each = min(K, S);   // lists of a row that remain
+    const bool all = K * S * K <= kBeamStage;
+    const int hop = all ? K : 1;
+    // (of a row without continuations by its logits, whatever lies there)
+    if (all)
+        for (int i = tid; i < K * S * K; i += threads) j.stage[i] = lists[i];
+    else
+        for (int i = tid; i < K * S; i += threads) j.stage[i] = lists[(int64_t)i * K];
+    for (int i = tid; i < K * each; i += threads) j.cand[i] = {0, 0};
+    if (tid < K) j.chosen[tid] = -1;
+    if (tid == 0) j.n = j.m = 0;
+    for (int k = w; k < K; k += threads / 64) {
         const int64_t row = row0 + k;
-        if (!beam_goes_on(a, row)) continue;
-        const float2* st = beam_stats(a, plan) + row * plan.chunks;
+        const float sc = a.scores[row];
+        const bool done = a.done && a.done[row];
+        const double weight = a.weight ? (double)a.weight[row] : 1.0;
+        const float2* st = beam_stats(a, plan) + row * S;
+        float2 x[kParts];
         float m = kBeamNegInf;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) x[i] = lane + 64 * i < S ? st[lane + 64 * i] : make_float2(kBeamNegInf, 0.f);
         bool nan = false;
-        for (int c = lane; c < plan.chunks; c += 64) m = fmaxf(m, st[c].x), nan |= st[c].x != st[c].x;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) m = fmaxf(m, x[i].x), nan |= x[i].x != x[i].x;
         m = group_max<64>(m);
         double z = 0.0;
-        for (int c = lane; c < plan.chunks; c += 64)
-            if (st[c].x != kBeamNegInf) z += (double)st[c].y * exp((double)st[c].x - (double)m);
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+            if (x[i].x != kBeamNegInf) z += (double)x[i].y * exp((double)x[i].x - (double)m);
         z = group_sum_d<64>(z);
-        const bool bad = __ballot(nan) != 0;
-        if (lane == 0) top[k] = m, logs[k] = bad ? __builtin_nan("") : log(z);
-        if (bad) continue;
-        constexpr int LL = 2;   // lists of a lane: 128 chunks at most
-        const uint64_t* at[LL];
-        uint64_t head[LL], next[LL];
-        int left[LL];
-#pragma unroll
-        for (int i = 0; i < LL; ++i) {
-            const int c = lane + 64 * i;
-            at[i] = beam_lists(a) + (row * plan.chunks + min(c, plan.chunks - 1)) * a.K;
-            left[i] = c < plan.chunks ? a.K : 0;
-            head[i] = left[i] > 0 ? at[i][0] : 0;
-            next[i] = left[i] > 1 ? at[i][1] : 0;
+        const int what = sc == kBeamNegInf ? kNone : sc != sc ? kNaN : done ? kItself : __ballot(nan) ? kNaN : kLogits;
+        if (lane == 0) j.kind[k] = what, j.top[k] = m, j.score[k] = sc, j.weight[k] = weight, j.logs[k] = log(z);
+    }
+    __syncthreads();
+
+    auto sum_of = [&](int k, uint64_t entry) {
+        return j.kind[k] == kLogits ? (double)j.score[k] + (((double)beam_logit((uint32_t)(entry >> 32)) - (double)j.top[k]) - j.logs[k])
+               : j.kind[k] == kItself ? (double)j.score[k] : __builtin_nan("");
+    };
+    auto ranked = [&](int k, uint64_t entry) -> BeamRank {   // {0, 0}: nothing
+        const double s = sum_of(k, entry), r = j.weight[k] * s;
+        if (s == (double)kBeamNegInf || r == (double)kBeamNegInf) return {0, 0};
+        const uint64_t rest = (uint64_t)(kBeamMost - 1 - k) << 52 | (entry >> 32) << 20 | (uint32_t)(entry - (0xffffffffull - (kBeamVocab - 1)));
+        return {rank_key(r), rest};
+    };
+    constexpr uint64_t kSelf = 0xffffffffull;   // the entry of a row that goes on as it is (a logit's key and a token of 0)
+    // a row's best heads
+    for (int i = tid; i < K * S; i += threads) {
+        const int k = i / S, c = i - k * S;
+        if (j.kind[k] == kNone) continue;
+        if (j.kind[k] != kLogits) {
+            if (c == 0) j.cand[k * each] = ranked(k, kSelf), j.from[k * each] = i;
+            continue;
         }
-        for (int j = 0; j < a.K; ++j) {
-            const uint64_t first = wave_max64(head[0] > head[1] ? head[0] : head[1]);
-            if (lane == 0) best[k][j] = first;
-#pragma unroll
-            for (int i = 0; i < LL; ++i)
-                if (first && head[i] == first) {   // keys hold their tokens: no two are alike
-                    head[i] = next[i];
-                    --left[i], ++at[i];
-                    next[i] = left[i] > 1 ? at[i][1] : 0;
-                }
+        const uint64_t x = j.stage[i * hop];
+        if (x == 0) continue;
+        int above = 0;
+        for (int o = k * S; o < k * S + S; ++o) above += j.stage[o * hop] > x;   // no two entries are alike
+        if (above < each) j.cand[k * each + above] = ranked(k, x), j.from[k * each + above] = i;
+    }
+    __syncthreads();
+    // of all rows': K of them are not below the least of the rows' best (where each row has one)
+    uint64_t least = ~0ull;
+    for (int k = 0; k < K; ++k) least = min(least, j.cand[k * each].rank);
+    for (int i = tid; i < K * each; i += threads)
+        if (j.cand[i].rank != 0 && j.cand[i].rank >= least) j.some[atomicAdd(&j.n, 1)] = i;
+    __syncthreads();
+    // G threads count what lies above the i-th of n
+    auto group = [&](int n) {
+        int G = 1;
+        while (G < 64 && 2 * G * n <= threads) G *= 2;
+        return G;
+    };
+    auto sum_group = [&](int x, int G) {
+        for (int off = 1; off < G; off *= 2) x += __shfl_xor(x, off, 64);
+        return x;
+    };
+    {
+        const int n = j.n, G = group(n);
+        for (int i0 = 0; i0 < n; i0 += threads / G) {   // (all of a wave's threads take part in the exchange)
+            const int i = i0 + tid / G;
+            const int at = j.some[min(i, n - 1)];
+            const BeamRank x = j.cand[at];
+            int above = 0;
+            for (int o = tid % G; o < n; o += G) above += j.cand[j.some[o]].above(x);
+            above = sum_group(above, G);
+            if (i < n && tid % G == 0 && above < K) {
+                j.chosen[above] = j.from[at];
+                if (above == K - 1) j.last = at;
+            }
         }
     }
     __syncthreads();
-    if (w != 0) return;
-    // lane k: the head of row k's list
-    const int k = lane;
-    const int64_t row = row0 + min(k, a.K - 1);
-    const float score = a.scores[row];
-    const bool goes = beam_goes_on(a, row), single = !goes && (a.done && a.done[row] ? score != kBeamNegInf : score != score);
-    const double weight = a.weight ? (double)a.weight[row] : 1.0, most = top[min(k, a.K - 1)], less = logs[min(k, a.K - 1)];
-    const bool bad = goes && less != less;
-    int j = 0;
-    double sum = 0.0;
-    uint64_t rank = 0;
-    auto take = [&] {   // the list's head: its score and rank; the least rank where there is none
-        rank = 0;
-        sum = (double)kBeamNegInf;
-        if (k >= a.K) return;
-        if (goes && !bad) {
-            const uint64_t b = j < a.K ? best[k][j] : 0;
-            if (b) sum = (double)score + (((double)beam_logit((uint32_t)(b >> 32)) - most) - less);
-        } else if (j == 0 && (single || bad)) {
-            sum = bad ? __builtin_nan("") : (double)score;
-        }
-        const double r = sum == (double)kBeamNegInf ? sum : weight * sum;
-        rank = r == (double)kBeamNegInf ? 0 : rank_key(r);
-    };
-    take();
-    for (int i = 0; i < a.K; ++i) {
-        const uint64_t first = wave_max64(rank);
-        const int64_t at = row0 + i;
-        if (first == 0) {
-            if (lane == 0) a.out[at] = kBeamNegInf, a.rows[at] = -1, a.tokens[at] = a.fill;
-            continue;
-        }
-        const int win = __ffsll((unsigned long long)__ballot(rank == first)) - 1;   // equals: the lower beam
-        if (lane == win) {
-            a.out[at] = (float)sum;
-            a.rows[at] = (int32_t)row;
-            a.tokens[at] = goes && !bad ? (int64_t)(0xffffffffu - (uint32_t)best[k][j]) : a.fill;
-            ++j;
-            take();
+    const uint64_t last = j.n >= K ? j.cand[j.last].rank : 1;
+    BeamRank x = {0, 0};
+    uint64_t entry = 0;
+    int k = 0;
+    if (tid < K * K) {
+        const int i = j.chosen[tid / K], o = tid % K;
+        if (i >= 0) {
+            k = i / S;
+            if (j.kind[k] == kLogits) entry = all ? j.stage[i * K + o] : lists[(int64_t)i * K + o];
+            else if (o == 0) entry = kSelf;
+            if (entry) x = ranked(k, entry);
         }
     }
+    __syncthreads();   // the heads have been read
+    if (x.rank >= last && x.rank != 0) {
+        const int at = atomicAdd(&j.m, 1);
+        j.cand[at] = x;
+        j.entry[at] = entry;
+        j.from[at] = k;
+    }
+    __syncthreads();
+    const int n = j.m, G = group(n);
+    for (int i0 = 0; i0 < n; i0 += threads / G) {
+        const int i = i0 + tid / G;
+        const BeamRank y = j.cand[min(i, n - 1)];
+        int above = 0;
+        for (int o = tid % G; o < n; o += G) above += j.cand[o].above(y);
+        above = sum_group(above, G);
+        if (i < n && tid % G == 0 && above < K) {
+            const int r = j.from[i];
+            a.out[row0 + above] = (float)sum_of(r, j.entry[i]);
+            a.rows[row0 + above] = (int32_t)(row0 + r);
+            a.tokens[row0 + above] = j.kind[r] == kLogits ? (int64_t)(0xffffffffu - (uint32_t)j.entry[i]) : a.fill;
+        }
+    }
+    for (int i = n + tid; i < K; i += threads) a.out[row0 + i] = kBeamNegInf, a.rows[row0 + i] = -1, a.tokens[row0 + i] = a.fill;
 }
 
+// Chunks of 8,192 places, or of 2,048 while that leaves CUs without one.  (A chunk's first logit may lie
+// inside a vector: so many places hold a vector's values less.)
 static BeamPlan beam_plan(int32_t B, int32_t K, int64_t V, bool bf16) {
     BeamPlan p{};
-    constexpr int64_t most = 8192;
-    p.chunks = (int32_t)((V + most - 1) / most);
-    p.length = (int32_t)(((V + p.chunks - 1) / p.chunks + 7) / 8 * 8);
+    const int64_t slack = bf16 ? 8 : 4, rows = (int64_t)B * K;
+    const bool few = rows * ((V + 8191) / 8192) <= device_cus() && V <= 2040 * kBeamChunks;
+    const int64_t most = (few ? 2048 : 8192) - slack;
+    p.few = few;
+    const int64_t n = (V + most - 1) / most;
+    p.length = (int32_t)(((V + n - 1) / n + slack - 1) / slack * slack);
     p.chunks = (int32_t)((V + p.length - 1) / p.length);
     return p;
 }
@@ -326,16 +428,18 @@ int beam_select(const BeamArgs& a, void* stream) {
     FX_REQUIRE(a.logits && a.scores && a.out && a.rows && a.tokens && a.work, "beam_select: null pointer");
     FX_REQUIRE((((uintptr_t)a.logits | (uintptr_t)a.work) & 15) == 0, "beam_select: logits and work must be 16-byte aligned");
     const BeamPlan p = beam_plan(a.B, a.K, a.V, a.bf16);
-    const int64_t grid = (int64_t)a.B * a.K * p.chunks;
-    FX_REQUIRE(grid < (1 << 23), "beam_select: too many rows");   // a launch has less than 2^32 work items
-    // NR vectors a thread: one more vector than the chunk's, where its first logit is not a vector's first
-    if (a.bf16)
-        hipLaunchKernelGGL((beam_chunk_kernel<true, 5>), dim3((unsigned)grid), dim3(kBeamThreads), 0, (hipStream_t)stream, a, p);
-    else
-        hipLaunchKernelGGL((beam_chunk_kernel<false, 9>), dim3((unsigned)grid), dim3(kBeamThreads), 0, (hipStream_t)stream, a, p);
+    const int64_t chunks = (int64_t)a.B * a.K * p.chunks;
+    FX_REQUIRE(chunks < (1 << 24) && p.chunks <= kBeamChunks, "beam_select: too many rows");   // a launch has less than 2^32 work items
+    const dim3 grid((unsigned)chunks), block(kBeamThreads);
+    const hipStream_t st = (hipStream_t)stream;
+    if (a.bf16 && p.few) hipLaunchKernelGGL((beam_chunk_kernel<true, 1>), grid, block, 0, st, a, p);
+    else if (a.bf16) hipLaunchKernelGGL((beam_chunk_kernel<true, 4>), grid, block, 0, st, a, p);
+    else if (p.few) hipLaunchKernelGGL((beam_chunk_kernel<false, 2>), grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL((beam_chunk_kernel<false, 8>), grid, block, 0, st, a, p);
     if (int e = check_launch("beam_select")) return e;
-    const int waves = a.K < 16 ? a.K : 16;
-    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)a.B), dim3(64 * waves), 0, (hipStream_t)stream, a, p);
+    // a wave a row, and a thread for each continuation of the last lists (K K <= 64 K up to 32 beams: two rows a wave past 16)
+    const int threads = 64 * (a.K < 4 ? 4 : a.K < 16 ? a.K : 16);
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)a.B), dim3((unsigned)threads), 0, st, a, p);
     return check_launch("beam_select_join");
 }
 
