@@ -99,7 +99,7 @@ struct PagedArgs {
     int32_t R, H, Hkv, N, shift, M, D;
     float scale;
 };
-int64_t paged_attention_workspace(int32_t R, int32_t H, int32_t Hkv, int32_t M, int32_t shift, int32_t D);
+int64_t paged_attention_workspace(int32_t R, int32_t H, int32_t Hkv, int32_t N, int32_t M, int32_t shift, int32_t D);
 int paged_attention(const PagedArgs& a, void* stream);
 
 // Pages and slots for tokens to be added (pages.hip).  slots (R, most) int64, out (R) int32 the lengths after it;

@@ -700,7 +700,7 @@ std::optional<std::tuple<Tensor, OptT>> paged_attention(const Tensor& q, const T
     if (want_lse) lse = at::empty({R, H}, as_f32(q));
     a.o = bf(o);
     a.lse = want_lse ? f32(*lse) : nullptr;
-    const int64_t nbytes = fx::paged_attention_workspace(a.R, a.H, a.Hkv, a.M, a.shift, a.D);
+    const int64_t nbytes = fx::paged_attention_workspace(a.R, a.H, a.Hkv, a.N, a.M, a.shift, a.D);
     if (nbytes) work = at::empty({nbytes / 4}, as_f32(q));
     a.work = nbytes ? f32(work) : nullptr;
     check(fx::paged_attention(a, stream_of(q)), "paged_attention");

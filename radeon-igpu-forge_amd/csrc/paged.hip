@@ -9,10 +9,13 @@
 // new token's key and value (knew, vnew), where given, are key lens[r] - 1 and are written to its page.
 //
 // HBM-bound: every key and value is read once (4 D bytes a token and key head).  So the keys are split
-// evenly, whatever the rows' lengths: all rows' and heads' steps (a tile of 32 keys for each wave of a
-// workgroup) lie in one line, and each workgroup of one full round of CUs takes an equal piece of it,
-// over the border of a row or a head if that falls in it.  A second kernel joins the rows that were cut.
-// Small caches are not split: a workgroup a row and key head, one launch.
+// evenly, whatever the rows' lengths: all rows' and heads' steps of 32 keys lie in one line, and each
+// workgroup of one full round of CUs takes an equal piece of it, over the border of a row or a head if
+// that falls in it.  A second kernel joins the rows that were cut.  Four waves a workgroup, each with a
+// key head of its own where there are as many: no wave waits for another.  Tables of up to 1,536 keys are not split: a
+// workgroup of eight waves a row and key head, one launch (one row of 12 heads over 217 keys 5.9 us against 9.3 split,
+// 1,500 keys 11.7 / 11.5, 3,000 18.5 / 15.6; 64 rows of up to 1,500 40.3 / 41.3).
+//
 #include <math.h>
 
 #include "fx_internal.h"
@@ -26,9 +29,10 @@ constexpr float kPagedNegInf = -__builtin_huge_valf();
 constexpr float kPagedLazy = 8.f;    // the running maximum moves only past this (log2 units): p stays <= 2^8
 
 // what a kernel needs besides the arguments: groups of query heads of a key head, query heads of a group,
-// workgroups of a split launch (0: not split)
+// workgroups of a split launch (0: not split), key heads and parts of the keys of a workgroup, whether loads go past the caches
 struct PagedPlan {
-    int32_t groups, gt, split;
+    int32_t groups, gt, split, hw, kw;
+    bool once;
 };
 
 __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
@@ -41,25 +45,30 @@ __device__ __forceinline__ int paged_len(const PagedArgs& a, int n) {
     return n < 0 ? 0 : n < most ? n : (int)most;
 }
 // its steps, one at least: a row without keys has its zeros written
-template <int NW>
+template <int KW>
 __device__ __forceinline__ uint32_t paged_steps(const PagedArgs& a, int n) {
     const uint32_t l = (uint32_t)paged_len(a, n);
-    return l ? (l + kPagedTile * NW - 1) / (kPagedTile * NW) : 1u;
+    return l ? (l + kPagedTile * KW - 1) / (kPagedTile * KW) : 1u;
 }
 
 // where the join finds the pieces of a row and head group: (first workgroup, count), behind the partials
 __device__ __forceinline__ uint2* paged_places(const PagedArgs& a, const PagedPlan& p) {
-    return reinterpret_cast<uint2*>(a.work + (int64_t)2 * p.split * p.gt * (a.D + 2));
+    return reinterpret_cast<uint2*>(a.work + (int64_t)2 * p.split * p.hw * p.gt * (a.D + 2));
 }
 
-// Workgroup: NW waves, each on a part of the keys of one row and key head.  Per tile S^T = K Q^T (a lane
-// holds 8 of the 32 keys of one query head), the softmax, and O^T += V^T P^T.  Keys come from memory in the operand's own
-// layout (64 bytes of 16 rows a load); values go through the wave's own LDS in whole rows and are read transposed
-// (fx_mfma.h), keys in the order that the scores lie in.  The next tile's loads are issued as soon as the scores are
-// formed.  P >= 16, so half a tile lies in one page: addresses are a base in scalar registers and an offset that
-// does not change.  The wave holds 64 entries of the row's table in a register, and the 64 behind them.
-template <int D, int NT, int NW>
-__global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedPlan plan) {
+// Workgroup: HW key heads x KW parts of a row's keys, a wave each.  Per tile of 32 keys S^T = K Q^T (a lane
+// holds 8 of the 32 keys of one query head), the softmax, and O^T += V^T P^T.  Keys and values go through the wave's own
+// LDS in whole rows (keys straight from memory in the operand's layout, 64 bytes of 16 rows a load: rows of 64 in
+// pools of 16 heads 103 us against 98); values are read transposed (fx_mfma.h), keys in the order that the scores
+// lie in.  The next tile is in flight in registers meanwhile.  P >= 16, so half a tile lies in one page: addresses
+// are a base in scalar registers and an offset that does not change.  The wave holds 64 entries of the row's table
+// in a register, and the 64 behind them.
+// ONCE: pools that are too large to stay in the caches from one call to the next are loaded past them (64 rows of up to 6,000
+// tokens 162 -> 152 us then; a batch whose 38 MB stay there would go from 10.5 to 13.9).  Else rows may share pages, and an eighth
+// of the line goes to each XCD, whose L2 then has what a prompt's beams have in common (35 beams 38.9 -> 31.5 us).
+template <int D, int NT, int HW, int KW, bool ONCE>
+__global__ void __launch_bounds__(64 * HW * KW, 2) paged_attn_kernel(PagedArgs a, PagedPlan plan) {
+    constexpr int NW = HW * KW;
     constexpr int LPR = D / 8;         // lanes of a row in 16-byte loads
     constexpr int RPI = 64 / LPR;      // rows of a wave-wide load
     constexpr int NV = kPagedTile / RPI;
@@ -67,22 +76,25 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
     constexpr int DT = D / 16;
     constexpr int VLD = D + 16;        // LDS row of V: 8 rows of a transposed read fall in distinct banks
     constexpr int OLD = D + 4;         // LDS row of a wave's fp32 output
-    constexpr int kV = kPagedTile * VLD * 2, kO = kPagedCols * OLD * 4;
+    constexpr int KLD = D + 8;         // LDS row of K: 16 rows of an operand read fall in distinct banks
+    constexpr int kV = kPagedTile * (VLD + KLD) * 2, kO = kPagedCols * OLD * 4;
     constexpr int kWave = kV > kO ? kV : kO;
     __shared__ __attribute__((aligned(16))) unsigned char lds[NW * kWave];
     __shared__ float2 ml[NW][kPagedCols];
 
     const int lane = threadIdx.x & 63, lc = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int G = a.H / a.Hkv, heads = plan.groups * a.Hkv, rowmask = (1 << a.shift) - 1;
+    const int hw = w % HW, kw = w / HW;
+    const int G = a.H / a.Hkv, heads = plan.groups * (a.Hkv / HW), rowmask = (1 << a.shift) - 1;
     uint16_t* const vt = reinterpret_cast<uint16_t*>(lds + w * kWave);
+    uint16_t* const kt = vt + kPagedTile * VLD;
     float* const ot = reinterpret_cast<float*>(lds + w * kWave);
     const float sc = a.scale * kLog2e;
     const int vr = lane / LPR, vc = (lane % LPR) * 8;   // this lane's row of a value load and its column
 
     // this workgroup's piece of the line, and where it begins: row, head group, step
     int r = 0, hr = 0;
-    uint32_t s0 = 0, parts = 1;
+    uint32_t s0 = 0, parts = 1, piece = blockIdx.x;
     uint64_t pos = 0, stop = 0, total = 0;
     if (plan.split == 0) {
         r = blockIdx.x / heads;
@@ -90,17 +102,21 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
         stop = 1;
     } else {
         uint32_t sum = 0;
-        for (int x = lane; x < a.R; x += 64) sum += paged_steps<NW>(a, a.lens[x]);
+        for (int x = lane; x < a.R; x += 64) sum += paged_steps<KW>(a, a.lens[x]);
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
         total = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(sum) * heads;
         parts = (uint32_t)(total < (uint32_t)plan.split ? total : plan.split);   // one step each at least
         if (blockIdx.x >= parts) return;
-        pos = total * blockIdx.x / parts;
-        stop = total * (blockIdx.x + 1) / parts;
+        if constexpr (!ONCE) {   // an eighth of the line for each XCD
+            const uint32_t x = blockIdx.x % 8, each = parts / 8, more = parts % 8;
+            piece = x * each + min(x, more) + blockIdx.x / 8;
+        }
+        pos = total * piece / parts;
+        stop = total * (piece + 1) / parts;
         uint32_t at = (uint32_t)(pos / heads), before = 0;   // in steps of one head group
         for (int x0 = 0; x0 < a.R; x0 += 64) {
-            const uint32_t k = x0 + lane < a.R ? paged_steps<NW>(a, a.lens[x0 + lane]) : 0u;
+            const uint32_t k = x0 + lane < a.R ? paged_steps<KW>(a, a.lens[x0 + lane]) : 0u;
             uint32_t up = k;   // inclusive scan
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
@@ -127,9 +143,9 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
 
     while (pos < stop) {
         const int len = __builtin_amdgcn_readfirstlane(paged_len(a, a.lens[r]));
-        const uint32_t steps = paged_steps<NW>(a, len);
+        const uint32_t steps = paged_steps<KW>(a, len);
         const uint32_t n = plan.split ? (uint32_t)(stop - pos < steps - s0 ? stop - pos : steps - s0) : steps;
-        const int h = hr % a.Hkv, grp = hr / a.Hkv;
+        const int grp = hr / (a.Hkv / HW), h = (hr - grp * (a.Hkv / HW)) * HW + hw;
         const int q0 = grp * plan.gt, rows = min(plan.gt, G - q0);   // this group's first query head and their number
 
         bf16x8 qf[NT][KS];
@@ -142,15 +158,12 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
 
         // this wave's tiles
         const int tiles = (len + kPagedTile - 1) / kPagedTile;
-        const int ta = min((int)(s0 * NW), tiles), cnt = min((int)((s0 + n) * NW), tiles) - ta;
-        int t = ta + cnt * w / NW;
-        const int t1 = ta + cnt * (w + 1) / NW;
+        const int ta = min((int)(s0 * KW), tiles), cnt = min((int)((s0 + n) * KW), tiles) - ta;
+        int t = ta + cnt * kw / KW;
+        const int t1 = ta + cnt * (kw + 1) / KW;
 
         const int32_t* tab = a.table + (int64_t)r * a.tab;
-        auto window = [&](int e0) {   // 64 entries from e0 on; -1 for one that is no page
-            const int id = tab[min(e0 + lane, a.M - 1)];
-            return (uint32_t)id < (uint32_t)a.N ? id : -1;
-        };
+        auto window = [&](int e0) { return tab[min(e0 + lane, a.M - 1)]; };   // 64 entries from e0 on
 
         f32x4 acc[NT][DT];
         float m[NT], l[NT];
@@ -164,11 +177,12 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
         if (t < t1) {
             int base = ((t * kPagedTile) >> a.shift) & ~63;
             int win = window(base), nxt = window(base + 64);
-            uint4 kr[2][KS], vv[NV];
+            uint4 kk[NV], vv[NV];
             int have[2];   // keys of the loaded tile's halves
             const char* const kh = reinterpret_cast<const char*>(a.k + (int64_t)h * a.kh);
             const char* const vh = reinterpret_cast<const char*>(a.v + (int64_t)h * a.vh);
             const uint32_t kt2 = (uint32_t)a.kt * 2u, vt2 = (uint32_t)a.vt * 2u;
+            auto get = [](const char* p) { return ONCE ? ld16_nt(p) : ld16(p); };
             auto load = [&](int j0) {
                 const int b0 = (j0 >> a.shift) & ~63;
                 if (b0 != base) {
@@ -180,32 +194,30 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
                 for (int half = 0; half < 2; ++half) {
                     const int js = j0 + 16 * half, jh = min(js, (len - 1) & ~15);   // a half without keys: the last one's rows again
                     const int id = __builtin_amdgcn_readlane(win, (jh >> a.shift) & 63);
-                    const int64_t page = id < 0 ? 0 : id;
-                    have[half] = id < 0 ? 0 : max(0, min(16, len - js));
+                    const bool is = (uint32_t)id < (uint32_t)a.N;   // keys of an entry that is no page are nobody's
+                    const int64_t page = is ? id : 0;
+                    have[half] = is ? max(0, min(16, len - js)) : 0;
                     const char* kp = kh + (page * a.kp + (int64_t)(jh & rowmask) * a.kt) * 2;
                     const char* vp = vh + (page * a.vp + (int64_t)(jh & rowmask) * a.vt) * 2;
                     // rows behind the last key are its own again
-                    const uint32_t lim = (uint32_t)(len - 1 - jh), ko = __umul24(min((uint32_t)lc, lim), kt2) + 16u * g;
+                    const uint32_t lim = (uint32_t)(len - 1 - jh);
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) kr[half][s] = ld16(kp + (ko + 64u * s));
-#pragma unroll
-                    for (int i = 0; i < NV / 2; ++i) vv[half * NV / 2 + i] = ld16(vp + (__umul24(min((uint32_t)(i * RPI + vr), lim), vt2) + 2u * vc));
+                    for (int i = 0; i < NV / 2; ++i) {
+                        const uint32_t row = min((uint32_t)(i * RPI + vr), lim);
+                        kk[half * NV / 2 + i] = get(kp + (__umul24(row, kt2) + 2u * vc));
+                        vv[half * NV / 2 + i] = get(vp + (__umul24(row, vt2) + 2u * vc));
+                    }
                     if (a.knew && js < len && lim < 16) {   // the new key and value: used from here, and kept
-                        const bool keep = grp == 0 && id >= 0;
-                        if ((uint32_t)lc == lim) {
-                            const uint16_t* np = a.knew + (int64_t)r * a.knr + (int64_t)h * a.knh + 8 * g;
-                            char* to = const_cast<char*>(kp) + ko;
-#pragma unroll
-                            for (int s = 0; s < KS; ++s) {
-                                kr[half][s] = ld16(np + 32 * s);
-                                if (keep) st16(to + 64 * s, kr[half][s]);
-                            }
-                        }
+                        const bool keep = grp == 0 && is;
 #pragma unroll
                         for (int i = 0; i < NV / 2; ++i)
                             if ((uint32_t)(i * RPI + vr) == lim) {
+                                kk[half * NV / 2 + i] = ld16(a.knew + (int64_t)r * a.knr + (int64_t)h * a.knh + vc);
                                 vv[half * NV / 2 + i] = ld16(a.vnew + (int64_t)r * a.vnr + (int64_t)h * a.vnh + vc);
-                                if (keep) st16(const_cast<char*>(vp) + (__umul24(lim, vt2) + 2u * vc), vv[half * NV / 2 + i]);
+                                if (keep) {
+                                    st16(const_cast<char*>(kp) + (__umul24(lim, kt2) + 2u * vc), kk[half * NV / 2 + i]);
+                                    st16(const_cast<char*>(vp) + (__umul24(lim, vt2) + 2u * vc), vv[half * NV / 2 + i]);
+                                }
                             }
                     }
                 }
@@ -225,7 +237,10 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the last tile's reads come first
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int i = 0; i < NV; ++i) st16(vt + (i * RPI + vr) * VLD + vc, vv[i]);
+                for (int i = 0; i < NV; ++i) st16(kt + (i * RPI + vr) * KLD + vc, kk[i]), st16(vt + (i * RPI + vr) * VLD + vc, vv[i]);
+                if (t + 1 < t1) load((t + 1) * kPagedTile);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
                 f32x4 s[NT][2];
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
@@ -233,11 +248,8 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
                     for (int half = 0; half < 2; ++half) {
                         s[x][half] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int c = 0; c < KS; ++c) s[x][half] = mfma16(__builtin_bit_cast(bf16x8, kr[half][c]), qf[x][c], s[x][half]);
+                        for (int c = 0; c < KS; ++c) s[x][half] = mfma16(*reinterpret_cast<const bf16x8*>(kt + (16 * half + lc) * KLD + 32 * c + 8 * g), qf[x][c], s[x][half]);
                     }
-                if (t + 1 < t1) load((t + 1) * kPagedTile);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
                 bf16x8 hi[NT], lo[NT];
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
@@ -286,62 +298,85 @@ __global__ void __launch_bounds__(64 * NW) paged_attn_kernel(PagedArgs a, PagedP
             }
         }
 
-        // join the waves, 16 query heads at a time
         const bool whole = n == steps;
         const int64_t per = (int64_t)plan.gt * (D + 2);   // floats of a piece
-        float* piece = whole ? nullptr : a.work + (2 * (int64_t)blockIdx.x + (s0 == 0)) * per;
+        float* pieces = a.work + (2 * (int64_t)piece + (s0 == 0)) * HW * per;
         if (plan.split && s0 == 0 && threadIdx.x == 0) {   // the workgroup with the row's last step: the last one that begins at or before it
-            const uint32_t last = whole ? blockIdx.x : (uint32_t)(((pos + steps) * parts - 1) / total);
-            paged_places(a, plan)[(int64_t)r * heads + hr] = make_uint2(blockIdx.x, last - blockIdx.x + 1);
+            const uint32_t last = whole ? piece : (uint32_t)(((pos + steps) * parts - 1) / total);
+            paged_places(a, plan)[(int64_t)r * heads + hr] = make_uint2(piece, last - piece + 1);
         }
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
             float lx = l[x];
             lx += __shfl_xor(lx, 16, 64);
             lx += __shfl_xor(lx, 32, 64);
-            if (x > 0) __syncthreads();   // the last round's sums are read
-            // the wave's own values are read: its LDS operations are done in order
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-                *reinterpret_cast<float4*>(ot + lc * OLD + 16 * d + 4 * g) = make_float4(acc[x][d][0], acc[x][d][1], acc[x][d][2], acc[x][d][3]);
-            if (g == 0) ml[w][lc] = make_float2(m[x] * sc, lx);
-            __syncthreads();
             const int some = min(kPagedCols, rows - x * kPagedCols);
-            for (int i = threadIdx.x; i < some * LPR; i += 64 * NW) {
-                const int q = i / LPR, c = (i % LPR) * 8;
-                float M = kPagedNegInf;
+            const float mx = m[x] * sc;
+            if constexpr (KW == 1) {   // a wave has all of its head's keys of the segment
+                if (lc < some) {
+                    const int q = x * kPagedCols + lc;
+                    if (whole) {
+                        const float inv = lx == 0.f ? 0.f : 1.f / lx;
+                        const int64_t at = (int64_t)r * a.H + h * G + q0 + q;
 #pragma unroll
-                for (int y = 0; y < NW; ++y) M = fmaxf(M, ml[y][q].x);
-                const float mu = M == kPagedNegInf ? 0.f : M;
-                float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                        for (int d = 0; d < DT; ++d) {
+                            f32x4 y = acc[x][d] * inv;
+                            if (lx == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
+                            *reinterpret_cast<uint2*>(a.o + at * D + 16 * d + 4 * g) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+                        }
+                        if (a.lse && g == 0) a.lse[at] = lx == 0.f ? kPagedNegInf : (mx + log2_fast(lx)) * kLn2;
+                    } else {
+                        float* u = pieces + hw * per;
 #pragma unroll
-                for (int y = 0; y < NW; ++y) {
-                    const float2 z = ml[y][q];
-                    const float f = exp2_fast(z.x - mu);
-                    L += z.y * f;
-                    const float* op = reinterpret_cast<const float*>(lds + y * kWave) + q * OLD + c;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] += op[e] * f;
+                        for (int d = 0; d < DT; ++d)
+                            *reinterpret_cast<float4*>(u + q * D + 16 * d + 4 * g) = make_float4(acc[x][d][0], acc[x][d][1], acc[x][d][2], acc[x][d][3]);
+                        if (g == 0) *reinterpret_cast<float2*>(u + (int64_t)plan.gt * D + 2 * q) = make_float2(mx, lx);
+                    }
                 }
-                if (whole) {
-                    const float inv = L == 0.f ? 0.f : 1.f / L;
-                    const int64_t at = (int64_t)r * a.H + h * G + q0 + x * kPagedCols + q;
+            } else {   // join the waves of a head, 16 query heads at a time
+                if (x > 0) __syncthreads();   // the last round's sums are read
+                // the wave's own values are read: its LDS operations are done in order
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] = L == 0.f ? 0.f : o[e] * inv;
-                    st16(a.o + at * D + c, pack8(o));
-                    if (a.lse && c == 0) a.lse[at] = L == 0.f ? kPagedNegInf : (M + log2_fast(L)) * kLn2;
-                } else {
-                    float* u = piece + (x * kPagedCols + q) * D + c;
-                    *reinterpret_cast<float4*>(u) = make_float4(o[0], o[1], o[2], o[3]);
-                    *reinterpret_cast<float4*>(u + 4) = make_float4(o[4], o[5], o[6], o[7]);
-                    if (c == 0) *reinterpret_cast<float2*>(piece + (int64_t)plan.gt * D + 2 * (x * kPagedCols + q)) = make_float2(M, L);
+                for (int d = 0; d < DT; ++d)
+                    *reinterpret_cast<float4*>(ot + lc * OLD + 16 * d + 4 * g) = make_float4(acc[x][d][0], acc[x][d][1], acc[x][d][2], acc[x][d][3]);
+                if (g == 0) ml[w][lc] = make_float2(mx, lx);
+                __syncthreads();
+                for (int i = threadIdx.x; i < HW * some * LPR; i += 64 * NW) {
+                    const int b = i / (some * LPR), in = i - b * some * LPR, q = in / LPR, c = (in % LPR) * 8;   // the head among the workgroup's
+                    float M = kPagedNegInf;
+#pragma unroll
+                    for (int y = 0; y < KW; ++y) M = fmaxf(M, ml[y * HW + b][q].x);
+                    const float mu = M == kPagedNegInf ? 0.f : M;
+                    float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+                    for (int y = 0; y < KW; ++y) {
+                        const float2 z = ml[y * HW + b][q];
+                        const float f = exp2_fast(z.x - mu);
+                        L += z.y * f;
+                        const float* op = reinterpret_cast<const float*>(lds + (y * HW + b) * kWave) + q * OLD + c;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] += op[e] * f;
+                    }
+                    if (whole) {
+                        const float inv = L == 0.f ? 0.f : 1.f / L;
+                        const int64_t at = (int64_t)r * a.H + (h - hw + b) * G + q0 + x * kPagedCols + q;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] = L == 0.f ? 0.f : o[e] * inv;
+                        st16(a.o + at * D + c, pack8(o));
+                        if (a.lse && c == 0) a.lse[at] = L == 0.f ? kPagedNegInf : (M + log2_fast(L)) * kLn2;
+                    } else {
+                        float* u = pieces + b * per;
+                        *reinterpret_cast<float4*>(u + (x * kPagedCols + q) * D + c) = make_float4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<float4*>(u + (x * kPagedCols + q) * D + c + 4) = make_float4(o[4], o[5], o[6], o[7]);
+                        if (c == 0) *reinterpret_cast<float2*>(u + (int64_t)plan.gt * D + 2 * (x * kPagedCols + q)) = make_float2(M, L);
+                    }
                 }
             }
         }
         if (plan.split == 0) return;
-        __syncthreads();   // before the next segment's values are written
+        if (KW > 1) __syncthreads();   // before the next segment's values are written
         pos += n;
         s0 = 0;
         if (++hr == heads) hr = 0, ++r;
@@ -353,11 +388,11 @@ template <int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, PagedPlan plan) {
     constexpr int LPR = D / 4, NS = 64 / LPR;   // pieces read side by side
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int G = a.H / a.Hkv, heads = plan.groups * a.Hkv;
+    const int G = a.H / a.Hkv, sets = a.Hkv / plan.hw, heads = plan.groups * sets;
     const int64_t at = (int64_t)blockIdx.x * 4 + w;
     if (at >= (int64_t)a.R * a.H) return;
     const int r = (int)(at / a.H), hq = (int)(at - (int64_t)r * a.H), h = hq / G, q = hq - h * G, grp = q / plan.gt, rr = q - grp * plan.gt;
-    const uint2 place = paged_places(a, plan)[(int64_t)r * heads + grp * a.Hkv + h];
+    const uint2 place = paged_places(a, plan)[(int64_t)r * heads + grp * sets + h / plan.hw];
     const uint32_t count = place.y;
     if (count == 1) return;   // written by its workgroup
     const int64_t per = (int64_t)plan.gt * (D + 2);
@@ -381,7 +416,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, PagedPlan 
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const uint32_t k = min(u + i * NS, count - 1);
-            const float* p = a.work + (2 * (int64_t)(place.x + k) + (k == 0)) * per;
+            const float* p = a.work + ((2 * (int64_t)(place.x + k) + (k == 0)) * plan.hw + h % plan.hw) * per;
             z[i] = *reinterpret_cast<const float2*>(p + (int64_t)plan.gt * D + 2 * rr);
             x[i] = *reinterpret_cast<const float4*>(p + rr * D + c);
         }
@@ -402,35 +437,45 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, PagedPlan 
     if (a.lse && lane == 0) a.lse[at] = L == 0.f ? kPagedNegInf : (M + log2_fast(L)) * kLn2;
 }
 
-constexpr int kPagedWaves = 8;
-
-// Launch shape.
-static PagedPlan paged_plan(int32_t R, int32_t H, int32_t Hkv, int32_t M, int32_t shift) {
+// Launch shape.  One round of CUs: with two workgroups a CU 134 us for 130 (64 rows of up to 6,000 tokens), 102 for 98
+// (long rows).
+static PagedPlan paged_plan(int32_t R, int32_t H, int32_t Hkv, int32_t N, int32_t M, int32_t shift, int32_t D) {
     PagedPlan p{};
     const int G = H / Hkv;
     const int tiles = G <= kPagedCols ? 1 : 2;
     p.gt = G < kPagedCols * tiles ? G : kPagedCols * tiles;
     p.groups = (G + p.gt - 1) / p.gt;
-    const int64_t steps = (((int64_t)M << shift) + kPagedTile * kPagedWaves - 1) / (kPagedTile * kPagedWaves);
-    if (steps <= 6) return p;
-    const int64_t all = steps * R * Hkv * p.groups, most = 2 * device_cus();
+    const int64_t keys = (int64_t)M << shift;
+    p.hw = 1, p.kw = 8;
+    const int64_t pages = (int64_t)R * M < N ? (int64_t)R * M : N;
+    p.once = (pages << shift) * Hkv * D * 4 >= (int64_t)256 << 20;
+    if (keys <= 6 * 8 * kPagedTile) return p;
+    p.hw = Hkv % 4 == 0 ? 4 : Hkv % 2 == 0 ? 2 : 1;
+    p.kw = 4 / p.hw;
+    const int64_t steps = (keys + kPagedTile * p.kw - 1) / (kPagedTile * p.kw), all = steps * R * (Hkv / p.hw) * p.groups, most = device_cus();
     p.split = (int32_t)(all < most ? all : most);
     return p;
 }
 
-int64_t paged_attention_workspace(int32_t R, int32_t H, int32_t Hkv, int32_t M, int32_t shift, int32_t D) {
-    if (R < 1 || Hkv < 1 || H < Hkv || H % Hkv || M < 1 || shift < 4 || shift > 20 || (D != 64 && D != 128)) return 0;
-    const PagedPlan p = paged_plan(R, H, Hkv, M, shift);
-    return p.split == 0 ? 0 : (int64_t)2 * p.split * p.gt * (D + 2) * (int64_t)sizeof(float) + (int64_t)R * Hkv * p.groups * (int64_t)sizeof(uint2);
+int64_t paged_attention_workspace(int32_t R, int32_t H, int32_t Hkv, int32_t N, int32_t M, int32_t shift, int32_t D) {
+    if (R < 1 || Hkv < 1 || H < Hkv || H % Hkv || N < 1 || M < 1 || shift < 4 || shift > 20 || (D != 64 && D != 128)) return 0;
+    const PagedPlan p = paged_plan(R, H, Hkv, N, M, shift, D);
+    return p.split == 0 ? 0 : (int64_t)2 * p.split * p.hw * p.gt * (D + 2) * (int64_t)sizeof(float) + (int64_t)R * (Hkv / p.hw) * p.groups * (int64_t)sizeof(uint2);
+}
+
+template <int D, int NT, bool ONCE>
+static void paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)(p.split ? p.split : a.R * a.Hkv * p.groups)), block(64 * p.hw * p.kw);
+    if (p.kw == 8) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, 8, ONCE>), grid, block, 0, st, a, p);
+    else if (p.hw == 4) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 4, 1, ONCE>), grid, block, 0, st, a, p);
+    else if (p.hw == 2) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 2, 2, ONCE>), grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, 4, ONCE>), grid, block, 0, st, a, p);
 }
 
 template <int D>
 static int paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
-    const dim3 grid((unsigned)(p.split ? p.split : a.R * a.Hkv * p.groups)), block(64 * kPagedWaves);
-    if (p.gt <= kPagedCols)
-        hipLaunchKernelGGL((paged_attn_kernel<D, 1, kPagedWaves>), grid, block, 0, st, a, p);
-    else
-        hipLaunchKernelGGL((paged_attn_kernel<D, 2, kPagedWaves>), grid, block, 0, st, a, p);
+    if (p.gt <= kPagedCols) p.once ? paged_launch<D, 1, true>(a, p, st) : paged_launch<D, 1, false>(a, p, st);
+    else p.once ? paged_launch<D, 2, true>(a, p, st) : paged_launch<D, 2, false>(a, p, st);
     if (int e = check_launch("paged_attention")) return e;
     if (p.split == 0) return 0;
     hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(((int64_t)a.R * a.H + 3) / 4)), dim3(256), 0, st, a, p);
@@ -453,9 +498,9 @@ int paged_attention(const PagedArgs& a, void* stream) {
     FX_REQUIRE((((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o | (uintptr_t)a.work | (uintptr_t)a.knew |
                  (uintptr_t)a.vnew) & 15) == 0,
                "paged_attention: q, k, v, o, work, knew and vnew must be 16-byte aligned");
-    const PagedPlan p = paged_plan(a.R, a.H, a.Hkv, a.M, a.shift);
+    const PagedPlan p = paged_plan(a.R, a.H, a.Hkv, a.N, a.M, a.shift, a.D);
     const int64_t pairs = (int64_t)a.R * a.Hkv * p.groups;
-    const int64_t steps = (((int64_t)a.M << a.shift) + kPagedTile * kPagedWaves - 1) / (kPagedTile * kPagedWaves);
+    const int64_t steps = (((int64_t)a.M << a.shift) + kPagedTile * p.kw - 1) / (kPagedTile * p.kw);
     // a launch has less than 2^32 work items; a row's steps and all rows' are counted in 32 bits
     FX_REQUIRE(pairs < (1 << 23) && (int64_t)a.R * a.H < (1 << 25) && a.R * steps < 0x7fffffffLL, "paged_attention: too many rows and heads");
     FX_REQUIRE(p.split == 0 || a.work, "paged_attention: null workspace");
