@@ -247,64 +247,36 @@ struct BeamRank {
     __device__ __forceinline__ bool above(const BeamRank& o) const { return rank > o.rank || (rank == o.rank && rest > o.rest); }
 };
 
-// A workgroup a sequence.  The chunks' lists are sorted, so of a set of lists the best K continuations lie in the K with the best
-// heads: first of each row's lists, then of all rows'; the continuations of these K that are not below the last of their heads are
-// ranked.  All ranking is by counting, of a few threads for each.
+// A workgroup a sequence.  The chunks' lists are sorted, so the best K continuations lie in the K lists with the best heads; of
+// these lists' continuations those that are not below the last of their heads are ranked.  Only heads that are not below the
+// least of the rows' best are looked at (where each row has one, K are not).  All ranking is by counting, of a few
+// threads for each.
 constexpr int kBeamJoin = 1024, kBeamChunks = 130;
 constexpr int kBeamStage = kBeamMost * kBeamChunks;   // entries in LDS
 
 struct BeamJoin {
     uint64_t stage[kBeamStage];                 // the lists, or their heads
-    BeamRank cand[kBeamMost * kBeamMost];       // the rows' best heads, then the last lists' continuations
+    BeamRank head[kBeamStage];                  // the heads that are ranked
+    int from[kBeamStage];                       // and their lists
+    BeamRank cand[kBeamMost * kBeamMost];       // the last lists' continuations
     uint64_t entry[kBeamMost * kBeamMost];      // and their entries
-    int from[kBeamMost * kBeamMost];            // the heads' lists, the continuations' rows
-    int some[kBeamMost * kBeamMost];            // which of the heads may be among the best
-    int chosen[kBeamMost], kind[kBeamMost], n, m, last;
-    float top[kBeamMost], score[kBeamMost];     // a row's largest logit, its score
-    double logs[kBeamMost], weight[kBeamMost];  // the logarithm of its sum, its weight
+    int row[kBeamMost * kBeamMost];             // and rows
+    uint64_t best[kBeamMost], last;             // the rank of a row's best, of the last of the best heads
+    double logs[kBeamMost], weight[kBeamMost];  // the logarithm of a row's sum, its weight
+    float top[kBeamMost], score[kBeamMost];     // its largest logit, its score
+    int chosen[kBeamMost], kind[kBeamMost], n, m;
 };
 
 __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPlan plan) {
     __shared__ BeamJoin j;
     enum { kNone, kLogits, kItself, kNaN };     // a row's continuations: none, those of its logits, itself, itself as NaN
     constexpr int kParts = (kBeamChunks + 63) / 64;
+    constexpr uint64_t kSelf = 0xffffffffull;   // the entry of a row that goes on as it is (a logit's key and a token of 0)
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, threads = blockDim.x, S = plan.chunks, K = a.K;
     const int64_t row0 = (int64_t)blockIdx.x * K;
     const uint64_t* lists = beam_lists(a) + row0 * S * K;
-    const int each = min(K, S);   // lists of a row that remain
     const bool all = K * S * K <= kBeamStage;
     const int hop = all ? K : 1;
-    // (of a row without continuations by its logits, whatever lies there)
-    if (all)
-        for (int i = tid; i < K * S * K; i += threads) j.stage[i] = lists[i];
-    else
-        for (int i = tid; i < K * S; i += threads) j.stage[i] = lists[(int64_t)i * K];
-    for (int i = tid; i < K * each; i += threads) j.cand[i] = {0, 0};
-    if (tid < K) j.chosen[tid] = -1;
-    if (tid == 0) j.n = j.m = 0;
-    for (int k = w; k < K; k += threads / 64) {
-        const int64_t row = row0 + k;
-        const float sc = a.scores[row];
-        const bool done = a.done && a.done[row];
-        const double weight = a.weight ? (double)a.weight[row] : 1.0;
-        const float2* st = beam_stats(a, plan) + row * S;
-        float2 x[kParts];
-        float m = kBeamNegInf;
-#pragma unroll
-        for (int i = 0; i < kParts; ++i) x[i] = lane + 64 * i < S ? st[lane + 64 * i] : make_float2(kBeamNegInf, 0.f);
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < kParts; ++i) m = fmaxf(m, x[i].x), nan |= x[i].x != x[i].x;
-        m = group_max<64>(m);
-        double z = 0.0;
-#pragma unroll
-        for (int i = 0; i < kParts; ++i)
-            if (x[i].x != kBeamNegInf) z += (double)x[i].y * exp((double)x[i].x - (double)m);
-        z = group_sum_d<64>(z);
-        const int what = sc == kBeamNegInf ? kNone : sc != sc ? kNaN : done ? kItself : __ballot(nan) ? kNaN : kLogits;
-        if (lane == 0) j.kind[k] = what, j.top[k] = m, j.score[k] = sc, j.weight[k] = weight, j.logs[k] = log(z);
-    }
-    __syncthreads();
 
     auto sum_of = [&](int k, uint64_t entry) {
         return j.kind[k] == kLogits ? (double)j.score[k] + (((double)beam_logit((uint32_t)(entry >> 32)) - (double)j.top[k]) - j.logs[k])
@@ -316,100 +288,126 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
         const uint64_t rest = (uint64_t)(kBeamMost - 1 - k) << 52 | (entry >> 32) << 20 | (uint32_t)(entry - (0xffffffffull - (kBeamVocab - 1)));
         return {rank_key(r), rest};
     };
-    constexpr uint64_t kSelf = 0xffffffffull;   // the entry of a row that goes on as it is (a logit's key and a token of 0)
-    // a row's best heads
-    for (int i = tid; i < K * S; i += threads) {
-        const int k = i / S, c = i - k * S;
-        if (j.kind[k] == kNone) continue;
-        if (j.kind[k] != kLogits) {
-            if (c == 0) j.cand[k * each] = ranked(k, kSelf), j.from[k * each] = i;
-            continue;
+
+    // (of a row without continuations by its logits, whatever lies there)
+    if (all)
+        for (int i = tid; i < K * S * K; i += threads) j.stage[i] = lists[i];
+    else
+        for (int i = tid; i < K * S; i += threads) j.stage[i] = lists[(int64_t)i * K];
+    if (tid < K) j.chosen[tid] = -1;
+    if (tid == 0) j.n = j.m = 0, j.last = 1;
+    for (int k = w; k < K; k += threads / 64) {
+        const int64_t row = row0 + k;
+        const float sc = a.scores[row];
+        const bool done = a.done && a.done[row];
+        const double weight = a.weight ? (double)a.weight[row] : 1.0;
+        const float2* st = beam_stats(a, plan) + row * S;
+        float2 x[kParts];
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            const int c = lane + 64 * i;
+            x[i] = c < S ? st[c] : make_float2(kBeamNegInf, 0.f);
+            const uint64_t h = c < S ? lists[((int64_t)k * S + c) * K] : 0;
+            best = h > best ? h : best;
         }
-        const uint64_t x = j.stage[i * hop];
-        if (x == 0) continue;
-        int above = 0;
-        for (int o = k * S; o < k * S + S; ++o) above += j.stage[o * hop] > x;   // no two entries are alike
-        if (above < each) j.cand[k * each + above] = ranked(k, x), j.from[k * each + above] = i;
+        float m = kBeamNegInf;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) m = fmaxf(m, x[i].x), nan |= x[i].x != x[i].x;
+        m = group_max<64>(m);
+        double z = 0.0;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+            if (x[i].x != kBeamNegInf) z += (double)x[i].y * exp((double)x[i].x - (double)m);
+        z = group_sum_d<64>(z);
+        best = wave_max64(best);
+        const int what = sc == kBeamNegInf ? kNone : sc != sc ? kNaN : done ? kItself : __ballot(nan) ? kNaN : kLogits;
+        if (lane == 0) {
+            j.kind[k] = what, j.top[k] = m, j.score[k] = sc, j.weight[k] = weight, j.logs[k] = log(z);
+            j.best[k] = what == kNone || (what == kLogits && best == 0) ? 0 : ranked(k, what == kLogits ? best : kSelf).rank;
+        }
     }
     __syncthreads();
-    // of all rows': K of them are not below the least of the rows' best (where each row has one)
+
     uint64_t least = ~0ull;
-    for (int k = 0; k < K; ++k) least = min(least, j.cand[k * each].rank);
-    for (int i = tid; i < K * each; i += threads)
-        if (j.cand[i].rank != 0 && j.cand[i].rank >= least) j.some[atomicAdd(&j.n, 1)] = i;
+#pragma unroll 4
+    for (int k = 0; k < K; ++k) least = min(least, j.best[k]);
+    for (int i = tid; i < K * S; i += threads) {
+        const int k = i / S, what = j.kind[k];
+        const uint64_t e = what == kLogits ? j.stage[i * hop] : what != kNone && i == k * S ? kSelf : 0;
+        if (e == 0) continue;
+        const BeamRank x = ranked(k, e);
+        if (x.rank == 0 || x.rank < least) continue;
+        const int at = atomicAdd(&j.n, 1);
+        j.head[at] = x;
+        j.from[at] = i;
+    }
     __syncthreads();
-    // G threads count what lies above the i-th of n
+    // a power of two of threads counts, for each of n, how many lie above it
     auto group = [&](int n) {
         int G = 1;
         while (G < 64 && 2 * G * n <= threads) G *= 2;
         return G;
     };
-    auto sum_group = [&](int x, int G) {
-        for (int off = 1; off < G; off *= 2) x += __shfl_xor(x, off, 64);
-        return x;
+    auto above = [&](const BeamRank* of, int n, const BeamRank& x, int G) {
+        int c = 0;
+#pragma unroll 4
+        for (int o = tid % G; o < n; o += G) c += of[o].above(x);
+        for (int off = 1; off < G; off *= 2) c += __shfl_xor(c, off, 64);
+        return c;
     };
     {
         const int n = j.n, G = group(n);
         for (int i0 = 0; i0 < n; i0 += threads / G) {   // (all of a wave's threads take part in the exchange)
             const int i = i0 + tid / G;
-            const int at = j.some[min(i, n - 1)];
-            const BeamRank x = j.cand[at];
-            int above = 0;
-            for (int o = tid % G; o < n; o += G) above += j.cand[j.some[o]].above(x);
-            above = sum_group(above, G);
-            if (i < n && tid % G == 0 && above < K) {
-                j.chosen[above] = j.from[at];
-                if (above == K - 1) j.last = at;
+            const BeamRank x = j.head[min(i, n - 1)];
+            const int c = above(j.head, n, x, G);
+            if (i < n && tid % G == 0 && c < K) {
+                j.chosen[c] = j.from[i];
+                if (c == K - 1) j.last = x.rank;
             }
         }
     }
     __syncthreads();
-    const uint64_t last = j.n >= K ? j.cand[j.last].rank : 1;
-    BeamRank x = {0, 0};
-    uint64_t entry = 0;
-    int k = 0;
     if (tid < K * K) {
         const int i = j.chosen[tid / K], o = tid % K;
         if (i >= 0) {
-            k = i / S;
-            if (j.kind[k] == kLogits) entry = all ? j.stage[i * K + o] : lists[(int64_t)i * K + o];
-            else if (o == 0) entry = kSelf;
-            if (entry) x = ranked(k, entry);
+            const int k = i / S;
+            const uint64_t e = j.kind[k] == kLogits ? (all ? j.stage[i * K + o] : lists[(int64_t)i * K + o]) : o == 0 ? kSelf : 0;
+            const BeamRank x = e ? ranked(k, e) : BeamRank{0, 0};
+            if (x.rank != 0 && x.rank >= j.last) {
+                const int at = atomicAdd(&j.m, 1);
+                j.cand[at] = x;
+                j.entry[at] = e;
+                j.row[at] = k;
+            }
         }
-    }
-    __syncthreads();   // the heads have been read
-    if (x.rank >= last && x.rank != 0) {
-        const int at = atomicAdd(&j.m, 1);
-        j.cand[at] = x;
-        j.entry[at] = entry;
-        j.from[at] = k;
     }
     __syncthreads();
     const int n = j.m, G = group(n);
     for (int i0 = 0; i0 < n; i0 += threads / G) {
         const int i = i0 + tid / G;
-        const BeamRank y = j.cand[min(i, n - 1)];
-        int above = 0;
-        for (int o = tid % G; o < n; o += G) above += j.cand[o].above(y);
-        above = sum_group(above, G);
-        if (i < n && tid % G == 0 && above < K) {
-            const int r = j.from[i];
-            a.out[row0 + above] = (float)sum_of(r, j.entry[i]);
-            a.rows[row0 + above] = (int32_t)(row0 + r);
-            a.tokens[row0 + above] = j.kind[r] == kLogits ? (int64_t)(0xffffffffu - (uint32_t)j.entry[i]) : a.fill;
+        const BeamRank x = j.cand[min(i, n - 1)];
+        const int c = above(j.cand, n, x, G);
+        if (i < n && tid % G == 0 && c < K) {
+            const int k = j.row[i];
+            a.out[row0 + c] = (float)sum_of(k, j.entry[i]);
+            a.rows[row0 + c] = (int32_t)(row0 + k);
+            a.tokens[row0 + c] = j.kind[k] == kLogits ? (int64_t)(0xffffffffu - (uint32_t)j.entry[i]) : a.fill;
         }
     }
     for (int i = n + tid; i < K; i += threads) a.out[row0 + i] = kBeamNegInf, a.rows[row0 + i] = -1, a.tokens[row0 + i] = a.fill;
 }
 
-// Chunks of 8,192 places, or of 2,048 while that leaves CUs without one.  (A chunk's first logit may lie
-// inside a vector: so many places hold a vector's values less.)
+// Chunks of as many places as 256 threads of eight vectors have, or of a quarter or an eighth while that leaves CUs without one.
+// (A chunk's first logit may lie inside a vector: so many places hold a vector's values less.)
 static BeamPlan beam_plan(int32_t B, int32_t K, int64_t V, bool bf16) {
     BeamPlan p{};
-    const int64_t slack = bf16 ? 8 : 4, rows = (int64_t)B * K;
-    const bool few = rows * ((V + 8191) / 8192) <= device_cus() && V <= 2040 * kBeamChunks;
-    const int64_t most = (few ? 2048 : 8192) - slack;
-    p.few = few;
+    const int64_t slack = bf16 ? 8 : 4, rows = (int64_t)B * K, full = kBeamThreads * 8 * slack;
+    p.few = rows * ((V + full - 1) / full) <= device_cus();
+    int64_t most = full / (p.few ? bf16 ? 8 : 4 : 1) - slack;
+    if (V > most * kBeamChunks) p.few = false, most = full - slack;
     const int64_t n = (V + most - 1) / most;
     p.length = (int32_t)(((V + n - 1) / n + slack - 1) / slack * slack);
     p.chunks = (int32_t)((V + p.length - 1) / p.length);
@@ -433,7 +431,7 @@ int beam_select(const BeamArgs& a, void* stream) {
     const dim3 grid((unsigned)chunks), block(kBeamThreads);
     const hipStream_t st = (hipStream_t)stream;
     if (a.bf16 && p.few) hipLaunchKernelGGL((beam_chunk_kernel<true, 1>), grid, block, 0, st, a, p);
-    else if (a.bf16) hipLaunchKernelGGL((beam_chunk_kernel<true, 4>), grid, block, 0, st, a, p);
+    else if (a.bf16) hipLaunchKernelGGL((beam_chunk_kernel<true, 8>), grid, block, 0, st, a, p);
     else if (p.few) hipLaunchKernelGGL((beam_chunk_kernel<false, 2>), grid, block, 0, st, a, p);
     else hipLaunchKernelGGL((beam_chunk_kernel<false, 8>), grid, block, 0, st, a, p);
     if (int e = check_launch("beam_select")) return e;

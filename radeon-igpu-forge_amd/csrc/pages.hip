@@ -48,89 +48,126 @@ __device__ __forceinline__ int block_before(int v, int* sh, int& sum) {
 // are about to write into it, none may; else the lowest of them may.  A row that wants some gets them if
 // all rows' wants up to and with its own do not exceed the free pages; else it gets nothing.
 //
-// One workgroup, bounded by its chain of round trips: lengths, open pages, their uses, who writes there, free
-// pages, tables.  The free pages are looked for only as far as they are wanted.
+// One workgroup, bounded by its chain of round trips: lengths, open pages, their uses, tables.  A thread has up to eight
+// rows in registers.  The first pages' uses are under way meanwhile; free ones are looked for only as far as they are wanted.
 
 // the workspace: a copy for each row, the page each wanted one is, and for each page (first writer, writers)
 __device__ __forceinline__ int32_t* extend_list(const ExtendArgs& a) { return a.work + 4 * (int64_t)a.R; }
 
-enum : uint8_t { kRowWants = 1, kRowCopies = 2, kRowShares = 4 };
-
-__device__ __forceinline__ int64_t slot_of(const ExtendArgs& a, int r, int64_t pos) {
+// the slot of row r's j-th new token, once its pages are in the table and its length in `out`
+__device__ __forceinline__ int64_t slot_of(const ExtendArgs& a, int r, int j) {
+    const int add = min(max(a.add[r], 0), a.most), len = pages_len(a.lens[r], a.M, a.shift), pos = len + j;
+    if (j >= add || a.out[r] != len + add) return -1;   // (a refused row keeps its length)
     return ((int64_t)a.table[(int64_t)r * a.tab + (pos >> a.shift)] << a.shift) + (pos & ((1 << a.shift) - 1));
 }
 
+constexpr int kPagesFew = 256;                           // rows that are compared with one another in LDS
+
+template <int kPagesEach>   // rows of a thread
 __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int64_t list, bool slots_too) {
-    extern __shared__ int32_t lds[];   // pre[R + 1], flags[R]
+    __shared__ int32_t pre[kPagesRows + 1], col0[kPagesRows];   // pages wanted before a row, and the column of its first
     __shared__ int sh[kPagesWaves];
-    int32_t* pre = lds;
-    uint8_t* flags = reinterpret_cast<uint8_t*>(lds + a.R + 1);
     int4* copies = reinterpret_cast<int4*>(a.work);
     int32_t *pages = extend_list(a), *writers = pages + list;
     const int tid = threadIdx.x, mask = (1 << a.shift) - 1;
+    const int off = (int)((reinterpret_cast<uintptr_t>(a.uses) >> 2) & 3);   // 16-byte loads at their addresses
 
-    auto length = [&](int r) { return pages_len(a.lens[r], a.M, a.shift); };
-    auto adds = [&](int r) { return min(max(a.add[r], 0), a.most); };
-    auto open_page = [&](int r, int len) { return a.table[(int64_t)r * a.tab + (len >> a.shift)]; };
+    // which of this thread's kPagesScan pages from p on are free
+    auto whole = [&](int p) { return p >= 0 && p + kPagesScan <= a.N; };
+    constexpr bool kAhead = kPagesEach == 1;   // (eight rows take the registers)
+    int4 ahead[kPagesScan / 4];
+    const int first = tid * kPagesScan - off;
+    if (kAhead && whole(first))
+#pragma unroll
+        for (int i = 0; i < kPagesScan / 4; ++i) ahead[i] = *reinterpret_cast<const int4*>(a.uses + first + 4 * i);
 
-    bool any = false;
-    for (int r = tid; r < a.R; r += kPagesThreads) {
-        const int len = length(r), add = adds(r);
-        uint8_t f = add > 0 && (int64_t)len + add <= (int64_t)a.M << a.shift ? kRowWants : 0;
-        if (f && (len & mask)) {
-            const int p = open_page(r, len);
-            if ((uint32_t)p >= (uint32_t)a.N) f = 0;
-            else if (a.uses[p] > 1) {
-                f = a.copies ? f | kRowShares : 0;
-                if (f) writers[2 * (int64_t)p] = 0x7fffffff, writers[2 * (int64_t)p + 1] = 0;
-            }
-        }
-        flags[r] = f;
-        any |= (f & kRowShares) != 0;
+    int len[kPagesEach], add[kPagesEach], open[kPagesEach];   // a row's tokens, the new ones it may have, its open page (-1: none)
+    bool copy[kPagesEach], any = false;
+#pragma unroll
+    for (int e = 0; e < kPagesEach; ++e) {
+        const int r = e * kPagesThreads + tid;
+        len[e] = add[e] = 0;
+        open[e] = -1;
+        copy[e] = false;
+        if (r < a.R) len[e] = pages_len(a.lens[r], a.M, a.shift), add[e] = min(max(a.add[r], 0), a.most);
+        if ((int64_t)len[e] + add[e] > (int64_t)a.M << a.shift) add[e] = 0;
     }
-    any = __syncthreads_or(any);
-    __syncthreads();   // what was written to memory is there
-    if (any) {
-        for (int r = tid; r < a.R; r += kPagesThreads)
-            if (flags[r] & kRowShares) {
-                const int64_t p = open_page(r, length(r));
-                atomicMin(&writers[2 * p], r);
-                atomicAdd(&writers[2 * p + 1], 1);
-            }
-        __syncthreads();
-        for (int r = tid; r < a.R; r += kPagesThreads)
-            if (flags[r] & kRowShares) {
-                const int64_t p = open_page(r, length(r));
-                const int first = __hip_atomic_load(&writers[2 * p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                const int count = __hip_atomic_load(&writers[2 * p + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (count < a.uses[p] || r != first) flags[r] |= kRowCopies;
-            }
+#pragma unroll
+    for (int e = 0; e < kPagesEach; ++e)
+        if (add[e] > 0 && (len[e] & mask)) {
+            open[e] = a.table[(int64_t)(e * kPagesThreads + tid) * a.tab + (len[e] >> a.shift)];
+            if ((uint32_t)open[e] >= (uint32_t)a.N) add[e] = 0;
+        }
+    int users[kPagesEach];
+#pragma unroll
+    for (int e = 0; e < kPagesEach; ++e) {
+        users[e] = add[e] > 0 && (len[e] & mask) ? a.uses[open[e]] : 0;
+        if (users[e] > 1 && !a.copies) add[e] = 0;
+        any |= users[e] > 1 && add[e] > 0;
+    }
+    auto shares = [&](int e) { return users[e] > 1 && add[e] > 0; };
+    if (__syncthreads_or(any)) {
+        // who else writes into a row's open page: the rows before it, and all
+        if (kPagesEach == 1 && a.R <= kPagesFew) {
+            int before = 0, writes = 0;
+            if (tid < a.R) col0[tid] = shares(0) ? open[0] : -1;
+            __syncthreads();
+            if (shares(0))
+                for (int r = 0; r < a.R; ++r) {
+                    const bool same = col0[r] == open[0];
+                    writes += same;
+                    before += same && r < tid;
+                }
+            copy[0] = shares(0) && (writes < users[0] || before > 0);
+            __syncthreads();   // col0 is used again
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPagesEach; ++e)
+                if (shares(e)) writers[2 * (int64_t)open[e]] = 0x7fffffff, writers[2 * (int64_t)open[e] + 1] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kPagesEach; ++e)
+                if (shares(e)) {
+                    atomicMin(&writers[2 * (int64_t)open[e]], e * kPagesThreads + tid);
+                    atomicAdd(&writers[2 * (int64_t)open[e] + 1], 1);
+                }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kPagesEach; ++e)
+                if (shares(e)) {
+                    const int lowest = __hip_atomic_load(&writers[2 * (int64_t)open[e]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    const int count = __hip_atomic_load(&writers[2 * (int64_t)open[e] + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    copy[e] = count < users[e] || e * kPagesThreads + tid != lowest;
+                }
+        }
     }
 
     int want = 0;   // of all rows so far
-    for (int r0 = 0; r0 < a.R; r0 += kPagesThreads) {
-        const int r = r0 + tid;
-        int n = 0;
-        if (r < a.R && (flags[r] & kRowWants)) {
-            const int len = length(r);
-            n = pages_of((int64_t)len + adds(r), a.shift) - pages_of(len, a.shift) + ((flags[r] & kRowCopies) != 0);
-        }
+    int need[kPagesEach];
+#pragma unroll
+    for (int e = 0; e < kPagesEach; ++e) {
+        need[e] = 0;
+        if (e * kPagesThreads >= a.R) continue;
+        const int r = e * kPagesThreads + tid, had = pages_of(len[e], a.shift);
+        if (add[e] > 0) need[e] = pages_of((int64_t)len[e] + add[e], a.shift) - had + copy[e];
         int sum;
-        const int before = block_before(n, sh, sum);
-        if (r < a.R) pre[r] = want + before;
+        const int begin = want + block_before(need[e], sh, sum);
+        if (r < a.R) pre[r] = begin, col0[r] = had - copy[e];
         want += sum;
     }
     if (tid == 0) pre[a.R] = want;
 
     int have = 0;   // free pages found, up to `want`
-    const int off = (int)((reinterpret_cast<uintptr_t>(a.uses) >> 2) & 3);   // 16-byte loads at their addresses
     for (int p0 = -off; p0 < a.N && have < want; p0 += kPagesThreads * kPagesScan) {
         const int p = p0 + tid * kPagesScan;
         uint32_t free = 0;
-        if (p >= 0 && p + kPagesScan <= a.N) {
+        if (whole(p)) {
+            if (!kAhead || p0 > 0)   // (the first are here)
+#pragma unroll
+                for (int i = 0; i < kPagesScan / 4; ++i) ahead[i] = *reinterpret_cast<const int4*>(a.uses + p + 4 * i);
 #pragma unroll
             for (int i = 0; i < kPagesScan / 4; ++i) {
-                const int4 u = *reinterpret_cast<const int4*>(a.uses + p + 4 * i);
+                const int4 u = ahead[i];
                 free |= (uint32_t)((u.x == 0) | (u.y == 0) << 1 | (u.z == 0) << 2 | (u.w == 0) << 3) << (4 * i);
             }
         } else {
@@ -147,21 +184,17 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
     }
     __syncthreads();
 
-    // rows: lengths, and the pages in place of open ones
-    auto gets = [&](int r) { return (flags[r] & kRowWants) && (pre[r + 1] == pre[r] || pre[r + 1] <= have); };
-    for (int r = tid; r < a.R; r += kPagesThreads) {
-        const int len = length(r), add = adds(r);
-        const bool ok = gets(r);
-        int4 c = make_int4(0, 0, 0, 0);
-        if (ok && (flags[r] & kRowCopies)) {
-            int32_t* at = a.table + (int64_t)r * a.tab + (len >> a.shift);
-            c = make_int4(*at, pages[pre[r]], len & mask, 0);
-            *at = c.y;
-            a.uses[c.y] = 1;
-            atomicAdd(&a.uses[c.x], -1);
-        }
-        copies[r] = c;
-        a.out[r] = ok ? len + add : a.lens[r];
+    // rows: their copies, lengths and, of single tokens, slots
+#pragma unroll
+    for (int e = 0; e < kPagesEach; ++e) {
+        const int r = e * kPagesThreads + tid;
+        if (r >= a.R) continue;
+        const bool ok = add[e] > 0 && (need[e] == 0 || pre[r] + need[e] <= have);
+        const int got = ok && need[e] > 0 ? pages[pre[r]] : -1;
+        copies[r] = ok && copy[e] ? make_int4(open[e], got, len[e] & mask, 0) : make_int4(0, 0, 0, 0);
+        if (ok && copy[e]) atomicAdd(&a.uses[open[e]], -1);
+        a.out[r] = ok ? len[e] + add[e] : a.lens[r];
+        if (a.most == 1) a.slots[r] = ok ? ((int64_t)(need[e] > 0 ? got : open[e]) << a.shift) + (len[e] & mask) : -1;
     }
     // new pages, each by the thread whose turn it is: its row is the last one that begins at or before it
     for (int i = tid; i < min(want, have); i += kPagesThreads) {
@@ -171,25 +204,19 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
             if (pre[mid] <= i) lo = mid;
             else hi = mid - 1;
         }
-        const int r = lo, j = i - pre[r], copy = (flags[r] & kRowCopies) != 0;
-        if (pre[r + 1] > have || j < copy) continue;
-        a.table[(int64_t)r * a.tab + pages_of(length(r), a.shift) + j - copy] = pages[i];
+        if (pre[lo + 1] > have) continue;
+        a.table[(int64_t)lo * a.tab + col0[lo] + i - pre[lo]] = pages[i];
         a.uses[pages[i]] = 1;
     }
-    if (!slots_too) return;
+    if (!slots_too || a.most == 1) return;
     __syncthreads();
-    for (int i = tid; i < a.R * a.most; i += kPagesThreads) {
-        const int r = i / a.most, j = i - r * a.most;
-        a.slots[i] = j < adds(r) && gets(r) ? slot_of(a, r, (int64_t)length(r) + j) : -1;
-    }
+    for (int i = tid; i < a.R * a.most; i += kPagesThreads) a.slots[i] = slot_of(a, i / a.most, i % a.most);
 }
 
 // the slots of longer additions
 __global__ void __launch_bounds__(256) slots_kernel(ExtendArgs a) {
-    const int r = blockIdx.x, add = min(max(a.add[r], 0), a.most), len = pages_len(a.lens[r], a.M, a.shift);
-    const bool ok = add > 0 && a.out[r] == len + add;   // refused rows keep their lengths
-    for (int j = blockIdx.y * 256 + threadIdx.x; j < a.most; j += gridDim.y * 256)
-        a.slots[(int64_t)r * a.most + j] = ok && j < add ? slot_of(a, r, (int64_t)len + j) : -1;
+    const int r = blockIdx.x;
+    for (int j = blockIdx.y * 256 + threadIdx.x; j < a.most; j += gridDim.y * 256) a.slots[(int64_t)r * a.most + j] = slot_of(a, r, j);
 }
 
 // pages that rows can want between them, in whole int4
@@ -212,8 +239,9 @@ int extend_pages(const ExtendArgs& a, void* stream) {
     FX_REQUIRE(a.table && a.uses && a.lens && a.add && a.slots && a.out && a.work, "extend_pages: null pointer");
     FX_REQUIRE(((uintptr_t)a.work & 15) == 0, "extend_pages: work must be 16-byte aligned");
     const bool one = (int64_t)a.R * a.most <= 8 * kPagesThreads;   // slots in the same launch
-    const size_t bytes = (size_t)(a.R + 1) * 4 + (size_t)((a.R + 3) & ~3);
-    hipLaunchKernelGGL(extend_kernel, dim3(1), dim3(kPagesThreads), bytes, (hipStream_t)stream, a, extend_most(a.R, a.M, a.N, a.shift, a.most), one);
+    const int64_t list = extend_most(a.R, a.M, a.N, a.shift, a.most);
+    if (a.R <= kPagesThreads) hipLaunchKernelGGL((extend_kernel<1>), dim3(1), dim3(kPagesThreads), 0, (hipStream_t)stream, a, list, one);
+    else hipLaunchKernelGGL((extend_kernel<kPagesRows / kPagesThreads>), dim3(1), dim3(kPagesThreads), 0, (hipStream_t)stream, a, list, one);
     if (int e = check_launch("extend_pages")) return e;
     if (one) return 0;
     const int y = (a.most + 1023) / 1024;
@@ -224,11 +252,20 @@ int extend_pages(const ExtendArgs& a, void* stream) {
 __global__ void __launch_bounds__(256) copy_pages_kernel(CopyPagesArgs a) {
     const int4 c = reinterpret_cast<const int4*>(a.copies)[blockIdx.x];
     const int t = blockIdx.y, per = a.D / 8, n = c.z * a.H * per;
-    uint16_t* const p = a.at[t];
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int d = i % per, hj = i / per, h = hj % a.H, j = hj / a.H;
-        const int64_t in = (int64_t)j * a.st[t] + (int64_t)h * a.sh[t] + d * 8;
-        st16(p + (int64_t)c.y * a.sp[t] + in, ld16(p + (int64_t)c.x * a.sp[t] + in));
+    uint16_t *const from = a.at[t] + c.x * a.sp[t], *const to = a.at[t] + c.y * a.sp[t];
+    constexpr int U = 4;
+    for (int i0 = threadIdx.x; i0 < n; i0 += 256 * U) {
+        uint4 x[U];
+        int64_t in[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = min(i0 + 256 * u, n - 1), d = i % per, hj = i / per, h = hj % a.H, j = hj / a.H;
+            in[u] = (int64_t)j * a.st[t] + (int64_t)h * a.sh[t] + d * 8;
+            x[u] = ld16(from + in[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + 256 * u < n) st16(to + in[u], x[u]);
     }
 }
 
@@ -241,45 +278,20 @@ int copy_pages(const CopyPagesArgs& a, void* stream) {
 
 // ---- store -------------------------------------------------------------------------------
 //
-// HBM-bound: every new row is read once and written once, 16 bytes a lane.  A workgroup takes some tokens of a row of
-// the batch, a thread four pieces of them at a time.
+// HBM-bound: every new row is read once and written once, a thread a 16-byte piece of a key and of its value.  The stores go past
+// the caches (24 prompts of up to 4,001 tokens, 525 MB: 98 us without, 90 with, 5.8 TB/s); the loads do not: what a projection
+// has just written is still there (33 MB 7.1 us, past them 8.8).  More pieces a thread are the slower: two 91 us, eight 111.
 
-struct StorePlan {
-    int32_t tokens, units;   // of a workgroup; 16-byte pieces of a token
-};
-
-__global__ void __launch_bounds__(256) store_pages_kernel(StorePagesArgs a, StorePlan p) {
-    const int r = blockIdx.y, t0 = blockIdx.x * p.tokens, n = min(p.tokens, a.T - t0) * p.units, per = a.D / 8;
-    const int64_t* slots = a.slots + r * a.sr;
-    const uint16_t *k = a.k + r * a.kr, *v = a.v + r * a.vr;
-    constexpr int U = 4;
-    for (int i0 = threadIdx.x; i0 < n; i0 += 256 * U) {
-        int64_t slot[U];
-        uint4 x[U], y[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + 256 * u, t = t0 + i / p.units;
-            slot[u] = i < n ? slots[t * a.st] : -1;
-            if (slot[u] >= a.N << a.shift) slot[u] = -1;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + 256 * u, tt = i / p.units, e = i - tt * p.units, h = e / per, d = (e - h * per) * 8;
-            if (slot[u] >= 0) {
-                x[u] = ld16_nt(k + (t0 + tt) * a.kt + h * a.kh + d);
-                y[u] = ld16_nt(v + (t0 + tt) * a.vt + h * a.vh + d);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + 256 * u, tt = i / p.units, e = i - tt * p.units, h = e / per, d = (e - h * per) * 8;
-            if (slot[u] >= 0) {
-                const int64_t page = slot[u] >> a.shift, j = slot[u] & ((1 << a.shift) - 1);
-                st16(a.kp + page * a.kpp + j * a.kpt + h * a.kph + d, x[u]);
-                st16(a.vp + page * a.vpp + j * a.vpt + h * a.vph + d, y[u]);
-            }
-        }
-    }
+__global__ void __launch_bounds__(256) store_pages_kernel(StorePagesArgs a) {
+    const int per = a.D / 8, units = a.H * per, i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.T * units) return;
+    const int r = blockIdx.y, t = i / units, e = i - t * units, h = e / per, d = (e - h * per) * 8;
+    const int64_t slot = a.slots[r * a.sr + t * a.st];
+    if (slot < 0 || slot >= a.N << a.shift) return;
+    const uint4 k = ld16(a.k + r * a.kr + t * a.kt + h * a.kh + d), v = ld16(a.v + r * a.vr + t * a.vt + h * a.vh + d);
+    const int64_t page = slot >> a.shift, j = slot & ((1 << a.shift) - 1);
+    st16_nt(a.kp + page * a.kpp + j * a.kpt + h * a.kph + d, k);
+    st16_nt(a.vp + page * a.vpp + j * a.vpt + h * a.vph + d, v);
 }
 
 int store_pages(const StorePagesArgs& a, void* stream) {
@@ -289,13 +301,9 @@ int store_pages(const StorePagesArgs& a, void* stream) {
     const int64_t s[] = {a.kr, a.kt, a.kh, a.vr, a.vt, a.vh, a.kpp, a.kpt, a.kph, a.vpp, a.vpt, a.vph};
     for (int64_t x : s) FX_REQUIRE(x % 8 == 0, "store_pages: strides must be multiples of 8 elements");
     FX_REQUIRE((((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15) == 0, "store_pages: 16-byte aligned tensors");
-    FX_REQUIRE((int64_t)a.H * (a.D / 8) < (1 << 24) && a.R <= 65535, "store_pages: %d rows of %d x %d are too many or too wide", a.R, a.H, a.D);
-    StorePlan p{};
-    p.units = a.H * (a.D / 8);
-    p.tokens = p.units >= 2048 ? 1 : 2048 / p.units;   // two turns of a thread
-    const dim3 grid((unsigned)((a.T + p.tokens - 1) / p.tokens), (unsigned)a.R);
-    FX_REQUIRE((int64_t)grid.x * 256 <= 0xffffffffLL, "store_pages: %d tokens are too many", a.T);
-    hipLaunchKernelGGL(store_pages_kernel, grid, dim3(256), 0, (hipStream_t)stream, a, p);
+    const int64_t n = (int64_t)a.T * a.H * (a.D / 8);
+    FX_REQUIRE(n <= 0x7fffff00 && a.R <= 65535, "store_pages: %d rows of %d x %d x %d are too many", a.R, a.T, a.H, a.D);
+    hipLaunchKernelGGL(store_pages_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)a.R), dim3(256), 0, (hipStream_t)stream, a);
     return check_launch("store_pages");
 }
 
