@@ -35,17 +35,46 @@ __device__ __forceinline__ uint64_t rank_key(double x) {
     const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
     return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
 }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int off) {
-    return (uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)x, off, 64) | (uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)(x >> 32), off, 64) << 32;
+// Reductions over a wave by lane shifts (row_shr 1, 2, 4, 8, then broadcasts of lanes 15 and 31): the last lane's, for all.
+// A lane that nothing is shifted to takes `old`.
+template <int CTRL>
+__device__ __forceinline__ uint32_t shifted(uint32_t old, uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)x, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ uint64_t shifted(uint64_t old, uint64_t x) {
+    return (uint64_t)shifted<CTRL>((uint32_t)(old >> 32), (uint32_t)(x >> 32)) << 32 | shifted<CTRL>((uint32_t)old, (uint32_t)x);
+}
+__device__ __forceinline__ float last_lane(float x) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63)); }
+__device__ __forceinline__ uint64_t last_lane(uint64_t x) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, 63);
+}
+#define FX_WAVE_STEPS(step) step(0x111) step(0x112) step(0x114) step(0x118) step(0x142) step(0x143)
+__device__ __forceinline__ float wave_max(float x) {
+#define FX_STEP(c) x = fmaxf(x, __uint_as_float(shifted<c>(__float_as_uint(x), __float_as_uint(x))));
+    FX_WAVE_STEPS(FX_STEP)
+#undef FX_STEP
+    return last_lane(x);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#define FX_STEP(c) x += __uint_as_float(shifted<c>(0u, __float_as_uint(x)));
+    FX_WAVE_STEPS(FX_STEP)
+#undef FX_STEP
+    return last_lane(x);
+}
+__device__ __forceinline__ double wave_sum(double x) {
+#define FX_STEP(c) x += __longlong_as_double((long long)shifted<c>((uint64_t)0, (uint64_t)__double_as_longlong(x)));
+    FX_WAVE_STEPS(FX_STEP)
+#undef FX_STEP
+    return __longlong_as_double((long long)last_lane((uint64_t)__double_as_longlong(x)));
 }
 __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint64_t o = shfl_xor64(x, off);
-        x = o > x ? o : x;
-    }
-    return x;
+#define FX_STEP(c) { const uint64_t o = shifted<c>(x, x); x = o > x ? o : x; }
+    FX_WAVE_STEPS(FX_STEP)
+#undef FX_STEP
+    return last_lane(x);
 }
+#undef FX_WAVE_STEPS
 
 // chunks of a row, and logits of each (a whole number of vectors; the last is shorter)
 struct BeamPlan {
@@ -61,7 +90,8 @@ __device__ __forceinline__ float2* beam_stats(const BeamArgs& a, const BeamPlan&
 // a beam with continuations by its logits
 __device__ __forceinline__ bool beam_goes_on(const BeamArgs& a, int64_t row) {
     const float s = a.scores[row];
-    return !(a.done && a.done[row]) && s == s && s != kBeamNegInf;
+    const int d = a.done ? a.done[row] : 0;   // (both loads at once)
+    return !d & (s == s) & (s != kBeamNegInf);
 }
 
 // A thread's part of a chunk: NR vectors of 16 bytes, as they lie in memory.  What a pass makes of a vector is not kept for the next.
@@ -126,30 +156,38 @@ __global__ void __launch_bounds__(kBeamThreads, 8) beam_chunk_kernel(BeamArgs a,
     BeamChunk<BF, NR> c;
     c.load(a.logits, i0, i1, row * a.V);
     if (tid == 0) listed = 0;
-    float own = c.edge, most[NR];   // the thread's largest, and each vector's
+    // One pass as the vectors come: the thread's largest and each vector's, and the sum of 2^(x log2 e - r) above a reference, the
+    // first vector's largest, r rounded (what it is rounded by is taken from the sum).  A reference too far from the thread's
+    // largest, a NaN or +inf: once more above the largest itself, which gives NaN for the last two.
+    float own = kBeamNegInf, most[NR], about = 0.f, ref = 0.f, s = 0.f;
     c.each([&](int i, const float* x, uint32_t) {
         most[i] = fmaxf(x[0], x[1]);
 #pragma unroll
         for (int e = 2; e < NP; e += 2) most[i] = fmaxf(most[i], fmaxf(x[e], x[e + 1]));
         own = fmaxf(own, most[i]);
+        if (i == 0) {
+            about = fabsf(own) < 1e38f ? own : 0.f;
+            ref = about * kLog2e;
+        }
+        float t = 0.f;
+#pragma unroll
+        for (int e = 0; e < NP; e += 2) {
+            s += exp2_fast(fmaf(x[e], kLog2e, -ref));
+            t += exp2_fast(fmaf(x[e + 1], kLog2e, -ref));
+        }
+        s += t;
+        asm volatile("" : "+v"(s), "+v"(own));
     });
-    // The sum above the thread's own maximum, before the workgroup waits for the slowest of its loads: the exponent x log2 e - c is
-    // rounded once, and what c, the maximum's, is rounded by is taken from the sum.  A NaN or +inf makes it NaN.
-    const float mine = own == kBeamNegInf ? 0.f : own, ref = mine * kLog2e;
-    float s;
-    if (fabsf(mine) < 1e38f) {
-        s = exp2_fast(fmaf(c.edge, kLog2e, -ref));
+    own = fmaxf(own, c.edge);   // (loaded last)
+    s += exp2_fast(fmaf(c.edge, kLog2e, -ref));
+    s *= exp2_fast(-fmaf(about, kLog2e, -ref));
+    if (own == kBeamNegInf && s == 0.f) about = own;   // none of its own
+    else if (!(fabsf(own - about) < 60.f)) {
+        about = own == kBeamNegInf ? 0.f : own;
+        s = exp2_fast((c.edge - about) * kLog2e);
         c.each([&](int, const float* x, uint32_t) {
 #pragma unroll
-            for (int e = 0; e < NP; ++e) s += exp2_fast(fmaf(x[e], kLog2e, -ref));
-            asm volatile("" : "+v"(s));
-        });
-        s *= exp2_fast(-fmaf(mine, kLog2e, -ref));
-    } else {   // c would be past the type's range (masks of its lowest value)
-        s = exp2_fast((c.edge - mine) * kLog2e);
-        c.each([&](int, const float* x, uint32_t) {
-#pragma unroll
-            for (int e = 0; e < NP; ++e) s += exp2_fast((x[e] - mine) * kLog2e);
+            for (int e = 0; e < NP; ++e) s += exp2_fast((x[e] - about) * kLog2e);
             asm volatile("" : "+v"(s));
         });
     }
@@ -160,7 +198,7 @@ __global__ void __launch_bounds__(kBeamThreads, 8) beam_chunk_kernel(BeamArgs a,
     bool bad = g != g;
 #pragma unroll
     for (int i = 1; i < kBeamWaves; ++i) bad |= gmax[i][lane] != gmax[i][lane], g = fmaxf(g, gmax[i][lane]);
-    const float m = group_max<64>(g);
+    const float m = wave_max(g);
     const int64_t place = row * plan.chunks + chunk;
     uint64_t* out = beam_lists(a) + place * a.K;
     float2* stat = beam_stats(a, plan) + place;
@@ -175,9 +213,7 @@ __global__ void __launch_bounds__(kBeamThreads, 8) beam_chunk_kernel(BeamArgs a,
     int have = __popcll(__ballot(k >= lo));
     if (have > a.K) {
         // the search begins above the least of the maxima
-        const uint32_t least = beam_key(-group_max<64>(k >= lo ? -g : kBeamNegInf));
-        lo = __builtin_amdgcn_readfirstlane(least);
-        hi = __builtin_amdgcn_readfirstlane(hi);
+        lo = beam_key(-wave_max(k >= lo ? -g : kBeamNegInf));
         while (lo < hi && have > a.K + a.K / 4) {
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
             const int n = __popcll(__ballot(k >= mid));
@@ -185,8 +221,8 @@ __global__ void __launch_bounds__(kBeamThreads, 8) beam_chunk_kernel(BeamArgs a,
             else hi = mid - 1;
         }
     }
-    s = own == kBeamNegInf ? 0.f : s * exp2_fast((mine - m) * kLog2e);
-    s = group_sum<64>(s);
+    s = about == kBeamNegInf ? 0.f : s * exp2_fast((about - m) * kLog2e);
+    s = wave_sum(s);
     if (lane == 0) shs[w] = s;
     const float least = beam_logit(lo);
     auto put = [&](float x, uint32_t tok) {
@@ -214,6 +250,7 @@ __global__ void __launch_bounds__(kBeamThreads, 8) beam_chunk_kernel(BeamArgs a,
         for (int i = tid; i < n; i += kBeamThreads) {
             const uint64_t x = list[i];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < n; ++j) rank += list[j] > x;
             if (rank < a.K) out[rank] = x;
         }
@@ -247,15 +284,15 @@ struct BeamRank {
     __device__ __forceinline__ bool above(const BeamRank& o) const { return rank > o.rank || (rank == o.rank && rest > o.rest); }
 };
 
-// A workgroup a sequence.  The chunks' lists are sorted, so the best K continuations lie in the K lists with the best heads; of
-// these lists' continuations those that are not below the last of their heads are ranked.  Only heads that are not below the
-// least of the rows' best are looked at (where each row has one, K are not).  All ranking is by counting, of a few
-// threads for each.
+// A workgroup a sequence, bounded by its chain of round trips and waits.  Only what is not below the least of the rows' best
+// continuations is looked at (where each row has one, K are not): of the chunks' lists, which are sorted, those with such a head;
+// where these are many, only the K lists with the best heads, in which the best K continuations lie, and what is
+// not below the last of their heads.  What remains is ranked by counting, of a few threads for each.
 constexpr int kBeamJoin = 1024, kBeamChunks = 130;
 constexpr int kBeamStage = kBeamMost * kBeamChunks;   // entries in LDS
 
 struct BeamJoin {
-    uint64_t stage[kBeamStage];                 // the lists, or their heads
+    uint64_t stage[kBeamStage];                 // the lists' heads
     BeamRank head[kBeamStage];                  // the heads that are ranked
     int from[kBeamStage];                       // and their lists
     BeamRank cand[kBeamMost * kBeamMost];       // the last lists' continuations
@@ -275,8 +312,6 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, threads = blockDim.x, S = plan.chunks, K = a.K;
     const int64_t row0 = (int64_t)blockIdx.x * K;
     const uint64_t* lists = beam_lists(a) + row0 * S * K;
-    const bool all = K * S * K <= kBeamStage;
-    const int hop = all ? K : 1;
 
     auto sum_of = [&](int k, uint64_t entry) {
         return j.kind[k] == kLogits ? (double)j.score[k] + (((double)beam_logit((uint32_t)(entry >> 32)) - (double)j.top[k]) - j.logs[k])
@@ -289,42 +324,41 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
         return {rank_key(r), rest};
     };
 
-    // (of a row without continuations by its logits, whatever lies there)
-    if (all)
-        for (int i = tid; i < K * S * K; i += threads) j.stage[i] = lists[i];
-    else
-        for (int i = tid; i < K * S; i += threads) j.stage[i] = lists[(int64_t)i * K];
     if (tid < K) j.chosen[tid] = -1;
     if (tid == 0) j.n = j.m = 0, j.last = 1;
     for (int k = w; k < K; k += threads / 64) {
         const int64_t row = row0 + k;
         const float sc = a.scores[row];
-        const bool done = a.done && a.done[row];
-        const double weight = a.weight ? (double)a.weight[row] : 1.0;
+        const bool done = a.done ? a.done[row] : false;
+        const float weight = a.weight ? a.weight[row] : 1.f;
         const float2* st = beam_stats(a, plan) + row * S;
+        // (of a row without continuations by its logits, whatever lies there)
         float2 x[kParts];
-        uint64_t best = 0;
+        uint64_t h[kParts], best = 0;
 #pragma unroll
         for (int i = 0; i < kParts; ++i) {
             const int c = lane + 64 * i;
             x[i] = c < S ? st[c] : make_float2(kBeamNegInf, 0.f);
-            const uint64_t h = c < S ? lists[((int64_t)k * S + c) * K] : 0;
-            best = h > best ? h : best;
+            h[i] = c < S ? lists[((int64_t)k * S + c) * K] : 0;
         }
         float m = kBeamNegInf;
         bool nan = false;
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) m = fmaxf(m, x[i].x), nan |= x[i].x != x[i].x;
-        m = group_max<64>(m);
-        double z = 0.0;
+        for (int i = 0; i < kParts; ++i) {
+            if (lane + 64 * i < S) j.stage[k * S + lane + 64 * i] = h[i];
+            best = h[i] > best ? h[i] : best;
+            m = fmaxf(m, x[i].x), nan |= x[i].x != x[i].x;
+        }
+        m = wave_max(m);
+        double z = 0.0;   // (an exponential in 32 bits is off by as much as those that the chunk's sum is of)
 #pragma unroll
         for (int i = 0; i < kParts; ++i)
-            if (x[i].x != kBeamNegInf) z += (double)x[i].y * exp((double)x[i].x - (double)m);
-        z = group_sum_d<64>(z);
+            if (x[i].x != kBeamNegInf) z += (double)(x[i].y * exp2_fast((x[i].x - m) * kLog2e));
+        z = wave_sum(z);
         best = wave_max64(best);
         const int what = sc == kBeamNegInf ? kNone : sc != sc ? kNaN : done ? kItself : __ballot(nan) ? kNaN : kLogits;
         if (lane == 0) {
-            j.kind[k] = what, j.top[k] = m, j.score[k] = sc, j.weight[k] = weight, j.logs[k] = log(z);
+            j.kind[k] = what, j.top[k] = m, j.score[k] = sc, j.weight[k] = (double)weight, j.logs[k] = log(z);
             j.best[k] = what == kNone || (what == kLogits && best == 0) ? 0 : ranked(k, what == kLogits ? best : kSelf).rank;
         }
     }
@@ -335,7 +369,7 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
     for (int k = 0; k < K; ++k) least = min(least, j.best[k]);
     for (int i = tid; i < K * S; i += threads) {
         const int k = i / S, what = j.kind[k];
-        const uint64_t e = what == kLogits ? j.stage[i * hop] : what != kNone && i == k * S ? kSelf : 0;
+        const uint64_t e = what == kLogits ? j.stage[i] : what != kNone && i == k * S ? kSelf : 0;
         if (e == 0) continue;
         const BeamRank x = ranked(k, e);
         if (x.rank == 0 || x.rank < least) continue;
@@ -357,7 +391,9 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
         for (int off = 1; off < G; off *= 2) c += __shfl_xor(c, off, 64);
         return c;
     };
-    {
+    // The lists of few heads are all looked at; of many, those of the best K.
+    const bool few = j.n * K <= threads / 4;
+    if (!few) {
         const int n = j.n, G = group(n);
         for (int i0 = 0; i0 < n; i0 += threads / G) {   // (all of a wave's threads take part in the exchange)
             const int i = i0 + tid / G;
@@ -368,21 +404,21 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
                 if (c == K - 1) j.last = x.rank;
             }
         }
+        __syncthreads();
     }
-    __syncthreads();
-    if (tid < K * K) {
-        const int i = j.chosen[tid / K], o = tid % K;
-        if (i >= 0) {
-            const int k = i / S;
-            const uint64_t e = j.kind[k] == kLogits ? (all ? j.stage[i * K + o] : lists[(int64_t)i * K + o]) : o == 0 ? kSelf : 0;
-            const BeamRank x = e ? ranked(k, e) : BeamRank{0, 0};
-            if (x.rank != 0 && x.rank >= j.last) {
-                const int at = atomicAdd(&j.m, 1);
-                j.cand[at] = x;
-                j.entry[at] = e;
-                j.row[at] = k;
-            }
-        }
+    const int* of = few ? j.from : j.chosen;
+    const uint64_t bound = few ? max(least, (uint64_t)1) : j.last;
+    for (int t = tid; t < (few ? j.n : K) * K; t += threads) {
+        const int i = of[t / K], o = t % K;
+        if (i < 0) continue;
+        const int k = i / S;
+        const uint64_t e = j.kind[k] == kLogits ? (o == 0 ? j.stage[i] : lists[(int64_t)i * K + o]) : o == 0 ? kSelf : 0;
+        const BeamRank x = e ? ranked(k, e) : BeamRank{0, 0};
+        if (x.rank < bound) continue;
+        const int at = atomicAdd(&j.m, 1);
+        j.cand[at] = x;
+        j.entry[at] = e;
+        j.row[at] = k;
     }
     __syncthreads();
     const int n = j.m, G = group(n);
