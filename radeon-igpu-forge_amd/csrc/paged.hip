@@ -51,9 +51,12 @@ __device__ __forceinline__ uint32_t paged_steps(const PagedArgs& a, int n) {
     return l ? (l + kPagedTile * KW - 1) / (kPagedTile * KW) : 1u;
 }
 
+// floats of a piece: its rows' outputs, their maxima and sums; whole 16-byte vectors
+__host__ __device__ __forceinline__ int64_t paged_piece(const PagedPlan& p, int D) { return ((int64_t)p.gt * (D + 2) + 3) & ~3ll; }
+
 // where the join finds the pieces of a row and head group: (first workgroup, count), behind the partials
 __device__ __forceinline__ uint2* paged_places(const PagedArgs& a, const PagedPlan& p) {
-    return reinterpret_cast<uint2*>(a.work + (int64_t)2 * p.split * p.hw * p.gt * (a.D + 2));
+    return reinterpret_cast<uint2*>(a.work + (int64_t)2 * p.split * p.hw * paged_piece(p, a.D));
 }
 
 // Workgroup: HW key heads x KW parts of a row's keys, a wave each.  Per tile of 32 keys S^T = K Q^T (a lane
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(64 * HW * KW, 2) paged_attn_kernel(PagedArgs a
     hr = __builtin_amdgcn_readfirstlane(hr);
     s0 = __builtin_amdgcn_readfirstlane(s0);
 
-    while (pos < stop) {
+    while (pos < stop && r < a.R) {
         const int len = __builtin_amdgcn_readfirstlane(paged_len(a, a.lens[r]));
         const uint32_t steps = paged_steps<KW>(a, len);
         const uint32_t n = plan.split ? (uint32_t)(stop - pos < steps - s0 ? stop - pos : steps - s0) : steps;
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(64 * HW * KW, 2) paged_attn_kernel(PagedArgs a
         }
 
         const bool whole = n == steps;
-        const int64_t per = (int64_t)plan.gt * (D + 2);   // floats of a piece
+        const int64_t per = paged_piece(plan, D);
         float* pieces = a.work + (2 * (int64_t)piece + (s0 == 0)) * HW * per;
         if (plan.split && s0 == 0 && threadIdx.x == 0) {   // the workgroup with the row's last step: the last one that begins at or before it
             const uint32_t last = whole ? piece : (uint32_t)(((pos + steps) * parts - 1) / total);
@@ -395,7 +398,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedArgs a, PagedPlan 
     const uint2 place = paged_places(a, plan)[(int64_t)r * heads + grp * sets + h / plan.hw];
     const uint32_t count = place.y;
     if (count == 1) return;   // written by its workgroup
-    const int64_t per = (int64_t)plan.gt * (D + 2);
+    const int64_t per = paged_piece(plan, D);
     const int st = lane / LPR, c = (lane % LPR) * 4;
     float M = kPagedNegInf, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -460,7 +463,7 @@ static PagedPlan paged_plan(int32_t R, int32_t H, int32_t Hkv, int32_t N, int32_
 int64_t paged_attention_workspace(int32_t R, int32_t H, int32_t Hkv, int32_t N, int32_t M, int32_t shift, int32_t D) {
     if (R < 1 || Hkv < 1 || H < Hkv || H % Hkv || N < 1 || M < 1 || shift < 4 || shift > 20 || (D != 64 && D != 128)) return 0;
     const PagedPlan p = paged_plan(R, H, Hkv, N, M, shift, D);
-    return p.split == 0 ? 0 : (int64_t)2 * p.split * p.hw * p.gt * (D + 2) * (int64_t)sizeof(float) + (int64_t)R * (Hkv / p.hw) * p.groups * (int64_t)sizeof(uint2);
+    return p.split == 0 ? 0 : 2 * (int64_t)p.split * p.hw * paged_piece(p, D) * (int64_t)sizeof(float) + (int64_t)R * (Hkv / p.hw) * p.groups * (int64_t)sizeof(uint2);
 }
 
 template <int D, int NT, bool ONCE>

@@ -51,7 +51,7 @@ __device__ __forceinline__ int block_before(int v, int* sh, int& sum) {
 // One workgroup, bounded by its chain of round trips: lengths, open pages, their uses, tables.  A thread has up to eight
 // rows in registers.  The first pages' uses are under way meanwhile; free ones are looked for only as far as they are wanted.
 
-// the workspace: a copy for each row, the page each wanted one is, and for each page (first writer, writers)
+// the workspace: a copy for each row, the page each wanted one is, and, of many rows, for each page (first writer, writers)
 __device__ __forceinline__ int32_t* extend_list(const ExtendArgs& a) { return a.work + 4 * (int64_t)a.R; }
 
 // the slot of row r's j-th new token, once its pages are in the table and its length in `out`
@@ -227,7 +227,7 @@ static int64_t extend_most(int32_t R, int32_t M, int32_t N, int32_t shift, int32
 
 int64_t extend_pages_workspace(int32_t R, int32_t M, int32_t N, int32_t shift, int32_t most) {
     if (R < 1 || M < 1 || N < 1 || shift < 0 || shift > 20 || most < 1) return 0;
-    return (4 * (int64_t)R + extend_most(R, M, N, shift, most) + 2 * (int64_t)N) * (int64_t)sizeof(int32_t);
+    return (4 * (int64_t)R + extend_most(R, M, N, shift, most) + (R > kPagesFew ? 2 * (int64_t)N : 0)) * (int64_t)sizeof(int32_t);
 }
 
 int extend_pages(const ExtendArgs& a, void* stream) {

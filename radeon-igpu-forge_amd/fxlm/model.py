@@ -403,8 +403,8 @@ class GPT(nn.Module):
         B, T = idx.shape
         if lens.shape != (B,) or B > cache.lens.numel() or (rows is not None and rows.shape != (B,)):
             raise ValueError(f"lens and rows ({B},) of a cache of {cache.lens.numel()} rows: {tuple(lens.shape)} {None if rows is None else tuple(rows.shape)}")
-        if T > self.cfg.seq_len:
-            raise ValueError(f"T={T} > seq_len={self.cfg.seq_len}")
+        if not 1 <= T <= self.cfg.seq_len:
+            raise ValueError(f"prompts of {T} tokens (1 to {self.cfg.seq_len})")
         if rows is None:
             rows = torch.arange(B, device=idx.device)
         cache.end(rows)

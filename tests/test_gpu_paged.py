@@ -203,6 +203,37 @@ def test_paged_attention_in_a_pool_past_32_bits(dev):
     assert _same(pools[0][N - n + page, 2499 % P], c["kn"][0]) and _same(pools[1][N - n + page, 2499 % P], c["vn"][0])
 
 
+# pools that are loaded past the caches: each of the kernel's forms, with the bits of the same rows in a small pool
+@pytest.mark.parametrize("R,H,Hkv,D,P,M,lens", [
+    (900, 4, 4, 64, 16, 20, [(53 * i) % 321 for i in range(900)]),      # not split
+    (500, 20, 1, 128, 64, 20, [(531 * i) % 1281 for i in range(500)]),
+    (6, 8, 4, 64, 256, 200, [3000, 0, 1, 2048, 255, 1700]),             # split: four heads a workgroup, two, one
+    (6, 8, 4, 128, 128, 200, [3000, 0, 1, 2048, 255, 1700]),
+    (6, 6, 6, 64, 256, 200, [3000, 0, 1, 2048, 255, 1700]),
+    (6, 40, 2, 128, 256, 200, [3000, 0, 1, 2048, 255, 1700]),
+    (6, 5, 5, 64, 256, 200, [3000, 0, 1, 2048, 255, 1700]),
+    (6, 32, 1, 64, 1024, 200, [3000, 0, 1, 2048, 255, 1700]),
+])
+@pytest.mark.parametrize("heads", [False, True])
+def test_paged_attention_in_large_pools(dev, R, H, Hkv, D, P, M, lens, heads):
+    from fxlm import paged_attention
+    c = _case(R, H, Hkv, D, P, M, lens, seed=D + P, heads=heads)
+    n = c["k"].shape[0]
+    N = max(n, (2 ** 28 + 2 ** 22) // (P * Hkv * D * 4))
+    assert min(R * M, N) * P * Hkv * D * 4 >= 2 ** 28 > min(R * M, n) * P * Hkv * D * 4
+    d = _to(dev, c)
+    kn, vn = d["kn"], d["vn"]
+    big = []
+    for t in ("k", "v"):
+        x = torch.full((N, Hkv, P, D) if heads else (N, P, Hkv, D), math.nan, device=dev, dtype=torch.bfloat16)
+        x = x.transpose(1, 2) if heads else x
+        x[N - n:] = d[t]
+        big.append(x)
+    o, l = paged_attention(d["q"], *big, d["table"] + (N - n), d["lens"], return_lse=True, k_new=kn, v_new=vn)   # noqa: E741
+    _, ro, rl = _check(dev, c, True) if R < 100 else (None, *paged_attention(*(d[t] for t in ("q", "k", "v", "table", "lens")), return_lse=True, k_new=kn, v_new=vn))
+    assert torch.equal(o, ro) and torch.equal(l, rl)
+
+
 def test_paged_attention_on_another_stream_and_in_graphs(dev):
     # two captured calls with workspaces of their own, replayed in turn between eager calls, lengths changed in between
     from fxlm import paged_attention
@@ -438,6 +469,40 @@ def test_a_cache_in_use(dev):
     assert refused > 0     # the pool was too small now and then
     c.end()
     assert not c.uses.any() and not c.lens.any()
+
+
+def test_tables_in_a_graph(dev):
+    # reordering, pages, stores and attention captured once and replayed between eager work, against the same calls one by one
+    from fxlm import extend_pages, paged_attention, reorder_pages, store_pages
+    g = torch.Generator().manual_seed(4)
+    R, M, P, N, H, D = 12, 9, 16, 200, 2, 64
+    table, lens, _, uses = _tables(g, R, M, P, N, 1, 0.3)
+    pools = [torch.randn(N, P, H, D, generator=g).bfloat16().to(dev) for _ in range(2)]
+    a = {"table": table.to(dev), "lens": lens.to(dev), "uses": uses.to(dev), "k": pools[0].clone(), "v": pools[1].clone(),
+         "par": torch.zeros(R, dtype=torch.int32, device=dev), "add": torch.zeros(R, dtype=torch.int32, device=dev), "x": torch.zeros(3, R, 3, H, D, device=dev).bfloat16()}
+    b = {n: t.clone() for n, t in a.items()}
+
+    def step(s):
+        n = reorder_pages(s["table"], s["lens"], s["par"], s["uses"], P)
+        slots, n = extend_pages(s["table"], n, s["add"], s["uses"], P, 3, [(s["k"], s["v"])])
+        s["lens"].copy_(n)
+        store_pages(s["x"][0], s["x"][1], slots, s["k"], s["v"])
+        return paged_attention(s["x"][2][:, 0], s["k"], s["v"], s["table"], n)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(a)
+    for i in range(6):
+        for n, t in (("par", torch.randint(-1, R, (R,), generator=g).int()), ("add", torch.randint(0, 4, (R,), generator=g).int()),
+                     ("x", torch.randn(3, R, 3, H, D, generator=g).bfloat16())):
+            a[n].copy_(t)
+            b[n].copy_(t)
+        graph.replay()
+        want = step(b)
+        torch.cuda.synchronize()
+        for n in a:
+            assert torch.equal(a[n].view(torch.int16) if a[n].dtype == torch.bfloat16 else a[n], b[n].view(torch.int16) if b[n].dtype == torch.bfloat16 else b[n]), (i, n)
+        assert torch.equal(out, want)
 
 
 # ---- beams ---------------------------------------------------------------------------------
