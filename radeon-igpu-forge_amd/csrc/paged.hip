@@ -51,6 +51,9 @@ __device__ __forceinline__ uint32_t paged_steps(const PagedArgs& a, int n) {
     return l ? (l + kPagedTile * KW - 1) / (kPagedTile * KW) : 1u;
 }
 
+// two tiles of query heads of 128 take more than the registers of two waves a SIMD: then four waves a workgroup
+constexpr bool paged_wide(int D, int NT) { return D == 128 && NT == 2; }
+
 // floats of a piece: its rows' outputs, their maxima and sums; whole 16-byte vectors
 __host__ __device__ __forceinline__ int64_t paged_piece(const PagedPlan& p, int D) { return ((int64_t)p.gt * (D + 2) + 3) & ~3ll; }
 
@@ -70,7 +73,7 @@ __device__ __forceinline__ uint2* paged_places(const PagedArgs& a, const PagedPl
 // tokens 162 -> 152 us then; a batch whose 38 MB stay there would go from 10.5 to 13.9).  Else rows may share pages, and an eighth
 // of the line goes to each XCD, whose L2 then has what a prompt's beams have in common (35 beams 38.9 -> 31.5 us).
 template <int D, int NT, int HW, int KW, bool ONCE>
-__global__ void __launch_bounds__(64 * HW * KW, 2) paged_attn_kernel(PagedArgs a, PagedPlan plan) {
+__global__ void __launch_bounds__(64 * HW * KW, paged_wide(D, NT) ? 1 : 2) paged_attn_kernel(PagedArgs a, PagedPlan plan) {
     constexpr int NW = HW * KW;
     constexpr int LPR = D / 8;         // lanes of a row in 16-byte loads
     constexpr int RPI = 64 / LPR;      // rows of a wave-wide load
@@ -449,7 +452,7 @@ static PagedPlan paged_plan(int32_t R, int32_t H, int32_t Hkv, int32_t N, int32_
     p.gt = G < kPagedCols * tiles ? G : kPagedCols * tiles;
     p.groups = (G + p.gt - 1) / p.gt;
     const int64_t keys = (int64_t)M << shift;
-    p.hw = 1, p.kw = 8;
+    p.hw = 1, p.kw = paged_wide(D, tiles) ? 4 : 8;
     const int64_t pages = (int64_t)R * M < N ? (int64_t)R * M : N;
     p.once = (pages << shift) * Hkv * D * 4 >= (int64_t)256 << 20;
     if (keys <= 6 * 8 * kPagedTile) return p;
@@ -469,8 +472,12 @@ int64_t paged_attention_workspace(int32_t R, int32_t H, int32_t Hkv, int32_t N, 
 template <int D, int NT, bool ONCE>
 static void paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)(p.split ? p.split : a.R * a.Hkv * p.groups)), block(64 * p.hw * p.kw);
-    if (p.kw == 8) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, 8, ONCE>), grid, block, 0, st, a, p);
-    else if (p.hw == 4) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 4, 1, ONCE>), grid, block, 0, st, a, p);
+    if constexpr (!paged_wide(D, NT))
+        if (p.kw == 8) {
+            hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, 8, ONCE>), grid, block, 0, st, a, p);
+            return;
+        }
+    if (p.hw == 4) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 4, 1, ONCE>), grid, block, 0, st, a, p);
     else if (p.hw == 2) hipLaunchKernelGGL((paged_attn_kernel<D, NT, 2, 2, ONCE>), grid, block, 0, st, a, p);
     else hipLaunchKernelGGL((paged_attn_kernel<D, NT, 1, 4, ONCE>), grid, block, 0, st, a, p);
 }
