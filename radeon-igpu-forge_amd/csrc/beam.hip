@@ -12,6 +12,10 @@
 // HBM-bound: the logits are read once.  A chunk lies in registers.  64 groups of its logits have a
 // maximum each; the K-th largest of these is at most the chunk's K-th logit, and few logits lie above
 // it: they are listed and ranked by counting.
+//
+// 32 sequences of 8 beams over 131,071 bf16 tokens, a quarter of the beams done (50 MB): 26 us, 18 of them the chunks (2.8 TB/s;
+// with nothing but its loads that kernel takes 13.5, the exponentials and the lists are 2.5 each), 7.5 the join.  512 beams
+// of 50,304 fp32 (103 MB) 33.  One sequence of 4 beams of 50,304 10.4: the two launches' chains of round trips.
 #include <math.h>
 
 #include "fx_device.h"

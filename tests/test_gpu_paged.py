@@ -262,6 +262,27 @@ def test_paged_attention_on_another_stream_and_in_graphs(dev):
                 assert torch.equal(a, b)
 
 
+def test_paged_attention_and_selection_on_two_streams_at_once(dev):
+    from fxlm import beam_select, paged_attention
+    cs = [_to(dev, _case(4, 4, 2, 64, 16, 130, [2000, 17, 900, 1300], seed=s)) for s in range(2)]
+    g = torch.Generator(device=dev).manual_seed(1)
+    xs = [(torch.randn(6, 4, 30011, device=dev, generator=g), torch.randn(6, 4, device=dev, generator=g)) for _ in range(2)]
+    run = lambda i: (*paged_attention(*(cs[i][n] for n in ("q", "k", "v", "table", "lens")), return_lse=True), *beam_select(*xs[i]))   # noqa: E731
+    want = [run(i) for i in range(2)]
+    streams = [torch.cuda.Stream(device=dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            for a, b in zip(out, want[i]):
+                assert torch.equal(a, b)
+
+
 # ---- tables --------------------------------------------------------------------------------
 
 
@@ -660,6 +681,33 @@ def test_paged_steps_are_the_models_forward(dev, R):
         with torch.no_grad():
             ref = m(torch.tensor([seqs[r]], device=dev))[0, lens[r] - 1:].float().cpu()
         assert ((lg[r] - ref).abs() <= LOGITS * ref.abs().max()).all(), float((lg[r] - ref).abs().max() / ref.abs().max())
+
+
+@pytest.mark.parametrize("kw", [{"tie_embeddings": False}, {"linear_impl": "torch", "norm_impl": "torch", "mlp_impl": "torch"}])
+def test_paged_steps_of_other_models(dev, kw):
+    # a head of its own, torch's own layers; a hook on the embedding, which is then called
+    from fxlm import GPT, GPTConfig
+    torch.manual_seed(2)
+    m = GPT(GPTConfig(**{**dict(vocab_size=64, seq_len=80, n_layer=2, n_head=2, d_model=128), **kw})).to(dev).bfloat16()
+    idx, lens = torch.randint(0, 64, (3, 20), device=dev), _ints([20, 3, 11], dev)
+    tok = torch.tensor([5, 63, 0], device=dev)
+    seen = []
+    outs = []
+    for hook in (False, True):
+        if hook:
+            m.tok_emb.register_forward_hook(lambda mod, args, out: seen.append(out.shape))
+        cache = m.paged_cache(3, 8, 16)
+        m.paged_prefill(idx, lens, cache)
+        seen.clear()
+        outs.append(m.paged_step(tok, cache))
+        assert len(seen) == hook
+    assert torch.equal(*outs)
+    for r, n in enumerate(lens.tolist()):
+        with torch.no_grad():
+            ref = m(torch.cat([idx[r, :n], tok[r:r + 1]])[None])[0, -1].float()
+        assert ((outs[0][r] - ref).abs() <= LOGITS * ref.abs().max()).all()
+    out, scores = m.beam_search(idx, 6, beams=3, lens=lens)
+    assert out.shape == (3, 3, 6) and torch.isfinite(scores).all()
 
 
 def test_paged_step_rows_that_cannot_go_on(dev):
