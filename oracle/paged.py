@@ -59,7 +59,7 @@ def extend_pages(table, lens, add, uses, page, most=1, cache=None):
     for r, _, _, held in rows:
         if held is not None and uses[held] > 1:
             writers.setdefault(held, []).append(r)
-    free = [p for p in range(N) if uses[p] == 0]
+    free = torch.nonzero(uses == 0)[:, 0].tolist()
     copied = {r for p, rs in writers.items() for r in (rs if len(rs) < uses[p] else rs[1:])}
     wanted = 0
     for r, n, a, held in rows:

@@ -64,8 +64,30 @@ __device__ __forceinline__ int64_t slot_of(const ExtendArgs& a, int r, int j) {
 
 constexpr int kPagesFew = 256;                           // rows that are compared with one another in LDS
 
-template <int kPagesEach>   // rows of a thread
-__global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int64_t list, bool slots_too) {
+// Large pools (from kPagesCounted on) have their free pages counted first, a turn's kPagesThreads kPagesScan pages a workgroup, so that
+// turns without any are passed over: of 1,000,000 pages with free ones at the end alone 92 us by one workgroup, 11 so.
+constexpr int kPagesTurn = kPagesThreads * kPagesScan, kPagesCounted = 1 << 18;
+
+__global__ void __launch_bounds__(kPagesThreads) count_kernel(const int32_t* uses, int N, int32_t* counts) {
+    __shared__ int sh[kPagesWaves];
+    const int off = (int)((reinterpret_cast<uintptr_t>(uses) >> 2) & 3), p = blockIdx.x * kPagesTurn + (int)threadIdx.x * kPagesScan - off;
+    int n = 0;
+    if (p >= 0 && p + kPagesScan <= N) {
+#pragma unroll
+        for (int i = 0; i < kPagesScan / 4; ++i) {
+            const int4 u = *reinterpret_cast<const int4*>(uses + p + 4 * i);
+            n += (u.x == 0) + (u.y == 0) + (u.z == 0) + (u.w == 0);
+        }
+    } else {
+        for (int i = max(0, -p); i < min(kPagesScan, N - p); ++i) n += uses[p + i] == 0;
+    }
+    int sum;
+    block_before(n, sh, sum);
+    if (threadIdx.x == 0) counts[blockIdx.x] = sum;
+}
+
+template <int kPagesEach, bool COUNTED>   // rows of a thread, whether `counts` are given
+__global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int64_t list, const int32_t* counts, bool slots_too) {
     __shared__ int32_t pre[kPagesRows + 1], col0[kPagesRows];   // pages wanted before a row, and the column of its first
     __shared__ int sh[kPagesWaves];
     int4* copies = reinterpret_cast<int4*>(a.work);
@@ -73,14 +95,35 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
     const int tid = threadIdx.x, mask = (1 << a.shift) - 1;
     const int off = (int)((reinterpret_cast<uintptr_t>(a.uses) >> 2) & 3);   // 16-byte loads at their addresses
 
-    // which of this thread's kPagesScan pages from p on are free
+    // This thread's pages of a turn, kPagesScan from place(turn) on, and the turns that have free pages (all, where these were
+    // not counted), 64 looked up at a time by every wave.
+    const int turns = (a.N + off + kPagesTurn - 1) / kPagesTurn;
+    auto place = [&](int turn) { return turn * kPagesTurn - off + tid * kPagesScan; };
     auto whole = [&](int p) { return p >= 0 && p + kPagesScan <= a.N; };
-    constexpr bool kAhead = kPagesEach == 1;   // (eight rows take the registers)
+    int window = -64;
+    uint64_t live = 0;
+    int turn = -1;
+    auto next = [&] {
+        if (!COUNTED) return turn + 1 < turns ? turn + 1 : -1;
+        while (live == 0) {
+            window += 64;
+            if (window >= turns) return -1;
+            const int t = window + (tid & 63);
+            live = __ballot(t < turns && counts[t] > 0);
+        }
+        const int t = window + __ffsll((unsigned long long)live) - 1;
+        live &= live - 1;
+        return t;
+    };
+    constexpr bool kAhead = kPagesEach == 1;   // the first turn's uses before all else (eight rows take the registers)
     int4 ahead[kPagesScan / 4];
-    const int first = tid * kPagesScan - off;
-    if (kAhead && whole(first))
+    auto look = [&](int turn) {
+        const int p = place(turn);
+        if (turn >= 0 && whole(p))
 #pragma unroll
-        for (int i = 0; i < kPagesScan / 4; ++i) ahead[i] = *reinterpret_cast<const int4*>(a.uses + first + 4 * i);
+            for (int i = 0; i < kPagesScan / 4; ++i) ahead[i] = *reinterpret_cast<const int4*>(a.uses + p + 4 * i);
+    };
+    if (kAhead) turn = next(), look(turn);
 
     int len[kPagesEach], add[kPagesEach], open[kPagesEach];   // a row's tokens, the new ones it may have, its open page (-1: none)
     bool copy[kPagesEach], any = false;
@@ -159,13 +202,11 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
     if (tid == 0) pre[a.R] = want;
 
     int have = 0;   // free pages found, up to `want`
-    for (int p0 = -off; p0 < a.N && have < want; p0 += kPagesThreads * kPagesScan) {
-        const int p = p0 + tid * kPagesScan;
+    if (!kAhead) turn = next(), look(turn);
+    while (turn >= 0 && have < want) {
+        const int p = place(turn);
         uint32_t free = 0;
         if (whole(p)) {
-            if (!kAhead || p0 > 0)   // (the first are here)
-#pragma unroll
-                for (int i = 0; i < kPagesScan / 4; ++i) ahead[i] = *reinterpret_cast<const int4*>(a.uses + p + 4 * i);
 #pragma unroll
             for (int i = 0; i < kPagesScan / 4; ++i) {
                 const int4 u = ahead[i];
@@ -174,6 +215,8 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
         } else {
             for (int i = max(0, -p); i < min(kPagesScan, a.N - p); ++i) free |= (uint32_t)(a.uses[p + i] == 0) << i;
         }
+        turn = next();
+        look(turn);   // behind this turn's sums
         int sum;
         int at = have + block_before(__popc(free), sh, sum);
         for (; free && at < want; ++at) {
@@ -226,9 +269,13 @@ static int64_t extend_most(int32_t R, int32_t M, int32_t N, int32_t shift, int32
     return ((all < N ? all : N) + 3) & ~3ll;
 }
 
+// (the kernel of eight rows a thread has one form: its registers do not take the other)
+static bool pages_counted(int32_t R, int32_t N) { return N >= kPagesCounted || R > kPagesThreads; }
+
 int64_t extend_pages_workspace(int32_t R, int32_t M, int32_t N, int32_t shift, int32_t most) {
     if (R < 1 || M < 1 || N < 1 || shift < 0 || shift > 20 || most < 1) return 0;
-    return (4 * (int64_t)R + extend_most(R, M, N, shift, most) + (R > kPagesFew ? 2 * (int64_t)N : 0)) * (int64_t)sizeof(int32_t);
+    return (4 * (int64_t)R + extend_most(R, M, N, shift, most) + (R > kPagesFew ? 2 * (int64_t)N : 0) +
+            (pages_counted(R, N) ? ((int64_t)N + 3) / kPagesTurn + 1 : 0)) * (int64_t)sizeof(int32_t);
 }
 
 int extend_pages(const ExtendArgs& a, void* stream) {
@@ -236,13 +283,25 @@ int extend_pages(const ExtendArgs& a, void* stream) {
     FX_REQUIRE(a.M >= 1 && a.N >= 1 && a.most >= 1 && a.shift >= 0 && a.shift <= 20, "extend_pages: bad shape M=%d N=%d most=%d shift=%d", a.M, a.N,
                a.most, a.shift);
     FX_REQUIRE(((int64_t)a.M << a.shift) <= 0x7fffffff - 128 && (int64_t)a.R * a.M < 0x7fffffff, "extend_pages: a table of %d x %d pages is too large", a.R, a.M);
-    FX_REQUIRE(a.N <= 0x7fffffff - kPagesThreads * kPagesScan, "extend_pages: %d pages are too many", a.N);
+    FX_REQUIRE(a.N <= 1 << 30, "extend_pages: %d pages are too many", a.N);
     FX_REQUIRE(a.table && a.uses && a.lens && a.add && a.slots && a.out && a.work, "extend_pages: null pointer");
     FX_REQUIRE(((uintptr_t)a.work & 15) == 0, "extend_pages: work must be 16-byte aligned");
     const bool one = (int64_t)a.R * a.most <= 8 * kPagesThreads;   // slots in the same launch
     const int64_t list = extend_most(a.R, a.M, a.N, a.shift, a.most);
-    if (a.R <= kPagesThreads) hipLaunchKernelGGL((extend_kernel<1>), dim3(1), dim3(kPagesThreads), 0, (hipStream_t)stream, a, list, one);
-    else hipLaunchKernelGGL((extend_kernel<kPagesRows / kPagesThreads>), dim3(1), dim3(kPagesThreads), 0, (hipStream_t)stream, a, list, one);
+    int32_t* counts = nullptr;
+    if (pages_counted(a.R, a.N)) {
+        counts = a.work + 4 * (int64_t)a.R + list + (a.R > kPagesFew ? 2 * (int64_t)a.N : 0);
+        const int off = (int)((reinterpret_cast<uintptr_t>(a.uses) >> 2) & 3);
+        hipLaunchKernelGGL(count_kernel, dim3((unsigned)((a.N + off + kPagesTurn - 1) / kPagesTurn)), dim3(kPagesThreads), 0, (hipStream_t)stream, a.uses, a.N,
+                           counts);
+        if (int e = check_launch("extend_pages_count")) return e;
+    }
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(kPagesThreads), 0, (hipStream_t)stream, a, list, counts, one);
+    };
+    constexpr int kMost = kPagesRows / kPagesThreads;
+    if (a.R > kPagesThreads) launch(extend_kernel<kMost, true>);
+    else counts ? launch(extend_kernel<1, true>) : launch(extend_kernel<1, false>);
     if (int e = check_launch("extend_pages")) return e;
     if (one) return 0;
     const int y = (a.most + 1023) / 1024;

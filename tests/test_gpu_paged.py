@@ -356,6 +356,23 @@ def test_extend_pages_of_a_pool_in_which_the_free_ones_are_far(dev):
         _check_extend(dev, table, lens, add, u, 16, 40, d=d)
 
 
+@pytest.mark.parametrize("R,N", [(7, 2 ** 18 - 1), (7, 2 ** 18), (300, 300001), (1500, 2 ** 20 + 70003)])
+def test_extend_pages_of_large_pools(dev, R, N):
+    # pools whose free pages are counted first: at the far end, here and there (more turns than a wave looks up at once), too few, none
+    g = torch.Generator().manual_seed(R)
+    buf = torch.ones(N + 3, dtype=torch.int32, device=dev)
+    table, lens = torch.randint(0, N, (R, 4), generator=g).int(), torch.randint(0, 33, (R,), generator=g).int()
+    add = torch.randint(0, 20, (R,), generator=g).int()
+    for free, first in ((torch.arange(N - 4000, N), 0), (torch.randperm(N, generator=g)[:5000], 1), (torch.tensor([5, N // 2, N - 1]), 2), (torch.tensor([], dtype=torch.int64), 3)):
+        u = torch.ones(N, dtype=torch.int32)
+        u[free] = 0
+        u[table[:, 0].long()] = 1
+        u[table[:, 1].long()] = 1
+        buf[first:N + first] = u.to(dev)
+        _check_extend(dev, table, lens, add, u, 16, 20, d={"table": table.to(dev), "uses": buf[first:N + first].clone() if first == 0 else buf[first:N + first]})
+        buf.fill_(1)
+
+
 def test_extend_pages_at_the_edges_of_its_arguments(dev):
     # lengths below zero and past the table, additions below zero and past `most`, an open page that is none, a table of too few
     # pages; strided views
