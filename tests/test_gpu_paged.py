@@ -635,6 +635,12 @@ def test_beam_select_adversarial_order(dev):
     _check_beams(dev, x, torch.zeros(1, K) - torch.arange(K) * 0.01)
 
 
+def test_beam_select_of_many_sequences(dev):
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(3000, 8, 50, generator=g) * 2
+    _check_beams(dev, x, -torch.rand(3000, 8, generator=g).cumsum(-1), torch.rand(3000, 8, generator=g) < 0.2)
+
+
 def test_beam_select_views_and_streams(dev):
     from fxlm import beam_select
     g = torch.Generator(device=dev).manual_seed(3)
@@ -746,6 +752,22 @@ def test_paged_step_rows_that_cannot_go_on(dev):
     assert torch.isfinite(lg2[2]).all() and lg2[[0, 1]].isnan().all() and cache.lens.tolist() == [48, 33, 0, 0]
 
 
+def test_paged_step_of_some_rows(dev):
+    m = _model(dev)
+    idx, lens = torch.randint(0, 64, (4, 20), device=dev), _ints([20, 5, 16, 11], dev)
+    a, b = m.paged_cache(4, 12, 16), m.paged_cache(4, 12, 16)
+    for c in (a, b):
+        m.paged_prefill(idx, lens, c)
+    tok = torch.tensor([1, 2, 3, 4], device=dev)
+    on = torch.tensor([True, False, True, False], device=dev)
+    want, got = m.paged_step(tok, a), m.paged_step(tok, b, on)
+    assert torch.equal(got[on], want[on]) and got[~on].isnan().all() and b.lens.tolist() == [21, 5, 17, 11]
+    # the others go on from where they were
+    got = m.paged_step(tok, b, ~on)
+    assert torch.equal(got[~on], want[~on]) and got[on].isnan().all() and b.lens.tolist() == a.lens.tolist()
+    assert not m.paged_step(tok, b, torch.zeros_like(on)).isfinite().any() and b.lens.tolist() == a.lens.tolist()
+
+
 def test_generate_with_lengths(dev):
     m = _model(dev)
     idx, lens = torch.randint(0, 64, (5, 30), device=dev), _ints([30, 1, 17, 16, 9], dev)
@@ -836,6 +858,9 @@ def test_refusals_on_the_gpu(dev):
                       (TypeError, (q, k.cpu(), k, t, n))]:
         with pytest.raises(err):
             paged_attention(*args)
+    far = torch.empty(16 * 2 ** 23, device=dev, dtype=torch.bfloat16).as_strided((1, 16, 1, 64), (8, 2 ** 23, 64, 1))
+    with pytest.raises(ValueError):     # a page's rows too far apart
+        paged_attention(q[:, :2], far, far, t, n)
     u = torch.zeros(5, dtype=torch.int32, device=dev)
     for err, args, kw in [(TypeError, (t, n, n, u.cpu(), 16), {}), (TypeError, (t, n[:1], n, u, 16), {}), (ValueError, (t, n, n, u, 16), {"most": 0}),
                           (ValueError, (t.expand(2, -1)[:1].expand(2, -1), n, n, u, 16), {}), (TypeError, (t, n, n, u.repeat_interleave(2)[::2], 16), {}),
