@@ -13,7 +13,7 @@
 // maximum each; the K-th largest of these is at most the chunk's K-th logit, and few logits lie above
 // it: they are listed and ranked by counting.
 //
-// 32 sequences of 8 beams over 131,071 bf16 tokens, a quarter of the beams done (50 MB): 26 us, 18 of them the chunks (2.8 TB/s;
+// 32 sequences of 8 beams over 131,071 bf16 tokens, a quarter of the beams done (50 MB): 27 us, 19 of them the chunks (2.6 TB/s;
 // with nothing but its loads that kernel takes 13.5, the exponentials and the lists are 2.5 each), 7.5 the join.  512 beams
 // of 50,304 fp32 (103 MB) 33.  One sequence of 4 beams of 50,304 10.4: the two launches' chains of round trips.
 #include <math.h>
@@ -440,15 +440,16 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
     for (int i = n + tid; i < K; i += threads) a.out[row0 + i] = kBeamNegInf, a.rows[row0 + i] = -1, a.tokens[row0 + i] = a.fill;
 }
 
-// Chunks of as many places as 256 threads of eight vectors have, or of a quarter or an eighth while that leaves CUs without one.
-// (A chunk's first logit may lie inside a vector: so many places hold a vector's values less.)
+// Chunks of as many places as 256 threads of nine vectors have, or of two (bf16: one) while that leaves CUs without one.  (A chunk's
+// first logit may lie inside a vector: so many places hold a vector's values less.  Nine: 131,072 logits are then a
+// power of two of chunks, and rows of them whole rounds of workgroups, 256 rows of 131,071 fp32 42 us against 44 with eight.)
+constexpr int kBeamVectors = 9;
+
 static BeamPlan beam_plan(int32_t B, int32_t K, int64_t V, bool bf16) {
     BeamPlan p{};
-    const int64_t slack = bf16 ? 8 : 4, rows = (int64_t)B * K, full = kBeamThreads * 8 * slack;
-    p.few = rows * ((V + full - 1) / full) <= device_cus();
-    int64_t most = full / (p.few ? bf16 ? 8 : 4 : 1) - slack;
-    if (V > most * kBeamChunks) p.few = false, most = full - slack;
-    const int64_t n = (V + most - 1) / most;
+    const int64_t slack = bf16 ? 8 : 4, rows = (int64_t)B * K, full = kBeamThreads * kBeamVectors * slack - slack, brief = 2048 - slack;
+    p.few = rows * ((V + full - 1) / full) <= device_cus() && V <= brief * kBeamChunks;
+    const int64_t n = (V + (p.few ? brief : full) - 1) / (p.few ? brief : full);
     p.length = (int32_t)(((V + n - 1) / n + slack - 1) / slack * slack);
     p.chunks = (int32_t)((V + p.length - 1) / p.length);
     return p;
@@ -471,9 +472,9 @@ int beam_select(const BeamArgs& a, void* stream) {
     const dim3 grid((unsigned)chunks), block(kBeamThreads);
     const hipStream_t st = (hipStream_t)stream;
     if (a.bf16 && p.few) hipLaunchKernelGGL((beam_chunk_kernel<true, 1>), grid, block, 0, st, a, p);
-    else if (a.bf16) hipLaunchKernelGGL((beam_chunk_kernel<true, 8>), grid, block, 0, st, a, p);
+    else if (a.bf16) hipLaunchKernelGGL((beam_chunk_kernel<true, kBeamVectors>), grid, block, 0, st, a, p);
     else if (p.few) hipLaunchKernelGGL((beam_chunk_kernel<false, 2>), grid, block, 0, st, a, p);
-    else hipLaunchKernelGGL((beam_chunk_kernel<false, 8>), grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL((beam_chunk_kernel<false, kBeamVectors>), grid, block, 0, st, a, p);
     if (int e = check_launch("beam_select")) return e;
     // a wave a row, and a thread for each continuation of the last lists (K K <= 64 K up to 32 beams: two rows a wave past 16)
     const int threads = 64 * (a.K < 4 ? 4 : a.K < 16 ? a.K : 16);
