@@ -106,6 +106,18 @@ def test_paged_attention_rows_share_pages(dev):
         _check(dev, _case(6, 4, 2, 64, 16, M, [n, n, n - 40, n + 17, 16, 40], seed=n, share=True), False)
 
 
+# long tables over a small pool, their rows sharing pages
+@pytest.mark.parametrize("R,H,Hkv,P,M,lens", [
+    (32, 12, 12, 64, 50, [(419 * i) % 1000 for i in range(31)] + [3200]),
+    (32, 12, 12, 64, 50, [i % 3 for i in range(32)]),            # fewer steps than workgroups
+    (170, 2, 2, 32, 100, [(97 * i) % 300 for i in range(169)] + [3200]),
+    (170, 33, 1, 32, 100, [(97 * i) % 300 for i in range(169)] + [3200]),
+])
+def test_paged_attention_of_many_rows_of_a_small_pool(dev, R, H, Hkv, P, M, lens):
+    for new in (False, True):
+        _check(dev, _case(R, H, Hkv, 64, P, M, lens, seed=R + H, share=not new), new)
+
+
 def test_paged_attention_lengths_outside_the_table(dev):
     # a negative length is none, one past the table is the table's
     for M in (3, 120):
