@@ -17,7 +17,7 @@ def beam_select(logits, scores, done=None, fill=0, weight=None):
     beams' sums of log-probabilities, -inf for one that does not exist (its logits are not read).  A
     beam's continuation by token v has the score scores[b, k] + log_softmax(logits[b, k])[v].  done
     (B, K) bool: a beam that has ended goes on as it is, by the token `fill`, its score unchanged.
-    weight (B, K) fp32, positive: continuations are ranked by weight times score (a length penalty).
+    weight (B, K) fp32, positive and finite: continuations are ranked by weight times score (a length penalty).
     A token whose logit is -inf continues nothing.  K <= 32, V <= 1,048,576.
 
     Returns, best first, scores (B, K) fp32; parents (B, K) int32, the row b * K + k that each goes on

@@ -19,7 +19,7 @@ from torch import nn
 from fxgpu.abi import host
 from fxgpu.fused_linear import FEW_ROWS, fused_linear, fused_mlp, linear, linear_ex
 
-from .attention import decode_attention, flash_attention_qkv, paged_attention, tree_attention
+from .attention import check_page, decode_attention, flash_attention_qkv, paged_attention, tree_attention
 from .beam import beam_select
 from .cross_entropy import linear_cross_entropy
 from .embedding import token_embedding
@@ -388,6 +388,7 @@ class GPT(nn.Module):
     def paged_cache(self, rows, pages, page=16, max_len=None):
         """A cache of `pages` pages of `page` rows for `rows` rows of up to max_len (seq_len) tokens each
         (fxlm.PagedCache)."""
+        check_page(page)
         cfg = self.cfg
         T = cfg.seq_len if max_len is None else min(int(max_len), cfg.seq_len)
         return PagedCache(rows, pages, page, -(-T // page), cfg.n_layer, cfg.n_head, cfg.d_model // cfg.n_head, self.pos_emb.device)
@@ -465,6 +466,9 @@ class GPT(nn.Module):
             raise ValueError(f"{T} + {max_new} tokens > seq_len={L}")
         if not 1 <= K <= 32:
             raise ValueError(f"{beams} beams (1 to 32)")
+        check_page(page)
+        if length_penalty and not abs(length_penalty) * math.log(L) < 80:   # weights up to L^penalty, in 32 bits
+            raise ValueError(f"length_penalty={length_penalty}: no weights for {L} tokens")
         dev, R = idx.device, B * K
         if lens is not None:
             _check_prompts(lens, T)

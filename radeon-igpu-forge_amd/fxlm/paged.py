@@ -121,7 +121,8 @@ class PagedCache:
 
     ``extend(add, most)`` gives rows pages for their next tokens and returns the slots; ``reorder(parents)``
     lets rows go on from others or end.  Both change ``table``, ``lens`` and ``uses`` in place, so that a
-    graph can hold them.  ``table`` has room for `width` pages a row."""
+    graph can hold them (one captured before the first ``reorder`` copies no pages: rows that would need
+    a copy get nothing there).  ``table`` has room for `width` pages a row."""
 
     def __init__(self, rows, pages, page, width, layers, heads, head_dim, device):
         check_page(page)

@@ -134,3 +134,14 @@ def test_beam_search_refuses():
         m.generate(idx, 13, lens=_i(20))
     with pytest.raises(ValueError):
         m.generate(idx, 3, lens=_i(0))
+
+
+def test_beam_search_refuses_pages_and_penalties():
+    from fxlm import GPT, GPTConfig
+    m = GPT(GPTConfig(vocab_size=8, seq_len=32, n_layer=1, n_head=1, d_model=64))
+    idx = torch.zeros(1, 20, dtype=torch.int64)
+    for kw in ({"page": 0}, {"page": 24}, {"length_penalty": math.nan}, {"length_penalty": math.inf}, {"length_penalty": -100.0}):
+        with pytest.raises(ValueError):
+            m.beam_search(idx, 4, **kw)
+    with pytest.raises(ValueError):
+        m.paged_cache(2, 4, 0)
