@@ -56,11 +56,12 @@ def extend_pages(table, lens, add, uses, page, most=1, cache=None):
             continue
         rows.append((r, n, a, held))
     writers = {}
-    for r, _, _, held in rows:
+    for r, n, _, held in rows:
         if held is not None and uses[held] > 1:
-            writers.setdefault(held, []).append(r)
+            writers.setdefault(held, []).append((-(n % page), r))
     free = torch.nonzero(uses == 0)[:, 0].tolist()
-    copied = {r for p, rs in writers.items() for r in (rs if len(rs) < uses[p] else rs[1:])}
+    # (the longest writes behind every other holder's tokens, so one that is refused its copy loses none)
+    copied = {r for p, rs in writers.items() for _, r in (rs if len(rs) < uses[p] else sorted(rs)[1:])}
     wanted = 0
     for r, n, a, held in rows:
         cols = ([n // page] if r in copied else []) + list(range(-(-n // page), -(-(n + a) // page)))

@@ -45,14 +45,15 @@ __device__ __forceinline__ int block_before(int v, int* sh, int& sum) {
 //
 // Row r wants ceil((len + add) / P) - ceil(len / P) pages, and one more in place of its open page (the
 // last one, where len is no multiple of P) if it may not write there: if more rows hold the page than
-// are about to write into it, none may; else the lowest of them may.  A row that wants some gets them if
-// all rows' wants up to and with its own do not exceed the free pages; else it gets nothing.
+// are about to write into it, none may; else the one with the most tokens there may, the lowest of equals:
+// it writes behind all of the others' tokens, so that one which is refused a page, and still holds this one, loses none.
+// A row that wants some gets them if all rows' wants up to and with its own do not exceed the free pages; else it gets nothing.
 //
 // One workgroup, bounded by its chain of round trips: lengths, open pages, their uses, tables.  A thread has up to eight
 // rows in registers.  The first pages' uses are under way meanwhile; free ones are looked for only as far as they are wanted.
 // 40 rows of beams 6.2 us and 4.5 for the copies in 24 pools; 48 prompts, about 3,100 pages among 65,536, 8.0 and 2.8 for the slots.
 
-// the workspace: a copy for each row, the page each wanted one is, and, of many rows, for each page (first writer, writers)
+// the workspace: a copy for each row, the page each wanted one is, and, of many rows, for each page (the writer that may keep it, writers)
 __device__ __forceinline__ int32_t* extend_list(const ExtendArgs& a) { return a.work + 4 * (int64_t)a.R; }
 
 // the slot of row r's j-th new token, once its pages are in the table and its length in `out`
@@ -151,19 +152,20 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
     }
     auto shares = [&](int e) { return users[e] > 1 && add[e] > 0; };
     if (__syncthreads_or(any)) {
-        // who else writes into a row's open page: the rows before it, and all
+        // who else writes into a row's open page: those that would rather keep it (a lower number: more tokens there, then a lower row), and all
+        auto order = [&](int e) { return (mask - (len[e] & mask)) * kPagesRows + e * kPagesThreads + tid; };
         if (kPagesEach == 1 && a.R <= kPagesFew) {
             int before = 0, writes = 0;
-            if (tid < a.R) col0[tid] = shares(0) ? open[0] : -1;
+            if (tid < a.R) col0[tid] = shares(0) ? open[0] : -1, pre[tid] = order(0);
             __syncthreads();
             if (shares(0))
                 for (int r = 0; r < a.R; ++r) {
                     const bool same = col0[r] == open[0];
                     writes += same;
-                    before += same && r < tid;
+                    before += same && pre[r] < order(0);
                 }
             copy[0] = shares(0) && (writes < users[0] || before > 0);
-            __syncthreads();   // col0 is used again
+            __syncthreads();   // col0 and pre are used again
         } else {
 #pragma unroll
             for (int e = 0; e < kPagesEach; ++e)
@@ -172,16 +174,16 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
 #pragma unroll
             for (int e = 0; e < kPagesEach; ++e)
                 if (shares(e)) {
-                    atomicMin(&writers[2 * (int64_t)open[e]], e * kPagesThreads + tid);
+                    atomicMin(&writers[2 * (int64_t)open[e]], order(e));
                     atomicAdd(&writers[2 * (int64_t)open[e] + 1], 1);
                 }
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < kPagesEach; ++e)
                 if (shares(e)) {
-                    const int lowest = __hip_atomic_load(&writers[2 * (int64_t)open[e]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    const int first = __hip_atomic_load(&writers[2 * (int64_t)open[e]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     const int count = __hip_atomic_load(&writers[2 * (int64_t)open[e] + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    copy[e] = count < users[e] || e * kPagesThreads + tid != lowest;
+                    copy[e] = count < users[e] || order(e) != first;
                 }
         }
     }
@@ -273,14 +275,15 @@ static int64_t extend_most(int32_t R, int32_t M, int32_t N, int32_t shift, int32
 static bool pages_counted(int32_t R, int32_t N) { return N >= kPagesCounted || R > kPagesThreads; }
 
 int64_t extend_pages_workspace(int32_t R, int32_t M, int32_t N, int32_t shift, int32_t most) {
-    if (R < 1 || M < 1 || N < 1 || shift < 0 || shift > 20 || most < 1) return 0;
+    if (R < 1 || M < 1 || N < 1 || shift < 0 || shift > 18 || most < 1) return 0;
     return (4 * (int64_t)R + extend_most(R, M, N, shift, most) + (R > kPagesFew ? 2 * (int64_t)N : 0) +
             (pages_counted(R, N) ? ((int64_t)N + 3) / kPagesTurn + 1 : 0)) * (int64_t)sizeof(int32_t);
 }
 
 int extend_pages(const ExtendArgs& a, void* stream) {
     FX_REQUIRE(a.R >= 1 && a.R <= kPagesRows, "extend_pages: %d rows (1 to %d)", a.R, kPagesRows);
-    FX_REQUIRE(a.M >= 1 && a.N >= 1 && a.most >= 1 && a.shift >= 0 && a.shift <= 20, "extend_pages: bad shape M=%d N=%d most=%d shift=%d", a.M, a.N,
+    // (2^18 rows of a page times kPagesRows are the most that order() takes)
+    FX_REQUIRE(a.M >= 1 && a.N >= 1 && a.most >= 1 && a.shift >= 0 && a.shift <= 18, "extend_pages: bad shape M=%d N=%d most=%d shift=%d", a.M, a.N,
                a.most, a.shift);
     FX_REQUIRE(((int64_t)a.M << a.shift) <= 0x7fffffff - 128 && (int64_t)a.R * a.M < 0x7fffffff, "extend_pages: a table of %d x %d pages is too large", a.R, a.M);
     FX_REQUIRE(a.N <= 1 << 30, "extend_pages: %d pages are too many", a.N);

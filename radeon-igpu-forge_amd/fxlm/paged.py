@@ -26,7 +26,8 @@ def extend_pages(table, lens, add, uses, page, most=1, cache=None):
     Free pages are taken from the lowest on, in the order of the rows; table and uses are changed in place.
     cache, a list of (k, v) pools (N, page, Hkv, Dh) bf16: where a row's last page is not full and other
     rows hold it too, the row gets one of its own with the same rows in it, in every pool; if all of the
-    holders are about to write there, the lowest of them keeps it.  Without cache such a row gets nothing.
+    holders are about to write there, the one with the most tokens keeps it, the lowest of equals (so that
+    nothing of a holder that is refused a page is written over).  Without cache such a row gets nothing.
 
     Returns slots (R, most) int64, the place page * P + row of each new token in the pools' rows, -1
     behind a row's own, and the new lengths (R,) int32.  A row that cannot have all of its pages (the
