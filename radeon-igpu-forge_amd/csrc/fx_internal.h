@@ -103,7 +103,7 @@ int64_t paged_attention_workspace(int32_t R, int32_t H, int32_t Hkv, int32_t N, 
 int paged_attention(const PagedArgs& a, void* stream);
 
 // Pages and slots for tokens to be added (pages.hip).  slots (R, most) int64, out (R) int32 the lengths after it;
-// `work`: extend_pages_workspace bytes, whose first R int4 are each row's copy: (page, to page, rows, 0), rows 0 for none.
+// `work`: extend_pages_workspace bytes, whose first R int4 are each row's copy: (page, to page, rows or 0 for none, whether the row has what it wanted).
 constexpr int kPagesRows = 8192;   // rows of a table, at most
 struct ExtendArgs {
     int32_t *table, *uses;

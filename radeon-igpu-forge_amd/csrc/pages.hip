@@ -56,10 +56,11 @@ __device__ __forceinline__ int block_before(int v, int* sh, int& sum) {
 // the workspace: a copy for each row, the page each wanted one is, and, of many rows, for each page (the writer that may keep it, writers)
 __device__ __forceinline__ int32_t* extend_list(const ExtendArgs& a) { return a.work + 4 * (int64_t)a.R; }
 
-// the slot of row r's j-th new token, once its pages are in the table and its length in `out`
+// the slot of row r's j-th new token, once its pages are in the table and its copy's entry says that it was served: then
+// its tokens lie in the table with all of the new ones (a refused row's length may be anything)
 __device__ __forceinline__ int64_t slot_of(const ExtendArgs& a, int r, int j) {
-    const int add = min(max(a.add[r], 0), a.most), len = pages_len(a.lens[r], a.M, a.shift), pos = len + j;
-    if (j >= add || a.out[r] != len + add) return -1;   // (a refused row keeps its length)
+    if (j >= a.add[r] || !reinterpret_cast<const int4*>(a.work)[r].w) return -1;
+    const int pos = max(a.lens[r], 0) + j;
     return ((int64_t)a.table[(int64_t)r * a.tab + (pos >> a.shift)] << a.shift) + (pos & ((1 << a.shift) - 1));
 }
 
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
         if (r >= a.R) continue;
         const bool ok = add[e] > 0 && (need[e] == 0 || pre[r] + need[e] <= have);
         const int got = ok && need[e] > 0 ? pages[pre[r]] : -1;
-        copies[r] = ok && copy[e] ? make_int4(open[e], got, len[e] & mask, 0) : make_int4(0, 0, 0, 0);
+        copies[r] = ok && copy[e] ? make_int4(open[e], got, len[e] & mask, 1) : make_int4(0, 0, 0, ok);
         if (ok && copy[e]) atomicAdd(&a.uses[open[e]], -1);
         a.out[r] = ok ? len[e] + add[e] : a.lens[r];
         if (a.most == 1) a.slots[r] = ok ? ((int64_t)(need[e] > 0 ? got : open[e]) << a.shift) + (len[e] & mask) : -1;

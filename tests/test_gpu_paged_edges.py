@@ -1,0 +1,31 @@
+"""Calls of a paged cache's functions at the ends of what they take, on the GPU, against the 64-bit oracle."""
+import pytest
+import torch
+
+from oracle import paged as op
+
+pytestmark = pytest.mark.gpu
+
+
+def _ints(x, dev=None):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+# slots in the same launch as the tables, and in one of their own; lengths past the table by what is added, by less and by more
+@pytest.mark.parametrize("R,most", [(4, 2), (4, 65), (4, 3000), (700, 2), (700, 40), (5000, 7)])
+def test_extend_pages_lengths_past_the_table(dev, R, most):
+    from fxlm import extend_pages
+    P, M = 16, 4
+    lens = _ints([64 + (r * 7 + most) % (most + 2) if r % 3 else 64 + min(most, 1 + r % 7) for r in range(R)])
+    add = torch.where(torch.arange(R) % 3 == 0, lens - 64, _ints([r * 5 % (most + 2) for r in range(R)])).int()
+    lens[1], add[1] = 40, 3                  # one that fits
+    lens[R - 1], add[R - 1] = 65, 1          # the last row: nothing is behind it
+    assert int(((lens - 64 == add.clamp(0, most)) & (add > 0)).sum()) >= 2
+    table = torch.arange(R * M, dtype=torch.int32).view(R, M)
+    uses = torch.cat([torch.ones(R * M, dtype=torch.int32), torch.zeros(9, dtype=torch.int32)])
+    want = op.extend_pages(table, lens, add, uses, P, most)
+    dt, du = table.to(dev), uses.to(dev)
+    got = extend_pages(dt, lens.to(dev), add.to(dev), du, P, most)
+    for a, b in zip((*got, dt, du), want):
+        assert torch.equal(a.cpu(), b)
+    assert (got[0].cpu()[lens > 64] == -1).all() and int((got[0] >= 0).sum()) == min(3, most)
