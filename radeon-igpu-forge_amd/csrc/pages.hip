@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
 // the slots of longer additions
 __global__ void __launch_bounds__(256) slots_kernel(ExtendArgs a) {
     const int r = blockIdx.x;
-    for (int j = blockIdx.y * 256 + threadIdx.x; j < a.most; j += gridDim.y * 256) a.slots[(int64_t)r * a.most + j] = slot_of(a, r, j);
+    // (64 bits: `most` may be the largest int)
+    for (int64_t j = blockIdx.y * 256 + threadIdx.x; j < a.most; j += gridDim.y * 256) a.slots[(int64_t)r * a.most + j] = slot_of(a, r, (int)j);
 }
 
 // pages that rows can want between them, in whole int4
@@ -308,7 +309,7 @@ int extend_pages(const ExtendArgs& a, void* stream) {
     else counts ? launch(extend_kernel<1, true>) : launch(extend_kernel<1, false>);
     if (int e = check_launch("extend_pages")) return e;
     if (one) return 0;
-    const int y = (a.most + 1023) / 1024;
+    const int y = (a.most - 1) / 1024 + 1;
     hipLaunchKernelGGL(slots_kernel, dim3((unsigned)a.R, (unsigned)(y < 64 ? y : 64)), dim3(256), 0, (hipStream_t)stream, a);
     return check_launch("extend_pages_slots");
 }

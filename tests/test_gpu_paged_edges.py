@@ -29,3 +29,14 @@ def test_extend_pages_lengths_past_the_table(dev, R, most):
     for a, b in zip((*got, dt, du), want):
         assert torch.equal(a.cpu(), b)
     assert (got[0].cpu()[lens > 64] == -1).all() and int((got[0] >= 0).sum()) == min(3, most)
+
+
+def test_extend_pages_of_as_many_tokens_as_there_can_be(dev):
+    # 2^31 - 1 slots of a row, 16 GiB: the last ones' numbers are just below the type's end
+    from fxlm import extend_pages
+    most = 2 ** 31 - 1
+    table, uses = torch.full((1, 4), -1, dtype=torch.int32, device=dev), torch.zeros(6, dtype=torch.int32, device=dev)
+    slots, n = extend_pages(table, _ints([0], dev), _ints([40], dev), uses, 16, most)
+    assert slots.shape == (1, most) and n.tolist() == [40] and slots[0, :40].tolist() == list(range(40))
+    assert int(slots[0, 40:].amax()) == -1 and int(slots[0, 40:].amin()) == -1
+    assert table.tolist() == [[0, 1, 2, -1]] and uses.tolist() == [1, 1, 1, 0, 0, 0]
