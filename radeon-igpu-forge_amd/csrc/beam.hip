@@ -6,8 +6,9 @@
 // a beam that is done has one continuation, itself.  Equal ranks go to the lower beam, then to the
 // larger logit, then to the lower token.  Within a beam the order is that of the logits, so each row is
 // cut into chunks, a workgroup each, which keep their best K logits and the sum of their exponentials;
-// a second kernel, a workgroup a sequence, joins them.  Sums beside the exponentials' own are in 64 bits: what
-// order two beams' continuations have is decided there.
+// a second kernel, a workgroup a sequence, joins them.  Exponentials and a chunk's sum of them are in 32 bits, which
+// leaves log sum exp off by at most 66 2^-23 and 3 2^-24 of the mean distance from the maximum, and all behind them in 64: rows of
+// equal logits have equal sums, and ranks of unlike rows that are nearer than that may go either way.
 //
 // HBM-bound: the logits are read once.  A chunk lies in registers.  64 groups of its logits have a
 // maximum each; the K-th largest of these is at most the chunk's K-th logit, and few logits lie above
@@ -15,7 +16,7 @@
 //
 // 32 sequences of 8 beams over 131,071 bf16 tokens, a quarter of the beams done (50 MB): 27 us, 19 of them the chunks (2.6 TB/s;
 // with nothing but its loads that kernel takes 13.5, the exponentials and the lists are 2.5 each), 7.5 the join.  512 beams
-// of 50,304 fp32 (103 MB) 33.  One sequence of 4 beams of 50,304 10.4: the two launches' chains of round trips.
+// of 50,304 fp32 (103 MB) 32.  One sequence of 4 beams of 50,304 9.5: the two launches' chains of round trips.
 #include <math.h>
 
 #include "fx_device.h"
@@ -99,36 +100,36 @@ __device__ __forceinline__ bool beam_goes_on(const BeamArgs& a, int64_t row) {
 }
 
 // A thread's part of a chunk: NR vectors of 16 bytes, as they lie in memory.  What a pass makes of a vector is not kept for the next.
+// Vectors begin with the chunk, at whatever address that is: so what a thread sums, and in which order, is a matter of the row's
+// places alone, and rows of equal logits have equal sums, bit for bit.
 template <bool BF, int NR>
 struct BeamChunk {
     static constexpr int NP = BF ? 8 : 4;
     uint4 raw[NR];
-    float edge;           // one logit of the ragged ends
-    int tok0, edge_tok;   // the tokens of the first vector's first value (below 0: of the row before) and of the edge
+    float edge;           // one logit of the ragged end
+    int tok0, edge_tok;   // the tokens of the first vector's first value and of the edge
 
     __device__ __forceinline__ static void unpack(const uint4& u, float* f) {
         if constexpr (BF) unpack8(u, f);
         else f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
     }
-    // flat places [i0, i1) of the logits, in a row that begins at `row`; what is not theirs is -inf: neither listed nor summed
-    __device__ __forceinline__ void load(const void* logits, int64_t i0, int64_t i1, int64_t row) {
-        const int64_t f0 = i0 / NP * NP;
-        const char* base = static_cast<const char*>(logits) + f0 * (BF ? 2 : 4);
-        const int lo = (int)(i0 - f0), hi = (int)(i1 - f0), tid = threadIdx.x, whole = hi / NP;   // places from f0 on; whole vectors end here
+    // flat places [i0, i1) of the logits, from token `tok` of a row on; what is not theirs is -inf: neither listed nor summed
+    __device__ __forceinline__ void load(const void* logits, int64_t i0, int64_t i1, int tok) {
+        struct __attribute__((packed, aligned(BF ? 2 : 4))) Vector { uint4 x; };   // at a logit's address
+        const char* base = static_cast<const char*>(logits) + i0 * (BF ? 2 : 4);
+        const int n = (int)(i1 - i0), tid = threadIdx.x, whole = n / NP;
         const uint32_t ninf = BF ? 0xff80ff80u : 0xff800000u;
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             const int v = tid + i * kBeamThreads;
             raw[i] = make_uint4(ninf, ninf, ninf, ninf);
-            if (v < whole && (v > 0 || lo == 0)) raw[i] = ld16(base + (uint32_t)v * 16u);
+            if (v < whole) raw[i] = reinterpret_cast<const Vector*>(base + (uint32_t)v * 16u)->x;
         }
-        // the first vector's, where it is not whole, by the first threads; the last one's by the next
-        const int at = tid < NP ? tid : whole * NP + tid - NP;
-        const bool mine = tid < NP ? (lo > 0 || whole == 0) && at >= lo && at < hi : tid < 2 * NP && whole > 0 && at < hi;
+        const int at = whole * NP + tid;
         edge = kBeamNegInf;
-        if (mine) edge = BF ? bf16_to_f32(reinterpret_cast<const uint16_t*>(base)[at]) : reinterpret_cast<const float*>(base)[at];
-        tok0 = (int)(f0 - row) + tid * NP;
-        edge_tok = (int)(f0 - row) + at;
+        if (at < n) edge = BF ? bf16_to_f32(reinterpret_cast<const uint16_t*>(base)[at]) : reinterpret_cast<const float*>(base)[at];
+        tok0 = tok + tid * NP;
+        edge_tok = tok + at;
     }
     // f(its number, its values, the first value's token) of every vector
     template <typename Fn>
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(kBeamThreads, 8) beam_chunk_kernel(BeamArgs a,
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int64_t i0 = row * a.V + (int64_t)chunk * plan.length, i1 = min(i0 + plan.length, (row + 1) * a.V);
     BeamChunk<BF, NR> c;
-    c.load(a.logits, i0, i1, row * a.V);
+    c.load(a.logits, i0, i1, chunk * plan.length);
     if (tid == 0) listed = 0;
     // One pass as the vectors come: the thread's largest and each vector's, and the sum of 2^(x log2 e - r) above a reference, the
     // first vector's largest, r rounded (what it is rounded by is taken from the sum).  A reference too far from the thread's
@@ -440,17 +441,17 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
     for (int i = n + tid; i < K; i += threads) a.out[row0 + i] = kBeamNegInf, a.rows[row0 + i] = -1, a.tokens[row0 + i] = a.fill;
 }
 
-// Chunks of as many places as 256 threads of nine vectors have, or of two (bf16: one) while that leaves CUs without one.  (A chunk's
-// first logit may lie inside a vector: so many places hold a vector's values less.  Nine: 131,072 logits are then a
-// power of two of chunks, and rows of them whole rounds of workgroups, 256 rows of 131,071 fp32 42 us against 44 with eight.)
-constexpr int kBeamVectors = 9;
+// Chunks of as many places as 256 threads of eight vectors have, or of two (bf16: one) while that leaves CUs without one.  (Eight:
+// rows of 131,072 logits are then whole rounds of workgroups, 256 rows of 131,071 fp32 39.5 us against 41.7 with nine, 32
+// sequences of 8 bf16 beams 26.6 / 27.4, 512 beams of 50,304 fp32 32.1 / 32.8, none the slower.)
+constexpr int kBeamVectors = 8;
 
 static BeamPlan beam_plan(int32_t B, int32_t K, int64_t V, bool bf16) {
     BeamPlan p{};
-    const int64_t slack = bf16 ? 8 : 4, rows = (int64_t)B * K, full = kBeamThreads * kBeamVectors * slack - slack, brief = 2048 - slack;
+    const int64_t vec = bf16 ? 8 : 4, rows = (int64_t)B * K, full = kBeamThreads * kBeamVectors * vec, brief = 2048;
     p.few = rows * ((V + full - 1) / full) <= device_cus() && V <= brief * kBeamChunks;
     const int64_t n = (V + (p.few ? brief : full) - 1) / (p.few ? brief : full);
-    p.length = (int32_t)(((V + n - 1) / n + slack - 1) / slack * slack);
+    p.length = (int32_t)(((V + n - 1) / n + vec - 1) / vec * vec);
     p.chunks = (int32_t)((V + p.length - 1) / p.length);
     return p;
 }
