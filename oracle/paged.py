@@ -129,6 +129,8 @@ def beam_select(logits, scores, done=None, fill=0, weight=None):
             s, w = float(scores[b, k]), 1.0 if weight is None else float(weight[b, k])
             if s == -math.inf:
                 continue
+            if not 0 < w < math.inf:
+                s = math.nan
             if s != s or (done is not None and bool(done[b, k])):
                 cand.append((s == s, -w * s if s == s else 0.0, k, 0.0, fill, s))
                 continue

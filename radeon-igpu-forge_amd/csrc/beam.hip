@@ -361,7 +361,8 @@ __global__ void __launch_bounds__(kBeamJoin) beam_join_kernel(BeamArgs a, BeamPl
             if (x[i].x != kBeamNegInf) z += (double)(x[i].y * exp2_fast((x[i].x - m) * kLog2e));
         z = wave_sum(z);
         best = wave_max64(best);
-        const int what = sc == kBeamNegInf ? kNone : sc != sc ? kNaN : done ? kItself : __ballot(nan) ? kNaN : kLogits;
+        const bool fair = weight > 0.f && weight < __builtin_huge_valf();
+        const int what = sc == kBeamNegInf ? kNone : sc != sc || !fair ? kNaN : done ? kItself : __ballot(nan) ? kNaN : kLogits;
         if (lane == 0) {
             j.kind[k] = what, j.top[k] = m, j.score[k] = sc, j.weight[k] = (double)weight, j.logs[k] = log(z);
             j.best[k] = what == kNone || (what == kLogits && best == 0) ? 0 : ranked(k, what == kLogits ? best : kSelf).rank;

@@ -25,8 +25,8 @@ def beam_select(logits, scores, done=None, fill=0, weight=None):
     larger logit, then to the lower token.  Exponentials are in 32 bits: beams of equal logits and scores rank
     alike, and the order of unlike beams' continuations is that of ranks off by about 1e-6.  Where there are fewer than K continuations the rest have
     score -inf, parent -1 and token `fill`.  A beam whose score or log-probabilities are not numbers
-    (a NaN or +inf among its logits) has one continuation, of score NaN and token `fill`, and NaN ranks
-    first: it is not lost silently.
+    (a NaN or +inf among its logits), or whose weight is not positive and finite, has one continuation, of
+    score NaN and token `fill`, and NaN ranks first: it is not lost silently.
     """
     r = host.beam_select(logits, scores, done, int(fill), weight)
     if r is None:

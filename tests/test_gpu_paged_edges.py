@@ -40,3 +40,23 @@ def test_extend_pages_of_as_many_tokens_as_there_can_be(dev):
     assert slots.shape == (1, most) and n.tolist() == [40] and slots[0, :40].tolist() == list(range(40))
     assert int(slots[0, 40:].amax()) == -1 and int(slots[0, 40:].amin()) == -1
     assert table.tolist() == [[0, 1, 2, -1]] and uses.tolist() == [1, 1, 1, 0, 0, 0]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("K,V", [(4, 2), (4, 9001), (32, 300)])
+def test_beam_select_of_weights_that_are_none(dev, K, V, bf16):
+    from fxlm import beam_select
+    g = torch.Generator().manual_seed(V)
+    x, s = torch.randn(6, K, V, generator=g), -torch.rand(6, K, generator=g)
+    x = x.bfloat16() if bf16 else x
+    s[:, 3], done, w = -torch.inf, torch.zeros(6, K, dtype=torch.bool), torch.ones(6, K)
+    done[:, 2] = True
+    for b, bad in enumerate((0.0, -1.0, torch.inf, -torch.inf, torch.nan)):     # (the last sequence's weights are good)
+        w[b, 1] = w[b, 2] = w[b, 3] = bad       # of a beam that goes on, one that is done and one that does not exist
+    ro, rr, rt, _ = op.beam_select(x, s, done, 1, w)
+    out, rows, toks = (t.cpu() for t in beam_select(x.to(dev), s.to(dev), done.to(dev), 1, w.to(dev)))
+    assert torch.equal(out.isnan(), ro.isnan()) and int(out.isnan().sum()) == 10 and out[:5, :2].isnan().all()
+    assert torch.equal(rows[:5, :2], rr[:5, :2]) and (toks[:5, :2] == 1).all()
+    # log sum exp: 66 2^-23 of exponentials and sums, 3 2^-24 of the mean distance from the maximum (below 9); the score's own rounding
+    num = ~ro.isnan()
+    assert ((out.double() - ro).abs()[num] <= 2.0 ** -23 * 80 + 2.0 ** -24 * ro.abs()[num]).all()

@@ -145,3 +145,12 @@ def test_beam_search_refuses_pages_and_penalties():
             m.beam_search(idx, 4, **kw)
     with pytest.raises(ValueError):
         m.paged_cache(2, 4, 0)
+
+
+def test_beam_selection_without_a_rank():
+    # a weight that is no positive finite number gives its beam no rank: NaN, and first
+    inf = math.inf
+    x, s = torch.tensor([[[0., 1.], [3., 2.], [1., 0.], [0., 0.]]]), torch.tensor([[-1., -2., -3., -inf]])
+    for bad in (0.0, -1.0, inf, -inf, math.nan):
+        out, rows, toks, _ = op.beam_select(x, s, fill=1, weight=torch.tensor([[1., bad, 1., bad]]))
+        assert out[0, 0].isnan() and rows[0, 0] == 1 and toks[0, 0] == 1 and not (rows[0, 1:] == 1).any() and torch.isfinite(out[0, 1:]).all()
