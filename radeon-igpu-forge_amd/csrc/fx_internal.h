@@ -114,7 +114,7 @@ struct ExtendArgs {
     int32_t R, M, N, shift, most;
     bool copies;   // false: rows whose open page others hold get nothing
 };
-int64_t extend_pages_workspace(int32_t R, int32_t M, int32_t N, int32_t shift, int32_t most);
+int64_t extend_pages_workspace(int32_t R, int32_t M, int32_t N, int32_t shift, int32_t most, bool copies);
 int extend_pages(const ExtendArgs& a, void* stream);
 // the copies of extend_pages in up to kCopyTensors pools of one shape
 constexpr int kCopyTensors = 64;

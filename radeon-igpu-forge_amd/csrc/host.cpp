@@ -733,7 +733,7 @@ std::optional<std::tuple<Tensor, Tensor>> extend_pages(const Tensor& table, cons
     a.R = (int32_t)R, a.M = (int32_t)M, a.N = (int32_t)N, a.shift = shift, a.most = (int32_t)most;
     a.copies = cache.has_value();
     Tensor slots = at::empty({R, most}, table.options().dtype(at::kLong)), out = at::empty({R}, lens.options());
-    Tensor work = at::empty({fx::extend_pages_workspace(a.R, a.M, a.N, a.shift, a.most) / 4}, lens.options());
+    Tensor work = at::empty({fx::extend_pages_workspace(a.R, a.M, a.N, a.shift, a.most, a.copies) / 4}, lens.options());
     a.slots = static_cast<int64_t*>(slots.data_ptr()), a.out = i32(out), a.work = i32(work);
     check(fx::extend_pages(a, stream_of(table)), "extend_pages");
     if (cache.has_value()) {

@@ -53,7 +53,8 @@ __device__ __forceinline__ int block_before(int v, int* sh, int& sum) {
 // rows in registers.  The first pages' uses are under way meanwhile; free ones are looked for only as far as they are wanted.
 // 40 rows of beams 6.2 us and 4.5 for the copies in 24 pools; 48 prompts, about 3,100 pages among 65,536, 8.0 and 2.8 for the slots.
 
-// the workspace: a copy for each row, the page each wanted one is, and, of many rows, for each page (the writer that may keep it, writers)
+// the workspace: a copy for each row, the page each wanted one is, and, of many rows that may have copies, for each page (the writer
+// that may keep it, writers)
 __device__ __forceinline__ int32_t* extend_list(const ExtendArgs& a) { return a.work + 4 * (int64_t)a.R; }
 
 // the slot of row r's j-th new token, once its pages are in the table and its copy's entry says that it was served: then
@@ -276,9 +277,11 @@ static int64_t extend_most(int32_t R, int32_t M, int32_t N, int32_t shift, int32
 // (the kernel of eight rows a thread has one form: its registers do not take the other)
 static bool pages_counted(int32_t R, int32_t N) { return N >= kPagesCounted || R > kPagesThreads; }
 
-int64_t extend_pages_workspace(int32_t R, int32_t M, int32_t N, int32_t shift, int32_t most) {
+static int64_t extend_writers(int32_t R, int32_t N, bool copies) { return copies && R > kPagesFew ? 2 * (int64_t)N : 0; }
+
+int64_t extend_pages_workspace(int32_t R, int32_t M, int32_t N, int32_t shift, int32_t most, bool copies) {
     if (R < 1 || M < 1 || N < 1 || shift < 0 || shift > 18 || most < 1) return 0;
-    return (4 * (int64_t)R + extend_most(R, M, N, shift, most) + (R > kPagesFew ? 2 * (int64_t)N : 0) +
+    return (4 * (int64_t)R + extend_most(R, M, N, shift, most) + extend_writers(R, N, copies) +
             (pages_counted(R, N) ? ((int64_t)N + 3) / kPagesTurn + 1 : 0)) * (int64_t)sizeof(int32_t);
 }
 
@@ -295,7 +298,7 @@ int extend_pages(const ExtendArgs& a, void* stream) {
     const int64_t list = extend_most(a.R, a.M, a.N, a.shift, a.most);
     int32_t* counts = nullptr;
     if (pages_counted(a.R, a.N)) {
-        counts = a.work + 4 * (int64_t)a.R + list + (a.R > kPagesFew ? 2 * (int64_t)a.N : 0);
+        counts = a.work + 4 * (int64_t)a.R + list + extend_writers(a.R, a.N, a.copies);
         const int off = (int)((reinterpret_cast<uintptr_t>(a.uses) >> 2) & 3);
         hipLaunchKernelGGL(count_kernel, dim3((unsigned)((a.N + off + kPagesTurn - 1) / kPagesTurn)), dim3(kPagesThreads), 0, (hipStream_t)stream, a.uses, a.N,
                            counts);

@@ -60,3 +60,17 @@ def test_beam_select_of_weights_that_are_none(dev, K, V, bf16):
     # log sum exp: 66 2^-23 of exponentials and sums, 3 2^-24 of the mean distance from the maximum (below 9); the score's own rounding
     num = ~ro.isnan()
     assert ((out.double() - ro).abs()[num] <= 2.0 ** -23 * 80 + 2.0 ** -24 * ro.abs()[num]).all()
+
+
+def test_extend_pages_without_copies_needs_nothing_for_each_page(dev):
+    # many rows over a large pool of their own pages
+    from fxlm import extend_pages
+    R, N = 300, 1 << 24
+    table, uses = torch.full((R, 2), -1, dtype=torch.int32, device=dev), torch.zeros(N, dtype=torch.int32, device=dev)
+    lens, add = torch.zeros(R, dtype=torch.int32, device=dev), torch.ones(R, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats(dev)
+    held = torch.cuda.memory_allocated(dev)
+    slots, n = extend_pages(table, lens, add, uses, 16)
+    assert torch.cuda.max_memory_allocated(dev) - held < N
+    assert slots[:, 0].tolist() == list(range(0, 16 * R, 16)) and (n == 1).all() and int(uses.sum()) == R
