@@ -459,7 +459,8 @@ class GPT(nn.Module):
         done and goes on by it without cost.  Beams are ranked by their log-probability over their length
         to the power length_penalty.  Returns tokens (B, beams, max_new) int64 and log-probabilities
         (B, beams) fp32, best first; a beam that does not exist (fewer than `beams` continuations) has
-        -inf.  The beams of a prompt share its pages; a step is replayed from a HIP graph when `graph`."""
+        -inf and tokens `eos` (0 without).  The beams of a prompt share its pages; a step is replayed from
+        a HIP graph when `graph`."""
         B, T = idx.shape
         K, L = int(beams), self.cfg.seq_len
         if T + max_new > L:
@@ -497,8 +498,9 @@ class GPT(nn.Module):
         _check_finite(not bool(scores.isnan().any()))
         row, out = torch.arange(R), torch.empty(R, max_new, dtype=torch.int64)
         for t in range(max_new - 1, -1, -1):
-            out[:, t] = toks[t, row]
-            row = parents[t, row].clamp_min(0)
+            # (a beam that does not exist goes on from none: its tokens are all the fill's)
+            out[:, t] = torch.where(row >= 0, toks[t, row], s.fill)
+            row = torch.where(row >= 0, parents[t, row], -1)
         return out.view(B, K, max_new).to(dev), s.scores.clone()
 
     @torch.no_grad()
@@ -671,6 +673,7 @@ class _Beams:
     def __init__(self, model, cache, K, eos, length_penalty):
         R, dev = cache.lens.numel(), cache.lens.device
         self.cache, self.eos, self.penalty = cache, -1 if eos is None else int(eos), float(length_penalty)
+        self.fill = max(self.eos, 0)
         self.scores = torch.full((R // K, K), -math.inf, device=dev)
         self.done = torch.zeros(R // K, K, dtype=torch.bool, device=dev)
         self.length = torch.zeros(R // K, K, device=dev)
@@ -681,7 +684,7 @@ class _Beams:
         """The best continuations by logits (B, K, V): the beams from here on."""
         length = self.length + (~self.done)
         weight = length.clamp_min(1).pow(-self.penalty) if self.penalty else None
-        scores, parents, tok = beam_select(logits, self.scores, self.done, max(self.eos, 0), weight)
+        scores, parents, tok = beam_select(logits, self.scores, self.done, self.fill, weight)
         row = parents.view(-1).clamp_min(0).long()
         self.scores.copy_(scores)
         self.parents.copy_(parents.view(-1))

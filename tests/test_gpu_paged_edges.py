@@ -74,3 +74,18 @@ def test_extend_pages_without_copies_needs_nothing_for_each_page(dev):
     slots, n = extend_pages(table, lens, add, uses, 16)
     assert torch.cuda.max_memory_allocated(dev) - held < N
     assert slots[:, 0].tolist() == list(range(0, 16 * R, 16)) and (n == 1).all() and int(uses.sum()) == R
+
+
+@pytest.mark.parametrize("eos", [None, 5])
+def test_beams_that_do_not_exist_have_no_prompts_tokens(dev, eos):
+    # 4 tokens: 16 continuations by two for 32 beams
+    from fxlm import GPT, GPTConfig
+    torch.manual_seed(4)
+    m = GPT(GPTConfig(vocab_size=4, seq_len=32, n_layer=1, n_head=1, d_model=64)).to(dev).bfloat16()
+    with torch.no_grad():
+        m.tok_emb.weight.mul_(8.0)
+    out, scores = m.beam_search(torch.randint(0, 4, (3, 9), device=dev), 2, beams=32, eos=eos)
+    assert torch.isfinite(scores[:, :16]).all() and (scores[:, 16:] == -torch.inf).all()
+    assert (out[:, 16:] == (eos or 0)).all()
+    for b in range(3):
+        assert len({tuple(t) for t in out[b, :16].tolist()}) == 16
