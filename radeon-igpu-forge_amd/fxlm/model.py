@@ -657,7 +657,7 @@ def _captured(step, state):
                 t.copy_(old)
     torch.cuda.current_stream(dev).wait_stream(s)
     g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
+    with torch.cuda.graph(g, stream=s):   # (torch's own stream for it may be another GPU's)
         out = step()
 
     def replay():
@@ -749,7 +749,7 @@ class _DecodeGraph:
                     model._decode(self.tok, cache, self.pos, self.lens)
             torch.cuda.current_stream(dev).wait_stream(s)
             self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph):
+            with torch.cuda.graph(self.graph, stream=s):   # (torch's own stream for it may be another GPU's)
                 self.logits = model._decode(self.tok, cache, self.pos, self.lens)
             for (k, v), (k0, v0) in zip(cache, saved):
                 k[:, :1].copy_(k0)
