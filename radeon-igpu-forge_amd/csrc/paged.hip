@@ -513,8 +513,9 @@ int paged_attention(const PagedArgs& a, void* stream) {
     const PagedPlan p = paged_plan(a.R, a.H, a.Hkv, a.N, a.M, a.shift, a.D);
     const int64_t pairs = (int64_t)a.R * a.Hkv * p.groups;
     const int64_t steps = (((int64_t)a.M << a.shift) + kPagedTile * p.kw - 1) / (kPagedTile * p.kw);
-    // a launch has less than 2^32 work items; a row's steps and all rows' are counted in 32 bits
-    FX_REQUIRE(pairs < (1 << 23) && (int64_t)a.R * a.H < (1 << 25) && a.R * steps < 0x7fffffffLL, "paged_attention: too many rows and heads");
+    // a launch has less than 2^32 work items; all rows' steps are counted in 32 bits, and so is a row's place among those of its heads
+    FX_REQUIRE(pairs < (1 << 23) && (int64_t)a.R * a.H < (1 << 25) && a.R * steps < 0x7fffffffLL && steps * p.groups * (a.Hkv / p.hw) <= 0xffffffffLL,
+               "paged_attention: too many rows and heads");
     FX_REQUIRE(p.split == 0 || a.work, "paged_attention: null workspace");
     return a.D == 64 ? paged_launch<64>(a, p, (hipStream_t)stream) : paged_launch<128>(a, p, (hipStream_t)stream);
 }

@@ -89,3 +89,16 @@ def test_beams_that_do_not_exist_have_no_prompts_tokens(dev, eos):
     assert (out[:, 16:] == (eos or 0)).all()
     for b in range(3):
         assert len({tuple(t) for t in out[b, :16].tolist()}) == 16
+
+
+def test_paged_attention_of_more_steps_than_are_counted(dev):
+    # 2^31 keys of 512 heads are 2^26 steps of 128 groups of heads: past 32 bits, where 256 heads are just below
+    from fxlm import paged_attention
+    table, lens = torch.zeros(1, 2 ** 21 - 1, dtype=torch.int32, device=dev), _ints([3], dev)
+    for H in (256, 512):
+        q, k = torch.ones(1, H, 64, device=dev).bfloat16(), torch.ones(1, 1024, H, 64, device=dev).bfloat16()
+        if H == 256:
+            assert (paged_attention(q, k, k, table, lens) == 1).all()
+        else:
+            with pytest.raises(ValueError):
+                paged_attention(q, k, k, table, lens)
