@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kPagesThreads) count_kernel(const int32_t* use
 
 template <int kPagesEach, bool COUNTED>   // rows of a thread, whether `counts` are given
 __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int64_t list, const int32_t* counts, bool slots_too) {
-    __shared__ int32_t pre[kPagesRows + 1], col0[kPagesRows];   // pages wanted before a row, and the column of its first
+    __shared__ __attribute__((aligned(8))) int32_t pre[kPagesRows + 1], col0[kPagesRows];   // pages wanted before a row, and the column of its first
     __shared__ int sh[kPagesWaves];
     int4* copies = reinterpret_cast<int4*>(a.work);
     int32_t *pages = extend_list(a), *writers = pages + list;
@@ -158,16 +158,19 @@ __global__ void __launch_bounds__(kPagesThreads) extend_kernel(ExtendArgs a, int
         auto order = [&](int e) { return (mask - (len[e] & mask)) * kPagesRows + e * kPagesThreads + tid; };
         if (kPagesEach == 1 && a.R <= kPagesFew) {
             int before = 0, writes = 0;
-            if (tid < a.R) col0[tid] = shares(0) ? open[0] : -1, pre[tid] = order(0);
+            int2* const writer = reinterpret_cast<int2*>(pre);   // (page, order)
+            const int mine = order(0);
+            if (tid < a.R) writer[tid] = make_int2(shares(0) ? open[0] : -1, mine);
             __syncthreads();
             if (shares(0))
+#pragma unroll 8
                 for (int r = 0; r < a.R; ++r) {
-                    const bool same = col0[r] == open[0];
-                    writes += same;
-                    before += same && pre[r] < order(0);
+                    const int2 o = writer[r];
+                    writes += o.x == open[0];
+                    before += (o.x == open[0]) & (o.y < mine);
                 }
             copy[0] = shares(0) && (writes < users[0] || before > 0);
-            __syncthreads();   // col0 and pre are used again
+            __syncthreads();   // pre is used again
         } else {
 #pragma unroll
             for (int e = 0; e < kPagesEach; ++e)
