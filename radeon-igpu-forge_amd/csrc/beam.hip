@@ -292,7 +292,8 @@ struct BeamRank {
 // A workgroup a sequence, bounded by its chain of round trips and waits.  Only what is not below the least of the rows' best
 // continuations is looked at (where each row has one, K are not): of the chunks' lists, which are sorted, those with such a head;
 // where these are many, only the K lists with the best heads, in which the best K continuations lie, and what is
-// not below the last of their heads.  What remains is ranked by counting, of a few threads for each.
+// not below the last of their heads.  What remains is ranked by counting, of a few threads for each.  (Of 32 beams with a chunk a row
+// that is most of K K, each compared with all: 4 sequences over 256 or 1,000 tokens 65 us, 9,000 45, 50,304 29; 16 beams 9 to 11.)
 constexpr int kBeamJoin = 1024, kBeamChunks = 130;
 constexpr int kBeamStage = kBeamMost * kBeamChunks;   // entries in LDS
 

@@ -8,7 +8,8 @@
 // key head are columns of one product, 16 to a wave's MFMA tile.  A row without keys gives zeros.  The
 // new token's key and value (knew, vnew), where given, are key lens[r] - 1 and are written to its page.
 //
-// HBM-bound: every key and value is read once (4 D bytes a token and key head).  So the keys are split
+// HBM-bound: a row's keys and values are read once for up to 32 query heads of a key head (4 D bytes a token and key head;
+// once more for every further 32, and a page that rows share once for each of them).  So the keys are split
 // evenly, whatever the rows' lengths: all rows' and heads' steps of 32 keys lie in one line, and each
 // workgroup of one full round of CUs takes an equal piece of it, over the border of a row or a head if
 // that falls in it.  A second kernel joins the rows that were cut.  Four waves a workgroup, each with a

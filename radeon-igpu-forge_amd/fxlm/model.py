@@ -456,11 +456,11 @@ class GPT(nn.Module):
     def beam_search(self, idx, max_new, beams=4, lens=None, eos=None, length_penalty=0.0, page=16, graph=True):
         """The `beams` likeliest continuations by max_new tokens that a beam search finds after each of the
         prompts idx (B, T), of lens (B,) int32 tokens (T by default).  A beam that draws the token `eos` is
-        done and goes on by it without cost.  Beams are ranked by their log-probability over their length
-        to the power length_penalty.  Returns tokens (B, beams, max_new) int64 and log-probabilities
-        (B, beams) fp32, best first; a beam that does not exist (fewer than `beams` continuations) has
-        -inf and tokens `eos` (0 without).  The beams of a prompt share its pages; a step is replayed from
-        a HIP graph when `graph`."""
+        done and goes on by it without cost (all max_new steps are run, whoever is done).  Beams are ranked
+        by their log-probability over their length to the power length_penalty.  Returns tokens
+        (B, beams, max_new) int64 and log-probabilities (B, beams) fp32, best first; a beam that does not
+        exist (fewer than `beams` continuations) has -inf and tokens `eos` (0 without).  The beams of a
+        prompt share its pages; a step is replayed from a HIP graph when `graph`."""
         B, T = idx.shape
         K, L = int(beams), self.cfg.seq_len
         if T + max_new > L:

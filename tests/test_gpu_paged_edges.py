@@ -102,3 +102,20 @@ def test_paged_attention_of_more_steps_than_are_counted(dev):
         else:
             with pytest.raises(ValueError):
                 paged_attention(q, k, k, table, lens)
+
+
+@pytest.mark.parametrize("R,H,Hkv,D,P,M", [(64, 32, 8, 128, 16, 512), (35, 20, 2, 128, 32, 300), (16, 12, 12, 64, 16, 64)])
+def test_paged_attention_repeats(dev, R, H, Hkv, D, P, M):
+    # ragged rows whose pieces are cut and joined, the new keys written by the first call and again by each: the same bits every time
+    from fxlm import paged_attention
+    g = torch.Generator(device=dev).manual_seed(R)
+    lens = torch.randint(0, M * P // 2 + 1, (R,), device=dev, generator=g).int()
+    N = R * M // 2 + 1
+    table = torch.randperm(N, device=dev, generator=g)[:R * (M // 2)].int().view(R, M // 2)
+    table = torch.cat([table, torch.full((R, M - M // 2), -1, device=dev, dtype=torch.int32)], 1)
+    q, k, v, kn, vn = (torch.randn(s, device=dev, generator=g).bfloat16() for s in ((R, H, D), (N, P, Hkv, D), (N, P, Hkv, D), (R, Hkv, D), (R, Hkv, D)))
+    want = None
+    for _ in range(20):
+        got = paged_attention(q, k, v, table, lens, return_lse=True, k_new=kn, v_new=vn)
+        want = want or got
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
