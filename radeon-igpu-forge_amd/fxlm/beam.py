@@ -22,9 +22,10 @@ def beam_select(logits, scores, done=None, fill=0, weight=None):
 
     Returns, best first, scores (B, K) fp32; parents (B, K) int32, the row b * K + k that each goes on
     from (reorder_pages' parents); tokens (B, K) int64.  Equal ranks go to the lower beam, then to the
-    larger logit, then to the lower token.  Exponentials are in 32 bits: beams of equal logits and scores rank
-    alike, and the order of unlike beams' continuations is that of ranks off by about 1e-6.  Where there are fewer than K continuations the rest have
-    score -inf, parent -1 and token `fill`.  A beam whose score or log-probabilities are not numbers
+    larger logit, then to the lower token.  Log-probabilities come from sums in 32 bits, off by 1e-5 at
+    most and by 1e-7 as a rule: unlike beams' continuations that are nearer than that may come in either
+    order; beams of equal logits and scores rank alike.  Where there are fewer than K continuations the
+    rest have score -inf, parent -1 and token `fill`.  A beam whose score or log-probabilities are not numbers
     (a NaN or +inf among its logits), or whose weight is not positive and finite, has one continuation, of
     score NaN and token `fill`, and NaN ranks first: it is not lost silently.
     """
